@@ -1,0 +1,750 @@
+// strasgpt_k_attn_tree: GQA attention of a tree of drafted tokens over the
+// cache that ends with the tree's own rows.
+//
+// Drafted token i and head h attend to the cached keys 0..n-1 and to the
+// drafted keys j (cache row n + j) whose bit j is set in row i of the mask:
+//   s = q.k / sqrt(head_dim),  att = sum exp(s) v / sum exp(s).
+//
+// All rows (i, h) of a kv head read the same cache, so a CTA takes 16, 32, 64
+// or 128 of them as the rows of matrix instructions and walks a share of the
+// keys, tile by tile, with the running maximum, sum and output of each row in
+// registers (one pass over the cache). The keys are split over as many CTAs
+// as fill the GPU; k_merge joins their parts.
+//
+// fp32 operands keep 21 bits or more: each is the sum of two tf32 values (the
+// upper 19 bits and what they leave), and a product takes three tf32 MMAs
+// (hi.hi + hi.lo + lo.hi). The bf16 form multiplies its inputs as they are
+// and carries the probabilities as two bf16 parts, so that the only rounding
+// to bf16 is that of the result.
+//
+// What bounds it: the cache's bytes while there are few rows, the tensor
+// cores' mma.sync rate from about 32 rows (fp32) or 64 (bf16) a kv head.
+#include "entry.h"
+
+#include <math.h>
+
+#include <algorithm>
+
+extern "C" {
+#include "strasgpt_kernels.h"
+}
+
+namespace {
+
+typedef unsigned long long u64;
+
+constexpr int kStages = 3;       // key/value tiles in flight
+constexpr int kMaxSplits = 256;
+
+struct TreeArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* att;
+  long long ldq, ldo;
+  int t, kh, group, ctx, words;
+  const int* cached;
+  const u64* mask;
+  int splits, min_tiles;
+  float* part;     // [splits][kh][t * group][HD] outputs before division
+  float2* ml;      // [splits][kh][t * group] running maximum (base 2) and sum
+};
+
+__device__ __forceinline__ uint32_t saddr(const void* p) {
+  return (uint32_t)__cvta_generic_to_shared(p);
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void mma_bf16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// x = hi + lo with hi its upper 19 bits (a tf32 value) and lo the exact
+// remainder cut to tf32: 21 bits of x at least.
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  hi = __float_as_uint(x) & 0xFFFFE000u;
+  lo = __float_as_uint(x - __uint_as_float(hi)) & 0xFFFFE000u;
+}
+// Two values -> their bf16 halves (x0 in the low 16 bits) and the bf16 of
+// what those leave.
+__device__ __forceinline__ void split_bf16(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(x1), "f"(x0));
+  const float r0 = x0 - __uint_as_float(hi << 16);
+  const float r1 = x1 - __uint_as_float(hi & 0xFFFF0000u);
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(r1), "f"(r0));
+}
+
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+__device__ __forceinline__ bool finite4(float4 v) {
+  return finite(v.x) && finite(v.y) && finite(v.z) && finite(v.w);
+}
+__device__ __forceinline__ bool finite_bf16x8(uint4 v) {
+  bool ok = true;
+  for (uint32_t w : {v.x, v.y, v.z, v.w})
+    ok = ok && (w & 0x7F80u) != 0x7F80u && (w & 0x7F800000u) != 0x7F800000u;
+  return ok;
+}
+
+// Keys of a tile and the padded rows in which it lies in shared memory. The
+// paddings make every fragment load below free of bank conflicts: 16 bytes
+// shift ldmatrix rows (bf16) and the fp32 value rows 2c apart by two 16-byte
+// groups; 64 bytes put neighbouring fp32 key rows on opposite banks.
+template <typename T, int HD>
+struct Tile {
+  static constexpr bool kF32 = sizeof(T) == 4;
+  static constexpr int kKeys = (kF32 ? 4096 : 8192) / HD;
+  static constexpr int kKRow = HD * (int)sizeof(T) + (kF32 ? 64 : 16);
+  static constexpr int kVRow = HD * (int)sizeof(T) + 16;
+  static constexpr int kStage = kKeys * (kKRow + kVRow);
+  static constexpr size_t kBytes = (size_t)kStages * kStage;
+};
+
+// MW warps side by side in rows (16 each), KW in keys.
+template <typename T, int HD, int MW, int KW>
+__global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(TreeArgs a) {
+  using L = Tile<T, HD>;
+  constexpr bool kF32 = L::kF32;
+  constexpr int kThreads = 32 * MW * KW;
+  constexpr int kRows = 16 * MW;
+  constexpr int kKeys = L::kKeys, kWarpKeys = kKeys / KW;
+  constexpr int kChunk = kWarpKeys < 32 ? kWarpKeys : 32;  // keys per softmax step of a warp
+  constexpr int kN8 = kChunk / 8;
+  constexpr int kOut = HD / 8;  // n8 tiles of the output
+  static_assert(kChunk % (kF32 ? 8 : 16) == 0, "a warp's keys fill k steps");
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, c4 = lane & 3;
+  const int mw = warp % MW, kw = warp / MW;
+  const int split = blockIdx.x, head = blockIdx.y, r0 = blockIdx.z * kRows;
+  const int R = a.t * a.group;
+  sg::pdl_trigger();
+  sg::pdl_wait();
+
+  // The cache's length is read on the device (a captured call serves every
+  // later length); one outside the cache is cut to it.
+  const int n = min(max(*a.cached, 0), a.ctx - a.t);
+  const int old_tiles = (n + kKeys - 1) / kKeys;
+  const int tiles = old_tiles + (a.t + kKeys - 1) / kKeys;
+  const int per = max((tiles + a.splits - 1) / a.splits, a.min_tiles);
+  const int tile0 = split * per, tile1 = min(tiles, tile0 + per);
+  if (tile0 >= tile1) return;
+
+  const T* kbase = static_cast<const T*>(a.k) + (size_t)head * a.ctx * HD;
+  const T* vbase = static_cast<const T*>(a.v) + (size_t)head * a.ctx * HD;
+  // First cache row of a tile and its rows: a tile holds cached keys or
+  // drafted ones, never both.
+  auto extent = [&](int tile, int& row, int& rows) {
+    const bool old = tile < old_tiles;
+    const int k0 = (old ? tile : tile - old_tiles) * kKeys;
+    row = old ? k0 : n + k0;
+    rows = min(kKeys, (old ? n : a.t) - k0);
+  };
+  auto fetch = [&](int tile) {
+    if (tile < tile1) {
+      int row, rows;
+      extent(tile, row, rows);
+      const uint32_t ks = saddr(smem) + (tile - tile0) % kStages * L::kStage;
+      const uint32_t vs = ks + kKeys * L::kKRow;
+      constexpr int kVecs = HD * (int)sizeof(T) / 16;
+#pragma unroll 8
+      for (int i = threadIdx.x; i < kKeys * kVecs; i += kThreads) {
+        const int r = i / kVecs, x = i % kVecs;
+        const int bytes = r < rows ? 16 : 0;  // rows behind the last key are zeros
+        const size_t at = (size_t)(row + (r < rows ? r : 0)) * HD + x * (16 / sizeof(T));
+        cp_async16(ks + r * L::kKRow + x * 16, kbase + at, bytes);
+        cp_async16(vs + r * L::kVRow + x * 16, vbase + at, bytes);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < kStages - 1; s++) fetch(tile0 + s);
+
+  // This lane's rows g8 and g8 + 8 of the warp's 16.
+  const int rA = r0 + 16 * mw + g8, rB = rA + 8;
+  const int tA = rA / a.group, tB = rB / a.group;
+  const bool inA = rA < R, inB = rB < R;
+  const T* qA = static_cast<const T*>(a.q) + (inA ? tA : 0) * a.ldq +
+                (size_t)(head * a.group + (inA ? rA - tA * a.group : 0)) * HD;
+  const T* qB = static_cast<const T*>(a.q) + (inB ? tB : 0) * a.ldq +
+                (size_t)(head * a.group + (inB ? rB - tB * a.group : 0)) * HD;
+  // Scores in units of log2, so that the softmax is exp2.
+  const float scale = 1.4426950408889634f / sqrtf((float)HD);
+
+  // Queries as A operands. fp32: raw values, 16 entries of the head per step;
+  // slots (c, c + 4) of its two k8 steps hold entries 4c, 4c+1 and 4c+2, 4c+3
+  // (keys are read in the same order, so one float4 feeds both steps).
+  // bf16: the fragment of m16n8k16.
+  constexpr int kQ = HD / 16;
+  float4 q4[kF32 ? kQ : 1][2];
+  uint32_t q16[kF32 ? 1 : kQ][4];
+#pragma unroll
+  for (int j = 0; j < kQ; j++) {
+    if constexpr (kF32) {
+      auto load = [&](const T* p, bool in) {
+        float4 v = *reinterpret_cast<const float4*>(p + 16 * j + 4 * c4);
+        return in ? make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale)
+                  : make_float4(0.f, 0.f, 0.f, 0.f);
+      };
+      q4[j][0] = load(qA, inA);
+      q4[j][1] = load(qB, inB);
+    } else {
+      auto load = [&](const T* p, bool in, int at) {
+        return in ? *reinterpret_cast<const uint32_t*>(p + 16 * j + at) : 0u;
+      };
+      q16[j][0] = load(qA, inA, 2 * c4);
+      q16[j][1] = load(qB, inB, 2 * c4);
+      q16[j][2] = load(qA, inA, 2 * c4 + 8);
+      q16[j][3] = load(qB, inB, 2 * c4 + 8);
+    }
+  }
+
+  // Output accumulators. fp32: n8 tile 4b + i holds head entries
+  // 32b + 4 column + i (one float4 of a value row feeds four tiles).
+  float o[kOut][4];
+#pragma unroll
+  for (int i = 0; i < kOut; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float mA = -INFINITY, mB = -INFINITY, lA = 0.f, lB = 0.f;
+
+  for (int tile = tile0; tile < tile1; tile++) {
+    cp_async_wait<kStages - 2>();
+    __syncthreads();
+    fetch(tile + kStages - 1);  // into the buffer that the last tile left
+    int row, rows;
+    extent(tile, row, rows);
+    const bool old = tile < old_tiles;
+    const unsigned char* ks = smem + (tile - tile0) % kStages * L::kStage;
+    const unsigned char* vs = ks + kKeys * L::kKRow;
+    // A drafted value row with an infinity or NaN may be hidden from some of
+    // the rows: 0 * NaN in a matrix instruction would reach them. Such a tile
+    // takes the slow product below. (Cached rows are seen by all.)
+    bool slow = false;
+    if (!old) {
+      bool bad = false;
+      constexpr int kVecs = HD * (int)sizeof(T) / 16;
+      for (int i = threadIdx.x; i < kKeys * kVecs; i += kThreads) {
+        const unsigned char* p = vs + i / kVecs * L::kVRow + i % kVecs * 16;
+        if constexpr (kF32)
+          bad = bad || !finite4(*reinterpret_cast<const float4*>(p));
+        else
+          bad = bad || !finite_bf16x8(*reinterpret_cast<const uint4*>(p));
+      }
+      slow = __syncthreads_or(bad);
+    }
+
+#pragma unroll 1
+    for (int ch = 0; ch < kWarpKeys; ch += kChunk) {
+      const int k0 = kw * kWarpKeys + ch;  // first key of the chunk in the tile
+      if (k0 >= rows) break;
+      float s[kN8][4];
+#pragma unroll
+      for (int i = 0; i < kN8; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+      if constexpr (kF32) {
+        // Three accumulator sets, one per product: independent chains.
+        float s1[kN8][4], s2[kN8][4];
+#pragma unroll
+        for (int i = 0; i < kN8; i++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) s1[i][e] = s2[i][e] = 0.f;
+        const unsigned char* kp = ks + (k0 + g8) * L::kKRow + c4 * 16;
+#pragma unroll
+        for (int j = 0; j < kQ; j++) {
+          uint32_t ah[2][4], al[2][4];
+          split_tf32(q4[j][0].x, ah[0][0], al[0][0]);
+          split_tf32(q4[j][1].x, ah[0][1], al[0][1]);
+          split_tf32(q4[j][0].y, ah[0][2], al[0][2]);
+          split_tf32(q4[j][1].y, ah[0][3], al[0][3]);
+          split_tf32(q4[j][0].z, ah[1][0], al[1][0]);
+          split_tf32(q4[j][1].z, ah[1][1], al[1][1]);
+          split_tf32(q4[j][0].w, ah[1][2], al[1][2]);
+          split_tf32(q4[j][1].w, ah[1][3], al[1][3]);
+#pragma unroll
+          for (int i = 0; i < kN8; i++) {
+            const float4 kv = *reinterpret_cast<const float4*>(kp + i * 8 * L::kKRow + j * 64);
+            uint32_t bh[4], bl[4];
+            split_tf32(kv.x, bh[0], bl[0]);
+            split_tf32(kv.y, bh[1], bl[1]);
+            split_tf32(kv.z, bh[2], bl[2]);
+            split_tf32(kv.w, bh[3], bl[3]);
+            mma_tf32(s[i], ah[0], bh[0], bh[1]);
+            mma_tf32(s1[i], ah[0], bl[0], bl[1]);
+            mma_tf32(s2[i], al[0], bh[0], bh[1]);
+            mma_tf32(s[i], ah[1], bh[2], bh[3]);
+            mma_tf32(s1[i], ah[1], bl[2], bl[3]);
+            mma_tf32(s2[i], al[1], bh[2], bh[3]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kN8; i++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) s[i][e] += s1[i][e] + s2[i][e];
+      } else {
+        const uint32_t kp = saddr(ks) + (k0 + (lane & 7) + (lane >> 4) * 8) * L::kKRow +
+                            ((lane >> 3) & 1) * 16;
+#pragma unroll
+        for (int j = 0; j < kQ; j++)
+#pragma unroll
+          for (int i = 0; i < kN8; i += 2) {
+            uint32_t b[4];
+            ldsm4(kp + i * 8 * L::kKRow + j * 32, b);
+            mma_bf16(s[i], q16[j], b[0], b[1]);
+            mma_bf16(s[i + 1], q16[j], b[2], b[3]);
+          }
+#pragma unroll
+        for (int i = 0; i < kN8; i++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) s[i][e] *= scale;
+      }
+
+      // What the rows may see: all cached keys, or the mask's bits.
+      if (!old) {
+        const int j0 = row - n + k0;  // drafted index, a multiple of 8
+        const u64 wA = inA ? a.mask[(size_t)tA * a.words + (j0 >> 6)] >> (j0 & 63) : 0;
+        const u64 wB = inB ? a.mask[(size_t)tB * a.words + (j0 >> 6)] >> (j0 & 63) : 0;
+#pragma unroll
+        for (int i = 0; i < kN8; i++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const int j = 8 * i + 2 * c4 + e;
+            const bool in = k0 + j < rows;
+            if (!(in && (wA >> j & 1))) s[i][e] = -INFINITY;
+            if (!(in && (wB >> j & 1))) s[i][2 + e] = -INFINITY;
+          }
+      } else if (k0 + kChunk > rows) {
+#pragma unroll
+        for (int i = 0; i < kN8; i++)
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+            if (k0 + 8 * i + 2 * c4 + e >= rows) s[i][e] = s[i][2 + e] = -INFINITY;
+      }
+
+      // Online softmax; the four lanes of a row share its keys.
+      float xA = -INFINITY, xB = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kN8; i++) {
+        xA = fmaxf(xA, fmaxf(s[i][0], s[i][1]));
+        xB = fmaxf(xB, fmaxf(s[i][2], s[i][3]));
+      }
+      xA = fmaxf(xA, __shfl_xor_sync(0xFFFFFFFFu, xA, 1));
+      xA = fmaxf(xA, __shfl_xor_sync(0xFFFFFFFFu, xA, 2));
+      xB = fmaxf(xB, __shfl_xor_sync(0xFFFFFFFFu, xB, 1));
+      xB = fmaxf(xB, __shfl_xor_sync(0xFFFFFFFFu, xB, 2));
+      const float nA = fmaxf(mA, xA), nB = fmaxf(mB, xB);
+      if (__any_sync(0xFFFFFFFFu, nA > mA || nB > mB)) {
+        // A row that has seen no key yet keeps m = -inf and zeros.
+        const float fA = nA == -INFINITY ? 1.f : exp2f(mA - nA);
+        const float fB = nB == -INFINITY ? 1.f : exp2f(mB - nB);
+        mA = nA;
+        mB = nB;
+        lA *= fA;
+        lB *= fB;
+#pragma unroll
+        for (int i = 0; i < kOut; i++) {
+          o[i][0] *= fA;
+          o[i][1] *= fA;
+          o[i][2] *= fB;
+          o[i][3] *= fB;
+        }
+      }
+      const float zA = mA == -INFINITY ? 0.f : mA, zB = mB == -INFINITY ? 0.f : mB;
+#pragma unroll
+      for (int i = 0; i < kN8; i++) {
+        s[i][0] = exp2f(s[i][0] - zA);
+        s[i][1] = exp2f(s[i][1] - zA);
+        s[i][2] = exp2f(s[i][2] - zB);
+        s[i][3] = exp2f(s[i][3] - zB);
+        lA += s[i][0] + s[i][1];
+        lB += s[i][2] + s[i][3];
+      }
+
+      if (slow) {
+        // Key by key, weights of exactly 0 left out.
+        for (int kk = 0; kk < kChunk && k0 + kk < rows; kk++) {
+          float pA = 0.f, pB = 0.f;
+#pragma unroll
+          for (int i = 0; i < kN8; i++)
+            if (i == kk / 8) {
+              pA = kk & 1 ? s[i][1] : s[i][0];
+              pB = kk & 1 ? s[i][3] : s[i][2];
+            }
+          const int from = (lane & ~3) | (kk % 8 / 2);
+          pA = __shfl_sync(0xFFFFFFFFu, pA, from);
+          pB = __shfl_sync(0xFFFFFFFFu, pB, from);
+          const T* vr = reinterpret_cast<const T*>(vs + (k0 + kk) * L::kVRow);
+#pragma unroll
+          for (int i = 0; i < kOut; i++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              float v;
+              if constexpr (kF32)
+                v = vr[32 * (i / 4) + 4 * (2 * c4 + e) + i % 4];
+              else
+                v = sg::bf16_to_f32(vr[8 * i + 2 * c4 + e]);
+              if (pA != 0.f) o[i][e] += pA * v;
+              if (pB != 0.f) o[i][2 + e] += pB * v;
+            }
+        }
+        continue;
+      }
+
+      if constexpr (kF32) {
+        // The score accumulators are the A operand as they lie: slots c and
+        // c + 4 of a k8 step are keys 2c and 2c + 1.
+#pragma unroll
+        for (int i = 0; i < kN8; i++) {
+          uint32_t ph[4], pl[4];
+          split_tf32(s[i][0], ph[0], pl[0]);
+          split_tf32(s[i][2], ph[1], pl[1]);
+          split_tf32(s[i][1], ph[2], pl[2]);
+          split_tf32(s[i][3], ph[3], pl[3]);
+          const unsigned char* vp = vs + (k0 + 8 * i + 2 * c4) * L::kVRow + g8 * 16;
+#pragma unroll
+          for (int b = 0; b < HD / 32; b++) {
+            const float4 v0 = *reinterpret_cast<const float4*>(vp + b * 128);
+            const float4 v1 = *reinterpret_cast<const float4*>(vp + L::kVRow + b * 128);
+            uint32_t h0[4], l0[4], h1[4], l1[4];
+            split_tf32(v0.x, h0[0], l0[0]);
+            split_tf32(v0.y, h0[1], l0[1]);
+            split_tf32(v0.z, h0[2], l0[2]);
+            split_tf32(v0.w, h0[3], l0[3]);
+            split_tf32(v1.x, h1[0], l1[0]);
+            split_tf32(v1.y, h1[1], l1[1]);
+            split_tf32(v1.z, h1[2], l1[2]);
+            split_tf32(v1.w, h1[3], l1[3]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) mma_tf32(o[4 * b + e], ph, h0[e], h1[e]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) mma_tf32(o[4 * b + e], ph, l0[e], l1[e]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) mma_tf32(o[4 * b + e], pl, h0[e], h1[e]);
+          }
+        }
+      } else {
+        const uint32_t vp = saddr(vs) + (k0 + (lane & 7) + ((lane >> 3) & 1) * 8) * L::kVRow +
+                            (lane >> 4) * 16;
+#pragma unroll
+        for (int i = 0; i < kN8; i += 2) {
+          uint32_t ph[4], pl[4];
+          split_bf16(s[i][0], s[i][1], ph[0], pl[0]);
+          split_bf16(s[i][2], s[i][3], ph[1], pl[1]);
+          split_bf16(s[i + 1][0], s[i + 1][1], ph[2], pl[2]);
+          split_bf16(s[i + 1][2], s[i + 1][3], ph[3], pl[3]);
+#pragma unroll
+          for (int b = 0; b < kOut; b += 2) {
+            uint32_t v[4];
+            ldsm4t(vp + i * 8 * L::kVRow + b * 16, v);
+            mma_bf16(o[b], ph, v[0], v[1]);
+            mma_bf16(o[b + 1], ph, v[2], v[3]);
+            mma_bf16(o[b], pl, v[0], v[1]);
+            mma_bf16(o[b + 1], pl, v[2], v[3]);
+          }
+        }
+      }
+    }
+  }
+  cp_async_wait<0>();
+  lA += __shfl_xor_sync(0xFFFFFFFFu, lA, 1);
+  lA += __shfl_xor_sync(0xFFFFFFFFu, lA, 2);
+  lB += __shfl_xor_sync(0xFFFFFFFFu, lB, 1);
+  lB += __shfl_xor_sync(0xFFFFFFFFu, lB, 2);
+
+  // The key warps' parts of the rows are joined in shared memory, warps of
+  // the upper half into the lower one.
+  if constexpr (KW > 1) {
+    constexpr int kLane = kOut * 4 + 4;  // values a lane hands over
+    float* x = reinterpret_cast<float*>(smem);
+    static_assert((size_t)MW * (KW / 2) * 32 * kLane * 4 <= L::kBytes, "join fits the tiles");
+#pragma unroll
+    for (int half = KW / 2; half > 0; half /= 2) {
+      __syncthreads();
+      // [value][warp][lane]: lanes side by side.
+      if (kw >= half && kw < 2 * half) {
+        float* p = x + ((kw - half) * MW + mw) * 32 + lane;
+        constexpr int kStep = MW * (KW / 2) * 32;
+#pragma unroll
+        for (int i = 0; i < kOut; i++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) p[(4 * i + e) * kStep] = o[i][e];
+        p[(4 * kOut) * kStep] = mA;
+        p[(4 * kOut + 1) * kStep] = mB;
+        p[(4 * kOut + 2) * kStep] = lA;
+        p[(4 * kOut + 3) * kStep] = lB;
+      }
+      __syncthreads();
+      if (kw < half) {
+        const float* p = x + (kw * MW + mw) * 32 + lane;
+        constexpr int kStep = MW * (KW / 2) * 32;
+        const float m2A = p[(4 * kOut) * kStep], m2B = p[(4 * kOut + 1) * kStep];
+        const float nA = fmaxf(mA, m2A), nB = fmaxf(mB, m2B);
+        const float fA = nA == -INFINITY ? 0.f : exp2f(mA - nA);
+        const float fB = nB == -INFINITY ? 0.f : exp2f(mB - nB);
+        const float gA = nA == -INFINITY ? 0.f : exp2f(m2A - nA);
+        const float gB = nB == -INFINITY ? 0.f : exp2f(m2B - nB);
+        lA = lA * fA + p[(4 * kOut + 2) * kStep] * gA;
+        lB = lB * fB + p[(4 * kOut + 3) * kStep] * gB;
+        mA = nA;
+        mB = nB;
+#pragma unroll
+        for (int i = 0; i < kOut; i++) {
+          o[i][0] = o[i][0] * fA + p[(4 * i) * kStep] * gA;
+          o[i][1] = o[i][1] * fA + p[(4 * i + 1) * kStep] * gA;
+          o[i][2] = o[i][2] * fB + p[(4 * i + 2) * kStep] * gB;
+          o[i][3] = o[i][3] * fB + p[(4 * i + 3) * kStep] * gB;
+        }
+      }
+    }
+    if (kw > 0) return;
+  }
+
+  // One split: the rows are complete (a row without keys is zeros). Else the
+  // parts go to the workspace as they are, in 32 bits.
+  const bool whole = a.splits == 1;
+#pragma unroll
+  for (int half = 0; half < 2; half++) {
+    const int r = half ? rB : rA, tok = half ? tB : tA;
+    if (r >= R) continue;
+    const float m = half ? mB : mA, l = half ? lB : lA;
+    const float f = whole ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
+    const size_t at = ((size_t)split * a.kh + head) * R + r;
+    if (!whole && c4 == 0) a.ml[at] = make_float2(m, l);
+    T* out = static_cast<T*>(a.att) + tok * a.ldo +
+             (size_t)(head * a.group + r - tok * a.group) * HD;
+    float* part = a.part + at * HD;
+    if constexpr (kF32) {
+      float* to = whole ? reinterpret_cast<float*>(out) : part;
+#pragma unroll
+      for (int b = 0; b < HD / 32; b++)
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+          *reinterpret_cast<float4*>(to + 32 * b + 8 * c4 + 4 * e) =
+              make_float4(o[4 * b][2 * half + e] * f, o[4 * b + 1][2 * half + e] * f,
+                          o[4 * b + 2][2 * half + e] * f, o[4 * b + 3][2 * half + e] * f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kOut; i++) {
+        const float x0 = o[i][2 * half] * f, x1 = o[i][2 * half + 1] * f;
+        if (whole) {
+          uint32_t w;
+          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(x1), "f"(x0));
+          *reinterpret_cast<uint32_t*>(out + 8 * i + 2 * c4) = w;
+        } else {
+          *reinterpret_cast<float2*>(part + 8 * i + 2 * c4) = make_float2(x0, x1);
+        }
+      }
+    }
+  }
+}
+
+// One warp joins the parts of one row: their common maximum, then the sum of
+// outputs and of sums, each scaled to it.
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) k_merge(TreeArgs a, int keys_per_tile) {
+  constexpr int V = HD / 32;  // entries per lane
+  const int lane = threadIdx.x & 31;
+  const int R = a.t * a.group, row = blockIdx.x * 4 + (threadIdx.x >> 5);
+  sg::pdl_trigger();
+  sg::pdl_wait();
+  if (row >= R * a.kh) return;
+  const int n = min(max(*a.cached, 0), a.ctx - a.t);
+  const int tiles = (n + keys_per_tile - 1) / keys_per_tile +
+                    (a.t + keys_per_tile - 1) / keys_per_tile;
+  const int per = max((tiles + a.splits - 1) / a.splits, a.min_tiles);
+  const int parts = (tiles + per - 1) / per;
+  const size_t step = (size_t)a.kh * R;
+  float m = -INFINITY;
+  for (int s = lane; s < parts; s += 32) m = fmaxf(m, a.ml[s * step + row].x);
+  m = sg::warp_max(m);
+  if (m == -INFINITY) m = 0.f;  // no key in any part: all weights are 0
+  float l = 0.f, acc[V];
+#pragma unroll
+  for (int e = 0; e < V; e++) acc[e] = 0.f;
+  for (int s0 = 0; s0 < parts; s0 += 32) {
+    float f = 0.f;
+    if (s0 + lane < parts) {
+      const float2 p = a.ml[(s0 + lane) * step + row];
+      f = exp2f(p.x - m);
+      l += p.y * f;
+    }
+    const int count = min(32, parts - s0);
+#pragma unroll 8
+    for (int s = 0; s < count; s++) {
+      const float w = __shfl_sync(0xFFFFFFFFu, f, s);
+      const float* p = a.part + ((s0 + s) * step + row) * HD + lane * V;
+#pragma unroll
+      for (int e = 0; e < V; e++) acc[e] += p[e] * w;
+    }
+  }
+  l = sg::warp_sum(l);
+  const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const int head = row / R, r = row - head * R, tok = r / a.group;
+  T* out = static_cast<T*>(a.att) + tok * a.ldo +
+           (size_t)(head * a.group + r - tok * a.group) * HD + lane * V;
+#pragma unroll
+  for (int e = 0; e < V; e++) {
+    const float x = acc[e] * f;
+    if constexpr (sizeof(T) == 4)
+      out[e] = x;
+    else
+      asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(out[e]) : "f"(x));
+  }
+}
+
+// Rows of a kv head -> warps in rows and in keys.
+struct Shape {
+  int mw, kw;
+};
+Shape shape_of(int rows) {
+  if (rows <= 16) return {1, 4};
+  if (rows <= 32) return {2, 2};
+  if (rows <= 64) return {4, 1};
+  return {8, 1};
+}
+
+// Splits of the keys: as many CTAs as the GPU holds at once.
+int splits_of(int sms, int t, int kh, int group) {
+  const int rows = t * group;
+  const Shape s = shape_of(rows);
+  const int resident = sms * (s.mw * s.kw <= 4 ? 2 : 1);
+  const long long others = (long long)kh * ((rows + 16 * s.mw - 1) / (16 * s.mw));
+  return (int)std::max(1ll, std::min((long long)kMaxSplits, resident / others));
+}
+
+size_t workspace_of(int splits, int t, int kh, int group, int hd) {
+  return splits == 1 ? 0 : (size_t)splits * kh * t * group * (hd + 2) * sizeof(float);
+}
+
+template <typename T, int HD, int MW, int KW>
+cudaError_t launch_shape(const TreeArgs& a, int dev, cudaStream_t s) {
+  static std::atomic<size_t> allowed[sg::kDevices];
+  constexpr size_t bytes = Tile<T, HD>::kBytes;
+  cudaError_t e = sg::allow_smem(k_tree<T, HD, MW, KW>, bytes, dev, allowed);
+  if (e != cudaSuccess) return e;
+  const int rows = a.t * a.group;
+  e = sg::try_launch(k_tree<T, HD, MW, KW>,
+                     dim3(a.splits, a.kh, (rows + 16 * MW - 1) / (16 * MW)),
+                     dim3(32 * MW * KW), bytes, 1, s, a);
+  if (e != cudaSuccess || a.splits == 1) return e;
+  return sg::try_launch(k_merge<T, HD>, dim3((rows * a.kh + 3) / 4), dim3(128), 0, 1, s, a,
+                        Tile<T, HD>::kKeys);
+}
+
+template <typename T, int HD>
+cudaError_t launch_hd(const TreeArgs& a, int dev, cudaStream_t s) {
+  const Shape f = shape_of(a.t * a.group);
+  if (f.mw == 1) return launch_shape<T, HD, 1, 4>(a, dev, s);
+  if (f.mw == 2) return launch_shape<T, HD, 2, 2>(a, dev, s);
+  if (f.mw == 4) return launch_shape<T, HD, 4, 1>(a, dev, s);
+  return launch_shape<T, HD, 8, 1>(a, dev, s);
+}
+
+template <typename T>
+cudaError_t launch_type(const TreeArgs& a, int hd, int dev, cudaStream_t s) {
+  if (hd == 128) return launch_hd<T, 128>(a, dev, s);
+  if (hd == 64) return launch_hd<T, 64>(a, dev, s);
+  return launch_hd<T, 32>(a, dev, s);
+}
+
+const char* bad_shape(int t, int kh, int group, int hd) {
+  if (t < 0 || kh <= 0 || group <= 0) return "empty shape";
+  if (t > STRASGPT_ATTN_TREE_MAX) return "more than 1024 drafted tokens";
+  if (group > 128 || kh > 65535) return "more than 128 q heads per kv head, or 65535 kv heads";
+  if (hd != 32 && hd != 64 && hd != 128) return "head_dim must be 32, 64 or 128";
+  return nullptr;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t strasgpt_k_attn_tree_workspace(int t, int kv_heads, int group, int head_dim) {
+  const char* const me = "strasgpt_k_attn_tree_workspace";
+  if (const char* why = bad_shape(t, kv_heads, group, head_dim)) {
+    sg::refuse(me, why);
+    return 0;
+  }
+  int dev = 0, sms = 0;
+  if (const char* why = sg::current_device(&dev, &sms)) {
+    sg::refuse(me, why);
+    return 0;
+  }
+  return workspace_of(t ? splits_of(sms, t, kv_heads, group) : 1, t, kv_heads, group, head_dim);
+}
+
+int strasgpt_k_attn_tree(const void* q, long long ldq, const void* k_cache, const void* v_cache,
+                         int type, int t, int kv_heads, int group, int head_dim, int ctx,
+                         const int* cached, const uint64_t* mask, void* att, long long ldo,
+                         void* workspace, size_t workspace_bytes, void* stream) {
+  const char* const me = "strasgpt_k_attn_tree";
+  if (type != STRASGPT_F32 && type != STRASGPT_BF16) return sg::refuse(me, "unknown type");
+  if (const char* why = bad_shape(t, kv_heads, group, head_dim)) return sg::refuse(me, why);
+  if (ctx < t) return sg::refuse(me, "the cache has fewer rows than the tree");
+  const long long row = (long long)kv_heads * group * head_dim;
+  if (t > 1 && (ldq < row || ldo < row)) return sg::refuse(me, "rows of q or att overlap");
+  if (t == 0) return 0;
+  if (!q || !k_cache || !v_cache || !cached || !mask || !att)
+    return sg::refuse(me, "null buffer");
+  const size_t size = type == STRASGPT_F32 ? 4 : 2;
+  if (!sg::aligned(q, 16) || !sg::aligned(k_cache, 16) || !sg::aligned(v_cache, 16) ||
+      !sg::aligned(att, 16) || (t > 1 && (ldq * size % 16 || ldo * size % 16)))
+    return sg::refuse(me, "q, the caches, att and their rows must be 16-byte aligned");
+  if (!sg::aligned(cached, 4) || !sg::aligned(mask, 8))
+    return sg::refuse(me, "a buffer is not aligned to its entries");
+  int dev = 0, sms = 0;
+  if (const char* why = sg::current_device(&dev, &sms)) return sg::refuse(me, why);
+  for (const void* p : {q, k_cache, v_cache, (const void*)cached, (const void*)mask,
+                        (const void*)att})
+    if (const char* why = sg::not_on_device(p, dev)) return sg::refuse(me, why);
+  const int splits = splits_of(sms, t, kv_heads, group);
+  const size_t need = workspace_of(splits, t, kv_heads, group, head_dim);
+  if (need) {
+    if (!workspace || workspace_bytes < need)
+      return sg::refuse(me, "the workspace is smaller than strasgpt_k_attn_tree_workspace says");
+    if (!sg::aligned(workspace, 16)) return sg::refuse(me, "workspace must be 16-byte aligned");
+    if (const char* why = sg::not_on_device(workspace, dev)) return sg::refuse(me, why);
+  }
+  TreeArgs a;
+  a.q = q; a.k = k_cache; a.v = v_cache; a.att = att;
+  a.ldq = ldq; a.ldo = ldo;
+  a.t = t; a.kh = kv_heads; a.group = group; a.ctx = ctx; a.words = (t + 63) / 64;
+  a.cached = cached; a.mask = (const u64*)mask;
+  a.splits = splits;
+  a.min_tiles = 1;
+  a.part = (float*)workspace;
+  a.ml = (float2*)(a.part + (size_t)splits * kv_heads * t * group * head_dim);
+  const cudaStream_t s = (cudaStream_t)stream;
+  const cudaError_t e = type == STRASGPT_F32 ? launch_type<float>(a, head_dim, dev, s)
+                                             : launch_type<uint16_t>(a, head_dim, dev, s);
+  if (e != cudaSuccess) return sg::refuse_cuda(me, "launch", e);
+  return 0;
+}
+
+}  // extern "C"

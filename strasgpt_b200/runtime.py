@@ -62,6 +62,24 @@ class KernelProfile(ctypes.Structure):
                 ("bytes", ctypes.c_double * 6)]
 
 
+F32, BF16 = 0, 1  # STRASGPT_F32, STRASGPT_BF16 (include/strasgpt_kernels.h)
+ROPE_NONE, ROPE_LINEAR, ROPE_BANDS = 0, 1, 2  # STRASGPT_ROPE_*
+
+
+class Rope(ctypes.Structure):
+    """strasgpt_rope_t (include/strasgpt_kernels.h): Rope(dim=..., theta=...)."""
+    _fields_ = [("dim", ctypes.c_int), ("interleaved", ctypes.c_int),
+                ("scaling", ctypes.c_int), ("original", ctypes.c_int),
+                ("theta", ctypes.c_double), ("factor", ctypes.c_double),
+                ("low", ctypes.c_double), ("high", ctypes.c_double),
+                ("magnitude", ctypes.c_double)]
+
+    def __init__(self, dim, theta, interleaved=0, scaling=ROPE_NONE, factor=1.0,
+                 low=1.0, high=4.0, original=8192, magnitude=1.0):
+        super().__init__(dim, interleaved, scaling, original, theta, factor, low,
+                         high, magnitude)
+
+
 def lib() -> ctypes.CDLL:
     """Load libstrasgpt.so (raises if it was not built)."""
     global _lib
@@ -113,6 +131,17 @@ def lib() -> ctypes.CDLL:
                                      vp, vp]
     L.strasgpt_k_rmsnorm_rows.restype = i32
     L.strasgpt_k_rmsnorm_rows.argtypes = [vp, i32, i32, vp, ctypes.c_float, vp, vp]
+    i64 = ctypes.c_longlong
+    L.strasgpt_k_rope.restype = i32
+    L.strasgpt_k_rope.argtypes = [vp, i64, i64, vp, i64, i64, i32, i32, i32, i32, vp,
+                                  ctypes.POINTER(Rope), vp]
+    L.strasgpt_k_attn_tree_workspace.restype = sz
+    L.strasgpt_k_attn_tree_workspace.argtypes = [i32, i32, i32, i32]
+    L.strasgpt_k_attn_tree.restype = i32
+    L.strasgpt_k_attn_tree.argtypes = [vp, i64, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp,
+                                       vp, i64, vp, sz, vp]
+    L.strasgpt_k_sample.restype = i32
+    L.strasgpt_k_sample.argtypes = [vp, i32, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp]
     _lib = L
     return L
 
