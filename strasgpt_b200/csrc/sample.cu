@@ -10,18 +10,27 @@
 // Weights are 64-bit: 2^(n / 256) from a table times a cubic, 2^-42 relative.
 // fp32 has an error of 1e-7 per weight, which moves a border between a
 // hundred thousand tokens by more than many of them weigh. Sums that atomics
-// gather are integers, in a unit of 2^-42 of the largest weight that can be
-// in their bin of the histogram, and all others are added in a fixed order:
-// the same row gives the same bits whatever the order of CTAs and threads.
+// gather are integers, in a unit of 2^-31 of the largest weight that can be
+// in their bin of the histogram (two 16-bit halves of up to 45056 entries fit
+// 32-bit sums; the roundings, to nearest, stay below 1e-11 of a row's mass in
+// the mean), and all others are added in a fixed order: the same row gives
+// the same bits whatever the order of CTAs and threads.
 //
 // A row is a thread-block cluster, each CTA holding a slice of it in shared
-// memory: logits are read from HBM once, whatever the filters then need. No
-// sort: one histogram over the logit's distance from M finds the bin in which
-// a filter's border lies (a count for top-k, a mass for top-p); the entries
-// of that bin, a few as a rule, are exchanged and ranked among themselves. A
-// bin with more entries than kList is divided again, by key, until few or
-// only equal ones are left.
+// memory: logits are read from HBM once, whatever the filters then need.
+// First a bound drops what cannot be kept, so that 64-bit work is done for
+// few entries:
+//   top-k   an entry below the k-th largest of 1024 or fewer groups' largest
+//           ones (the groups' maxima are exchanged with the row's own);
+//   min-p   one below it.
+// No sort of the row: one histogram over the logit's distance from M finds
+// the bin in which a filter's border lies (a count for top-k, a mass for
+// top-p); the entries of that bin, a few as a rule, are exchanged and ranked
+// among themselves. A bin with more entries than kList is divided again, by
+// distance and then by key, until few or only equal ones are left. Where top-k's bound leaves at
+// most kThreads entries of the row, one CTA sorts those and does the rest.
 #include <cooperative_groups.h>
+#include <float.h>
 
 #include "entry.h"
 
@@ -38,9 +47,13 @@ typedef unsigned long long u64;
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr int kBins = 1024;      // two per thread
+constexpr int kBins = kThreads;  // one per thread
+constexpr int kGroups = kThreads / 4;  // of a CTA, whose maxima bound top-k
 constexpr int kList = 256;       // entries ranked against each other
-constexpr int kUnit = 42;        // a weight in its bin's unit is at most 2^kUnit
+constexpr int kWords = 3;        // a thread's entries (at most 96) as bits
+constexpr int kKept = 4096;      // entries of a slice listed behind a bound
+constexpr int kUnit = 31;        // a weight in its bin's unit is at most 2^kUnit
+constexpr int kFine = 11;        // bits more of the weights of ranked entries
 constexpr int kReach = 72;       // octaves of weight that the bins divide evenly
 
 struct SampleArgs {
@@ -61,7 +74,7 @@ struct SampleArgs {
 struct Entry {
   unsigned key;
   int idx;
-  u64 w;                         // in the bin's unit
+  u64 w;                         // in the bin's unit / 2^kFine
 };
 
 // What a CTA's threads share, before its slice of the row.
@@ -69,19 +82,35 @@ struct alignas(16) Shared {
   double table[256];             // 2^(i / 256)
   u64 gmass[kBins];              // histogram of the row: mass, count
   unsigned gcount[kBins];
-  unsigned count[kBins];         // of this slice: count, mass as two words
-  unsigned lo[kBins], hi[kBins];
-  Entry list[2][kList];          // border entries of top-k, of top-p
+  unsigned count[kBins];         // of this slice: count, and the mass as the
+  unsigned lo[kBins], hi[kBins]; // sums of the weights' lower and upper 16 bits
+  union {
+    Entry list[2][kList];        // border entries of top-k, of top-p
+    struct {
+      u64 few[kThreads];         // the row's entries that the bound leaves,
+      u64 order[kThreads];       // when they are few: key, index
+    };
+  };
+  union {
+    float maxima[kMaxCluster * kGroups];  // the groups' largest logits
+    unsigned short kept[kKept];  // places of the entries that a bound leaves
+  };
   // One slot per CTA of the cluster, written by that CTA in all of them.
-  u64 best[kMaxCluster];
   float least[kMaxCluster];
   unsigned kmin[kMaxCluster], kmax[kMaxCluster];
   unsigned number[kMaxCluster];
   double mass[kMaxCluster];
   unsigned total[kMaxCluster];
+  unsigned left[kMaxCluster];    // entries that the bound leaves in each slice
   u64 wred[kWarps];
   double wsum[kWarps];
   unsigned wmin[kWarps], wmax[kWarps];
+  float wleast[kWarps];
+  double before_mass[kMaxCluster];    // what each slice has before the border's
+  unsigned before_count[kMaxCluster]; // entries, then what it keeps in all
+  u64 slice_mass[kMaxCluster];   // of the border's entries, what is kept of
+  unsigned slice_count[kMaxCluster];  // each slice
+  unsigned few_count;
   double bbase;
   u64 bmass;
   unsigned bcount, bbin, fill;
@@ -99,6 +128,10 @@ __device__ __forceinline__ float of_key(unsigned k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
+__device__ __forceinline__ void store_f(float& to, float v) { to = v; }
+__device__ __forceinline__ void store_f(uint16_t& to, float v) {
+  to = (uint16_t)(__float_as_uint(v) >> 16);  // 0, or cut to bf16's lowest value
+}
 __device__ __forceinline__ float load_f(float v) { return v; }
 __device__ __forceinline__ float load_f(uint16_t v) { return sg::bf16_to_f32(v); }
 
@@ -123,18 +156,40 @@ __device__ __forceinline__ N block_prefix(N v, N* red, N* total) {
   __syncthreads();
   if (lane == 31) red[warp] = v;
   __syncthreads();
-  N before = 0, all = 0;
+  N w = lane < kWarps ? red[lane] : N(0);
 #pragma unroll
-  for (int w = 0; w < kWarps; w++) {
-    if (w == warp) before = all;
-    all += red[w];
+  for (int o = 1; o < kWarps; o <<= 1) {
+    const N n = shfl_up(w, o);
+    if (lane >= o) w += n;
   }
-  *total = all;
-  return before + v;
+  *total = __shfl_sync(0xFFFFFFFFu, w, kWarps - 1);
+  const N before = __shfl_sync(0xFFFFFFFFu, w, (warp + 31) & 31);
+  return warp ? before + v : v;
 }
 
 // 2^e for -1022 <= e <= 1023.
 __device__ __forceinline__ double pow2(int e) { return __hiloint2double((1023 + e) << 20, 0); }
+
+// Descending bitonic sort of the first n threads' values (the others' are 0
+// and smaller than all); `x` holds kThreads words.
+__device__ __forceinline__ u64 block_sort(u64 v, int n, u64* x) {
+  const int i = threadIdx.x;
+  for (int size = 2; size < 2 * n; size *= 2)
+    for (int step = size / 2; step; step /= 2) {
+      u64 o;
+      if (step < 32) {
+        o = __shfl_xor_sync(0xFFFFFFFFu, v, step);
+      } else {
+        __syncthreads();
+        x[i] = v;
+        __syncthreads();
+        o = x[i ^ step];
+      }
+      const bool larger = ((i & size) == 0) == ((i & step) == 0);
+      v = larger == (v > o) ? v : o;
+    }
+  return v;
+}
 
 template <typename T>
 struct Row {
@@ -142,87 +197,152 @@ struct Row {
   const T* xs;                   // this CTA's slice
   cg::cluster_group cluster;
   int rank, ranks;
-  int start;                     // the slice's first index
-  int c0, c1;                    // this thread's entries [c0, c1) of it
+  int start, per;                // the slice's first index, a slice's length
+  int c0, c1;                    // this thread's entries [c0, c1) of it, or
+  bool listed;                   // of those listed in sh->kept
+  float floor;                   // entries below are out
   float M;
   double scale;                  // log2(e) / T
   float bins_per;                // histogram bins per unit of logit
+  float octaves;                 // octaves of weight per bin
+  float last;                    // bins from M to where weights are 0
 
   __device__ float at(int i) const { return clean(load_f(xs[i])); }
 
-  // exp((x - M) / T): 2^t with t in units of 1/256 taken apart by adding
-  // 1.5 * 2^44, a cubic for the rest (|r ln 2| < 1.4e-3, the next term is
-  // below 1.5e-13). 0 below 2^-1000.
-  __device__ double weight(float x) const {
-    if (x == M) return 1.0;
+  // Drops the entries below `least` (and -inf) and returns how many stay. Up
+  // to kKept of them are listed, so that the threads get equal shares;
+  // otherwise each thread keeps its part of the slice.
+  __device__ unsigned bound(float least) {
+    floor = fmaxf(least, -FLT_MAX);
+    unsigned in[kWords], mine = 0;
+#pragma unroll
+    for (int w = 0; w < kWords; w++) {
+      unsigned m = 0;
+      const int a = c0 + 32 * w, n = min(32, c1 - a);
+#pragma unroll 8
+      for (int j = 0; j < n; j++) m |= (unsigned)(load_f(xs[a + j]) >= floor) << j;
+      in[w] = m;
+      mine += __popc(m);
+    }
+    u64 total;
+    unsigned at = (unsigned)block_prefix((u64)mine, sh->wred, &total) - mine;
+    listed = total <= kKept;
+    if (listed) {
+#pragma unroll
+      for (int w = 0; w < kWords; w++)
+        for (unsigned m = in[w]; m; m &= m - 1)
+          sh->kept[at++] = (unsigned short)(c0 + 32 * w + __ffs(m) - 1);
+      const int share = ((int)total + kThreads - 1) / kThreads;
+      c0 = min((int)threadIdx.x * share, (int)total);
+      c1 = min(c0 + share, (int)total);
+      __syncthreads();
+    }
+    return (unsigned)total;
+  }
+  __device__ int place(int j) const { return listed ? sh->kept[j] : j; }
+  // f(logit, place in the slice) for what is left, in index order.
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    for (int j = c0; j < c1; j++) {
+      const int i = place(j);
+      const float x = at(i);
+      if (x >= floor) f(x, i);
+    }
+  }
+
+  // Distance from M in bins (-inf and NaN: FLT_MAX). Every step is monotone,
+  // so larger logits come first whatever the roundings.
+  __device__ float pos(float x) const { return fminf((M - x) * bins_per, FLT_MAX); }
+  // The integer below, by adding 2^23 rounded down.
+  __device__ static int whole(float f) { return __float_as_int(__fadd_rd(f, 8388608.f)) & 0x7FFFFF; }
+  // Histogram bin; the last one is open to below.
+  __device__ static int bin_at(float f) { return whole(fminf(f, (float)(kBins - 1))); }
+  __device__ int bin_of(float x) const { return bin_at(pos(x)); }
+  // The weights of bin b are at most 2^-e: their unit is 2^-(e + kUnit).
+  __device__ int unit_of(int b) const { return kUnit + whole((float)b * octaves); }
+
+  // exp((x - M) / T) as (v, e): v 2^e, with 1 <= v < 2 or nearly so. 2^t with
+  // t in units of 1/256 taken apart by adding 1.5 * 2^44, a cubic for the
+  // rest (|r ln 2| < 1.4e-3, the next term is below 1.5e-13). No branches, so
+  // that a loop's weights overlap.
+  __device__ double power(float x, int* e) const {
     const double t = ((double)x - (double)M) * scale;
-    if (!(t > -1000.0)) return 0.0;      // also -inf, and NaN of M = inf
     const double magic = 6755399441055744.0 / 256;
     const double z = t + magic;
     const int n = __double2loint(z);
-    const double r = (t - (z - magic)) * 0.6931471805599453;
-    const double p = fma(fma(fma(r, 1.0 / 6, 0.5), r, 1.0), r, 1.0);
-    return sh->table[n & 255] * p * pow2(n >> 8);
+    const double r = t - (z - magic);
+    const double p = fma(fma(fma(r, 0.05550410866482158, 0.2402265069591007), r,
+                             0.6931471805599453), r, 1.0);
+    *e = n >> 8;
+    return sh->table[n & 255] * p;
   }
-
-  // Histogram bin, larger logits first; the last one is open to below.
-  __device__ int bin_of(float x) const {
-    if (x == M) return 0;
-    return min(kBins - 1, (int)fminf((M - x) * bins_per, (float)kBins));
+  __device__ static double shifted(double v, int e) {
+    return __hiloint2double(__double2hiint(v) + e * (1 << 20), __double2loint(v));
   }
-  // The weights of bin b are at most 2^-e: their unit is 2^-(e + kUnit).
-  __device__ int unit_of(int b) const {
-    return kUnit + (int)fmin(b * (scale / (double)bins_per), 2.0 * kReach);
+  // The weight; 0 below 2^-1000 (and for -inf and NaN).
+  __device__ double weight(float x) const {
+    int e;
+    const double v = power(x, &e);
+    return pos(x) < last ? shifted(v, e) : 0.0;
   }
   // A weight in units of 2^-unit, rounded: adding 2^52 leaves the nearest
   // integer in the low 52 bits. (A rounding of the bin's border may let a
-  // weight exceed 2^kUnit by a little, not by 2^10.)
+  // weight exceed 2^kUnit by a little.)
   __device__ u64 in_units(double w, int unit) const {
     return (u64)__double_as_longlong(fma(w, pow2(unit), 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
   }
-
-  // The cluster's histogram of the entries that `digit` puts in [0, kBins);
-  // unit(bin) is the unit of a bin's weights.
-  template <typename F, typename G>
-  __device__ void histogram(F digit, G unit) {
-    for (int b = threadIdx.x; b < kBins; b += kThreads) sh->count[b] = sh->lo[b] = sh->hi[b] = 0;
-    __syncthreads();
-    for (int i = c0; i < c1; i++) {
-      const float x = at(i);
-      const int b = digit(x);
-      if (b < 0) continue;
-      atomicAdd(&sh->count[b], 1u);
-      const u64 w = in_units(weight(x), unit(b));
-      if (w) {
-        const unsigned l = (unsigned)w;
-        const unsigned old = atomicAdd(&sh->lo[b], l);
-        const unsigned h = (unsigned)(w >> 32) + (old + l < old);
-        if (h) atomicAdd(&sh->hi[b], h);
-      }
-    }
-    cluster.sync();
-    // Each CTA adds up its share of the bins and hands it to all.
-    const int share = kBins / ranks;
-    for (int i = threadIdx.x; i < share; i += kThreads) {
-      const int b = rank * share + i;
-      unsigned c = 0;
-      u64 m = 0;
-      for (int r = 0; r < ranks; r++) {
-        const Shared* o = cluster.map_shared_rank(sh, r);
-        c += o->count[b];
-        m += ((u64)o->hi[b] << 32) + o->lo[b];
-      }
-      for (int r = 0; r < ranks; r++) {
-        Shared* o = cluster.map_shared_rank(sh, r);
-        o->gcount[b] = c;
-        o->gmass[b] = m;
-      }
-    }
-    cluster.sync();
+  // Adds the weight of x, f bins from M, to bin b.
+  __device__ void add(int b, float x, float f, int unit) {
+    int e;
+    const double v = power(x, &e);
+    const unsigned w = (unsigned)__double2loint(shifted(v, e + unit) + 4503599627370496.0);
+    if (!(f < last) || w == 0) return;
+    atomicAdd(&sh->lo[b], w & 0xFFFFu);
+    atomicAdd(&sh->hi[b], w >> 16);
   }
+  __device__ static u64 join(unsigned lo, unsigned hi) { return ((u64)hi << 16) + lo; }
+  __device__ void clear() {
+    sh->count[threadIdx.x] = sh->lo[threadIdx.x] = sh->hi[threadIdx.x] = 0;
+    __syncthreads();
+  }
+
+  // The histogram of what is left, with counts.
   __device__ void histogram() {
-    histogram([&](float x) { return x == -INFINITY ? -1 : bin_of(x); },
-              [&](int b) { return unit_of(b); });
+    clear();
+    each([&](float x, int) {
+      const float f = pos(x);
+      const int b = bin_at(f);
+      atomicAdd(&sh->count[b], 1u);
+      add(b, x, f, unit_of(b));
+    });
+    gather_histogram();
+  }
+  // The masses alone, of all of the row.
+  __device__ void histogram_of_all() {
+    clear();
+#pragma unroll 2
+    for (int i = c0; i < c1; i++) {
+      const float x = load_f(xs[i]), f = pos(x);
+      const int b = bin_at(f);
+      add(b, x, f, unit_of(b));
+    }
+    gather_histogram();
+  }
+  // The slices' histograms become the row's, in every CTA: each adds up its
+  // share of the bins and hands it to all, a thread per bin and CTA.
+  __device__ void gather_histogram() {
+    cluster.sync();
+    const int b = rank * (kBins / ranks) + threadIdx.x / ranks;
+    Shared* o = cluster.map_shared_rank(sh, threadIdx.x % ranks);
+    unsigned c = o->count[b];
+    u64 m = join(o->lo[b], o->hi[b]);
+    for (int d = 1; d < ranks; d *= 2) {
+      c += __shfl_xor_sync(0xFFFFFFFFu, c, d);
+      m += __shfl_xor_sync(0xFFFFFFFFu, m, d);
+    }
+    o->gcount[b] = c;
+    o->gmass[b] = m;
+    cluster.sync();
   }
 
   // The mass of a bin of the whole row's histogram.
@@ -231,71 +351,63 @@ struct Row {
   // The row's mass, from its histogram.
   __device__ double mass() {
     double all;
-    const int b = 2 * threadIdx.x;
-    block_prefix(mass_of(b) + mass_of(b + 1), sh->wsum, &all);
+    block_prefix(mass_of(threadIdx.x), sh->wsum, &all);
     return all;
   }
 
-  // The bin with the border: the first whose entries bring the count to k
-  // (by_mass: the mass to target). Leaves it in sh->bbin, the count before it
-  // in sh->bcount, the mass in sh->bbase (whole row) or, in units, in
-  // sh->bmass (within a bin of it); false: no bin does.
-  __device__ bool find_bin(bool by_mass, double target, unsigned k) {
-    const int b = 2 * threadIdx.x;
-    const unsigned c[2] = {sh->gcount[b], sh->gcount[b + 1]};
-    const double m[2] = {mass_of(b), mass_of(b + 1)};
-    u64 all;
-    double mall;
-    const unsigned upto = (unsigned)block_prefix((u64)(c[0] + c[1]), sh->wred, &all);
-    const double mupto = block_prefix(m[0] + m[1], sh->wsum, &mall);
+  // The lowest bin whose thread says so; kBins: none.
+  __device__ unsigned first_bin(bool here) {
     if (threadIdx.x == 0) sh->bbin = kBins;
     __syncthreads();
-    // A bin without entries is no border, whatever its sums' roundings say.
-    const bool first = c[0] && (by_mass ? mupto - m[1] >= target : upto - c[1] >= k);
-    const bool second = c[1] && (by_mass ? mupto >= target : upto >= k);
-    if (first || second) atomicMin(&sh->bbin, (unsigned)(first ? b : b + 1));
+    const unsigned who = __ballot_sync(0xFFFFFFFFu, here);
+    if (who && (threadIdx.x & 31) == __ffs(who) - 1) atomicMin(&sh->bbin, threadIdx.x);
     __syncthreads();
-    const unsigned bin = sh->bbin;
-    if ((bin >> 1) == threadIdx.x) {
-      sh->bcount = upto - c[1] - (bin & 1 ? 0 : c[0]);
-      sh->bbase = bin & 1 ? mupto - m[1] : mupto - m[1] - m[0];
+    return sh->bbin;
+  }
+
+  // The bin with the border: the first whose entries bring the count to k
+  // (by_mass: the mass to target; a bin without mass is no border, whatever
+  // its sums' roundings say). Leaves it in sh->bbin, the count before it in
+  // sh->bcount, the mass in sh->bbase; false: no bin does.
+  __device__ bool find_bin(bool by_mass, double target, unsigned k) {
+    const unsigned c = sh->gcount[threadIdx.x];
+    const double m = mass_of(threadIdx.x);
+    u64 all;
+    double mall;
+    const unsigned upto = (unsigned)block_prefix((u64)c, sh->wred, &all);
+    const double mupto = block_prefix(m, sh->wsum, &mall);
+    const unsigned bin = first_bin(by_mass ? m > 0 && mupto >= target : c && upto >= k);
+    if (bin == threadIdx.x) {
+      sh->bcount = upto - c;
+      sh->bbase = mupto - m;
     }
     __syncthreads();
     return bin < kBins;
   }
 
   // The same within one bin of the row's histogram: integers, on top of
-  // `count`, `base` and `mass` before it.
+  // `count`, `base` and `mass` before it; the mass goes to sh->bmass.
   __device__ void find_sub_bin(bool by_mass, double target, unsigned k, unsigned count,
                                double base, u64 mass, double unit) {
-    const int b = 2 * threadIdx.x;
-    const unsigned c1_ = sh->gcount[b + 1], c0_ = sh->gcount[b];
-    const u64 m1 = sh->gmass[b + 1], m0 = sh->gmass[b];
+    const unsigned c = sh->gcount[threadIdx.x];
+    const u64 m = sh->gmass[threadIdx.x];
     u64 all;
-    const unsigned upto = count + (unsigned)block_prefix((u64)(c0_ + c1_), sh->wred, &all);
-    const u64 mupto = mass + block_prefix(m0 + m1, sh->wred, &all);
-    if (threadIdx.x == 0) sh->bbin = kBins;
-    __syncthreads();
-    const bool first =
-        c0_ && (by_mass ? base + (double)(mupto - m1) * unit >= target : upto - c1_ >= k);
-    const bool second =
-        c1_ && (by_mass ? base + (double)mupto * unit >= target : upto >= k);
-    if (first || second) atomicMin(&sh->bbin, (unsigned)(first ? b : b + 1));
-    __syncthreads();
-    unsigned bin = sh->bbin;
+    const unsigned upto = count + (unsigned)block_prefix((u64)c, sh->wred, &all);
+    const u64 mupto = mass + block_prefix(m, sh->wred, &all);
+    unsigned bin = first_bin(c && (by_mass ? base + (double)mupto * unit >= target : upto >= k));
     if (bin == kBins) {
       // Roundings of the row's sums left the border behind the bin's last
       // entry: that one it is.
       __syncthreads();
       if (threadIdx.x == 0) sh->bbin = 0;
       __syncthreads();
-      if (c0_ || c1_) atomicMax(&sh->bbin, (unsigned)(c1_ ? b + 1 : b));
+      if (c) atomicMax(&sh->bbin, threadIdx.x);
       __syncthreads();
       bin = sh->bbin;
     }
-    if ((bin >> 1) == threadIdx.x) {
-      sh->bcount = upto - c1_ - (bin & 1 ? 0 : c0_);
-      sh->bmass = mupto - m1 - (bin & 1 ? 0 : m0);
+    if (bin == threadIdx.x) {
+      sh->bcount = upto - c;
+      sh->bmass = mupto - m;
     }
     __syncthreads();
   }
@@ -324,9 +436,9 @@ struct Row {
       double run = __shfl_sync(0xFFFFFFFFu, upto - mine, from);
       const int a = __shfl_sync(0xFFFFFFFFu, c0, from), b = __shfl_sync(0xFFFFFFFFu, c1, from);
       int last = -1;
-      for (int i0 = a; i0 < b; i0 += 32) {
-        const int i = i0 + lane;
-        const double v = i < b ? value(at(i), start + i) : 0.0;
+      for (int j0 = a; j0 < b; j0 += 32) {
+        const int i = place(min(j0 + lane, b - 1));
+        const double v = j0 + lane < b ? value(at(i), start + i) : 0.0;
         double s = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -335,36 +447,35 @@ struct Row {
         }
         const unsigned some = __ballot_sync(0xFFFFFFFFu, v > 0);
         const unsigned over = __ballot_sync(0xFFFFFFFFu, v > 0 && run + s > target);
-        if (some) last = i0 + 31 - __clz(some);
+        if (some) last = j0 + 31 - __clz(some);
         if (over) {
-          last = i0 + __ffs(over) - 1;
+          last = j0 + __ffs(over) - 1;
           break;
         }
         run += __shfl_sync(0xFFFFFFFFu, s, 31);
       }
-      if (lane == 0) sh->found = last;
+      if (lane == 0) sh->found = place(last);
     }
     __syncthreads();
     return start + sh->found;
   }
 
   // The prefix of the order that a filter keeps: its last entry (key and
-  // index) and, of top-k, its mass. tail: the border lies among entries of
-  // weight 0; all others are kept, and `zeros` of those.
+  // index) and its mass. tail: the border lies among entries of weight 0; all
+  // others are kept, and `zeros` of those. sums: sh->before_mass and
+  // sh->before_count say what is kept of each slice.
   struct Cut {
     unsigned key;
     int idx;
     double mass;
-    bool tail;
+    bool tail, sums;
     unsigned zeros;
   };
 
   // by_mass: the shortest prefix whose mass reaches `target`; else the first
-  // k. ready: the row's histogram is there.
+  // k. The row's histogram is there.
   __device__ Cut select(bool by_mass, double target, unsigned k, bool& ready, int which) {
-    Cut cut = {0u, INT_MAX, 0.0, false, 0u};
-    if (!ready) histogram();
-    ready = true;
+    Cut cut = {0u, INT_MAX, 0.0, false, false, 0u};
     if (!find_bin(by_mass, target, k)) {  // fewer than k entries: all are kept
       cut.mass = mass();
       return cut;
@@ -373,29 +484,92 @@ struct Row {
     const double step = pow2(-unit), base = sh->bbase;
     unsigned count = sh->bcount, number = sh->gcount[bin];
     u64 mass = 0;                         // within the bin, before its border
-    if (bin == kBins - 1 && sh->gmass[bin] == 0) {
+    if (!by_mass && bin == kBins - 1 && sh->gmass[bin] == 0) {
       cut.tail = true;
       cut.zeros = k - count;
       cut.mass = base;
       return cut;
     }
-    unsigned lo = 0, hi = 0xFFFFFFFFu;    // keys of the bin that are left
+    // The entries in question: a range of distances, and of keys.
+    float from = (float)bin, to = bin < kBins - 1 ? (float)(bin + 1) : INFINITY;
+    unsigned lo = 0, hi = 0xFFFFFFFFu;
     int digit = bin;
+    bool few = false;                     // sh->kept lists them
+    unsigned own = 0;                     // how many are this slice's
     auto in_set = [&](float x) {
-      if (x == -INFINITY || bin_of(x) != bin) return false;
+      const float f = pos(x);
+      if (!(f >= from && f < to)) return false;
       const unsigned key = key_of(x);
       return key >= lo && key <= hi;
     };
+    if (by_mass || number > kList) {
+      // Divide the bin evenly (f - bin and its multiple are exact). On the
+      // way: what the slice has before it.
+      double slice, fine;
+      block_prefix((int)threadIdx.x < bin ? (double)join(sh->lo[threadIdx.x], sh->hi[threadIdx.x]) *
+                                                pow2(-unit_of(threadIdx.x))
+                                          : 0.0,
+                   sh->wsum, &slice);
+      unsigned above = 0;
+      if (threadIdx.x == 0) sh->fill = 0;
+      clear();
+      auto divide = [&](float x, float f) {
+        const int d = bin_at((f - from) * kBins);
+        atomicAdd(&sh->count[d], 1u);
+        add(d, x, f, unit);
+      };
+      if (listed) {
+        each([&](float x, int) {
+          const float f = pos(x);
+          above += f < from;
+          if (f >= from && f < to) divide(x, f);
+        });
+      } else {
+        // The bin's entries are listed for the last look at them.
+#pragma unroll 4
+        for (int i = c0; i < c1; i++) {
+          const float x = load_f(xs[i]), f = pos(x);
+          above += f < from;
+          if (f >= from && f < to && x >= floor) {
+            divide(x, f);
+            const unsigned p = atomicAdd(&sh->fill, 1u);
+            if (p < kKept) sh->kept[p] = (unsigned short)i;
+          }
+        }
+      }
+      gather_histogram();
+      own = sh->fill;
+      few = !listed && own <= kKept;
+      ready = false;
+      find_sub_bin(by_mass, target, k, count, base, mass, step);
+      digit = (int)sh->bbin;
+      count = sh->bcount;
+      mass = sh->bmass;
+      number = sh->gcount[digit];
+      const bool before = (int)threadIdx.x < digit;
+      block_prefix(before ? (double)join(sh->lo[threadIdx.x], sh->hi[threadIdx.x]) : 0.0, sh->wsum,
+                   &fine);
+      u64 counts;
+      block_prefix((u64)(above + (before ? sh->count[threadIdx.x] : 0u)), sh->wred, &counts);
+      if (threadIdx.x < ranks) {
+        Shared* o = cluster.map_shared_rank(sh, threadIdx.x);
+        o->before_mass[rank] = slice + fine * step;
+        o->before_count[rank] = (unsigned)counts;
+      }
+      if (digit < kBins - 1) to = from + (float)(digit + 1) / kBins;
+      from += (float)digit / kBins;
+      cut.sums = true;
+    }
     while (number > kList) {
+      cut.sums = false;
       unsigned kmin = 0xFFFFFFFFu, kmax = 0, mine = 0;
-      for (int i = c0; i < c1; i++) {
-        const float x = at(i);
-        if (!in_set(x)) continue;
+      each([&](float x, int) {
+        if (!in_set(x)) return;
         mine++;
         const unsigned key = key_of(x);
         kmin = min(kmin, key);
         kmax = max(kmax, key);
-      }
+      });
       kmin = __reduce_min_sync(0xFFFFFFFFu, kmin);
       kmax = __reduce_max_sync(0xFFFFFFFFu, kmax);
       if ((threadIdx.x & 31) == 0) {
@@ -426,19 +600,20 @@ struct Row {
       if (kmin == kmax) {
         // Equal logits only: the first `take` by index are kept, while the
         // mass before them is below the target.
-        const u64 w = in_units(weight(of_key(kmin)), unit);
+        const double w = weight(of_key(kmin)), ahead = base + (double)mass * step;
         unsigned take = by_mass ? number : k - count;
         if (by_mass && w > 0) {
-          const double need = (target - (base + (double)mass * step)) / ((double)w * step);
+          const double need = (target - ahead) / w;
           if (need < (double)number) take = need > 1.0 ? (unsigned)ceil(need) : 1u;
         }
         cut.key = kmin;
-        cut.mass = base + (double)(mass + take * w) * step;
+        cut.mass = ahead + take * w;
         if (take < number) {
           // The take-th of them lies in one slice.
           if (before < take && take <= before + (unsigned)total) {
-            const int i = find_index([&](float x, int) { return in_set(x) ? 1.0 : 0.0; },
-                                     (double)mine, upto, (double)(take - 1 - before));
+            const int i = find_index(
+                [&](float x, int) { return x >= floor && in_set(x) ? 1.0 : 0.0; }, (double)mine,
+                upto, (double)(take - 1 - before));
             if (threadIdx.x < ranks) cluster.map_shared_rank(sh, threadIdx.x)->cut_idx = i;
           }
           cluster.sync();
@@ -448,11 +623,14 @@ struct Row {
       }
       int shift = 0;
       while (((kmax - kmin) >> shift) >= (unsigned)kBins) shift++;
-      lo = kmin;
-      hi = kmax;
-      histogram([&](float x) { return in_set(x) ? (int)((kmax - key_of(x)) >> shift) : -1; },
-                [&](int) { return unit; });
-      ready = false;
+      clear();
+      each([&](float x, int) {
+        if (!in_set(x)) return;
+        const int d = (int)((kmax - key_of(x)) >> shift);
+        atomicAdd(&sh->count[d], 1u);
+        add(d, x, pos(x), unit);
+      });
+      gather_histogram();
       find_sub_bin(by_mass, target, k, count, base, mass, step);
       digit = (int)sh->bbin;
       count = sh->bcount;
@@ -464,23 +642,33 @@ struct Row {
     }
     // The set's entries go to every CTA, this CTA's behind those of the CTAs
     // before it, and are ranked there.
+    __syncthreads();
     if (threadIdx.x == 0) {
       unsigned before = 0;
       for (int r = 0; r < rank; r++) before += cluster.map_shared_rank(sh, r)->count[digit];
       sh->fill = before;
     }
+    if (threadIdx.x < ranks) {
+      sh->slice_mass[threadIdx.x] = 0;
+      sh->slice_count[threadIdx.x] = 0;
+    }
     __syncthreads();
-    for (int i = c0; i < c1; i++) {
-      const float x = at(i);
-      if (!in_set(x)) continue;
+    auto send = [&](float x, int i) {
+      if (!in_set(x)) return;
       const unsigned p = atomicAdd(&sh->fill, 1u);
-      const Entry e = {key_of(x), start + i, in_units(weight(x), unit)};
+      const Entry e = {key_of(x), start + i, in_units(weight(x), unit + kFine)};
       for (int r = 0; r < ranks; r++) cluster.map_shared_rank(sh, r)->list[which][p] = e;
+    };
+    if (few) {
+      for (unsigned j = threadIdx.x; j < own; j += kThreads) send(at(sh->kept[j]), sh->kept[j]);
+    } else {
+      each(send);
     }
     cluster.sync();
+    const double ahead = base + (double)mass * step, fine = pow2(-unit - kFine);
     bool kept = false;
     unsigned place = 0;
-    u64 ahead = mass;
+    u64 before = 0;
     Entry e = {0u, 0, 0ull};
     if (threadIdx.x < number) {
       e = sh->list[which][threadIdx.x];
@@ -488,23 +676,31 @@ struct Row {
         const Entry o = sh->list[which][j];
         if (o.key > e.key || (o.key == e.key && o.idx < e.idx)) {
           place++;
-          ahead += o.w;
+          before += o.w;
         }
       }
       // The border is in this set: its first entry is kept.
       kept = place == 0 ||
-             (by_mass ? base + (double)ahead * step < target : count + place < k);
+             (by_mass ? ahead + (double)before * fine < target : count + place < k);
+      if (kept) {
+        atomicAdd(&sh->slice_mass[e.idx / per], e.w);
+        atomicAdd(&sh->slice_count[e.idx / per], 1u);
+      }
     }
     const unsigned keeps = __syncthreads_count(kept);
     if (kept && place == keeps - 1) {
       sh->cut_key = e.key;
       sh->cut_idx = e.idx;
-      sh->bmass = ahead + e.w;
+      sh->bmass = before + e.w;
+    }
+    if (cut.sums && threadIdx.x < ranks) {
+      sh->before_mass[threadIdx.x] += (double)sh->slice_mass[threadIdx.x] * fine;
+      sh->before_count[threadIdx.x] += sh->slice_count[threadIdx.x];
     }
     __syncthreads();
     cut.key = sh->cut_key;
     cut.idx = sh->cut_idx;
-    cut.mass = base + (double)sh->bmass * step;
+    cut.mass = ahead + (double)sh->bmass * fine;
     return cut;
   }
 };
@@ -517,108 +713,222 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleArgs a) {
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int row = blockIdx.x / ranks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  cluster.barrier_arrive();  // waited for before the first access to another CTA
   if (threadIdx.x < 256) sh->table[threadIdx.x] = exp2(threadIdx.x / 256.0);
   sg::pdl_trigger();
   sg::pdl_wait();
 
   const int start = min(rank * a.per, a.vocab), n = min(a.per, a.vocab - start);
   const T* src = static_cast<const T*>(a.logits) + row * a.ld + start;
-  // Slice into shared memory; its largest key (with the lowest index that has
-  // it) and its smallest finite logit.
-  u64 best = 0;
-  float least = INFINITY;
-  auto take = [&](float x, int i) {
-    const u64 b = ((u64)key_of(x) << 32) | (unsigned)(0x7FFFFFFF - (start + i));
-    if (x > -INFINITY) {
-      best = b > best ? b : best;
-      least = fminf(least, x);
-    }
+  // Slice into shared memory; its largest logit and its smallest finite one.
+  float top = -INFINITY, least = INFINITY;
+  auto take = [&](float x) {
+    top = fmaxf(top, x);         // a NaN is passed over
+    least = fminf(least, x > -INFINITY ? x : INFINITY);
   };
   constexpr int V = 16 / sizeof(T);
   const int nv = a.vec ? n / V : 0;
-#pragma unroll 4
+#pragma unroll 8
   for (int v = threadIdx.x; v < nv; v += kThreads) {
     const uint4 r = sg::ldg_stream(src + v * V);
     T e[V];
     memcpy(e, &r, 16);
 #pragma unroll
-    for (int j = 0; j < V; j++) take(clean(load_f(e[j])), v * V + j);
+    for (int j = 0; j < V; j++) take(load_f(e[j]));
     reinterpret_cast<uint4*>(xs)[v] = r;
   }
   for (int i = nv * V + threadIdx.x; i < n; i += kThreads) {
     xs[i] = src[i];
-    take(clean(load_f(xs[i])), i);
+    take(load_f(xs[i]));
   }
+  // The largest of each group of four threads goes to every CTA.
+  top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+  top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const u64 b = __shfl_xor_sync(0xFFFFFFFFu, best, o);
-    best = b > best ? b : best;
-    least = fminf(least, __shfl_xor_sync(0xFFFFFFFFu, least, o));
-  }
-  if (lane == 0) {
-    sh->wred[warp] = best;
-    sh->wmin[warp] = __float_as_uint(least);
-  }
+  for (int o = 16; o; o >>= 1) least = fminf(least, __shfl_xor_sync(0xFFFFFFFFu, least, o));
+  if (lane == 0) sh->wleast[warp] = least;
+  if (threadIdx.x == 0) sh->few_count = 0;
   __syncthreads();
-  cluster.sync();  // every CTA of the cluster runs: its shared memory is there
+  cluster.barrier_wait();
+  for (int q = lane & 3; q < ranks; q += 4)
+    cluster.map_shared_rank(sh, q)->maxima[rank * kGroups + (threadIdx.x >> 2)] = top;
   if (threadIdx.x < ranks) {
-    for (int w = 0; w < kWarps; w++) {
-      best = sh->wred[w] > best ? sh->wred[w] : best;
-      least = fminf(least, __uint_as_float(sh->wmin[w]));
-    }
-    Shared* o = cluster.map_shared_rank(sh, threadIdx.x);
-    o->best[rank] = best;
-    o->least[rank] = least;
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) least = fminf(least, sh->wleast[w]);
+    cluster.map_shared_rank(sh, threadIdx.x)->least[rank] = least;
   }
-  const float T_ = a.temperature ? a.temperature[row] : 1.f;
+  float T_ = a.temperature ? a.temperature[row] : 1.f;
   const int k_ = a.top_k ? a.top_k[row] : 0;
   const float p_ = a.top_p ? a.top_p[row] : 1.f;
   const float m_ = a.min_p ? a.min_p[row] : 0.f;
   const float u_ = a.u[row];
   cluster.sync();
-  best = 0;
   least = INFINITY;
-  for (int r = 0; r < ranks; r++) {
-    best = sh->best[r] > best ? sh->best[r] : best;
-    least = fminf(least, sh->least[r]);
-  }
-  const bool empty = best == 0;
-  if (empty || !(T_ > 0.f) || k_ == 1 || p_ <= 0.f) {
+  for (int r = 0; r < ranks; r++) least = fminf(least, sh->least[r]);
+  // Each warp looks at all groups: the row's largest logit, and the first
+  // slice that has it.
+  top = -INFINITY;
+  for (int g = lane; g < ranks * kGroups; g += 32) top = fmaxf(top, sh->maxima[g]);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+  top += 0.f;                    // -0 is 0
+  if (top == -INFINITY) {        // nothing but -inf and NaN
     if (rank == 0 && threadIdx.x == 0) {
-      a.token[row] = empty ? -1 : 0x7FFFFFFF - (int)(unsigned)best;
-      if (a.prob) a.prob[row] = empty ? 0.f : 1.f;
-      if (a.kept) a.kept[row] = empty ? 0 : 1;
+      a.token[row] = -1;
+      if (a.prob) a.prob[row] = 0.f;
+      if (a.kept) a.kept[row] = 0;
+    }
+    return;
+  }
+  if (!(T_ > 0.f) || k_ == 1 || p_ <= 0.f) {
+    // The largest, at its lowest index.
+    int first = ranks;
+    for (int g = lane; g < ranks * kGroups; g += 32)
+      if (sh->maxima[g] == top) first = min(first, g / kGroups);
+    if (rank != __reduce_min_sync(0xFFFFFFFFu, first)) return;
+    if (threadIdx.x == 0) sh->found = INT_MAX;
+    __syncthreads();
+    int i = threadIdx.x;
+    while (i < n && load_f(xs[i]) != top) i += kThreads;
+    if (i < n) atomicMin(&sh->found, i);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      a.token[row] = start + sh->found;
+      if (a.prob) a.prob[row] = 1.f;
+      if (a.kept) a.kept[row] = 1;
     }
     return;
   }
 
   const int chunk = ((a.per + kThreads - 1) / kThreads) | 1;  // odd: no bank conflicts
-  Row<T> r{sh, xs, cluster, rank, ranks, start};
+  Row<T> r{sh, xs, cluster, rank, ranks, start, a.per};
   r.c0 = min((int)threadIdx.x * chunk, n);
   r.c1 = min(r.c0 + chunk, n);
-  r.M = of_key((unsigned)(best >> 32));
+  if (top == INFINITY) {
+    // Infinite logits share all of the mass: they become 0, the others the
+    // lowest value, at a temperature of 1.
+    T_ = 1.f;
+    for (int i = r.c0; i < r.c1; i++) {
+      const float x = load_f(xs[i]);
+      if (x > -INFINITY) store_f(xs[i], x == INFINITY ? 0.f : -FLT_MAX);
+    }
+    __syncthreads();
+    for (int g = threadIdx.x; g < ranks * kGroups; g += kThreads)
+      if (sh->maxima[g] > -INFINITY) sh->maxima[g] = sh->maxima[g] == INFINITY ? 0.f : -FLT_MAX;
+    __syncthreads();
+    top = 0.f;
+    least = -FLT_MAX;
+  }
+  r.M = top;
+  r.listed = false;
+  r.floor = -FLT_MAX;
   r.scale = 1.4426950408889634 / (double)T_;
   // The bins share what is within kReach octaves of the largest weight, or
-  // down to the smallest logit if that is nearer.
-  double range = fmin(kReach / r.scale, ((double)r.M - (double)least) * (1 + 1e-6));
-  if (!(range < 1e300)) range = 1;  // infinite logits at an infinite temperature
-  r.bins_per = (float)((kBins - 1) / range);
+  // down to the smallest logit if that is nearer. (Bins in 32 bits: all CTAs
+  // compute the same ones, and any monotone ones do.)
+  const float bits = (float)fmin(r.scale, 1e37);
+  const float range = fminf(kReach / bits, (r.M - least) * 1.00001f);
+  r.bins_per = fminf((kBins - 1) / range, 1e37f);
+  r.octaves = fminf(bits / r.bins_per, 2.0f * kReach / kBins);
+  r.last = fminf(1000.f / (bits / r.bins_per), 1e38f);
   const double min_w = m_ > 0.f ? fmin((double)m_, 1.0) : 0.0;
+  // A logit just below M + T ln(w).
+  auto logit_of = [&](double w) {
+    return __double2float_rd((double)r.M + log2(w) * (1 + 1e-12) / r.scale - 1e-12 * fabs(r.M));
+  };
 
-  typename Row<T>::Cut cut = {0u, INT_MAX, 0.0, false, 0u};
-  bool ready = false, cut_k = false;
+  typename Row<T>::Cut cut = {0u, INT_MAX, 0.0, false, false, 0u};
+  bool ready = false;
   if (k_ > 1 && k_ < a.vocab) {
-    cut = r.select(false, 0.0, (unsigned)k_, ready, 0);
-    cut_k = true;
-  }
-  if (p_ < 1.f) {
-    if (!cut_k) {
-      r.histogram();
-      ready = true;
-      cut.mass = r.mass();
+    // The k-th largest of the groups' largest logits is not above the k-th
+    // largest of all: find its bin.
+    sh->gcount[threadIdx.x] = 0;
+    sh->gmass[threadIdx.x] = 0;
+    __syncthreads();
+    for (int g = threadIdx.x; g < ranks * kGroups; g += kThreads) {
+      const float x = sh->maxima[g] + 0.f;
+      if (x > -INFINITY) atomicAdd(&sh->gcount[r.bin_of(x)], 1u);
     }
-    cut = r.select(true, (double)p_ * cut.mass, 0u, ready, 1);
+    __syncthreads();
+    float least_kept = -INFINITY;
+    if (k_ <= ranks * kGroups && r.find_bin(false, 0.0, (unsigned)k_)) {
+      // Everything down to that bin's end stays.
+      const int b = (int)sh->bbin;
+      if (b < kBins - 1)
+        least_kept = __double2float_rd((double)r.M - (b + 1.01) / (double)r.bins_per -
+                                       1e-6 * (fabs((double)r.M) + range));
+    }
+    const unsigned mine = r.bound(least_kept);
+    // How many of the row are left; this slice's go to CTA 0 if it has few.
+    Shared* o = cluster.map_shared_rank(sh, 0);
+    if (threadIdx.x < ranks) cluster.map_shared_rank(sh, threadIdx.x)->left[rank] = mine;
+    if (mine <= kThreads) {
+      if (threadIdx.x == 0) sh->fill = atomicAdd(&o->few_count, mine);
+      __syncthreads();
+      r.each([&](float x, int i) {
+        const unsigned at = atomicAdd(&sh->fill, 1u);
+        if (at < kThreads) o->few[at] = ((u64)key_of(x) << 32) | (unsigned)(INT_MAX - start - i);
+      });
+    }
+    cluster.sync();
+    unsigned all = 0;
+    for (int q = 0; q < ranks; q++) all += sh->left[q];
+    if (all <= kThreads) {
+      // Few: CTA 0 does the rest alone. Sorted, entry `tid` of the order is
+      // thread tid's.
+      if (rank > 0) return;
+      const int tid = threadIdx.x;
+      const bool real = tid < (int)all;
+      const u64 v = block_sort(real ? sh->few[tid] : 0, (int)all, sh->order);
+      double w = real ? r.weight(of_key((unsigned)(v >> 32))) : 0.0;
+      bool stays = real && tid < k_;
+      double mass;
+      const double upto_w = block_prefix(stays ? w : 0.0, sh->wsum, &mass);
+      if (p_ < 1.f) stays = stays && (tid == 0 || upto_w - w < (double)p_ * mass);
+      stays = stays && w >= min_w;
+      const int kept = __syncthreads_count(stays);
+      // What stays, by index.
+      double* weights = reinterpret_cast<double*>(sh->few);
+      weights[tid] = w;
+      const u64 byi =
+          block_sort(stays ? (u64)(unsigned)v << 32 | (unsigned)tid : 0, (int)all, sh->order);
+      __syncthreads();
+      w = tid < kept ? weights[(unsigned)byi] : 0.0;
+      double total;
+      const double run = block_prefix(w, sh->wsum, &total);
+      const double target = u_ > 0.f ? (double)u_ * total : 0.0;
+      if (tid == 0) {
+        sh->found = kThreads;
+        sh->fill = 0;
+      }
+      __syncthreads();
+      if (w > 0) {
+        if (run > target) atomicMin(&sh->found, tid);
+        atomicMax(&sh->fill, tid);
+      }
+      __syncthreads();
+      if (tid == min(sh->found, (int)sh->fill)) {
+        a.token[row] = INT_MAX - (int)(unsigned)(byi >> 32);
+        if (a.prob) a.prob[row] = (float)(w / total);
+        if (a.kept) a.kept[row] = kept;
+      }
+      return;
+    }
+    r.histogram();
+    ready = true;
+    cut = r.select(false, 0.0, (unsigned)k_, ready, 0);
+    if (p_ < 1.f) {
+      if (!ready) r.histogram();
+      cut = r.select(true, (double)p_ * cut.mass, 0u, ready, 1);
+    }
+  } else if (p_ < 1.f) {
+    r.histogram_of_all();
+    cut = r.select(true, (double)p_ * r.mass(), 0u, ready, 1);
+  } else {
+    r.bound(min_w > 0 ? logit_of(min_w * 0.999) : -INFINITY);
   }
+  // min-p counts where it drops the last entry that is kept so far.
+  if (min_w > 0 && cut.sums) cut.sums = r.weight(of_key(cut.key)) >= min_w;
 
   // What is kept, in index order.
   auto kept_weight = [&](float x, int i, bool& kept) -> double {
@@ -634,28 +944,36 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleArgs a) {
     kept = w >= min_w;
     return kept ? w : 0.0;
   };
-  double mine = 0;
-  int number = 0;
-  for (int i = r.c0; i < r.c1; i++) {
-    bool kept;
-    mine += kept_weight(r.at(i), start + i, kept);
-    number += kept;
+  double mine = 0, upto = 0;
+  auto add_up = [&](u64* numbers) {
+    int number = 0;
+    r.each([&](float x, int i) {
+      bool kept;
+      mine += kept_weight(x, start + i, kept);
+      number += kept;
+    });
+    double total;
+    upto = block_prefix(mine, sh->wsum, &total);
+    if (numbers) block_prefix((u64)number, sh->wred, numbers);
+    return total;
+  };
+  const bool known = cut.sums;  // what each slice keeps
+  if (!known) {
+    u64 numbers;
+    const double total = add_up(&numbers);
+    if (threadIdx.x < ranks) {
+      Shared* o = cluster.map_shared_rank(sh, threadIdx.x);
+      o->mass[rank] = total;
+      o->total[rank] = (unsigned)numbers;
+    }
+    cluster.sync();
   }
-  double total;
-  u64 numbers;
-  const double upto = block_prefix(mine, sh->wsum, &total);
-  block_prefix((u64)number, sh->wred, &numbers);
-  if (threadIdx.x < ranks) {
-    Shared* o = cluster.map_shared_rank(sh, threadIdx.x);
-    o->mass[rank] = total;
-    o->total[rank] = (unsigned)numbers;
-  }
-  cluster.sync();
-  total = 0;
+  const double* slices = known ? sh->before_mass : sh->mass;
+  double total = 0;
   unsigned kept = 0;
   for (int q = 0; q < ranks; q++) {
-    total += sh->mass[q];
-    kept += sh->total[q];
+    total += slices[q];
+    kept += known ? sh->before_count[q] : sh->total[q];
   }
   // The slice in which the running mass exceeds u total; the last with any
   // if none (u at or above 1).
@@ -663,7 +981,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleArgs a) {
   double run = 0, before = 0;
   int owner = -1;
   for (int q = 0; q < ranks; q++) {
-    const double v = sh->mass[q];
+    const double v = slices[q];
     if (v > 0 && (owner < 0 || !(run > target))) {
       owner = q;
       before = run;
@@ -671,6 +989,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleArgs a) {
     run += v;
   }
   if (rank != owner) return;
+  if (known) add_up(nullptr);
   const int token = r.find_index(
       [&](float x, int i) {
         bool in;
