@@ -19,7 +19,7 @@
 //
 // What bounds it: the cache's bytes while there are few rows, the tensor
 // cores' mma.sync rate from about 32 rows (fp32) or 64 (bf16) a kv head.
-#include "entry.h"
+#include "attn_tree.h"
 
 #include <math.h>
 
@@ -36,19 +36,7 @@ typedef unsigned long long u64;
 constexpr int kStages = 3;       // key/value tiles in flight
 constexpr int kMaxSplits = 256;
 
-struct TreeArgs {
-  const void* q;
-  const void* k;
-  const void* v;
-  void* att;
-  long long ldq, ldo;
-  int t, kh, group, ctx, words;
-  const int* cached;
-  const u64* mask;
-  int splits, min_tiles;
-  float* part;     // [splits][kh][t * group][HD] outputs before division
-  float2* ml;      // [splits][kh][t * group] running maximum (base 2) and sum
-};
+using sg::TreeArgs;
 
 __device__ __forceinline__ uint32_t saddr(const void* p) {
   return (uint32_t)__cvta_generic_to_shared(p);
@@ -151,10 +139,10 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Tree
 
   // The cache's length is read on the device (a captured call serves every
   // later length); one outside the cache is cut to it.
-  const int n = min(max(*a.cached, 0), a.ctx - a.t);
+  const int n = sg::tree_cached(a);
   const int old_tiles = (n + kKeys - 1) / kKeys;
   const int tiles = old_tiles + (a.t + kKeys - 1) / kKeys;
-  const int per = max((tiles + a.splits - 1) / a.splits, a.min_tiles);
+  const int per = (tiles + a.splits - 1) / a.splits;
   const int tile0 = split * per, tile1 = min(tiles, tile0 + per);
   if (tile0 >= tile1) return;
 
@@ -564,57 +552,138 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Tree
   }
 }
 
-// One warp joins the parts of one row: their common maximum, then the sum of
-// outputs and of sums, each scaled to it.
-template <typename T, int HD>
+// One warp joins the parts of one row: outputs and sums of all parts, each
+// scaled to their common maximum. Four groups of eight lanes take the parts
+// in turn, a lane having HD / 8 entries of the head.
+//
+// DRAFTED: the parts have the cached keys only. The drafted ones that the row
+// sees, its ancestors in the tree and itself, come first, a group per key
+// with a running softmax of its own: a few keys as a rule, for which a matrix
+// tile would be nearly empty, and rows it does not see are not even read.
+template <typename T, int HD, bool DRAFTED>
 __global__ void __launch_bounds__(128) k_merge(TreeArgs a, int keys_per_tile) {
-  constexpr int V = HD / 32;  // entries per lane
-  const int lane = threadIdx.x & 31;
+  constexpr int V = HD / 8;  // entries per lane
+  constexpr bool kF32 = sizeof(T) == 4;
+  const int lane = threadIdx.x & 31, group = lane >> 3, e0 = (lane & 7) * V;
   const int R = a.t * a.group, row = blockIdx.x * 4 + (threadIdx.x >> 5);
   sg::pdl_trigger();
   sg::pdl_wait();
   if (row >= R * a.kh) return;
-  const int n = min(max(*a.cached, 0), a.ctx - a.t);
+  const int n = sg::tree_cached(a);
   const int tiles = (n + keys_per_tile - 1) / keys_per_tile +
-                    (a.t + keys_per_tile - 1) / keys_per_tile;
-  const int per = max((tiles + a.splits - 1) / a.splits, a.min_tiles);
-  const int parts = (tiles + per - 1) / per;
-  const size_t step = (size_t)a.kh * R;
-  float m = -INFINITY;
-  for (int s = lane; s < parts; s += 32) m = fmaxf(m, a.ml[s * step + row].x);
-  m = sg::warp_max(m);
-  if (m == -INFINITY) m = 0.f;  // no key in any part: all weights are 0
-  float l = 0.f, acc[V];
+                    (DRAFTED ? 0 : (a.t + keys_per_tile - 1) / keys_per_tile);
+  const int per = (tiles + a.splits - 1) / a.splits;
+  const int parts = tiles ? (tiles + per - 1) / per : 0;
+  const int head = row / R, r = row - head * R, tok = r / a.group;
+  const size_t at = (size_t)(head * a.group + r - tok * a.group) * HD + e0;
+  auto read = [&](const T* p, float* x) {
+    if constexpr (kF32) {
 #pragma unroll
-  for (int e = 0; e < V; e++) acc[e] = 0.f;
-  for (int s0 = 0; s0 < parts; s0 += 32) {
-    float f = 0.f;
-    if (s0 + lane < parts) {
-      const float2 p = a.ml[(s0 + lane) * step + row];
-      f = exp2f(p.x - m);
-      l += p.y * f;
+      for (int i = 0; i < V; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(p + i);
+        x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; i += 4) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p + i);
+        x[i] = sg::bf16_lo(v.x); x[i + 1] = sg::bf16_hi(v.x);
+        x[i + 2] = sg::bf16_lo(v.y); x[i + 3] = sg::bf16_hi(v.y);
+      }
     }
-    const int count = min(32, parts - s0);
-#pragma unroll 8
-    for (int s = 0; s < count; s++) {
-      const float w = __shfl_sync(0xFFFFFFFFu, f, s);
-      const float* p = a.part + ((s0 + s) * step + row) * HD + lane * V;
+  };
+  float m = -INFINITY, l = 0.f, o[V];
 #pragma unroll
-      for (int e = 0; e < V; e++) acc[e] += p[e] * w;
+  for (int i = 0; i < V; i++) o[i] = 0.f;
+  if constexpr (DRAFTED) {
+    const float scale = 1.4426950408889634f / sqrtf((float)HD);
+    float q[V];
+    read(static_cast<const T*>(a.q) + tok * a.ldq + at, q);
+#pragma unroll
+    for (int i = 0; i < V; i++) q[i] *= scale;
+    const size_t base = ((size_t)head * a.ctx + n) * HD + e0;
+    const T* k = static_cast<const T*>(a.k) + base;
+    const T* v = static_cast<const T*>(a.v) + base;
+    for (int w = 0; w < a.words; w++) {
+      u64 bits = a.mask[(size_t)tok * a.words + w];
+      if (a.t - 64 * w < 64) bits &= (1ull << (a.t - 64 * w)) - 1;
+      while (bits) {
+        // The next four keys, one per group (fewer at the end).
+        int j = -1;
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          const int next = bits ? __ffsll((long long)bits) - 1 : -1;
+          bits &= bits - 1;
+          if (g == group) j = next;
+        }
+        float x[V], s = 0.f;
+        if (j >= 0) {
+          read(k + (size_t)(64 * w + j) * HD, x);
+#pragma unroll
+          for (int i = 0; i < V; i++) s = fmaf(q[i], x[i], s);
+          read(v + (size_t)(64 * w + j) * HD, x);
+        }
+        s += __shfl_xor_sync(0xFFFFFFFFu, s, 1);
+        s += __shfl_xor_sync(0xFFFFFFFFu, s, 2);
+        s += __shfl_xor_sync(0xFFFFFFFFu, s, 4);
+        if (j >= 0) {
+          const float next = fmaxf(m, s);
+          const float f = next == -INFINITY ? 1.f : exp2f(m - next);
+          const float p = exp2f(s - (next == -INFINITY ? 0.f : next));
+          m = next;
+          l = l * f + p;
+#pragma unroll
+          for (int i = 0; i < V; i++) o[i] = fmaf(p, x[i], o[i] * f);
+        }
+      }
     }
   }
-  l = sg::warp_sum(l);
-  const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  const int head = row / R, r = row - head * R, tok = r / a.group;
-  T* out = static_cast<T*>(a.att) + tok * a.ldo +
-           (size_t)(head * a.group + r - tok * a.group) * HD + lane * V;
+  const size_t step = (size_t)a.kh * R;
+  float top = m;
+  for (int s = lane; s < parts; s += 32) top = fmaxf(top, a.ml[s * step + row].x);
+  top = sg::warp_max(top);
+  if (top == -INFINITY) top = 0.f;  // no key at all: all weights are 0
+  {
+    const float f = exp2f(m - top);
+    l *= f;
 #pragma unroll
-  for (int e = 0; e < V; e++) {
-    const float x = acc[e] * f;
-    if constexpr (sizeof(T) == 4)
-      out[e] = x;
-    else
-      asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(out[e]) : "f"(x));
+    for (int i = 0; i < V; i++) o[i] *= f;
+  }
+#pragma unroll 4
+  for (int s = group; s < parts; s += 4) {
+    const float2 p = a.ml[s * step + row];
+    const float f = exp2f(p.x - top);
+    l += p.y * f;
+    const float* x = a.part + (s * step + row) * HD + e0;
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const float4 y = *reinterpret_cast<const float4*>(x + i);
+      o[i] = fmaf(y.x, f, o[i]);
+      o[i + 1] = fmaf(y.y, f, o[i + 1]);
+      o[i + 2] = fmaf(y.z, f, o[i + 2]);
+      o[i + 3] = fmaf(y.w, f, o[i + 3]);
+    }
+  }
+#pragma unroll
+  for (int d = 8; d < 32; d *= 2) {
+    l += __shfl_xor_sync(0xFFFFFFFFu, l, d);
+#pragma unroll
+    for (int i = 0; i < V; i++) o[i] += __shfl_xor_sync(0xFFFFFFFFu, o[i], d);
+  }
+  if (group > 0) return;
+  const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  T* out = static_cast<T*>(a.att) + tok * a.ldo + at;
+#pragma unroll
+  for (int i = 0; i < V; i += 4) {
+    if constexpr (kF32) {
+      *reinterpret_cast<float4*>(out + i) =
+          make_float4(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f);
+    } else {
+      uint2 w;
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w.x) : "f"(o[i + 1] * f), "f"(o[i] * f));
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w.y) : "f"(o[i + 3] * f), "f"(o[i + 2] * f));
+      *reinterpret_cast<uint2*>(out + i) = w;
+    }
   }
 }
 
@@ -629,17 +698,26 @@ Shape shape_of(int rows) {
   return {8, 1};
 }
 
+// Whether the cached keys go to tcgen05 (attn_tree_tc.cu): from 33 rows a kv
+// head on, where mma.sync is what bounds this file's kernel. Not for many
+// drafted tokens, whose own keys the merge reads one by one, and not for
+// head_dim 32.
+bool on_tc(int t, int group, int hd) { return t * group > 32 && t <= 256 && hd >= 64; }
+
 // Splits of the keys: as many CTAs as the GPU holds at once.
-int splits_of(int sms, int t, int kh, int group) {
+int splits_of(int sms, int t, int kh, int group, int hd) {
   const int rows = t * group;
   const Shape s = shape_of(rows);
-  const int resident = sms * (s.mw * s.kw <= 4 ? 2 : 1);
-  const long long others = (long long)kh * ((rows + 16 * s.mw - 1) / (16 * s.mw));
+  const bool tc = on_tc(t, group, hd);
+  const int resident = sms * (!tc && s.mw * s.kw <= 4 ? 2 : 1);
+  const int tile = tc ? sg::kTreeTcRows : 16 * s.mw;
+  const long long others = (long long)kh * ((rows + tile - 1) / tile);
   return (int)std::max(1ll, std::min((long long)kMaxSplits, resident / others));
 }
 
 size_t workspace_of(int splits, int t, int kh, int group, int hd) {
-  return splits == 1 ? 0 : (size_t)splits * kh * t * group * (hd + 2) * sizeof(float);
+  if (splits == 1 && !on_tc(t, group, hd)) return 0;
+  return (size_t)splits * kh * t * group * (hd + 2) * sizeof(float);
 }
 
 template <typename T, int HD, int MW, int KW>
@@ -653,12 +731,21 @@ cudaError_t launch_shape(const TreeArgs& a, int dev, cudaStream_t s) {
                      dim3(a.splits, a.kh, (rows + 16 * MW - 1) / (16 * MW)),
                      dim3(32 * MW * KW), bytes, 1, s, a);
   if (e != cudaSuccess || a.splits == 1) return e;
-  return sg::try_launch(k_merge<T, HD>, dim3((rows * a.kh + 3) / 4), dim3(128), 0, 1, s, a,
+  return sg::try_launch(k_merge<T, HD, false>, dim3((rows * a.kh + 3) / 4), dim3(128), 0, 1, s, a,
                         Tile<T, HD>::kKeys);
 }
 
 template <typename T, int HD>
 cudaError_t launch_hd(const TreeArgs& a, int dev, cudaStream_t s) {
+  if (on_tc(a.t, a.group, HD)) {
+    if constexpr (HD >= 64) {
+      constexpr bool kF32 = sizeof(T) == 4;
+      const cudaError_t e = sg::tree_tc(a, kF32, HD, dev, s);
+      if (e != cudaSuccess) return e;
+      return sg::try_launch(k_merge<T, HD, true>, dim3((a.t * a.group * a.kh + 3) / 4), dim3(128),
+                            0, 1, s, a, sg::tree_tc_keys(kF32));
+    }
+  }
   const Shape f = shape_of(a.t * a.group);
   if (f.mw == 1) return launch_shape<T, HD, 1, 4>(a, dev, s);
   if (f.mw == 2) return launch_shape<T, HD, 2, 2>(a, dev, s);
@@ -696,7 +783,9 @@ size_t strasgpt_k_attn_tree_workspace(int t, int kv_heads, int group, int head_d
     sg::refuse(me, why);
     return 0;
   }
-  return workspace_of(t ? splits_of(sms, t, kv_heads, group) : 1, t, kv_heads, group, head_dim);
+  return t ? workspace_of(splits_of(sms, t, kv_heads, group, head_dim), t, kv_heads, group,
+                          head_dim)
+           : 0;
 }
 
 int strasgpt_k_attn_tree(const void* q, long long ldq, const void* k_cache, const void* v_cache,
@@ -723,7 +812,7 @@ int strasgpt_k_attn_tree(const void* q, long long ldq, const void* k_cache, cons
   for (const void* p : {q, k_cache, v_cache, (const void*)cached, (const void*)mask,
                         (const void*)att})
     if (const char* why = sg::not_on_device(p, dev)) return sg::refuse(me, why);
-  const int splits = splits_of(sms, t, kv_heads, group);
+  const int splits = splits_of(sms, t, kv_heads, group, head_dim);
   const size_t need = workspace_of(splits, t, kv_heads, group, head_dim);
   if (need) {
     if (!workspace || workspace_bytes < need)
@@ -737,7 +826,6 @@ int strasgpt_k_attn_tree(const void* q, long long ldq, const void* k_cache, cons
   a.t = t; a.kh = kv_heads; a.group = group; a.ctx = ctx; a.words = (t + 63) / 64;
   a.cached = cached; a.mask = (const u64*)mask;
   a.splits = splits;
-  a.min_tiles = 1;
   a.part = (float*)workspace;
   a.ml = (float2*)(a.part + (size_t)splits * kv_heads * t * group * head_dim);
   const cudaStream_t s = (cudaStream_t)stream;

@@ -1,0 +1,35 @@
+// What the two kernels behind strasgpt_k_attn_tree share: attn_tree.cu (the
+// entry point, few rows per kv head) and attn_tree_tc.cu (many).
+#pragma once
+
+#include "entry.h"
+
+namespace sg {
+
+struct TreeArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* att;
+  long long ldq, ldo;
+  int t, kh, group, ctx, words;
+  const int* cached;
+  const unsigned long long* mask;
+  int splits;
+  float* part;     // [splits][kh][t * group][HD] outputs before division
+  float2* ml;      // [splits][kh][t * group] running maximum (base 2) and sum
+};
+
+// Cached keys, cut to what the cache holds.
+__device__ __forceinline__ int tree_cached(const TreeArgs& a) {
+  return min(max(*a.cached, 0), a.ctx - a.t);
+}
+
+// The cached keys [0, *cached) on the fifth-generation tensor cores, 128 rows
+// per CTA; the drafted ones are k_merge's. head_dim 64 or 128.
+constexpr int kTreeTcRows = 128;
+cudaError_t tree_tc(const TreeArgs& a, bool f32, int head_dim, int dev, cudaStream_t s);
+// Keys per tile: what a split's share is a multiple of.
+int tree_tc_keys(bool f32);
+
+}  // namespace sg
