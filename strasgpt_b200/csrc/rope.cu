@@ -9,11 +9,17 @@
 // at most half a turn, becomes an fp32 sine and cosine.
 //
 // What bounds it: bytes (each entry read and written once) for a chunk, one
-// launch for a token. A block computes the sines of its tokens once, in
-// shared memory, for all of its heads: their 64-bit part costs one multiply
-// per pair and token instead of one per entry.
+// launch for a token. A block has a run of items (two a thread), loads them
+// first, and computes the sines of their tokens, once for all heads, in
+// shared memory while they are on their way: the sines' 64-bit part costs a
+// multiply per pair and token instead of one per entry. Measured on a B200:
+// 1.8 us for one token of 40 heads of 128 fp32 entries, 4.5 us (3.7 TB/s) for
+// 2048 tokens of 8 such heads into a cache, 44 us (3.8 TB/s; a plain copy of
+// as many contiguous bytes takes 33) for 8191 tokens of 40 heads of 128 bf16
+// entries, half of each turned, out of rows twice as wide.
 #include "entry.h"
 
+#include <limits.h>
 #include <math.h>
 
 extern "C" {
@@ -24,7 +30,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxPairs = 256;    // dim <= 512
-constexpr int kUnroll = 4;        // items in flight per thread
+constexpr int kUnroll = 2;        // items in flight per thread
 constexpr int kSinesMax = 2048;   // (token, pair) sines of a block: 16 KB
 
 struct RopeArgs {
@@ -33,7 +39,7 @@ struct RopeArgs {
   long long xt, xh, yt, yh;  // token and head strides, in entries
   const int* pos;
   int t, heads, hd, dim;
-  int tokens, heads_per_block;
+  int per_block;             // items of a block
   float magnitude;
   double turns[kMaxPairs];   // f_j / 2 pi
 };
@@ -52,96 +58,93 @@ __device__ __forceinline__ void from_f(float v, uint16_t& o) {
   asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(o) : "f"(v));
 }
 
-// An item is V pairs of one head (two accesses of V entries), or V entries
-// behind the turned ones, which are copied.
-template <typename T, int V, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads) k_rope(const __grid_constant__ RopeArgs a) {
+// How the pairs of a head are read.
+enum Layout {
+  kHalves,    // (j, j + dim / 2): V pairs are two accesses of V entries
+  kAdjacent,  // (2j, 2j + 1): V / 2 pairs are one access (V >= 2)
+  kSingle     // (2j, 2j + 1), entry by entry (V == 1)
+};
+
+// Blocks per SM that the registers are held to: two accesses an item need 64
+// a thread (4 blocks; at 6 they spill, 22 us for 17 us on 4096 x 32 x 128 bf16
+// entries), one gets by with 40 (6; 44 us for 55 us on 8191 x 40 x 128).
+constexpr int blocks_of(Layout l) { return l == kHalves ? 4 : 6; }
+
+// An item is the pairs of one access, or V entries behind the turned ones,
+// which are copied.
+template <typename T, int V, Layout LAYOUT>
+__global__ void __launch_bounds__(kThreads, blocks_of(LAYOUT)) k_rope(const __grid_constant__ RopeArgs a) {
+  constexpr int kPairs = LAYOUT == kAdjacent ? V / 2 : V;  // of an item
+  constexpr bool kTwo = LAYOUT != kAdjacent;               // two accesses
   __shared__ float2 cs[kSinesMax];
+  const int half = a.dim / 2, next = LAYOUT == kSingle ? 1 : half;
+  // Items in the order token, head, place: a block has a run of them, of
+  // tokens t0 to t0 + nt - 1, and starts at place `skip` of the first.
+  const int turned = half / kPairs, per_head = turned + (a.hd - a.dim) / V;
+  const int per_token = a.heads * per_head;
+  const long long first = (long long)blockIdx.x * a.per_block, all = (long long)a.t * per_token;
+  const int t0 = (int)(first / per_token), skip = (int)(first - (long long)t0 * per_token);
+  const int items = (int)min((long long)a.per_block, all - first);
+  const int nt = (skip + items - 1) / per_token + 1;
+  const T* x = static_cast<const T*>(a.x);
+  T* y = static_cast<T*>(a.y);
+  using Access = Vec<T, V>;
+  Access p[kUnroll], q[kTwo ? kUnroll : 1];
+  long long to[kUnroll];
+  int pair[kUnroll];  // where the item's sines are, or -1: copied
   sg::pdl_trigger();
   sg::pdl_wait();
-  const int half = a.dim / 2;
-  const int t0 = blockIdx.x * a.tokens, nt = min(a.tokens, a.t - t0);
-  const int h0 = blockIdx.y * a.heads_per_block, nh = min(a.heads_per_block, a.heads - h0);
+  // The entries are on their way while the sines are computed.
+#pragma unroll
+  for (int u = 0; u < kUnroll; u++) {
+    const int i = threadIdx.x + u * kThreads;
+    if (i >= items) break;
+    const int token = (skip + i) / per_token, place = skip + i - token * per_token;
+    const int h = place / per_head, v = place - h * per_head;
+    const bool turn = v < turned;
+    const int at = !turn ? a.dim + (v - turned) * V : LAYOUT == kSingle ? 2 * v : v * V;
+    const T* from = x + (t0 + token) * a.xt + h * a.xh + at;
+    p[u] = *reinterpret_cast<const Access*>(from);
+    if (kTwo && turn) q[kTwo ? u : 0] = *reinterpret_cast<const Access*>(from + next);
+    to[u] = (t0 + token) * a.yt + h * a.yh + at;
+    pair[u] = turn ? token * half + v : -1;
+  }
   for (int i = threadIdx.x; i < nt * half; i += kThreads) {
     const int token = i / half, j = i - token * half;
     const double turns = (double)a.pos[t0 + token] * a.turns[j];
     float s, c;
     sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-    cs[i] = make_float2(c * a.magnitude, s * a.magnitude);
+    // Pair kPairs v + e of a token lies at e turned + v: the sines of an item
+    // are read by neighbouring threads side by side.
+    cs[token * half + j % kPairs * turned + j / kPairs] =
+        make_float2(c * a.magnitude, s * a.magnitude);
   }
   __syncthreads();
 
-  const int turned = half / V, per_head = turned + (a.hd - a.dim) / V;
-  const int items = nt * nh * per_head;
-  const T* x = static_cast<const T*>(a.x);
-  T* y = static_cast<T*>(a.y);
-  using Access = Vec<T, V>;
-  for (int i0 = threadIdx.x; i0 < items; i0 += kThreads * kUnroll) {
-    Access p[kUnroll], q[kUnroll];
-    long long to[kUnroll];
-    int pair[kUnroll];  // index of the first pair's sine, or -1: copied
 #pragma unroll
-    for (int u = 0; u < kUnroll; u++) {
-      const int i = i0 + u * kThreads;
-      if (i >= items) break;
-      const int row = i / per_head, v = i - row * per_head;
-      const int token = row / nh, h = h0 + row - token * nh;
-      const long long from = (t0 + token) * a.xt + h * a.xh;
-      to[u] = (t0 + token) * a.yt + h * a.yh;
-      if (v < turned) {
-        const int at = INTERLEAVED ? 2 * v * V : v * V;
-        const int next = INTERLEAVED ? V : half;
-        p[u] = *reinterpret_cast<const Access*>(x + from + at);
-        q[u] = *reinterpret_cast<const Access*>(x + from + at + next);
-        to[u] += at;
-        pair[u] = token * half + v * V;
-      } else {
-        const int at = a.dim + (v - turned) * V;
-        p[u] = *reinterpret_cast<const Access*>(x + from + at);
-        to[u] += at;
-        pair[u] = -1;
+  for (int u = 0; u < kUnroll; u++) {
+    if (threadIdx.x + u * kThreads >= items) break;
+    if (pair[u] >= 0) {
+#pragma unroll
+      for (int e = 0; e < kPairs; e++) {
+        const float2 k = cs[pair[u] + e * turned];
+        T& one = kTwo ? p[u].e[e] : p[u].e[2 * e % V];
+        T& two = kTwo ? q[kTwo ? u : 0].e[e] : p[u].e[(2 * e + 1) % V];
+        const float f = to_f(one), g = to_f(two);
+        from_f(f * k.x - g * k.y, one);
+        from_f(f * k.y + g * k.x, two);
       }
+      if (kTwo) *reinterpret_cast<Access*>(y + to[u] + next) = q[kTwo ? u : 0];
     }
-#pragma unroll
-    for (int u = 0; u < kUnroll; u++) {
-      if (i0 + u * kThreads >= items) break;
-      if (pair[u] < 0) {
-        *reinterpret_cast<Access*>(y + to[u]) = p[u];
-        continue;
-      }
-      Access r, s;
-#pragma unroll
-      for (int e = 0; e < V; e++) {
-        const float2 k = cs[pair[u] + e];
-        // Adjacent layout: the two accesses hold entries 0..V-1 and V..2V-1
-        // of the run, and pair e is its entries 2e and 2e + 1.
-        float f, g;
-        if (INTERLEAVED) {
-          f = to_f(2 * e < V ? p[u].e[2 * e % V] : q[u].e[2 * e % V]);
-          g = to_f(2 * e + 1 < V ? p[u].e[(2 * e + 1) % V] : q[u].e[(2 * e + 1) % V]);
-        } else {
-          f = to_f(p[u].e[e]);
-          g = to_f(q[u].e[e]);
-        }
-        const float n = f * k.x - g * k.y, m = f * k.y + g * k.x;
-        if (INTERLEAVED) {
-          from_f(n, 2 * e < V ? r.e[2 * e % V] : s.e[2 * e % V]);
-          from_f(m, 2 * e + 1 < V ? r.e[(2 * e + 1) % V] : s.e[(2 * e + 1) % V]);
-        } else {
-          from_f(n, r.e[e]);
-          from_f(m, s.e[e]);
-        }
-      }
-      *reinterpret_cast<Access*>(y + to[u]) = r;
-      *reinterpret_cast<Access*>(y + to[u] + (INTERLEAVED ? V : half)) = s;
-    }
+    *reinterpret_cast<Access*>(y + to[u]) = p[u];
   }
 }
 
 template <typename T, int V>
 cudaError_t launch(const RopeArgs& a, bool interleaved, dim3 grid, cudaStream_t s) {
-  return interleaved ? sg::try_launch(k_rope<T, V, true>, grid, kThreads, 0, 1, s, a)
-                     : sg::try_launch(k_rope<T, V, false>, grid, kThreads, 0, 1, s, a);
+  constexpr Layout kPaired = V > 1 ? kAdjacent : kSingle;
+  return interleaved ? sg::try_launch(k_rope<T, V, kPaired>, grid, kThreads, 0, 1, s, a)
+                     : sg::try_launch(k_rope<T, V, kHalves>, grid, kThreads, 0, 1, s, a);
 }
 
 // Whether rows of `hd` entries at i st + j sh (i < t, j < heads) share no
@@ -217,33 +220,37 @@ extern "C" int strasgpt_k_rope(const void* x, long long x_token_stride, long lon
     a.turns[j] = g / two_pi;
   }
 
-  // 16-byte accesses where every run of V entries starts on 16 bytes, single
-  // entries otherwise.
-  const int wide = (int)(16 / size);
-  const bool vec = half % wide == 0 && (head_dim - rope->dim) % wide == 0 &&
-                   a.xt % wide == 0 && a.xh % wide == 0 && a.yt % wide == 0 &&
-                   a.yh % wide == 0 && sg::aligned(x, 16) && sg::aligned(y, 16);
-  const int v = vec ? wide : 1;
-  const int per_head = half / v + (head_dim - rope->dim) / v;
-  // Blocks of one item per thread while they all fit on the GPU at once
-  // (8 blocks per SM), of kUnroll items per thread after that.
-  const long long all = (long long)t * heads * per_head;
-  const int target = all <= (long long)sms * 8 * kThreads ? kThreads : kThreads * kUnroll;
-  a.heads_per_block = (target + per_head - 1) / per_head;
-  if (a.heads_per_block > heads) a.heads_per_block = heads;
-  a.tokens = target / (a.heads_per_block * per_head);
-  if (a.tokens > kSinesMax / half) a.tokens = kSinesMax / half;
-  if (a.tokens > t) a.tokens = t;
-  if (a.tokens < 1) a.tokens = 1;
-  const dim3 grid((t + a.tokens - 1) / a.tokens,
-                  (heads + a.heads_per_block - 1) / a.heads_per_block);
+  // 16-byte accesses where every run of their entries starts on 16 bytes; for
+  // adjacent pairs, else, an access per pair where pairs start on their size;
+  // single entries otherwise.
   const bool il = rope->interleaved != 0;
+  auto fits = [&](int v, int unit) {
+    return unit % v == 0 && (head_dim - rope->dim) % v == 0 && a.xt % v == 0 && a.xh % v == 0 &&
+           a.yt % v == 0 && a.yh % v == 0 && sg::aligned(x, v * size) && sg::aligned(y, v * size);
+  };
+  const int wide = (int)(16 / size), unit = il ? rope->dim : half;
+  const int v = fits(wide, unit) ? wide : il && fits(2, unit) ? 2 : 1;
+  const int per_head = (il && v > 1 ? rope->dim : half) / v + (head_dim - rope->dim) / v;
+  // Blocks of one item per thread while they all fit on the GPU at once
+  // (8 blocks per SM), of kUnroll after that; no more tokens than have room
+  // for their sines (a block's run may start and end within a token).
+  const long long per_token = (long long)heads * per_head, all = t * per_token;
+  long long per_block = all <= (long long)sms * 8 * kThreads ? kThreads : kThreads * kUnroll;
+  const long long room = (kSinesMax / half - 2) * per_token;
+  a.per_block = (int)(room < per_block ? room : per_block);
+  const long long blocks = (all + a.per_block - 1) / a.per_block;
+  if (per_token > INT_MAX / 2 || blocks > INT_MAX) return sg::refuse(me, "too many entries");
+  const dim3 grid((unsigned)blocks);
   const cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e;
   if (type == STRASGPT_F32)
-    e = vec ? launch<float, 4>(a, il, grid, s) : launch<float, 1>(a, il, grid, s);
+    e = v == 4   ? launch<float, 4>(a, il, grid, s)
+        : v == 2 ? launch<float, 2>(a, true, grid, s)
+                 : launch<float, 1>(a, il, grid, s);
   else
-    e = vec ? launch<uint16_t, 8>(a, il, grid, s) : launch<uint16_t, 1>(a, il, grid, s);
+    e = v == 8   ? launch<uint16_t, 8>(a, il, grid, s)
+        : v == 2 ? launch<uint16_t, 2>(a, true, grid, s)
+                 : launch<uint16_t, 1>(a, il, grid, s);
   if (e != cudaSuccess) return sg::refuse_cuda(me, "launch", e);
   return 0;
 }
