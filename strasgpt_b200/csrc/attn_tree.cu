@@ -743,7 +743,7 @@ cudaError_t launch_hd(const TreeArgs& a, int dev, cudaStream_t s) {
       const cudaError_t e = sg::tree_tc(a, kF32, HD, dev, s);
       if (e != cudaSuccess) return e;
       return sg::try_launch(k_merge<T, HD, true>, dim3((a.t * a.group * a.kh + 3) / 4), dim3(128),
-                            0, 1, s, a, sg::tree_tc_keys(kF32));
+                            0, 1, s, a, sg::tree_tc_keys());
     }
   }
   const Shape f = shape_of(a.t * a.group);

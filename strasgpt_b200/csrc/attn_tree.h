@@ -30,6 +30,6 @@ __device__ __forceinline__ int tree_cached(const TreeArgs& a) {
 constexpr int kTreeTcRows = 128;
 cudaError_t tree_tc(const TreeArgs& a, bool f32, int head_dim, int dev, cudaStream_t s);
 // Keys per tile: what a split's share is a multiple of.
-int tree_tc_keys(bool f32);
+int tree_tc_keys();
 
 }  // namespace sg

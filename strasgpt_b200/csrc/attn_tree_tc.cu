@@ -1,27 +1,29 @@
 // strasgpt_k_attn_tree, cached keys, for many rows per kv head: tcgen05.
 //
 // A CTA has 128 rows (drafted token, q head) of one kv head and a share of
-// the cached keys, which all of its rows see. Twelve warps: two warpgroups of
-// softmax, one thread per row, that take the key tiles in turn; one thread
-// that issues the matrix instructions; three warps that bring in keys and
-// values. Per tile: S = Q K^T into tensor memory; its warpgroup reads S,
-// subtracts the running maximum and writes P = 2^(S - m) over it, as bf16
-// parts; O = P V (P read from tensor memory) into tensor memory; the
-// warpgroup adds O, scaled, to its registers. Each warpgroup has its own
-// maximum, sum and output, joined at the end, so that one's softmax runs
-// under the other's matrix instructions and nothing is rescaled in place.
+// the cached keys, which all of its rows see. Sixteen warps: two warpgroups
+// of softmax, one thread per row, that take the key tiles in turn; one thread
+// that issues the matrix instructions; seven warps that bring in keys and
+// values. Per tile of 64 keys: S = Q K^T into tensor memory; its warpgroup
+// reads S, subtracts the running maximum and writes P = 2^(S - m) over it, as
+// bf16 parts; O = P V into tensor memory; the warpgroup adds O, scaled, to
+// its registers. Each warpgroup has its own maximum, sum and output, joined
+// at the end, so that one's softmax runs under the other's matrix
+// instructions and nothing is rescaled in place.
 //
-// Keys and values lie in shared memory as rows of 64 head entries (128 bytes,
-// 128-byte swizzle): K-major for Q K^T, the same rows MN-major for P V.
+// Q and P are operands in tensor memory: read from shared memory, Q alone
+// would take two thirds of its bandwidth at 64 keys a tile. Keys and values
+// lie in shared memory as rows of 64 head entries (128 bytes, 128-byte
+// swizzle): K-major for Q K^T, the same rows MN-major for P V.
 //
 // Precision. bf16: operands as they are, P as two bf16 parts (2^-17). fp32:
 // every operand as three bf16 parts, the six products that matter (the others
 // are below 2^-24); sums of a tile stay in the tensor cores' fp32, tiles are
 // added in registers, rounded to nearest.
 //
-// Bound: for bf16 with 128 rows the cache's bytes (23 cycles a key at 6.5
-// TB/s, against 8 for the matrix instructions and 8 for exp2), with more rows
-// the three come together; fp32's six products take 60 cycles a key.
+// Bound, in cycles per key and SM: the cache's bytes 23 (bf16, one row tile;
+// fp32 46; row tiles of the same keys share what L2 holds), exp2 8, issue of
+// the softmax 11, matrix instructions 12 (bf16) or 48 (fp32's six products).
 #include "attn_tree.h"
 
 #include <math.h>
@@ -30,8 +32,10 @@ namespace sg {
 namespace {
 
 constexpr int kRows = kTreeTcRows;
-constexpr int kThreads = 384;
-constexpr int kLoaders = 96;
+constexpr int kThreads = 512;
+constexpr int kKeys = 64;        // of a tile
+constexpr int kLoadWarps = 7;
+constexpr int kLoaders = 32 * kLoadWarps;
 constexpr unsigned long long kTimeoutNs = 2000000000ULL;
 
 template <typename T, int HD>
@@ -39,31 +43,36 @@ struct Tc {
   static constexpr bool kF32 = sizeof(T) == 4;
   static constexpr int kParts = kF32 ? 3 : 1;           // of q, k, v
   static constexpr int kPParts = kF32 ? 3 : 2;          // of the probabilities
-  static constexpr int kKeys = kF32 ? 64 : 128;
-  static constexpr int kQPart = kRows * HD * 2;         // bytes of one part
-  static constexpr int kPart = kKeys * HD * 2;
+  static constexpr int kPart = kKeys * HD * 2;          // bytes of a tile's part
   static constexpr int kTile = kParts * kPart;          // of K, or of V
-  // First column of S in its region: P's parts of 32 keys, which overwrite
-  // it from the region's start, reach no scores that are still to be read.
-  static constexpr int kS = kF32 ? 32 : 0;
-  static constexpr int kStages = kF32 ? 1 : 3;
+  // bf16: each loader warp has a stage. fp32: one, and rows on their way to
+  // parts in a ring of units of 32 keys.
+  static constexpr int kStages = kF32 ? 1 : kLoadWarps;
   static constexpr int kLoaded = kF32 ? kLoaders : 32;  // arrivals per filled tile
-  // fp32 rows on their way to parts: two buffers of 32 keys.
-  static constexpr int kRawKeys = 32;
-  static constexpr int kRaw = kF32 ? 2 * kRawKeys * HD * 4 : 0;
+  static constexpr int kUnitKeys = 32;
+  static constexpr int kUnit = kUnitKeys * HD * 4;
+  static constexpr int kRing = kF32 ? 8 : 0;
   static constexpr int kJoin = kRows * (HD + 4) * 4;    // the warpgroups' join
-  static constexpr int kOperands = kParts * kQPart + kStages * 2 * kTile + kRaw;
+  static constexpr int kOperands = kStages * 2 * kTile + kRing * kUnit;
   static constexpr int kUsed = (kOperands > kJoin ? kOperands : kJoin) + 1024;
   // At least half of an SM's: the CTA has all of the SM's tensor memory.
   static constexpr int kBytes = kUsed > 120 * 1024 ? kUsed : 120 * 1024;
-  // Instruction descriptors: fp32 sums of bf16, M = 128; S: N = keys, both
+  // Tensor memory columns: Q; regions of S and then P (in an fp32 region S
+  // starts at column 32: P's parts of 16 keys, which overwrite it from the
+  // start, reach no scores that are still to be read); O.
+  static constexpr int kSBuffers = kF32 ? 2 : 3, kOBuffers = kF32 ? 1 : 2;
+  static constexpr uint32_t kRegion = kF32 ? 96 : 64, kS = kF32 ? 32 : 0;
+  static constexpr uint32_t kColS = kParts * HD / 2;
+  static constexpr uint32_t kColO = kColS + kSBuffers * kRegion;
+  static_assert(kColO + kOBuffers * HD <= 512, "tensor memory has 512 columns");
+  // Instruction descriptors: fp32 sums of bf16, M = 128; S: N = keys, K
   // K-major; O: N = head entries, V MN-major.
-  static constexpr uint32_t kBase = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kRows >> 4) << 24);
+  static constexpr uint32_t kBase =
+      (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kRows >> 4) << 24);
   static constexpr uint32_t kDescS = kBase | ((uint32_t)(kKeys >> 3) << 17);
   static constexpr uint32_t kDescO = kBase | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
 };
-// Tensor memory columns: S (then P) and O of each warpgroup.
-constexpr uint32_t kColumns = 512, kColS = 128, kColO = 256;
+constexpr uint32_t kColumns = 512;
 
 // Products of parts, small ones first: part x of A times part y of B.
 __device__ constexpr int part_a(int x) { return x == 0 ? 2 : x == 2 || x == 3 ? 1 : 0; }
@@ -104,17 +113,21 @@ __device__ void mbar_drain(uint32_t bar) {
 __device__ bool mbar_wait(uint32_t bar, unsigned parity, volatile int* failed) {
   if (mbar_try_wait(bar, parity)) return true;
   const unsigned long long t0 = now_ns();
-  unsigned spins = 0;
   while (!mbar_try_wait(bar, parity)) {
-    if ((++spins & 63) == 0) {
-      if (*failed) return false;
-      if (now_ns() - t0 > kTimeoutNs) {
-        *failed = 1;
-        return false;
-      }
+    if (*failed) return false;
+    if (now_ns() - t0 > kTimeoutNs) {
+      *failed = 1;
+      return false;
     }
   }
   return true;
+}
+
+// The same for a whole warp, which stays together: the tensor-memory and
+// barrier instructions that follow are for converged warps.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, unsigned parity, volatile int* failed) {
+  const bool ok = mbar_wait(bar, parity, failed);
+  return __all_sync(0xFFFFFFFFu, ok);
 }
 
 // Operand tiles of 128-byte rows with 128-byte swizzle, 8-row atoms of 1024
@@ -129,14 +142,7 @@ __device__ __forceinline__ uint64_t sw128(uint32_t addr, uint32_t lead) {
   d |= (uint64_t)2 << 61;
   return d;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                       bool add) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
-      : "memory");
-}
+// D (+)= A B, A in tensor memory.
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
                                        bool add) {
   asm volatile(
@@ -156,31 +162,29 @@ __device__ __forceinline__ void fence_before() {
 __device__ __forceinline__ void fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
-// 32 columns of this thread's lane.
-__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t* r) {
+// 16 columns of this thread's lane.
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
         "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-        "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
-        "=r"(r[31])
+        "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(addr));
 }
-__device__ __forceinline__ void tmem_wait_ld() {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+// Until the loads issued have arrived; r is what one of them fills (no use of
+// it may move ahead of the wait).
+__device__ __forceinline__ void tmem_wait_ld(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
-// 16 columns of this thread's lane.
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+// 8 columns of this thread's lane.
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
-      "r"(r[15])
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() {
@@ -235,20 +239,18 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
   using C = Tc<T, HD>;
   constexpr bool kF32 = C::kF32;
-  constexpr int kKeys = C::kKeys, kStages = C::kStages;
+  constexpr int kStages = C::kStages;
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t k_full[kStages], k_empty[kStages], v_full[kStages],
-      v_empty[kStages], s_full[2], p_full[2], o_full[2], o_empty[2], done;
+      v_empty[kStages], s_full[C::kSBuffers], p_full[C::kSBuffers], o_full[2], o_empty[2], done;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int failed;
   __shared__ float2 ml[kRows];  // of the second warpgroup
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (saddr(raw) + 1023u) & ~1023u;
   uint8_t* const gbase = raw + (base - saddr(raw));
-  const uint32_t sq = base, skv = base + C::kParts * C::kQPart;
-  const uint32_t sraw = skv + kStages * 2 * C::kTile;
-  auto k_tile = [&](int s) { return skv + s * 2 * C::kTile; };
-  auto v_tile = [&](int s) { return skv + s * 2 * C::kTile + C::kTile; };
+  auto k_tile = [&](int s) { return base + s * 2 * C::kTile; };
+  auto v_tile = [&](int s) { return base + s * 2 * C::kTile + C::kTile; };
   const int split = blockIdx.x, head = blockIdx.y, r0 = blockIdx.z * kRows;
   const int R = a.t * a.group;
   pdl_trigger();
@@ -265,9 +267,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
       mbar_init(saddr(&k_empty[s]), 1);
       mbar_init(saddr(&v_empty[s]), 1);
     }
+    for (int b = 0; b < C::kSBuffers; b++) {
+      mbar_init(saddr(&s_full[b]), 1);
+      mbar_init(saddr(&p_full[b]), 128);
+    }
     for (int w = 0; w < 2; w++) {
-      mbar_init(saddr(&s_full[w]), 1);
-      mbar_init(saddr(&p_full[w]), 128);
       mbar_init(saddr(&o_full[w]), 1);
       mbar_init(saddr(&o_empty[w]), 128);
     }
@@ -283,46 +287,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     fence_before();
   }
-  // Queries, zeros for rows behind the last.
-  for (int i = threadIdx.x; i < kRows * (HD / 8); i += kThreads) {
-    const int r = i / (HD / 8), c = i % (HD / 8), row = r0 + r;
-    uint4 w[C::kParts];
-#pragma unroll
-    for (int p = 0; p < C::kParts; p++) w[p] = make_uint4(0, 0, 0, 0);
-    if (row < R) {
-      const int tok = row / a.group;
-      const T* q = static_cast<const T*>(a.q) + tok * a.ldq +
-                   (size_t)(head * a.group + row - tok * a.group) * HD + c * 8;
-      if constexpr (kF32) {
-        const float4 x = reinterpret_cast<const float4*>(q)[0];
-        const float4 y = reinterpret_cast<const float4*>(q)[1];
-        uint32_t e[4][3];
-        parts<3>(x.x, x.y, e[0]);
-        parts<3>(x.z, x.w, e[1]);
-        parts<3>(y.x, y.y, e[2]);
-        parts<3>(y.z, y.w, e[3]);
-#pragma unroll
-        for (int p = 0; p < 3; p++) w[p] = make_uint4(e[0][p], e[1][p], e[2][p], e[3][p]);
-      } else {
-        w[0] = *reinterpret_cast<const uint4*>(q);
-      }
-    }
-#pragma unroll
-    for (int p = 0; p < C::kParts; p++)
-      *reinterpret_cast<uint4*>(gbase + p * C::kQPart + at_sw128(kRows, r, c)) = w[p];
-  }
-  fence_operands();
   __syncthreads();
   fence_after();
   const uint32_t tmem = tmem_slot;
 
+  // 512 threads of 128 registers: 2 x 128 x 208 + 2 x 128 x 48 make as many.
   if (warp >= 8) {
-    // 384 threads of 168 registers: 2 x 128 x 208 + 128 x 88 make as many.
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp == 8) {
+      // Queries are there once the first warpgroup has written them.
+      asm volatile("bar.sync 3, 160;" ::: "memory");
       if (lane == 0) {
+        fence_after();
         auto scores = [&](int i) {  // S of tile i
-          const int s = i % kStages, w = i & 1;
+          const int s = i % kStages, b = i % C::kSBuffers;
           if (!mbar_wait(saddr(&k_full[s]), (i / kStages) & 1, &failed)) return false;
           fence_after();
           bool add = false;
@@ -331,22 +309,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
             const int pq = kF32 ? part_a(x) : 0, pk = kF32 ? part_b(x) : 0;
 #pragma unroll
             for (int k = 0; k < HD / 16; k++) {
-              const uint32_t at = (k / 4), in = (k % 4) * 32;
-              mma_ss(tmem + w * kColS + C::kS, sw128(sq + pq * C::kQPart + at * kRows * 128 + in, 16),
-                     sw128(k_tile(s) + pk * C::kPart + at * kKeys * 128 + in, 16), C::kDescS, add);
+              mma_ts(tmem + C::kColS + b * C::kRegion + C::kS, tmem + pq * (HD / 2) + k * 8,
+                     sw128(k_tile(s) + pk * C::kPart + (k / 4) * kKeys * 128 + (k % 4) * 32, 16),
+                     C::kDescS, add);
               add = true;
             }
           }
-          mma_commit(saddr(&s_full[w]));
+          mma_commit(saddr(&s_full[b]));
           mma_commit(saddr(&k_empty[s]));
           return true;
         };
-        bool ok = scores(0) && (nt < 2 || scores(1));
+        bool ok = true;
+        for (int i = 0; ok && i < C::kSBuffers && i < nt; i++) ok = scores(i);
         for (int i = 0; ok && i < nt; i++) {
-          const int s = i % kStages, w = i & 1, turn = i >> 1;
-          ok = mbar_wait(saddr(&p_full[w]), turn & 1, &failed) &&
+          const int s = i % kStages, b = i % C::kSBuffers, o = i % C::kOBuffers, w = i & 1;
+          // The last product in these columns has been read. (O's barriers go
+          // by warpgroup, so that who waits on one has seen all its phases.)
+          const int last = i - C::kOBuffers;
+          ok = mbar_wait(saddr(&p_full[b]), (i / C::kSBuffers) & 1, &failed) &&
                mbar_wait(saddr(&v_full[s]), (i / kStages) & 1, &failed) &&
-               (turn == 0 || mbar_wait(saddr(&o_empty[w]), (turn - 1) & 1, &failed));
+               (last < 0 || mbar_wait(saddr(&o_empty[last & 1]), (last >> 1) & 1, &failed));
           if (!ok) break;
           fence_after();
           bool add = false;
@@ -357,17 +339,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
             for (int k = 0; k < kKeys / 16; k++) {
               // P's columns: per 32 keys, 16 of each part.
               const uint32_t p = (k / 2) * C::kPParts * 16 + pp * 16 + (k % 2) * 8;
-              mma_ts(tmem + kColO + w * 128, tmem + w * kColS + p,
+              mma_ts(tmem + C::kColO + o * HD, tmem + C::kColS + b * C::kRegion + p,
                      sw128(v_tile(s) + pv * C::kPart + k * 2048, kKeys * 128), C::kDescO, add);
               add = true;
             }
           }
           mma_commit(saddr(&o_full[w]));
           mma_commit(saddr(&v_empty[s]));
-          // The next scores of this warpgroup overwrite the P that this
-          // product reads.
-          if (i + 2 < nt)
-            ok = mbar_wait(saddr(&o_full[w]), turn & 1, &failed) && scores(i + 2);
+          // The next scores in this region overwrite the P that this product
+          // reads.
+          if (i + C::kSBuffers < nt)
+            ok = mbar_wait(saddr(&o_full[w]), (i >> 1) & 1, &failed) && scores(i + C::kSBuffers);
         }
         // Nothing issued here outlives the tensor memory.
         mma_commit(saddr(&done));
@@ -378,8 +360,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
       const T* kbase = static_cast<const T*>(a.k) + (size_t)head * a.ctx * HD;
       const T* vbase = static_cast<const T*>(a.v) + (size_t)head * a.ctx * HD;
       if constexpr (!kF32) {
-        // Each loader warp has one of the three stages: it waits for what it
-        // copied without holding up the other stages.
+        // Each loader warp has one of the stages: it waits for what it copied
+        // without holding up the others.
         const int s = warp - 9;
         for (int i = s; i < nt; i += kStages) {
           const unsigned turn = (unsigned)(i / kStages);
@@ -394,9 +376,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
             }
             cp_async_commit();
           };
-          if (turn && !mbar_wait(saddr(&k_empty[s]), (turn - 1) & 1, &failed)) break;
+          if (turn && !warp_wait(saddr(&k_empty[s]), (turn - 1) & 1, &failed)) break;
           copy(kbase, k_tile(s));
-          if (turn && !mbar_wait(saddr(&v_empty[s]), (turn - 1) & 1, &failed)) break;
+          if (turn && !warp_wait(saddr(&v_empty[s]), (turn - 1) & 1, &failed)) break;
           copy(vbase, v_tile(s));
           cp_async_wait<1>();
           fence_operands();
@@ -407,64 +389,74 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
         }
         cp_async_wait<0>();
       } else {
-        const int id = threadIdx.x - 288;
-        // Units of 32 keys: K, K, V, V of each tile. The next unit's rows
-        // stream into the other raw buffer while this one's become parts.
-        constexpr int kUnits = kKeys / C::kRawKeys;
+        // Half tiles in the order of their use: K of tile 0, then K of tile
+        // i + 1 and V of tile i. Rows of the next kRing - 1 units stream into
+        // the ring while this one's become parts.
+        constexpr int kRing = C::kRing, kUnitKeys = C::kUnitKeys;
+        const int id = threadIdx.x - 288, units = 4 * nt;
+        const uint32_t ring = base + kStages * 2 * C::kTile;
+        // Tile of unit u, whether it is of V; its half is u & 1.
+        auto unit = [&](int u, bool& is_v) {
+          const int x = u >> 1;  // K0, K1, V0, K2, V1, ..., V of the last
+          if (x == 0) { is_v = false; return 0; }
+          if (x == 2 * nt - 1) { is_v = true; return nt - 1; }
+          is_v = !(x & 1);
+          return is_v ? x / 2 - 1 : (x + 1) / 2;
+        };
         auto fetch = [&](int u) {
-          if (u < nt * 2 * kUnits) {
-            const int tile = u / (2 * kUnits), half = u % kUnits;
-            const bool is_v = u / kUnits & 1;
-            const int row = (tile0 + tile) * kKeys + half * C::kRawKeys;
-            const int rows = min(C::kRawKeys, n - row);
+          if (u < units) {
+            bool is_v;
+            const int row = (tile0 + unit(u, is_v)) * kKeys + (u & 1) * kUnitKeys;
+            const int rows = min(kUnitKeys, n - row);
             const T* from = is_v ? vbase : kbase;
-            const uint32_t to = sraw + (u & 1) * (C::kRaw / 2);
+            const uint32_t to = ring + (u % kRing) * C::kUnit;
 #pragma unroll 4
-            for (int x = id; x < C::kRawKeys * (HD / 4); x += kLoaders) {
+            for (int x = id; x < kUnitKeys * (HD / 4); x += kLoaders) {
               const int r = x / (HD / 4), c = x % (HD / 4);
-              const bool in = r < rows;
+              const bool in = r < rows;  // zeros behind the last key
               cp_async16(to + x * 16, from + (size_t)(in ? row + r : 0) * HD + c * 4, in ? 16 : 0);
             }
           }
           cp_async_commit();
         };
-        fetch(0);
+#pragma unroll 1
+        for (int u = 0; u < kRing - 1; u++) fetch(u);
         bool ok = true;
-        for (int u = 0; u < nt * 2 * kUnits; u++) {
-          const int i = u / (2 * kUnits), half = u % kUnits, s = i % kStages;
-          const bool is_v = u / kUnits & 1;
-          cp_async_wait<0>();
+#pragma unroll 1
+        for (int u = 0; u < units; u++) {
+          bool is_v;
+          const int i = unit(u, is_v), half = u & 1;
+          cp_async_wait<kRing - 2>();
           // All loaders' copies of this unit have landed, and all are done
-          // with the other buffer.
+          // with the buffer that the next fetch fills.
           asm volatile("bar.sync 1, %0;" ::"n"(kLoaders) : "memory");
-          fetch(u + 1);
-          if (half == 0 && i >= kStages)
-            ok = ok && mbar_wait(saddr(is_v ? &v_empty[s] : &k_empty[s]), (i / kStages - 1) & 1,
-                                 &failed);
+          fetch(u + kRing - 1);
           // (A wait that ran out leaves nothing to do but to stay in step.)
-          const uint8_t* from = gbase + (sraw - base) + (u & 1) * (C::kRaw / 2);
-          uint8_t* to = gbase + ((is_v ? v_tile(s) : k_tile(s)) - base);
+          if (half == 0 && i > 0)
+            ok = ok && warp_wait(saddr(is_v ? &v_empty[0] : &k_empty[0]), (i - 1) & 1, &failed);
           if (ok) {
-#pragma unroll 2
-            for (int x = id; x < C::kRawKeys * (HD / 8); x += kLoaders) {
+            const uint8_t* from = gbase + (ring - base) + (u % kRing) * C::kUnit;
+            uint8_t* to = gbase + (is_v ? C::kTile : 0);
+#pragma unroll 1
+            for (int x = id; x < kUnitKeys * (HD / 8); x += kLoaders) {
               const int r = x / (HD / 8), c = x % (HD / 8);
-              const float4 f = *reinterpret_cast<const float4*>(from + (r * HD + c * 8) * 4);
-              const float4 g = *reinterpret_cast<const float4*>(from + (r * HD + c * 8) * 4 + 16);
+              const float4 f = *reinterpret_cast<const float4*>(from + x * 32);
+              const float4 g = *reinterpret_cast<const float4*>(from + x * 32 + 16);
               uint32_t e[4][3];
               parts<3>(f.x, f.y, e[0]);
               parts<3>(f.z, f.w, e[1]);
               parts<3>(g.x, g.y, e[2]);
               parts<3>(g.z, g.w, e[3]);
-              const uint32_t at = at_sw128(kKeys, half * C::kRawKeys + r, c);
+              const uint32_t at = at_sw128(kKeys, half * kUnitKeys + r, c);
 #pragma unroll
               for (int p = 0; p < 3; p++)
                 *reinterpret_cast<uint4*>(to + p * C::kPart + at) =
                     make_uint4(e[0][p], e[1][p], e[2][p], e[3][p]);
             }
-          }
-          if (half == kUnits - 1 && ok) {
-            fence_operands();
-            mbar_arrive(saddr(is_v ? &v_full[s] : &k_full[s]));
+            if (half) {
+              fence_operands();
+              mbar_arrive(saddr(is_v ? &v_full[0] : &k_full[0]));
+            }
           }
         }
         cp_async_wait<0>();
@@ -474,51 +466,89 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // Softmax: this thread's row is lane 32 (warp % 4) + lane of the tile.
     const int w = warp >> 2, r = threadIdx.x & 127;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tp = tmem + w * kColS + lanes, ts = tp + C::kS, to = tmem + kColO + w * 128 + lanes;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    if (w == 0) {
+      // Queries into tensor memory, zeros for rows behind the last.
+      const int row = r0 + r, tok = row < R ? row / a.group : 0;
+      const T* q = static_cast<const T*>(a.q) + tok * a.ldq +
+                   (size_t)(head * a.group + (row < R ? row - tok * a.group : 0)) * HD;
+#pragma unroll
+      for (int c = 0; c < HD / 16; c++) {
+        uint32_t e[C::kParts][8];
+        if constexpr (kF32) {
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            float4 x = reinterpret_cast<const float4*>(q)[c * 4 + j];
+            if (row >= R) x = make_float4(0.f, 0.f, 0.f, 0.f);
+            uint32_t y[2][3];
+            parts<3>(x.x, x.y, y[0]);
+            parts<3>(x.z, x.w, y[1]);
+#pragma unroll
+            for (int p = 0; p < 3; p++) {
+              e[p][2 * j] = y[0][p];
+              e[p][2 * j + 1] = y[1][p];
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            uint4 x = reinterpret_cast<const uint4*>(q)[c * 2 + j];
+            if (row >= R) x = make_uint4(0, 0, 0, 0);
+            e[0][4 * j] = x.x;
+            e[0][4 * j + 1] = x.y;
+            e[0][4 * j + 2] = x.z;
+            e[0][4 * j + 3] = x.w;
+          }
+        }
+#pragma unroll
+        for (int p = 0; p < C::kParts; p++) tmem_st8(lanes + p * (HD / 2) + c * 8, e[p]);
+      }
+      tmem_wait_st();
+      fence_before();
+      asm volatile("bar.arrive 3, 160;" ::: "memory");
+    }
     // Scores in units of log2, so that the softmax is exp2.
     const float scale = 1.4426950408889634f / sqrtf((float)HD);
     float o[HD], m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int i = 0; i < HD; i++) o[i] = 0.f;
+#pragma unroll 1
     for (int i = w; i < nt; i += 2) {
-      const int turn = i >> 1;
+      const int b = i % C::kSBuffers;
+      const uint32_t tp = lanes + C::kColS + b * C::kRegion, ts = tp + C::kS;
+      const uint32_t to = lanes + C::kColO + i % C::kOBuffers * HD;
       const int keys = min(kKeys, n - (tile0 + i) * kKeys);
-      if (!mbar_wait(saddr(&s_full[w]), turn & 1, &failed)) break;
+      if (!warp_wait(saddr(&s_full[b]), (i / C::kSBuffers) & 1, &failed)) break;
       fence_after();
+      uint32_t s[2][16];
       float top = -INFINITY;
+      tmem_ld16(ts, s[0]);
 #pragma unroll
-      for (int c = 0; c < kKeys / 32; c++) {
-        uint32_t s[32];
-        tmem_ld(ts + c * 32, s);
-        tmem_wait_ld();
-        if ((c + 1) * 32 <= keys) {
+      for (int c = 0; c < kKeys / 16; c++) {
+        tmem_wait_ld(s[c & 1]);
+        // After the last, the first again, for the second pass.
+        tmem_ld16(ts + (c + 1) % (kKeys / 16) * 16, s[(c + 1) & 1]);
 #pragma unroll
-          for (int j = 0; j < 32; j++) top = fmaxf(top, __uint_as_float(s[j]));
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; j++)
-            if (c * 32 + j < keys) top = fmaxf(top, __uint_as_float(s[j]));
-        }
+        for (int j = 0; j < 16; j++)
+          if (keys == kKeys || c * 16 + j < keys) top = fmaxf(top, __uint_as_float(s[c & 1][j]));
       }
       const float next = fmaxf(m, top * scale);
-      const float keep = ex2(m - next);  // 0 before the first key
       const float shift = next == -INFINITY ? 0.f : next;
+      const float keep = next == -INFINITY ? 1.f : ex2(m - next);  // 0 before the first key
       m = next;
       float sum = 0.f;
 #pragma unroll
-      for (int c = 0; c < kKeys / 32; c++) {
-        uint32_t s[32];
-        tmem_ld(ts + c * 32, s);
-        tmem_wait_ld();
-        uint32_t p[C::kPParts][16];
+      for (int c = 0; c < kKeys / 16; c++) {
+        tmem_wait_ld(s[c & 1]);
+        if (c + 1 < kKeys / 16) tmem_ld16(ts + (c + 1) * 16, s[(c + 1) & 1]);
+        uint32_t p[C::kPParts][8];
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          float x0 = ex2(fmaf(__uint_as_float(s[j]), scale, -shift));
-          float x1 = ex2(fmaf(__uint_as_float(s[j + 1]), scale, -shift));
-          if ((c + 1) * 32 > keys) {
-            if (c * 32 + j >= keys) x0 = 0.f;
-            if (c * 32 + j + 1 >= keys) x1 = 0.f;
+        for (int j = 0; j < 16; j += 2) {
+          float x0 = ex2(fmaf(__uint_as_float(s[c & 1][j]), scale, -shift));
+          float x1 = ex2(fmaf(__uint_as_float(s[c & 1][j + 1]), scale, -shift));
+          if (keys < kKeys) {
+            if (c * 16 + j >= keys) x0 = 0.f;
+            if (c * 16 + j + 1 >= keys) x1 = 0.f;
           }
           sum += x0 + x1;
           uint32_t e[C::kPParts];
@@ -526,23 +556,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
 #pragma unroll
           for (int y = 0; y < C::kPParts; y++) p[y][j / 2] = e[y];
         }
+        // The scores that these columns held have been read.
+        tmem_wait_ld(s[(c + 1) & 1]);
 #pragma unroll
-        for (int y = 0; y < C::kPParts; y++) tmem_st16(tp + (c * C::kPParts + y) * 16, p[y]);
+        for (int y = 0; y < C::kPParts; y++)
+          tmem_st8(tp + (c / 2) * C::kPParts * 16 + y * 16 + (c % 2) * 8, p[y]);
       }
-      l = l * (m == -INFINITY ? 1.f : keep) + sum;
+      l = l * keep + sum;
       tmem_wait_st();
       fence_before();
-      mbar_arrive(saddr(&p_full[w]));
-      if (!mbar_wait(saddr(&o_full[w]), turn & 1, &failed)) break;
+      mbar_arrive(saddr(&p_full[b]));
+      if (!warp_wait(saddr(&o_full[w]), (i >> 1) & 1, &failed)) break;
       fence_after();
+      tmem_ld16(to, s[0]);
 #pragma unroll
-      for (int c = 0; c < HD / 32; c++) {
-        uint32_t x[32];
-        tmem_ld(to + c * 32, x);
-        tmem_wait_ld();
+      for (int c = 0; c < HD / 16; c++) {
+        tmem_wait_ld(s[c & 1]);
+        if (c + 1 < HD / 16) tmem_ld16(to + (c + 1) * 16, s[(c + 1) & 1]);
 #pragma unroll
-        for (int j = 0; j < 32; j++)
-          o[c * 32 + j] = fmaf(o[c * 32 + j], m == -INFINITY ? 1.f : keep, __uint_as_float(x[j]));
+        for (int j = 0; j < 16; j++)
+          o[c * 16 + j] = fmaf(o[c * 16 + j], keep, __uint_as_float(s[c & 1][j]));
       }
       fence_before();
       mbar_arrive(saddr(&o_empty[w]));
@@ -608,7 +641,7 @@ cudaError_t launch_tc(const TreeArgs& a, int dev, cudaStream_t s) {
 
 }  // namespace
 
-int tree_tc_keys(bool f32) { return f32 ? Tc<float, 128>::kKeys : Tc<uint16_t, 128>::kKeys; }
+int tree_tc_keys() { return kKeys; }
 
 cudaError_t tree_tc(const TreeArgs& a, bool f32, int head_dim, int dev, cudaStream_t s) {
   if (f32) return head_dim == 128 ? launch_tc<float, 128>(a, dev, s) : launch_tc<float, 64>(a, dev, s);

@@ -247,7 +247,7 @@ def inputs(torch, t, kh, g, hd, ctx, type_, seed):
     (1, 1, 1, 0), (1, 2, 4, 1), (1, 2, 8, 333), (2, 1, 5, 31), (5, 2, 3, 32), (4, 1, 4, 33),
     (6, 2, 4, 63), (8, 1, 4, 64), (9, 1, 4, 65), (16, 1, 4, 127), (17, 2, 4, 128),
     (11, 1, 7, 129), (64, 1, 2, 700), (33, 1, 8, 255), (70, 1, 1, 40), (130, 1, 3, 0),
-    (3, 1, 2, 5000), (40, 1, 4, 1500)])
+    (3, 1, 2, 5000), (40, 1, 4, 1500), (33, 8, 4, 2999), (256, 2, 1, 77), (257, 2, 1, 130)])
 def test_tree_matches_float64(cuda, type_, hd, t, kh, g, n):
     torch = cuda
     q, k, v = inputs(torch, t, kh, g, hd, n + t + 13, type_, t * 131 + n)
