@@ -6,10 +6,15 @@
 // that issues the matrix instructions; seven warps that bring in keys and
 // values. Per tile of 64 keys: S = Q K^T into tensor memory; its warpgroup
 // reads S, subtracts the running maximum and writes P = 2^(S - m) over it, as
-// bf16 parts; O = P V into tensor memory; the warpgroup adds O, scaled, to
-// its registers. Each warpgroup has its own maximum, sum and output, joined
-// at the end, so that one's softmax runs under the other's matrix
-// instructions and nothing is rescaled in place.
+// bf16 parts; then O (+)= P V in tensor memory. Each warpgroup has its own
+// maximum, sum and output, joined at the end, so that one's softmax runs
+// under the other's matrix instructions.
+//
+// bf16: O stays in tensor memory. A new maximum rescales it only when it is
+// 2^8 above the one that P is relative to (P is at most 2^8 then), which
+// happens in the first few tiles as a rule. fp32: the tensor cores' sums are
+// cut, not rounded, so each tile's O starts from zero and is added, scaled,
+// to the warpgroup's registers.
 //
 // Q and P are operands in tensor memory: read from shared memory, Q alone
 // would take two thirds of its bandwidth at 64 keys a tile. Keys and values
@@ -17,9 +22,8 @@
 // swizzle): K-major for Q K^T, the same rows MN-major for P V.
 //
 // Precision. bf16: operands as they are, P as two bf16 parts (2^-17). fp32:
-// every operand as three bf16 parts, the six products that matter (the others
-// are below 2^-24); sums of a tile stay in the tensor cores' fp32, tiles are
-// added in registers, rounded to nearest.
+// every operand as three bf16 parts of 8 bits each, all 24 of them, and the six
+// products that matter (the others are below 2^-24).
 //
 // Bound, in cycles per key and SM: the cache's bytes 23 (bf16, one row tile;
 // fp32 46; row tiles of the same keys share what L2 holds), exp2 8, issue of
@@ -142,18 +146,32 @@ __device__ __forceinline__ uint64_t sw128(uint32_t addr, uint32_t lead) {
   d |= (uint64_t)2 << 61;
   return d;
 }
+// One thread of a converged warp. The matrix instructions are issued under
+// its predicate and not inside a branch, so that their operands, the same in
+// all threads, can stay in uniform registers: a branch took 100 cycles per
+// instruction.
+__device__ __forceinline__ uint32_t elect() {
+  uint32_t one;
+  asm volatile(
+      "{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(one));
+  return one;
+}
 // D (+)= A B, A in tensor memory.
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                       bool add) {
+                                       bool add, uint32_t issue) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(issue)
       : "memory");
 }
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
+__device__ __forceinline__ void mma_commit(uint32_t bar, uint32_t issue) {
   asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(
+          bar),
+      "r"(issue)
       : "memory");
 }
 __device__ __forceinline__ void fence_before() {
@@ -180,7 +198,24 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t* r) {
                  "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
                  "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
-// 8 columns of this thread's lane.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
+  tmem_ld16(addr, r);
+  tmem_ld16(addr + 16, r + 16);
+}
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t* r) {
+  tmem_wait_ld(r);
+  tmem_wait_ld(r + 16);
+}
+// 16, 8 columns of this thread's lane.
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr),
@@ -216,17 +251,25 @@ __device__ __forceinline__ uint32_t bf16x2(float x0, float x1) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(x1), "f"(x0));
   return w;
 }
-__device__ __forceinline__ float low(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float high(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
-// Two values as N bf16 parts each: x = p[0] + p[1] + ..., each the rounding
-// of what the ones before leave.
+// The upper halves of two words: two values cut to bf16.
+__device__ __forceinline__ uint32_t upper(float x0, float x1) {
+  return __byte_perm(__float_as_uint(x0), __float_as_uint(x1), 0x7632);
+}
+__device__ __forceinline__ float rest(float x) {  // what the cut leaves, exact
+  return x - __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
+}
+// Two values as bf16 parts, x = p[0] + p[1] + ...: N = 3 cuts 8 bits off each
+// time and loses nothing; N = 2 rounds the second part.
 template <int N>
 __device__ __forceinline__ void parts(float x0, float x1, uint32_t* p) {
-#pragma unroll
-  for (int i = 0; i < N; i++) {
-    p[i] = bf16x2(x0, x1);
-    x0 -= low(p[i]);
-    x1 -= high(p[i]);
+  p[0] = upper(x0, x1);
+  x0 = rest(x0);
+  x1 = rest(x1);
+  if constexpr (N == 2) {
+    p[1] = bf16x2(x0, x1);
+  } else {
+    p[1] = upper(x0, x1);
+    p[2] = upper(rest(x0), rest(x1));
   }
 }
 
@@ -297,64 +340,62 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
     if (warp == 8) {
       // Queries are there once the first warpgroup has written them.
       asm volatile("bar.sync 3, 160;" ::: "memory");
-      if (lane == 0) {
+      fence_after();
+      const uint32_t one = elect();
+      auto scores = [&](int i) {  // S of tile i
+        const int s = i % kStages, b = i % C::kSBuffers;
+        if (!warp_wait(saddr(&k_full[s]), (i / kStages) & 1, &failed)) return false;
         fence_after();
-        auto scores = [&](int i) {  // S of tile i
-          const int s = i % kStages, b = i % C::kSBuffers;
-          if (!mbar_wait(saddr(&k_full[s]), (i / kStages) & 1, &failed)) return false;
-          fence_after();
-          bool add = false;
+        const uint64_t k0 = sw128(k_tile(s), 16);
+        const uint32_t d = tmem + C::kColS + b * C::kRegion + C::kS;
 #pragma unroll
-          for (int x = 0; x < (kF32 ? 6 : 1); x++) {
-            const int pq = kF32 ? part_a(x) : 0, pk = kF32 ? part_b(x) : 0;
+        for (int x = 0; x < (kF32 ? 6 : 1); x++) {
+          const int pq = kF32 ? part_a(x) : 0, pk = kF32 ? part_b(x) : 0;
 #pragma unroll
-            for (int k = 0; k < HD / 16; k++) {
-              mma_ts(tmem + C::kColS + b * C::kRegion + C::kS, tmem + pq * (HD / 2) + k * 8,
-                     sw128(k_tile(s) + pk * C::kPart + (k / 4) * kKeys * 128 + (k % 4) * 32, 16),
-                     C::kDescS, add);
-              add = true;
-            }
-          }
-          mma_commit(saddr(&s_full[b]));
-          mma_commit(saddr(&k_empty[s]));
-          return true;
-        };
-        bool ok = true;
-        for (int i = 0; ok && i < C::kSBuffers && i < nt; i++) ok = scores(i);
-        for (int i = 0; ok && i < nt; i++) {
-          const int s = i % kStages, b = i % C::kSBuffers, o = i % C::kOBuffers, w = i & 1;
-          // The last product in these columns has been read. (O's barriers go
-          // by warpgroup, so that who waits on one has seen all its phases.)
-          const int last = i - C::kOBuffers;
-          ok = mbar_wait(saddr(&p_full[b]), (i / C::kSBuffers) & 1, &failed) &&
-               mbar_wait(saddr(&v_full[s]), (i / kStages) & 1, &failed) &&
-               (last < 0 || mbar_wait(saddr(&o_empty[last & 1]), (last >> 1) & 1, &failed));
-          if (!ok) break;
-          fence_after();
-          bool add = false;
-#pragma unroll
-          for (int x = 0; x < (kF32 ? 6 : 2); x++) {
-            const int pp = kF32 ? part_a(x) : 1 - x, pv = kF32 ? part_b(x) : 0;
-#pragma unroll
-            for (int k = 0; k < kKeys / 16; k++) {
-              // P's columns: per 32 keys, 16 of each part.
-              const uint32_t p = (k / 2) * C::kPParts * 16 + pp * 16 + (k % 2) * 8;
-              mma_ts(tmem + C::kColO + o * HD, tmem + C::kColS + b * C::kRegion + p,
-                     sw128(v_tile(s) + pv * C::kPart + k * 2048, kKeys * 128), C::kDescO, add);
-              add = true;
-            }
-          }
-          mma_commit(saddr(&o_full[w]));
-          mma_commit(saddr(&v_empty[s]));
-          // The next scores in this region overwrite the P that this product
-          // reads.
-          if (i + C::kSBuffers < nt)
-            ok = mbar_wait(saddr(&o_full[w]), (i >> 1) & 1, &failed) && scores(i + C::kSBuffers);
+          for (int k = 0; k < HD / 16; k++)
+            mma_ts(d, tmem + pq * (HD / 2) + k * 8,
+                   k0 + ((pk * C::kPart + (k / 4) * kKeys * 128 + (k % 4) * 32) >> 4), C::kDescS,
+                   x + k > 0, one);
         }
-        // Nothing issued here outlives the tensor memory.
-        mma_commit(saddr(&done));
-        mbar_drain(saddr(&done));
+        mma_commit(saddr(&s_full[b]), one);
+        mma_commit(saddr(&k_empty[s]), one);
+        return true;
+      };
+      bool ok = true;
+      for (int i = 0; ok && i < C::kSBuffers && i < nt; i++) ok = scores(i);
+      for (int i = 0; ok && i < nt; i++) {
+        const int s = i % kStages, b = i % C::kSBuffers, w = i & 1, o = kF32 ? 0 : w;
+        // fp32: the last product in these columns has been read. (O's barriers
+        // go by warpgroup, so that who waits on one has seen all its phases.)
+        const int last = i - 1;
+        ok = warp_wait(saddr(&p_full[b]), (i / C::kSBuffers) & 1, &failed) &&
+             warp_wait(saddr(&v_full[s]), (i / kStages) & 1, &failed) &&
+             (!kF32 || last < 0 ||
+              warp_wait(saddr(&o_empty[last & 1]), (last >> 1) & 1, &failed));
+        if (!ok) break;
+        fence_after();
+        const uint64_t v0 = sw128(v_tile(s), kKeys * 128);
+        const uint32_t d = tmem + C::kColO + o * HD, p0 = tmem + C::kColS + b * C::kRegion;
+#pragma unroll
+        for (int x = 0; x < (kF32 ? 6 : 2); x++) {
+          const int pp = kF32 ? part_a(x) : 1 - x, pv = kF32 ? part_b(x) : 0;
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; k++)
+            // P's columns: per 32 keys, 16 of each part.
+            mma_ts(d, p0 + (k / 2) * C::kPParts * 16 + pp * 16 + (k % 2) * 8,
+                   v0 + ((pv * C::kPart + k * 2048) >> 4), C::kDescO,
+                   x + k > 0 || (!kF32 && i >= 2), one);
+        }
+        mma_commit(saddr(&o_full[w]), one);
+        mma_commit(saddr(&v_empty[s]), one);
+        // The next scores in this region overwrite the P that this product
+        // reads.
+        if (i + C::kSBuffers < nt)
+          ok = warp_wait(saddr(&o_full[w]), (i >> 1) & 1, &failed) && scores(i + C::kSBuffers);
       }
+      // Nothing issued here outlives the tensor memory.
+      mma_commit(saddr(&done), one);
+      mbar_drain(saddr(&done));
       __syncwarp();
     } else {
       const T* kbase = static_cast<const T*>(a.k) + (size_t)head * a.ctx * HD;
@@ -437,21 +478,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
           if (ok) {
             const uint8_t* from = gbase + (ring - base) + (u % kRing) * C::kUnit;
             uint8_t* to = gbase + (is_v ? C::kTile : 0);
-#pragma unroll 1
+#pragma unroll 2
             for (int x = id; x < kUnitKeys * (HD / 8); x += kLoaders) {
               const int r = x / (HD / 8), c = x % (HD / 8);
               const float4 f = *reinterpret_cast<const float4*>(from + x * 32);
               const float4 g = *reinterpret_cast<const float4*>(from + x * 32 + 16);
-              uint32_t e[4][3];
-              parts<3>(f.x, f.y, e[0]);
-              parts<3>(f.z, f.w, e[1]);
-              parts<3>(g.x, g.y, e[2]);
-              parts<3>(g.z, g.w, e[3]);
-              const uint32_t at = at_sw128(kKeys, half * kUnitKeys + r, c);
+              float e[8] = {f.x, f.y, f.z, f.w, g.x, g.y, g.z, g.w};
+              uint8_t* at = to + at_sw128(kKeys, half * kUnitKeys + r, c);
 #pragma unroll
-              for (int p = 0; p < 3; p++)
-                *reinterpret_cast<uint4*>(to + p * C::kPart + at) =
-                    make_uint4(e[0][p], e[1][p], e[2][p], e[3][p]);
+              for (int p = 0; p < 3; p++) {
+                *reinterpret_cast<uint4*>(at + p * C::kPart) =
+                    make_uint4(upper(e[0], e[1]), upper(e[2], e[3]), upper(e[4], e[5]),
+                               upper(e[6], e[7]));
+#pragma unroll
+                for (int j = 0; j < 8; j++) e[j] = rest(e[j]);
+              }
             }
             if (half) {
               fence_operands();
@@ -472,36 +513,45 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
       const int row = r0 + r, tok = row < R ? row / a.group : 0;
       const T* q = static_cast<const T*>(a.q) + tok * a.ldq +
                    (size_t)(head * a.group + (row < R ? row - tok * a.group : 0)) * HD;
+      constexpr int kVec = 16 / sizeof(T), kBatch = 8;  // 16-byte loads in flight
 #pragma unroll
-      for (int c = 0; c < HD / 16; c++) {
-        uint32_t e[C::kParts][8];
-        if constexpr (kF32) {
+      for (int c = 0; c < HD / (kVec * kBatch); c++) {
+        uint4 x[kBatch];
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            float4 x = reinterpret_cast<const float4*>(q)[c * 4 + j];
-            if (row >= R) x = make_float4(0.f, 0.f, 0.f, 0.f);
-            uint32_t y[2][3];
-            parts<3>(x.x, x.y, y[0]);
-            parts<3>(x.z, x.w, y[1]);
-#pragma unroll
-            for (int p = 0; p < 3; p++) {
-              e[p][2 * j] = y[0][p];
-              e[p][2 * j + 1] = y[1][p];
-            }
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 2; j++) {
-            uint4 x = reinterpret_cast<const uint4*>(q)[c * 2 + j];
-            if (row >= R) x = make_uint4(0, 0, 0, 0);
-            e[0][4 * j] = x.x;
-            e[0][4 * j + 1] = x.y;
-            e[0][4 * j + 2] = x.z;
-            e[0][4 * j + 3] = x.w;
-          }
+        for (int j = 0; j < kBatch; j++) {
+          x[j] = reinterpret_cast<const uint4*>(q)[c * kBatch + j];
+          if (row >= R) x[j] = make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
-        for (int p = 0; p < C::kParts; p++) tmem_st8(lanes + p * (HD / 2) + c * 8, e[p]);
+        for (int h = 0; h < kBatch * kVec / 16; h++) {  // 16 entries, 8 columns a part
+          uint32_t e[C::kParts][8];
+          if constexpr (kF32) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const uint4 v = x[4 * h + j];
+              uint32_t y[2][3];
+              parts<3>(__uint_as_float(v.x), __uint_as_float(v.y), y[0]);
+              parts<3>(__uint_as_float(v.z), __uint_as_float(v.w), y[1]);
+#pragma unroll
+              for (int p = 0; p < 3; p++) {
+                e[p][2 * j] = y[0][p];
+                e[p][2 * j + 1] = y[1][p];
+              }
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+              const uint4 v = x[2 * h + j];
+              e[0][4 * j] = v.x;
+              e[0][4 * j + 1] = v.y;
+              e[0][4 * j + 2] = v.z;
+              e[0][4 * j + 3] = v.w;
+            }
+          }
+#pragma unroll
+          for (int p = 0; p < C::kParts; p++)
+            tmem_st8(lanes + p * (HD / 2) + (c * kBatch * kVec / 16 + h) * 8, e[p]);
+        }
       }
       tmem_wait_st();
       fence_before();
@@ -509,46 +559,30 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
     }
     // Scores in units of log2, so that the softmax is exp2.
     const float scale = 1.4426950408889634f / sqrtf((float)HD);
-    float o[HD], m = -INFINITY, l = 0.f;
+    float o[kF32 ? HD : 1], m = -INFINITY, l = 0.f;
+    const uint32_t to = lanes + C::kColO + (kF32 ? 0 : w * HD);
 #pragma unroll
-    for (int i = 0; i < HD; i++) o[i] = 0.f;
+    for (int i = 0; i < (kF32 ? HD : 1); i++) o[i] = 0.f;
+    bool ok = true;
 #pragma unroll 1
     for (int i = w; i < nt; i += 2) {
       const int b = i % C::kSBuffers;
       const uint32_t tp = lanes + C::kColS + b * C::kRegion, ts = tp + C::kS;
-      const uint32_t to = lanes + C::kColO + i % C::kOBuffers * HD;
       const int keys = min(kKeys, n - (tile0 + i) * kKeys);
-      if (!warp_wait(saddr(&s_full[b]), (i / C::kSBuffers) & 1, &failed)) break;
+      ok = warp_wait(saddr(&s_full[b]), (i / C::kSBuffers) & 1, &failed);
+      if (!ok) break;
       fence_after();
-      uint32_t s[2][16];
-      float top = -INFINITY;
-      tmem_ld16(ts, s[0]);
+      float top = -INFINITY, sum = 0.f, keep = 1.f;
+      // P of 32 keys: this thread's scores -> its columns of the region.
+      auto probabilities = [&](const uint32_t* s, int c, float shift) {
+        uint32_t p[C::kPParts][16];
 #pragma unroll
-      for (int c = 0; c < kKeys / 16; c++) {
-        tmem_wait_ld(s[c & 1]);
-        // After the last, the first again, for the second pass.
-        tmem_ld16(ts + (c + 1) % (kKeys / 16) * 16, s[(c + 1) & 1]);
-#pragma unroll
-        for (int j = 0; j < 16; j++)
-          if (keys == kKeys || c * 16 + j < keys) top = fmaxf(top, __uint_as_float(s[c & 1][j]));
-      }
-      const float next = fmaxf(m, top * scale);
-      const float shift = next == -INFINITY ? 0.f : next;
-      const float keep = next == -INFINITY ? 1.f : ex2(m - next);  // 0 before the first key
-      m = next;
-      float sum = 0.f;
-#pragma unroll
-      for (int c = 0; c < kKeys / 16; c++) {
-        tmem_wait_ld(s[c & 1]);
-        if (c + 1 < kKeys / 16) tmem_ld16(ts + (c + 1) * 16, s[(c + 1) & 1]);
-        uint32_t p[C::kPParts][8];
-#pragma unroll
-        for (int j = 0; j < 16; j += 2) {
-          float x0 = ex2(fmaf(__uint_as_float(s[c & 1][j]), scale, -shift));
-          float x1 = ex2(fmaf(__uint_as_float(s[c & 1][j + 1]), scale, -shift));
+        for (int j = 0; j < 32; j += 2) {
+          float x0 = ex2(fmaf(__uint_as_float(s[j]), scale, -shift));
+          float x1 = ex2(fmaf(__uint_as_float(s[j + 1]), scale, -shift));
           if (keys < kKeys) {
-            if (c * 16 + j >= keys) x0 = 0.f;
-            if (c * 16 + j + 1 >= keys) x1 = 0.f;
+            if (c * 32 + j >= keys) x0 = 0.f;
+            if (c * 32 + j + 1 >= keys) x1 = 0.f;
           }
           sum += x0 + x1;
           uint32_t e[C::kPParts];
@@ -556,67 +590,159 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
 #pragma unroll
           for (int y = 0; y < C::kPParts; y++) p[y][j / 2] = e[y];
         }
-        // The scores that these columns held have been read.
-        tmem_wait_ld(s[(c + 1) & 1]);
 #pragma unroll
         for (int y = 0; y < C::kPParts; y++)
-          tmem_st8(tp + (c / 2) * C::kPParts * 16 + y * 16 + (c % 2) * 8, p[y]);
+          tmem_st16(tp + (c * C::kPParts + y) * 16, p[y]);
+      };
+      auto largest = [&](const uint32_t* s, int c) {
+#pragma unroll
+        for (int j = 0; j < 32; j++)
+          if (keys == kKeys || c * 32 + j < keys) top = fmaxf(top, __uint_as_float(s[j]));
+      };
+      if constexpr (!kF32) {
+        uint32_t s[2][32];
+        tmem_ld32(ts, s[0]);
+        tmem_ld32(ts + 32, s[1]);
+        tmem_wait_ld32(s[0]);
+        tmem_wait_ld32(s[1]);
+        largest(s[0], 0);
+        largest(s[1], 1);
+        const float next = fmaxf(m, top * scale);
+        if (__any_sync(0xFFFFFFFFu, next > m + 8.f)) {
+          // m is what P and O are relative to. (The wait is for the last
+          // tile's product; this tile's scores say that the one before is
+          // complete, so the parity is not an older phase's.)
+          const float f = next == -INFINITY ? 1.f : ex2(m - next);
+          m = next;
+          l *= f;
+          if (i >= 2) {
+            ok = warp_wait(saddr(&o_full[w]), ((i - 2) >> 1) & 1, &failed);
+            if (!ok) break;
+            fence_after();
+#pragma unroll 1
+            for (int c = 0; c < HD / 16; c++) {
+              uint32_t x[16];
+              tmem_ld16(to + c * 16, x);
+              tmem_wait_ld(x);
+#pragma unroll
+              for (int j = 0; j < 16; j++) x[j] = __float_as_uint(__uint_as_float(x[j]) * f);
+              tmem_st16(to + c * 16, x);
+            }
+          }
+        }
+        const float shift = m == -INFINITY ? 0.f : m;
+        probabilities(s[0], 0, shift);
+        probabilities(s[1], 1, shift);
+      } else {
+        // The scores are read twice: with O in registers there is no room to
+        // keep them.
+        uint32_t s[32];
+        tmem_ld32(ts, s);
+        tmem_wait_ld32(s);
+        largest(s, 0);
+        tmem_ld32(ts + 32, s);
+        tmem_wait_ld32(s);
+        largest(s, 1);
+        const float next = fmaxf(m, top * scale);
+        keep = next == -INFINITY ? 1.f : ex2(m - next);  // 0 before the first key
+        m = next;
+        const float shift = next == -INFINITY ? 0.f : next;
+        tmem_ld32(ts, s);
+        tmem_wait_ld32(s);
+        probabilities(s, 0, shift);
+        tmem_ld32(ts + 32, s);
+        tmem_wait_ld32(s);
+        probabilities(s, 1, shift);
       }
       l = l * keep + sum;
       tmem_wait_st();
       fence_before();
       mbar_arrive(saddr(&p_full[b]));
-      if (!warp_wait(saddr(&o_full[w]), (i >> 1) & 1, &failed)) break;
-      fence_after();
-      tmem_ld16(to, s[0]);
+      if constexpr (kF32) {
+        ok = warp_wait(saddr(&o_full[w]), (i >> 1) & 1, &failed);
+        if (!ok) break;
+        fence_after();
 #pragma unroll
-      for (int c = 0; c < HD / 16; c++) {
-        tmem_wait_ld(s[c & 1]);
-        if (c + 1 < HD / 16) tmem_ld16(to + (c + 1) * 16, s[(c + 1) & 1]);
+        for (int c = 0; c < HD / 32; c++) {
+          uint32_t x[32];
+          tmem_ld32(to + c * 32, x);
+          tmem_wait_ld32(x);
 #pragma unroll
-        for (int j = 0; j < 16; j++)
-          o[c * 16 + j] = fmaf(o[c * 16 + j], keep, __uint_as_float(s[c & 1][j]));
+          for (int j = 0; j < 32; j++)
+            o[c * 32 + j] = fmaf(o[c * 32 + j], keep, __uint_as_float(x[j]));
+        }
+        fence_before();
+        mbar_arrive(saddr(&o_empty[w]));
       }
-      fence_before();
-      mbar_arrive(saddr(&o_empty[w]));
+    }
+    const bool any = nt > w;  // this warpgroup had a tile
+    if constexpr (!kF32) {
+      // The last product of this warpgroup, behind the one before (whose
+      // older phase has the last one's parity).
+      const int turn = (nt - 1 - w) >> 1;
+      if (ok && any && turn > 0) ok = warp_wait(saddr(&o_full[w]), (turn - 1) & 1, &failed);
+      if (ok && any) ok = warp_wait(saddr(&o_full[w]), turn & 1, &failed);
+      fence_after();
     }
     // A wait that ran out leaves NaN: no result passes for a complete one.
-    if (failed) l = o[0] = __int_as_float(0x7FC00000);
-    if (w == 1) ml[r] = make_float2(m, l);
-    // Both warpgroups are past their last matrix instruction: the operands'
-    // memory is free.
-    asm volatile("bar.sync 2, 256;" ::: "memory");
-    float* join = reinterpret_cast<float*>(gbase) + r * (HD + 4);
-    if (w == 1) {
+    if (failed || !ok) l = __int_as_float(0x7FC00000);
+    // 32 outputs of this thread's row.
+    auto outputs = [&](int c, float* x) {
+      if constexpr (kF32) {
 #pragma unroll
-      for (int i = 0; i < HD; i += 4)
-        *reinterpret_cast<float4*>(join + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        for (int j = 0; j < 32; j++) x[j] = o[c * 32 + j];
+      } else {
+        uint32_t y[32];
+        tmem_ld32(to + c * 32, y);
+        tmem_wait_ld32(y);
+#pragma unroll
+        for (int j = 0; j < 32; j++) x[j] = __uint_as_float(y[j]);
+      }
+    };
+    float* join = reinterpret_cast<float*>(gbase) + r * (HD + 4);
+    if (nt > 1) {
+      if (w == 1) ml[r] = make_float2(m, l);
+      // Both warpgroups are past their last matrix instruction: the operands'
+      // memory is free.
+      asm volatile("bar.sync 2, 256;" ::: "memory");
+      if (w == 1) {
+#pragma unroll
+        for (int c = 0; c < HD / 32; c++) {
+          float x[32];
+          outputs(c, x);
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<float4*>(join + c * 32 + j) =
+                make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+        }
+      }
+      asm volatile("bar.sync 2, 256;" ::: "memory");
     }
-    asm volatile("bar.sync 2, 256;" ::: "memory");
     if (w == 0) {
-      const float2 y = ml[r];
+      const float2 y = nt > 1 ? ml[r] : make_float2(-INFINITY, 0.f);
       const float both = fmaxf(m, y.x);
       const float f = both == -INFINITY ? 1.f : ex2(m - both);
       const float g = both == -INFINITY ? 1.f : ex2(y.x - both);
+      const size_t at = ((size_t)split * a.kh + head) * R + r0 + r;
+      if (r0 + r < R) a.ml[at] = make_float2(both, l * f + y.y * g);
 #pragma unroll
-      for (int i = 0; i < HD; i += 4) {
-        float4 v = *reinterpret_cast<float4*>(join + i);
-        v.x = fmaf(o[i], f, v.x * g);
-        v.y = fmaf(o[i + 1], f, v.y * g);
-        v.z = fmaf(o[i + 2], f, v.z * g);
-        v.w = fmaf(o[i + 3], f, v.w * g);
-        *reinterpret_cast<float4*>(join + i) = v;
+      for (int c = 0; c < HD / 32; c++) {
+        float x[32];
+        outputs(c, x);
+        float4* part = reinterpret_cast<float4*>(a.part + at * HD + c * 32);
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          float4 v = make_float4(x[j] * f, x[j + 1] * f, x[j + 2] * f, x[j + 3] * f);
+          if (nt > 1) {
+            const float4 z = *reinterpret_cast<const float4*>(join + c * 32 + j);
+            v.x = fmaf(z.x, g, v.x);
+            v.y = fmaf(z.y, g, v.y);
+            v.z = fmaf(z.z, g, v.z);
+            v.w = fmaf(z.w, g, v.w);
+          }
+          if (r0 + r < R) part[j / 4] = v;
+        }
       }
-      if (r0 + r < R)
-        a.ml[((size_t)split * a.kh + head) * R + r0 + r] = make_float2(both, l * f + y.y * g);
-    }
-    asm volatile("bar.sync 2, 256;" ::: "memory");
-    float* part = a.part + (((size_t)split * a.kh + head) * R + r0) * HD;
-    const int rows = min(kRows, R - r0);
-    for (int i = threadIdx.x; i < rows * (HD / 4); i += 256) {
-      const int rr = i / (HD / 4), c = i % (HD / 4);
-      reinterpret_cast<float4*>(part)[i] =
-          *reinterpret_cast<float4*>(reinterpret_cast<float*>(gbase) + rr * (HD + 4) + c * 4);
     }
     fence_before();
   }
