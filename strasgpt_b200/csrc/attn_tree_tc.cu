@@ -2,9 +2,9 @@
 //
 // A CTA has 128 rows (drafted token, q head) of one kv head and a share of
 // the cached keys, which all of its rows see. Sixteen warps: two warpgroups
-// of softmax, one thread per row, that take the key tiles in turn; one thread
-// that issues the matrix instructions; seven warps that bring in keys and
-// values. Per tile of 64 keys: S = Q K^T into tensor memory; its warpgroup
+// of softmax, one thread per row, that take the key tiles in turn; two warps
+// that issue the matrix instructions, one Q K^T and one P V, so that neither
+// waits for what the other waits for; six that bring in keys and values. Per tile of 64 keys: S = Q K^T into tensor memory; its warpgroup
 // reads S, subtracts the running maximum and writes P = 2^(S - m) over it, as
 // bf16 parts; then O (+)= P V in tensor memory. Each warpgroup has its own
 // maximum, sum and output, joined at the end, so that one's softmax runs
@@ -30,7 +30,11 @@
 // the softmax 11, matrix instructions 12 (bf16) or 48 (fp32's six products).
 #include "attn_tree.h"
 
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <math.h>
+
+#include <type_traits>
 
 namespace sg {
 namespace {
@@ -38,7 +42,7 @@ namespace {
 constexpr int kRows = kTreeTcRows;
 constexpr int kThreads = 512;
 constexpr int kKeys = 64;        // of a tile
-constexpr int kLoadWarps = 7;
+constexpr int kLoadWarps = 6;
 constexpr int kLoaders = 32 * kLoadWarps;
 constexpr unsigned long long kTimeoutNs = 2000000000ULL;
 
@@ -49,10 +53,10 @@ struct Tc {
   static constexpr int kPParts = kF32 ? 3 : 2;          // of the probabilities
   static constexpr int kPart = kKeys * HD * 2;          // bytes of a tile's part
   static constexpr int kTile = kParts * kPart;          // of K, or of V
-  // bf16: each loader warp has a stage. fp32: one, and rows on their way to
-  // parts in a ring of units of 32 keys.
-  static constexpr int kStages = kF32 ? 1 : kLoadWarps;
-  static constexpr int kLoaded = kF32 ? kLoaders : 32;  // arrivals per filled tile
+  // bf16: stages filled by TMA. fp32: one, and rows on their way to parts in
+  // a ring of units of 32 keys.
+  static constexpr int kStages = kF32 ? 1 : 7;
+  static constexpr int kLoaded = kF32 ? kLoaders : 1;  // arrivals per filled tile
   static constexpr int kUnitKeys = 32;
   static constexpr int kUnit = kUnitKeys * HD * 4;
   static constexpr int kRing = kF32 ? 8 : 0;
@@ -95,6 +99,28 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, unsigned count) {
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, unsigned bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+// 64 head entries (x a multiple of 64: 128 bytes) of 64 cache rows from `row`
+// on into a tile's panel.
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int x, int row,
+                                         int head, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(row), "r"(head), "r"(bar)
+      : "memory");
+}
+// `bytes` (a multiple of 16) as they are; both addresses 16-byte aligned.
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+          "r"(dst), "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
 }
 __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, unsigned parity) {
   unsigned ok;
@@ -279,13 +305,16 @@ __device__ __forceinline__ uint32_t at_sw128(int rows, int r, int c) {
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
+__global__ void __launch_bounds__(kThreads, 1)
+    k_tree_tc(TreeArgs a, const __grid_constant__ CUtensorMap k_map,
+              const __grid_constant__ CUtensorMap v_map) {
   using C = Tc<T, HD>;
   constexpr bool kF32 = C::kF32;
   constexpr int kStages = C::kStages;
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t k_full[kStages], k_empty[kStages], v_full[kStages],
-      v_empty[kStages], s_full[C::kSBuffers], p_full[C::kSBuffers], o_full[2], o_empty[2], done;
+      v_empty[kStages], s_full[C::kSBuffers], p_full[C::kSBuffers], s_empty[C::kSBuffers],
+      o_full[2], o_empty[2], raw_full[C::kRing ? C::kRing : 1], done;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int failed;
   __shared__ float2 ml[kRows];  // of the second warpgroup
@@ -313,12 +342,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
     for (int b = 0; b < C::kSBuffers; b++) {
       mbar_init(saddr(&s_full[b]), 1);
       mbar_init(saddr(&p_full[b]), 128);
+      mbar_init(saddr(&s_empty[b]), 1);
     }
     for (int w = 0; w < 2; w++) {
       mbar_init(saddr(&o_full[w]), 1);
       mbar_init(saddr(&o_empty[w]), 128);
     }
-    mbar_init(saddr(&done), 1);
+    for (int x = 0; x < C::kRing; x++) mbar_init(saddr(&raw_full[x]), 1);
+    mbar_init(saddr(&done), 2);
     failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -337,14 +368,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
   // 512 threads of 128 registers: 2 x 128 x 208 + 2 x 128 x 48 make as many.
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    const uint32_t one = elect();
     if (warp == 8) {
-      // Queries are there once the first warpgroup has written them.
+      // S of every tile. Queries are there once the first warpgroup has
+      // written them.
       asm volatile("bar.sync 3, 160;" ::: "memory");
       fence_after();
-      const uint32_t one = elect();
-      auto scores = [&](int i) {  // S of tile i
+#pragma unroll 1
+      for (int i = 0; i < nt; i++) {
         const int s = i % kStages, b = i % C::kSBuffers;
-        if (!warp_wait(saddr(&k_full[s]), (i / kStages) & 1, &failed)) return false;
+        // The region's last P has been multiplied.
+        if (i >= C::kSBuffers &&
+            !warp_wait(saddr(&s_empty[b]), (i / C::kSBuffers - 1) & 1, &failed))
+          break;
+        if (!warp_wait(saddr(&k_full[s]), (i / kStages) & 1, &failed)) break;
         fence_after();
         const uint64_t k0 = sw128(k_tile(s), 16);
         const uint32_t d = tmem + C::kColS + b * C::kRegion + C::kS;
@@ -359,20 +396,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
         }
         mma_commit(saddr(&s_full[b]), one);
         mma_commit(saddr(&k_empty[s]), one);
-        return true;
-      };
-      bool ok = true;
-      for (int i = 0; ok && i < C::kSBuffers && i < nt; i++) ok = scores(i);
-      for (int i = 0; ok && i < nt; i++) {
+      }
+      // Nothing issued here outlives the tensor memory.
+      mma_commit(saddr(&done), one);
+      mbar_drain(saddr(&done));
+      __syncwarp();
+    } else if (warp == 9) {
+      // O of every tile.
+#pragma unroll 1
+      for (int i = 0; i < nt; i++) {
         const int s = i % kStages, b = i % C::kSBuffers, w = i & 1, o = kF32 ? 0 : w;
         // fp32: the last product in these columns has been read. (O's barriers
         // go by warpgroup, so that who waits on one has seen all its phases.)
         const int last = i - 1;
-        ok = warp_wait(saddr(&p_full[b]), (i / C::kSBuffers) & 1, &failed) &&
-             warp_wait(saddr(&v_full[s]), (i / kStages) & 1, &failed) &&
-             (!kF32 || last < 0 ||
-              warp_wait(saddr(&o_empty[last & 1]), (last >> 1) & 1, &failed));
-        if (!ok) break;
+        if (!warp_wait(saddr(&p_full[b]), (i / C::kSBuffers) & 1, &failed) ||
+            !warp_wait(saddr(&v_full[s]), (i / kStages) & 1, &failed) ||
+            (kF32 && last >= 0 &&
+             !warp_wait(saddr(&o_empty[last & 1]), (last >> 1) & 1, &failed)))
+          break;
         fence_after();
         const uint64_t v0 = sw128(v_tile(s), kKeys * 128);
         const uint32_t d = tmem + C::kColO + o * HD, p0 = tmem + C::kColS + b * C::kRegion;
@@ -387,13 +428,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
                    x + k > 0 || (!kF32 && i >= 2), one);
         }
         mma_commit(saddr(&o_full[w]), one);
+        mma_commit(saddr(&s_empty[b]), one);
         mma_commit(saddr(&v_empty[s]), one);
-        // The next scores in this region overwrite the P that this product
-        // reads.
-        if (i + C::kSBuffers < nt)
-          ok = warp_wait(saddr(&o_full[w]), (i >> 1) & 1, &failed) && scores(i + C::kSBuffers);
       }
-      // Nothing issued here outlives the tensor memory.
       mma_commit(saddr(&done), one);
       mbar_drain(saddr(&done));
       __syncwarp();
@@ -401,40 +438,53 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
       const T* kbase = static_cast<const T*>(a.k) + (size_t)head * a.ctx * HD;
       const T* vbase = static_cast<const T*>(a.v) + (size_t)head * a.ctx * HD;
       if constexpr (!kF32) {
-        // Each loader warp has one of the stages: it waits for what it copied
-        // without holding up the others.
-        const int s = warp - 9;
-        for (int i = s; i < nt; i += kStages) {
-          const unsigned turn = (unsigned)(i / kStages);
-          const int row = (tile0 + i) * kKeys, rows = min(kKeys, n - row);
-          auto copy = [&](const T* from, uint32_t to) {
-#pragma unroll 8
-            for (int x = lane; x < kKeys * (HD / 8); x += 32) {
-              const int r = x / (HD / 8), c = x % (HD / 8);
-              const bool in = r < rows;  // zeros behind the last key
-              cp_async16(to + at_sw128(kKeys, r, c),
-                         from + (size_t)(in ? row + r : 0) * HD + c * 8, in ? 16 : 0);
+        // One warp for the keys, one for the values.
+        auto load = [&](const CUtensorMap* map, const T* from, bool is_v, uint64_t* full,
+                        uint64_t* empty) {
+#pragma unroll 1
+          for (int i = 0; i < nt; i++) {
+            const int s = i % kStages, row = (tile0 + i) * kKeys, rows = min(kKeys, n - row);
+            const uint32_t to = is_v ? v_tile(s) : k_tile(s);
+            if (i >= kStages && !warp_wait(saddr(&empty[s]), (i / kStages - 1) & 1, &failed))
+              break;
+            if (rows == kKeys) {
+              if (one) {
+                mbar_expect_tx(saddr(&full[s]), C::kPart);
+#pragma unroll
+                for (int p = 0; p < HD / 64; p++)
+                  tma_rows(to + p * kKeys * 128, map, p * 64, row, head, saddr(&full[s]));
+              }
+            } else {
+              // The last tile: rows behind the last cached key are zeros and
+              // not what the cache has there.
+#pragma unroll 4
+              for (int x = lane; x < kKeys * (HD / 8); x += 32) {
+                const int r = x / (HD / 8), c = x % (HD / 8);
+                const bool in = r < rows;
+                cp_async16(to + at_sw128(kKeys, r, c),
+                           from + (size_t)(in ? row + r : 0) * HD + c * 8, in ? 16 : 0);
+              }
+              cp_async_commit();
+              cp_async_wait<0>();
+              fence_operands();
+              __syncwarp();
+              if (one) mbar_arrive(saddr(&full[s]));
             }
-            cp_async_commit();
-          };
-          if (turn && !warp_wait(saddr(&k_empty[s]), (turn - 1) & 1, &failed)) break;
-          copy(kbase, k_tile(s));
-          if (turn && !warp_wait(saddr(&v_empty[s]), (turn - 1) & 1, &failed)) break;
-          copy(vbase, v_tile(s));
-          cp_async_wait<1>();
-          fence_operands();
-          mbar_arrive(saddr(&k_full[s]));
-          cp_async_wait<0>();
-          fence_operands();
-          mbar_arrive(saddr(&v_full[s]));
-        }
-        cp_async_wait<0>();
+            __syncwarp();
+          }
+          // Nothing is on its way when the CTA ends: every tile that was asked
+          // for is waited for here (or by the matrix instructions before).
+          if (failed)
+            for (int s = 0; s < kStages && s < nt; s++) mbar_drain(saddr(&full[s]));
+        };
+        if (warp == 10) load(&k_map, kbase, false, k_full, k_empty);
+        if (warp == 11) load(&v_map, vbase, true, v_full, v_empty);
       } else {
         // Half tiles in the order of their use: K of tile 0, then K of tile
-        // i + 1 and V of tile i. Rows of the next kRing - 1 units stream into
-        // the ring while this one's become parts.
+        // i + 1 and V of tile i. Rows of the next kRing units stream into the
+        // ring while this one's become parts.
         constexpr int kRing = C::kRing, kUnitKeys = C::kUnitKeys;
-        const int id = threadIdx.x - 288, units = 4 * nt;
+        const int id = threadIdx.x - 320, units = 4 * nt;
         const uint32_t ring = base + kStages * 2 * C::kTile;
         // Tile of unit u, whether it is of V; its half is u & 1.
         auto unit = [&](int u, bool& is_v) {
@@ -444,45 +494,45 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
           is_v = !(x & 1);
           return is_v ? x / 2 - 1 : (x + 1) / 2;
         };
-        auto fetch = [&](int u) {
-          if (u < units) {
-            bool is_v;
-            const int row = (tile0 + unit(u, is_v)) * kKeys + (u & 1) * kUnitKeys;
-            const int rows = min(kUnitKeys, n - row);
-            const T* from = is_v ? vbase : kbase;
-            const uint32_t to = ring + (u % kRing) * C::kUnit;
-#pragma unroll 4
-            for (int x = id; x < kUnitKeys * (HD / 4); x += kLoaders) {
-              const int r = x / (HD / 4), c = x % (HD / 4);
-              const bool in = r < rows;  // zeros behind the last key
-              cp_async16(to + x * 16, from + (size_t)(in ? row + r : 0) * HD + c * 4, in ? 16 : 0);
-            }
-          }
-          cp_async_commit();
+        auto rows_of = [&](int u, bool& is_v, int& row) {
+          row = (tile0 + unit(u, is_v)) * kKeys + (u & 1) * kUnitKeys;
+          return max(0, min(kUnitKeys, n - row));
         };
-#pragma unroll 1
-        for (int u = 0; u < kRing - 1; u++) fetch(u);
+        auto fetch = [&](int u) {
+          bool is_v;
+          int row;
+          const int rows = u < units ? rows_of(u, is_v, row) : 0;
+          if (rows == 0) return;
+          const uint32_t bar = saddr(&raw_full[u % kRing]), bytes = rows * HD * 4;
+          mbar_expect_tx(bar, bytes);
+          bulk_copy(ring + (u % kRing) * C::kUnit, (is_v ? vbase : kbase) + (size_t)row * HD, bytes,
+                    bar);
+        };
+        if (id == 0)
+          for (int u = 0; u < kRing; u++) fetch(u);
         bool ok = true;
 #pragma unroll 1
         for (int u = 0; u < units; u++) {
           bool is_v;
-          const int i = unit(u, is_v), half = u & 1;
-          cp_async_wait<kRing - 2>();
-          // All loaders' copies of this unit have landed, and all are done
-          // with the buffer that the next fetch fills.
-          asm volatile("bar.sync 1, %0;" ::"n"(kLoaders) : "memory");
-          fetch(u + kRing - 1);
+          int row;
+          const int rows = rows_of(u, is_v, row), i = unit(u, is_v), half = u & 1;
           // (A wait that ran out leaves nothing to do but to stay in step.)
+          if (rows) ok = ok && warp_wait(saddr(&raw_full[u % kRing]), (u / kRing) & 1, &failed);
           if (half == 0 && i > 0)
             ok = ok && warp_wait(saddr(is_v ? &v_empty[0] : &k_empty[0]), (i - 1) & 1, &failed);
           if (ok) {
             const uint8_t* from = gbase + (ring - base) + (u % kRing) * C::kUnit;
             uint8_t* to = gbase + (is_v ? C::kTile : 0);
-#pragma unroll 2
-            for (int x = id; x < kUnitKeys * (HD / 8); x += kLoaders) {
-              const int r = x / (HD / 8), c = x % (HD / 8);
-              const float4 f = *reinterpret_cast<const float4*>(from + x * 32);
-              const float4 g = *reinterpret_cast<const float4*>(from + x * 32 + 16);
+            constexpr int kItems = kUnitKeys * (HD / 8);
+#pragma unroll
+            for (int y = 0; y < (kItems + kLoaders - 1) / kLoaders; y++) {
+              const int x = id + y * kLoaders, r = x / (HD / 8), c = x % (HD / 8);
+              if (x >= kItems) break;
+              float4 f = make_float4(0.f, 0.f, 0.f, 0.f), g = f;
+              if (r < rows) {  // zeros behind the last key
+                f = *reinterpret_cast<const float4*>(from + x * 32);
+                g = *reinterpret_cast<const float4*>(from + x * 32 + 16);
+              }
               float e[8] = {f.x, f.y, f.z, f.w, g.x, g.y, g.z, g.w};
               uint8_t* at = to + at_sw128(kKeys, half * kUnitKeys + r, c);
 #pragma unroll
@@ -499,8 +549,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
               mbar_arrive(saddr(is_v ? &v_full[0] : &k_full[0]));
             }
           }
+          // All loaders are done with the unit's buffer.
+          asm volatile("bar.sync 1, %0;" ::"n"(kLoaders) : "memory");
+          if (id == 0 && ok) fetch(u + kRing);
         }
-        cp_async_wait<0>();
+        // After a failure units may still be on their way: their memory is
+        // this CTA's until they have landed.
+        if (failed && id == 0) {
+          const unsigned long long t0 = now_ns();
+          while (now_ns() - t0 < 10000000ULL) {
+          }
+        }
       }
     }
   } else {
@@ -574,13 +633,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
       fence_after();
       float top = -INFINITY, sum = 0.f, keep = 1.f;
       // P of 32 keys: this thread's scores -> its columns of the region.
-      auto probabilities = [&](const uint32_t* s, int c, float shift) {
+      // `all`: none of the tile's keys is behind the last.
+      auto probabilities = [&](const uint32_t* s, int c, float shift, auto all) {
         uint32_t p[C::kPParts][16];
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
           float x0 = ex2(fmaf(__uint_as_float(s[j]), scale, -shift));
           float x1 = ex2(fmaf(__uint_as_float(s[j + 1]), scale, -shift));
-          if (keys < kKeys) {
+          if constexpr (!decltype(all)::value) {
             if (c * 32 + j >= keys) x0 = 0.f;
             if (c * 32 + j + 1 >= keys) x1 = 0.f;
           }
@@ -594,19 +654,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
         for (int y = 0; y < C::kPParts; y++)
           tmem_st16(tp + (c * C::kPParts + y) * 16, p[y]);
       };
-      auto largest = [&](const uint32_t* s, int c) {
+      auto largest = [&](const uint32_t* s, int c, auto all) {
 #pragma unroll
         for (int j = 0; j < 32; j++)
-          if (keys == kKeys || c * 32 + j < keys) top = fmaxf(top, __uint_as_float(s[j]));
+          if (decltype(all)::value || c * 32 + j < keys) top = fmaxf(top, __uint_as_float(s[j]));
       };
+      const std::true_type full;
+      const std::false_type part;
+      const bool whole = keys == kKeys;
       if constexpr (!kF32) {
         uint32_t s[2][32];
         tmem_ld32(ts, s[0]);
         tmem_ld32(ts + 32, s[1]);
         tmem_wait_ld32(s[0]);
         tmem_wait_ld32(s[1]);
-        largest(s[0], 0);
-        largest(s[1], 1);
+        if (whole) {
+          largest(s[0], 0, full);
+          largest(s[1], 1, full);
+        } else {
+          largest(s[0], 0, part);
+          largest(s[1], 1, part);
+        }
         const float next = fmaxf(m, top * scale);
         if (__any_sync(0xFFFFFFFFu, next > m + 8.f)) {
           // m is what P and O are relative to. (The wait is for the last
@@ -631,28 +699,39 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
           }
         }
         const float shift = m == -INFINITY ? 0.f : m;
-        probabilities(s[0], 0, shift);
-        probabilities(s[1], 1, shift);
+        if (whole) {
+          probabilities(s[0], 0, shift, full);
+          probabilities(s[1], 1, shift, full);
+        } else {
+          probabilities(s[0], 0, shift, part);
+          probabilities(s[1], 1, shift, part);
+        }
       } else {
         // The scores are read twice: with O in registers there is no room to
         // keep them.
         uint32_t s[32];
-        tmem_ld32(ts, s);
-        tmem_wait_ld32(s);
-        largest(s, 0);
-        tmem_ld32(ts + 32, s);
-        tmem_wait_ld32(s);
-        largest(s, 1);
-        const float next = fmaxf(m, top * scale);
-        keep = next == -INFINITY ? 1.f : ex2(m - next);  // 0 before the first key
-        m = next;
-        const float shift = next == -INFINITY ? 0.f : next;
-        tmem_ld32(ts, s);
-        tmem_wait_ld32(s);
-        probabilities(s, 0, shift);
-        tmem_ld32(ts + 32, s);
-        tmem_wait_ld32(s);
-        probabilities(s, 1, shift);
+        auto tile = [&](auto all) {
+          tmem_ld32(ts, s);
+          tmem_wait_ld32(s);
+          largest(s, 0, all);
+          tmem_ld32(ts + 32, s);
+          tmem_wait_ld32(s);
+          largest(s, 1, all);
+          const float next = fmaxf(m, top * scale);
+          keep = next == -INFINITY ? 1.f : ex2(m - next);  // 0 before the first key
+          m = next;
+          const float shift = next == -INFINITY ? 0.f : next;
+          tmem_ld32(ts, s);
+          tmem_wait_ld32(s);
+          probabilities(s, 0, shift, all);
+          tmem_ld32(ts + 32, s);
+          tmem_wait_ld32(s);
+          probabilities(s, 1, shift, all);
+        };
+        if (whole)
+          tile(full);
+        else
+          tile(part);
       }
       l = l * keep + sum;
       tmem_wait_st();
@@ -754,15 +833,48 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_tc(TreeArgs a) {
   }
 }
 
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static std::atomic<void*> known;
+  void* fn = known.load(std::memory_order_relaxed);
+  if (!fn) {
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) !=
+            cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return nullptr;
+    known.store(fn, std::memory_order_relaxed);
+  }
+  return (PFN_cuTensorMapEncodeTiled_v12000)fn;
+}
+
+// Map of a bf16 cache [kh][ctx][hd]: boxes of 64 entries of 64 rows.
+cudaError_t cache_map(CUtensorMap* map, const void* base, int kh, int ctx, int hd) {
+  const auto encode = encode_fn();
+  if (!encode) return cudaErrorNotSupported;
+  const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)ctx, (cuuint64_t)kh};
+  const cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)ctx * hd * 2};
+  const cuuint32_t box[3] = {64, kKeys, 1}, step[3] = {1, 1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims,
+                            strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 template <typename T, int HD>
 cudaError_t launch_tc(const TreeArgs& a, int dev, cudaStream_t s) {
   static std::atomic<size_t> allowed[kDevices];
   constexpr size_t bytes = Tc<T, HD>::kBytes;
-  const cudaError_t e = allow_smem(k_tree_tc<T, HD>, bytes, dev, allowed);
+  cudaError_t e = allow_smem(k_tree_tc<T, HD>, bytes, dev, allowed);
   if (e != cudaSuccess) return e;
+  CUtensorMap k = {}, v = {};
+  if (!Tc<T, HD>::kF32) {
+    if ((e = cache_map(&k, a.k, a.kh, a.ctx, HD)) != cudaSuccess) return e;
+    if ((e = cache_map(&v, a.v, a.kh, a.ctx, HD)) != cudaSuccess) return e;
+  }
   const int rows = a.t * a.group;
   return try_launch(k_tree_tc<T, HD>, dim3(a.splits, a.kh, (rows + kRows - 1) / kRows),
-                    dim3(kThreads), bytes, 1, s, a);
+                    dim3(kThreads), bytes, 1, s, a, k, v);
 }
 
 }  // namespace
