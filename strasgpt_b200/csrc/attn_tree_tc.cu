@@ -54,23 +54,26 @@ struct Tc {
   static constexpr int kPart = kKeys * HD * 2;          // bytes of a tile's part
   static constexpr int kTile = kParts * kPart;          // of K, or of V
   // bf16: stages filled by TMA. fp32: one, and rows on their way to parts in
-  // a ring of units of 32 keys.
-  static constexpr int kStages = kF32 ? 1 : 7;
+  // a ring of units, a tile's keys or values.
+  static constexpr int kStages = kF32 ? 1 : HD == 128 ? 6 : 8;
   static constexpr int kLoaded = kF32 ? kLoaders : 1;  // arrivals per filled tile
-  static constexpr int kUnitKeys = 32;
-  static constexpr int kUnit = kUnitKeys * HD * 4;
-  static constexpr int kRing = kF32 ? 8 : 0;
+  static constexpr int kUnit = kKeys * HD * 4;
+  static constexpr int kRing = kF32 ? 4 : 0;
   static constexpr int kJoin = kRows * (HD + 4) * 4;    // the warpgroups' join
-  static constexpr int kOperands = kStages * 2 * kTile + kRing * kUnit;
+  // Where Q has no room in tensor memory beside four regions of scores (bf16,
+  // 128 entries) it lies in shared memory.
+  static constexpr bool kQShared = !kF32 && HD == 128;
+  static constexpr int kQ = kQShared ? kRows * HD * 2 : 0;
+  static constexpr int kOperands = kStages * 2 * kTile + kRing * kUnit + kQ;
   static constexpr int kUsed = (kOperands > kJoin ? kOperands : kJoin) + 1024;
   // At least half of an SM's: the CTA has all of the SM's tensor memory.
   static constexpr int kBytes = kUsed > 120 * 1024 ? kUsed : 120 * 1024;
   // Tensor memory columns: Q; regions of S and then P (in an fp32 region S
   // starts at column 32: P's parts of 16 keys, which overwrite it from the
   // start, reach no scores that are still to be read); O.
-  static constexpr int kSBuffers = kF32 ? 2 : 3, kOBuffers = kF32 ? 1 : 2;
+  static constexpr int kSBuffers = kF32 ? 2 : 4, kOBuffers = kF32 ? 1 : 2;
   static constexpr uint32_t kRegion = kF32 ? 96 : 64, kS = kF32 ? 32 : 0;
-  static constexpr uint32_t kColS = kParts * HD / 2;
+  static constexpr uint32_t kColS = kQShared ? 0 : kParts * HD / 2;
   static constexpr uint32_t kColO = kColS + kSBuffers * kRegion;
   static_assert(kColO + kOBuffers * HD <= 512, "tensor memory has 512 columns");
   // Instruction descriptors: fp32 sums of bf16, M = 128; S: N = keys, K
@@ -183,7 +186,15 @@ __device__ __forceinline__ uint32_t elect() {
       : "=r"(one));
   return one;
 }
-// D (+)= A B, A in tensor memory.
+// D (+)= A B, A in shared memory; in tensor memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       bool add, uint32_t issue) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(issue)
+      : "memory");
+}
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
                                        bool add, uint32_t issue) {
   asm volatile(
@@ -314,7 +325,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t k_full[kStages], k_empty[kStages], v_full[kStages],
       v_empty[kStages], s_full[C::kSBuffers], p_full[C::kSBuffers], s_empty[C::kSBuffers],
-      o_full[2], o_empty[2], raw_full[C::kRing ? C::kRing : 1], done;
+      o_full[2], o_empty[2], raw_full[C::kRing ? C::kRing : 1],
+      raw_empty[C::kRing ? C::kRing : 1], done;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int failed;
   __shared__ float2 ml[kRows];  // of the second warpgroup
@@ -323,6 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* const gbase = raw + (base - saddr(raw));
   auto k_tile = [&](int s) { return base + s * 2 * C::kTile; };
   auto v_tile = [&](int s) { return base + s * 2 * C::kTile + C::kTile; };
+  const uint32_t q_at = base + kStages * 2 * C::kTile;
   const int split = blockIdx.x, head = blockIdx.y, r0 = blockIdx.z * kRows;
   const int R = a.t * a.group;
   pdl_trigger();
@@ -348,7 +361,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(saddr(&o_full[w]), 1);
       mbar_init(saddr(&o_empty[w]), 128);
     }
-    for (int x = 0; x < C::kRing; x++) mbar_init(saddr(&raw_full[x]), 1);
+    for (int x = 0; x < C::kRing; x++) {
+      mbar_init(saddr(&raw_full[x]), 1);
+      mbar_init(saddr(&raw_empty[x]), kLoaders);
+    }
     mbar_init(saddr(&done), 2);
     failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -383,16 +399,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         if (!warp_wait(saddr(&k_full[s]), (i / kStages) & 1, &failed)) break;
         fence_after();
-        const uint64_t k0 = sw128(k_tile(s), 16);
+        const uint64_t k0 = sw128(k_tile(s), 16), q0 = sw128(q_at, 16);
         const uint32_t d = tmem + C::kColS + b * C::kRegion + C::kS;
 #pragma unroll
         for (int x = 0; x < (kF32 ? 6 : 1); x++) {
           const int pq = kF32 ? part_a(x) : 0, pk = kF32 ? part_b(x) : 0;
 #pragma unroll
-          for (int k = 0; k < HD / 16; k++)
-            mma_ts(d, tmem + pq * (HD / 2) + k * 8,
-                   k0 + ((pk * C::kPart + (k / 4) * kKeys * 128 + (k % 4) * 32) >> 4), C::kDescS,
-                   x + k > 0, one);
+          for (int k = 0; k < HD / 16; k++) {
+            const uint64_t kd = k0 + ((pk * C::kPart + (k / 4) * kKeys * 128 + (k % 4) * 32) >> 4);
+            if constexpr (C::kQShared)
+              mma_ss(d, q0 + (((k / 4) * kRows * 128 + (k % 4) * 32) >> 4), kd, C::kDescS,
+                     x + k > 0, one);
+            else
+              mma_ts(d, tmem + pq * (HD / 2) + k * 8, kd, C::kDescS, x + k > 0, one);
+          }
         }
         mma_commit(saddr(&s_full[b]), one);
         mma_commit(saddr(&k_empty[s]), one);
@@ -480,30 +500,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (warp == 10) load(&k_map, kbase, false, k_full, k_empty);
         if (warp == 11) load(&v_map, vbase, true, v_full, v_empty);
       } else {
-        // Half tiles in the order of their use: K of tile 0, then K of tile
-        // i + 1 and V of tile i. Rows of the next kRing units stream into the
-        // ring while this one's become parts.
-        constexpr int kRing = C::kRing, kUnitKeys = C::kUnitKeys;
-        const int id = threadIdx.x - 320, units = 4 * nt;
+        // Units in the order of their use: K of tile 0, then K of tile i + 1
+        // and V of tile i. The rows of the next kRing stream into the ring
+        // while this one's become parts.
+        constexpr int kRing = C::kRing;
+        const int id = threadIdx.x - 320, units = 2 * nt;
         const uint32_t ring = base + kStages * 2 * C::kTile;
-        // Tile of unit u, whether it is of V; its half is u & 1.
+        // Tile of unit u, and whether it is of V.
         auto unit = [&](int u, bool& is_v) {
-          const int x = u >> 1;  // K0, K1, V0, K2, V1, ..., V of the last
-          if (x == 0) { is_v = false; return 0; }
-          if (x == 2 * nt - 1) { is_v = true; return nt - 1; }
-          is_v = !(x & 1);
-          return is_v ? x / 2 - 1 : (x + 1) / 2;
-        };
-        auto rows_of = [&](int u, bool& is_v, int& row) {
-          row = (tile0 + unit(u, is_v)) * kKeys + (u & 1) * kUnitKeys;
-          return max(0, min(kUnitKeys, n - row));
+          is_v = u > 0 && (!(u & 1) || u == units - 1);
+          return u == 0 ? 0 : u == units - 1 ? nt - 1 : is_v ? u / 2 - 1 : (u + 1) / 2;
         };
         auto fetch = [&](int u) {
+          if (u >= units) return;
           bool is_v;
-          int row;
-          const int rows = u < units ? rows_of(u, is_v, row) : 0;
-          if (rows == 0) return;
-          const uint32_t bar = saddr(&raw_full[u % kRing]), bytes = rows * HD * 4;
+          const int row = (tile0 + unit(u, is_v)) * kKeys;
+          const uint32_t bar = saddr(&raw_full[u % kRing]), bytes = min(kKeys, n - row) * HD * 4;
           mbar_expect_tx(bar, bytes);
           bulk_copy(ring + (u % kRing) * C::kUnit, (is_v ? vbase : kbase) + (size_t)row * HD, bytes,
                     bar);
@@ -514,27 +526,24 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int u = 0; u < units; u++) {
           bool is_v;
-          int row;
-          const int rows = rows_of(u, is_v, row), i = unit(u, is_v), half = u & 1;
+          const int i = unit(u, is_v), rows = min(kKeys, n - (tile0 + i) * kKeys);
           // (A wait that ran out leaves nothing to do but to stay in step.)
-          if (rows) ok = ok && warp_wait(saddr(&raw_full[u % kRing]), (u / kRing) & 1, &failed);
-          if (half == 0 && i > 0)
-            ok = ok && warp_wait(saddr(is_v ? &v_empty[0] : &k_empty[0]), (i - 1) & 1, &failed);
+          ok = ok && warp_wait(saddr(&raw_full[u % kRing]), (u / kRing) & 1, &failed) &&
+               (i == 0 || warp_wait(saddr(is_v ? &v_empty[0] : &k_empty[0]), (i - 1) & 1, &failed));
           if (ok) {
             const uint8_t* from = gbase + (ring - base) + (u % kRing) * C::kUnit;
             uint8_t* to = gbase + (is_v ? C::kTile : 0);
-            constexpr int kItems = kUnitKeys * (HD / 8);
-#pragma unroll
-            for (int y = 0; y < (kItems + kLoaders - 1) / kLoaders; y++) {
-              const int x = id + y * kLoaders, r = x / (HD / 8), c = x % (HD / 8);
-              if (x >= kItems) break;
+            constexpr int kItems = kKeys * (HD / 8);
+#pragma unroll 3
+            for (int x = id; x < kItems; x += kLoaders) {
+              const int r = x / (HD / 8), c = x % (HD / 8);
               float4 f = make_float4(0.f, 0.f, 0.f, 0.f), g = f;
               if (r < rows) {  // zeros behind the last key
                 f = *reinterpret_cast<const float4*>(from + x * 32);
                 g = *reinterpret_cast<const float4*>(from + x * 32 + 16);
               }
               float e[8] = {f.x, f.y, f.z, f.w, g.x, g.y, g.z, g.w};
-              uint8_t* at = to + at_sw128(kKeys, half * kUnitKeys + r, c);
+              uint8_t* at = to + at_sw128(kKeys, r, c);
 #pragma unroll
               for (int p = 0; p < 3; p++) {
                 *reinterpret_cast<uint4*>(at + p * C::kPart) =
@@ -544,14 +553,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int j = 0; j < 8; j++) e[j] = rest(e[j]);
               }
             }
-            if (half) {
-              fence_operands();
-              mbar_arrive(saddr(is_v ? &v_full[0] : &k_full[0]));
-            }
+            fence_operands();
+            mbar_arrive(saddr(is_v ? &v_full[0] : &k_full[0]));
           }
-          // All loaders are done with the unit's buffer.
-          asm volatile("bar.sync 1, %0;" ::"n"(kLoaders) : "memory");
-          if (id == 0 && ok) fetch(u + kRing);
+          mbar_arrive(saddr(&raw_empty[u % kRing]));
+          // The first warp refills the buffer of the unit before, which the
+          // others are done with by now as a rule.
+          if (warp == 10 && u > 0 && u - 1 + kRing < units) {
+            ok = ok && warp_wait(saddr(&raw_empty[(u - 1) % kRing]), ((u - 1) / kRing) & 1,
+                                 &failed);
+            if (id == 0 && ok) fetch(u - 1 + kRing);
+            __syncwarp();
+          }
         }
         // After a failure units may still be on their way: their memory is
         // this CTA's until they have landed.
@@ -568,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int w = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     if (w == 0) {
-      // Queries into tensor memory, zeros for rows behind the last.
+      // Queries into tensor (or shared) memory, zeros for rows behind the last.
       const int row = r0 + r, tok = row < R ? row / a.group : 0;
       const T* q = static_cast<const T*>(a.q) + tok * a.ldq +
                    (size_t)(head * a.group + (row < R ? row - tok * a.group : 0)) * HD;
@@ -580,6 +593,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < kBatch; j++) {
           x[j] = reinterpret_cast<const uint4*>(q)[c * kBatch + j];
           if (row >= R) x[j] = make_uint4(0, 0, 0, 0);
+        }
+        if constexpr (C::kQShared) {
+#pragma unroll
+          for (int j = 0; j < kBatch; j++)
+            *reinterpret_cast<uint4*>(gbase + (q_at - base) + at_sw128(kRows, r, c * kBatch + j)) =
+                x[j];
+          continue;
         }
 #pragma unroll
         for (int h = 0; h < kBatch * kVec / 16; h++) {  // 16 entries, 8 columns a part
@@ -612,8 +632,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_st8(lanes + p * (HD / 2) + (c * kBatch * kVec / 16 + h) * 8, e[p]);
         }
       }
-      tmem_wait_st();
-      fence_before();
+      if constexpr (C::kQShared) {
+        fence_operands();
+      } else {
+        tmem_wait_st();
+        fence_before();
+      }
       asm volatile("bar.arrive 3, 160;" ::: "memory");
     }
     // Scores in units of log2, so that the softmax is exp2.
