@@ -552,30 +552,35 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Tree
   }
 }
 
-// One warp joins the parts of one row: outputs and sums of all parts, each
-// scaled to their common maximum. Four groups of eight lanes take the parts
-// in turn, a lane having HD / 8 entries of the head.
+// A block joins the parts of one row: sixteen groups of eight lanes, a lane
+// having HD / 8 entries of the head, take the parts in turn, each with a
+// running maximum of its own, so that a row's loads are all on their way at
+// once; then the groups are joined.
 //
 // DRAFTED: the parts have the cached keys only. The drafted ones that the row
-// sees, its ancestors in the tree and itself, come first, a group per key
-// with a running softmax of its own: a few keys as a rule, for which a matrix
-// tile would be nearly empty, and rows it does not see are not even read.
+// sees, its ancestors in the tree and itself, come first, a group per key: a
+// few keys as a rule, for which a matrix tile would be nearly empty, and rows
+// it does not see are not even read.
+constexpr int kMergeThreads = 128, kMergeGroups = kMergeThreads / 8;
+
 template <typename T, int HD, bool DRAFTED>
-__global__ void __launch_bounds__(128) k_merge(TreeArgs a, int keys_per_tile) {
+__global__ void __launch_bounds__(kMergeThreads) k_merge(TreeArgs a, int keys_per_tile) {
   constexpr int V = HD / 8;  // entries per lane
   constexpr bool kF32 = sizeof(T) == 4;
-  const int lane = threadIdx.x & 31, group = lane >> 3, e0 = (lane & 7) * V;
-  const int R = a.t * a.group, row = blockIdx.x * 4 + (threadIdx.x >> 5);
+  __shared__ float warp_o[kMergeThreads / 32][HD];
+  __shared__ float2 warp_ml[kMergeThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int group = threadIdx.x >> 3, e0 = (threadIdx.x & 7) * V;
+  const int R = a.t * a.group, row = blockIdx.x;
   sg::pdl_trigger();
   sg::pdl_wait();
-  if (row >= R * a.kh) return;
   const int n = sg::tree_cached(a);
   const int tiles = (n + keys_per_tile - 1) / keys_per_tile +
                     (DRAFTED ? 0 : (a.t + keys_per_tile - 1) / keys_per_tile);
   const int per = (tiles + a.splits - 1) / a.splits;
   const int parts = tiles ? (tiles + per - 1) / per : 0;
   const int head = row / R, r = row - head * R, tok = r / a.group;
-  const size_t at = (size_t)(head * a.group + r - tok * a.group) * HD + e0;
+  const size_t at = (size_t)(head * a.group + r - tok * a.group) * HD;
   auto read = [&](const T* p, float* x) {
     if constexpr (kF32) {
 #pragma unroll
@@ -595,96 +600,107 @@ __global__ void __launch_bounds__(128) k_merge(TreeArgs a, int keys_per_tile) {
   float m = -INFINITY, l = 0.f, o[V];
 #pragma unroll
   for (int i = 0; i < V; i++) o[i] = 0.f;
+  // Adds outputs x with maximum and sum (m2, l2).
+  auto join = [&](float m2, float l2, const float* x) {
+    const float next = fmaxf(m, m2);
+    const float f = next == -INFINITY ? 1.f : exp2f(m - next);
+    const float g = next == -INFINITY ? 1.f : exp2f(m2 - next);
+    m = next;
+    l = l * f + l2 * g;
+#pragma unroll
+    for (int i = 0; i < V; i++) o[i] = fmaf(x[i], g, o[i] * f);
+  };
   if constexpr (DRAFTED) {
     const float scale = 1.4426950408889634f / sqrtf((float)HD);
     float q[V];
-    read(static_cast<const T*>(a.q) + tok * a.ldq + at, q);
+    read(static_cast<const T*>(a.q) + tok * a.ldq + at + e0, q);
 #pragma unroll
     for (int i = 0; i < V; i++) q[i] *= scale;
     const size_t base = ((size_t)head * a.ctx + n) * HD + e0;
     const T* k = static_cast<const T*>(a.k) + base;
     const T* v = static_cast<const T*>(a.v) + base;
+    int seen = 0;  // keys in the words before
     for (int w = 0; w < a.words; w++) {
       u64 bits = a.mask[(size_t)tok * a.words + w];
       if (a.t - 64 * w < 64) bits &= (1ull << (a.t - 64 * w)) - 1;
-      while (bits) {
-        // The next four keys, one per group (fewer at the end).
-        int j = -1;
-#pragma unroll
-        for (int g = 0; g < 4; g++) {
-          const int next = bits ? __ffsll((long long)bits) - 1 : -1;
-          bits &= bits - 1;
-          if (g == group) j = next;
+      // This group's keys: those whose number among the row's is the group's,
+      // modulo the groups. (Lanes of a warp come out of the loop together.)
+      const int count = __popcll(bits);
+      int mine = (group - seen % kMergeGroups + kMergeGroups) % kMergeGroups;
+      seen += count;
+      for (int first = 0; first < count; first += kMergeGroups, mine += kMergeGroups) {
+        const bool in = mine < count;
+        int j = 0;
+        if (in) {  // the mine-th set bit
+          u64 b = bits;
+          for (int x = 0; x < mine; x++) b &= b - 1;
+          j = 64 * w + __ffsll((long long)b) - 1;
         }
         float x[V], s = 0.f;
-        if (j >= 0) {
-          read(k + (size_t)(64 * w + j) * HD, x);
+        if (in) {
+          read(k + (size_t)j * HD, x);
 #pragma unroll
           for (int i = 0; i < V; i++) s = fmaf(q[i], x[i], s);
-          read(v + (size_t)(64 * w + j) * HD, x);
+          read(v + (size_t)j * HD, x);
         }
         s += __shfl_xor_sync(0xFFFFFFFFu, s, 1);
         s += __shfl_xor_sync(0xFFFFFFFFu, s, 2);
         s += __shfl_xor_sync(0xFFFFFFFFu, s, 4);
-        if (j >= 0) {
-          const float next = fmaxf(m, s);
-          const float f = next == -INFINITY ? 1.f : exp2f(m - next);
-          const float p = exp2f(s - (next == -INFINITY ? 0.f : next));
-          m = next;
-          l = l * f + p;
-#pragma unroll
-          for (int i = 0; i < V; i++) o[i] = fmaf(p, x[i], o[i] * f);
-        }
+        // exp2(s - s) is 1, and NaN where the score is: as one part of sum 1.
+        // A score of -inf weighs nothing.
+        if (in && s != -INFINITY) join(s == s ? s : m, s == s ? 1.f : s, x);
       }
     }
   }
   const size_t step = (size_t)a.kh * R;
-  float top = m;
-  for (int s = lane; s < parts; s += 32) top = fmaxf(top, a.ml[s * step + row].x);
-  top = sg::warp_max(top);
-  if (top == -INFINITY) top = 0.f;  // no key at all: all weights are 0
-  {
-    const float f = exp2f(m - top);
-    l *= f;
-#pragma unroll
-    for (int i = 0; i < V; i++) o[i] *= f;
-  }
-#pragma unroll 4
-  for (int s = group; s < parts; s += 4) {
+#pragma unroll 2
+  for (int s = group; s < parts; s += kMergeGroups) {
     const float2 p = a.ml[s * step + row];
-    const float f = exp2f(p.x - top);
-    l += p.y * f;
-    const float* x = a.part + (s * step + row) * HD + e0;
+    const float* from = a.part + (s * step + row) * HD + e0;
+    float x[V];
 #pragma unroll
     for (int i = 0; i < V; i += 4) {
-      const float4 y = *reinterpret_cast<const float4*>(x + i);
-      o[i] = fmaf(y.x, f, o[i]);
-      o[i + 1] = fmaf(y.y, f, o[i + 1]);
-      o[i + 2] = fmaf(y.z, f, o[i + 2]);
-      o[i + 3] = fmaf(y.w, f, o[i + 3]);
+      const float4 y = *reinterpret_cast<const float4*>(from + i);
+      x[i] = y.x; x[i + 1] = y.y; x[i + 2] = y.z; x[i + 3] = y.w;
     }
+    join(p.x, p.y, x);
   }
+  // The warp's four groups, then the warps.
+  float top = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 8));
+  top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
+  const float f = top == -INFINITY ? 1.f : exp2f(m - top);
+  l *= f;
+#pragma unroll
+  for (int i = 0; i < V; i++) o[i] *= f;
 #pragma unroll
   for (int d = 8; d < 32; d *= 2) {
     l += __shfl_xor_sync(0xFFFFFFFFu, l, d);
 #pragma unroll
     for (int i = 0; i < V; i++) o[i] += __shfl_xor_sync(0xFFFFFFFFu, o[i], d);
   }
-  if (group > 0) return;
-  const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  T* out = static_cast<T*>(a.att) + tok * a.ldo + at;
+  if (lane < 8) {
 #pragma unroll
-  for (int i = 0; i < V; i += 4) {
-    if constexpr (kF32) {
-      *reinterpret_cast<float4*>(out + i) =
-          make_float4(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f);
-    } else {
-      uint2 w;
-      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w.x) : "f"(o[i + 1] * f), "f"(o[i] * f));
-      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w.y) : "f"(o[i + 3] * f), "f"(o[i + 2] * f));
-      *reinterpret_cast<uint2*>(out + i) = w;
-    }
+    for (int i = 0; i < V; i++) warp_o[warp][e0 + i] = o[i];
+    if (lane == 0) warp_ml[warp] = make_float2(top, l);
   }
+  __syncthreads();
+  if (threadIdx.x >= HD) return;
+  float all = -INFINITY, sum = 0.f, out = 0.f;
+#pragma unroll
+  for (int w = 0; w < kMergeThreads / 32; w++) all = fmaxf(all, warp_ml[w].x);
+#pragma unroll
+  for (int w = 0; w < kMergeThreads / 32; w++) {
+    const float g = all == -INFINITY ? 1.f : exp2f(warp_ml[w].x - all);
+    sum += warp_ml[w].y * g;
+    out += warp_o[w][threadIdx.x] * g;
+  }
+  // A row without keys is zeros.
+  out *= sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+  T* to = static_cast<T*>(a.att) + tok * a.ldo + at + threadIdx.x;
+  if constexpr (kF32)
+    *to = out;
+  else
+    asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(*to) : "f"(out));
 }
 
 // Rows of a kv head -> warps in rows and in keys.
@@ -731,7 +747,7 @@ cudaError_t launch_shape(const TreeArgs& a, int dev, cudaStream_t s) {
                      dim3(a.splits, a.kh, (rows + 16 * MW - 1) / (16 * MW)),
                      dim3(32 * MW * KW), bytes, 1, s, a);
   if (e != cudaSuccess || a.splits == 1) return e;
-  return sg::try_launch(k_merge<T, HD, false>, dim3((rows * a.kh + 3) / 4), dim3(128), 0, 1, s, a,
+  return sg::try_launch(k_merge<T, HD, false>, dim3(rows * a.kh), dim3(kMergeThreads), 0, 1, s, a,
                         Tile<T, HD>::kKeys);
 }
 
@@ -742,7 +758,7 @@ cudaError_t launch_hd(const TreeArgs& a, int dev, cudaStream_t s) {
       constexpr bool kF32 = sizeof(T) == 4;
       const cudaError_t e = sg::tree_tc(a, kF32, HD, dev, s);
       if (e != cudaSuccess) return e;
-      return sg::try_launch(k_merge<T, HD, true>, dim3((a.t * a.group * a.kh + 3) / 4), dim3(128),
+      return sg::try_launch(k_merge<T, HD, true>, dim3(a.t * a.group * a.kh), dim3(kMergeThreads),
                             0, 1, s, a, sg::tree_tc_keys());
     }
   }

@@ -655,7 +655,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = warp_wait(saddr(&s_full[b]), (i / C::kSBuffers) & 1, &failed);
       if (!ok) break;
       fence_after();
-      float top = -INFINITY, sum = 0.f, keep = 1.f;
+      float keep = 1.f;
+      // Four partial maxima and sums: chains of 16, not of 64.
+      float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, sum4[4] = {0.f, 0.f, 0.f, 0.f};
       // P of 32 keys: this thread's scores -> its columns of the region.
       // `all`: none of the tile's keys is behind the last.
       auto probabilities = [&](const uint32_t* s, int c, float shift, auto all) {
@@ -668,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (c * 32 + j >= keys) x0 = 0.f;
             if (c * 32 + j + 1 >= keys) x1 = 0.f;
           }
-          sum += x0 + x1;
+          sum4[j / 2 % 4] += x0 + x1;
           uint32_t e[C::kPParts];
           parts<C::kPParts>(x0, x1, e);
 #pragma unroll
@@ -681,7 +683,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto largest = [&](const uint32_t* s, int c, auto all) {
 #pragma unroll
         for (int j = 0; j < 32; j++)
-          if (decltype(all)::value || c * 32 + j < keys) top = fmaxf(top, __uint_as_float(s[j]));
+          if (decltype(all)::value || c * 32 + j < keys)
+            top4[j % 4] = fmaxf(top4[j % 4], __uint_as_float(s[j]));
       };
       const std::true_type full;
       const std::false_type part;
@@ -699,7 +702,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           largest(s[0], 0, part);
           largest(s[1], 1, part);
         }
-        const float next = fmaxf(m, top * scale);
+        const float next = fmaxf(m, fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * scale);
         if (__any_sync(0xFFFFFFFFu, next > m + 8.f)) {
           // m is what P and O are relative to. (The wait is for the last
           // tile's product; this tile's scores say that the one before is
@@ -741,7 +744,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld32(ts + 32, s);
           tmem_wait_ld32(s);
           largest(s, 1, all);
-          const float next = fmaxf(m, top * scale);
+          const float next = fmaxf(m, fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * scale);
           keep = next == -INFINITY ? 1.f : ex2(m - next);  // 0 before the first key
           m = next;
           const float shift = next == -INFINITY ? 0.f : next;
@@ -757,7 +760,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         else
           tile(part);
       }
-      l = l * keep + sum;
+      l = l * keep + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
       tmem_wait_st();
       fence_before();
       mbar_arrive(saddr(&p_full[b]));
