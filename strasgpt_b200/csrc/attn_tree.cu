@@ -17,8 +17,10 @@
 // and carries the probabilities as two bf16 parts, so that the only rounding
 // to bf16 is that of the result.
 //
-// What bounds it: the cache's bytes while there are few rows, the tensor
-// cores' mma.sync rate from about 32 rows (fp32) or 64 (bf16) a kv head.
+// What bounds it: the cache's bytes with up to 16 rows a kv head (90 us for
+// 8 heads of 128000 bf16 keys of 128 entries, 5.8 TB/s; 238 us, 4.4 TB/s, in
+// fp32), mma.sync above; from 17 or 33 rows on the cached keys are
+// attn_tree_tc.cu's (see on_tc).
 #include "attn_tree.h"
 
 #include <math.h>
@@ -257,12 +259,8 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Tree
 #pragma unroll
       for (int i = 0; i < kN8; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
       if constexpr (kF32) {
-        // Three accumulator sets, one per product: independent chains.
-        float s1[kN8][4], s2[kN8][4];
-#pragma unroll
-        for (int i = 0; i < kN8; i++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) s1[i][e] = s2[i][e] = 0.f;
+        // The tensor cores cut their sums: 16 entries at a time from zero,
+        // small products first, then added with rounding.
         const unsigned char* kp = ks + (k0 + g8) * L::kKRow + c4 * 16;
 #pragma unroll
         for (int j = 0; j < kQ; j++) {
@@ -283,18 +281,17 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Tree
             split_tf32(kv.y, bh[1], bl[1]);
             split_tf32(kv.z, bh[2], bl[2]);
             split_tf32(kv.w, bh[3], bl[3]);
-            mma_tf32(s[i], ah[0], bh[0], bh[1]);
-            mma_tf32(s1[i], ah[0], bl[0], bl[1]);
-            mma_tf32(s2[i], al[0], bh[0], bh[1]);
-            mma_tf32(s[i], ah[1], bh[2], bh[3]);
-            mma_tf32(s1[i], ah[1], bl[2], bl[3]);
-            mma_tf32(s2[i], al[1], bh[2], bh[3]);
+            float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_tf32(x, ah[0], bl[0], bl[1]);
+            mma_tf32(y, ah[1], bl[2], bl[3]);
+            mma_tf32(x, al[0], bh[0], bh[1]);
+            mma_tf32(y, al[1], bh[2], bh[3]);
+            mma_tf32(x, ah[0], bh[0], bh[1]);
+            mma_tf32(y, ah[1], bh[2], bh[3]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[i][e] += x[e] + y[e];
           }
         }
-#pragma unroll
-        for (int i = 0; i < kN8; i++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) s[i][e] += s1[i][e] + s2[i][e];
       } else {
         const uint32_t kp = saddr(ks) + (k0 + (lane & 7) + (lane >> 4) * 8) * L::kKRow +
                             ((lane >> 3) & 1) * 16;
@@ -406,19 +403,28 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Tree
 
       if constexpr (kF32) {
         // The score accumulators are the A operand as they lie: slots c and
-        // c + 4 of a k8 step are keys 2c and 2c + 1.
+        // c + 4 of a k8 step are keys 2c and 2c + 1. A chunk's products are
+        // summed from zero and then added, as above.
+        uint32_t ph[kN8][4], pl[kN8][4];
 #pragma unroll
         for (int i = 0; i < kN8; i++) {
-          uint32_t ph[4], pl[4];
-          split_tf32(s[i][0], ph[0], pl[0]);
-          split_tf32(s[i][2], ph[1], pl[1]);
-          split_tf32(s[i][1], ph[2], pl[2]);
-          split_tf32(s[i][3], ph[3], pl[3]);
-          const unsigned char* vp = vs + (k0 + 8 * i + 2 * c4) * L::kVRow + g8 * 16;
+          split_tf32(s[i][0], ph[i][0], pl[i][0]);
+          split_tf32(s[i][2], ph[i][1], pl[i][1]);
+          split_tf32(s[i][1], ph[i][2], pl[i][2]);
+          split_tf32(s[i][3], ph[i][3], pl[i][3]);
+        }
+        const unsigned char* vp = vs + (k0 + 2 * c4) * L::kVRow + g8 * 16;
 #pragma unroll
-          for (int b = 0; b < HD / 32; b++) {
-            const float4 v0 = *reinterpret_cast<const float4*>(vp + b * 128);
-            const float4 v1 = *reinterpret_cast<const float4*>(vp + L::kVRow + b * 128);
+        for (int b = 0; b < HD / 32; b++) {
+          float x[4][4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) x[e][0] = x[e][1] = x[e][2] = x[e][3] = 0.f;
+#pragma unroll
+          for (int i = 0; i < kN8; i++) {
+            const float4 v0 =
+                *reinterpret_cast<const float4*>(vp + i * 8 * L::kVRow + b * 128);
+            const float4 v1 =
+                *reinterpret_cast<const float4*>(vp + (i * 8 + 1) * L::kVRow + b * 128);
             uint32_t h0[4], l0[4], h1[4], l1[4];
             split_tf32(v0.x, h0[0], l0[0]);
             split_tf32(v0.y, h0[1], l0[1]);
@@ -429,12 +435,16 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Tree
             split_tf32(v1.z, h1[2], l1[2]);
             split_tf32(v1.w, h1[3], l1[3]);
 #pragma unroll
-            for (int e = 0; e < 4; e++) mma_tf32(o[4 * b + e], ph, h0[e], h1[e]);
+            for (int e = 0; e < 4; e++) mma_tf32(x[e], ph[i], l0[e], l1[e]);
 #pragma unroll
-            for (int e = 0; e < 4; e++) mma_tf32(o[4 * b + e], ph, l0[e], l1[e]);
+            for (int e = 0; e < 4; e++) mma_tf32(x[e], pl[i], h0[e], h1[e]);
 #pragma unroll
-            for (int e = 0; e < 4; e++) mma_tf32(o[4 * b + e], pl, h0[e], h1[e]);
+            for (int e = 0; e < 4; e++) mma_tf32(x[e], ph[i], h0[e], h1[e]);
           }
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int y = 0; y < 4; y++) o[4 * b + e][y] += x[e][y];
         }
       } else {
         const uint32_t vp = saddr(vs) + (k0 + (lane & 7) + ((lane >> 3) & 1) * 8) * L::kVRow +
@@ -714,11 +724,19 @@ Shape shape_of(int rows) {
   return {8, 1};
 }
 
-// Whether the cached keys go to tcgen05 (attn_tree_tc.cu): from 33 rows a kv
-// head on, where mma.sync is what bounds this file's kernel. Not for many
-// drafted tokens, whose own keys the merge reads one by one, and not for
-// head_dim 32.
-bool on_tc(int t, int group, int hd) { return t * group > 32 && t <= 256 && hd >= 64; }
+// Whether the cached keys go to tcgen05 (attn_tree_tc.cu): where mma.sync, not
+// the cache's bytes, is what bounds this file's kernel. Measured with 8 kv
+// heads, us here / there:
+//   head_dim 128, 16 rows: bf16 128000 keys 92 / 92, 8000 13.5 / 15.4;
+//                          fp32 128000 keys 245 / 335
+//                 32 rows: bf16 119 / 92, 19.1 / 16.3; fp32 431 / 337
+//   head_dim 64,  32 rows: bf16 77 / 70, 11.4 / 13.2; fp32 191 / 241
+//                 48 rows: bf16 121 / 71, 14.2 / 13.6; fp32 338 / 241
+// Not for many drafted tokens, whose own keys the merge reads one by one, and
+// not for head_dim 32.
+bool on_tc(int t, int group, int hd) {
+  return t <= 256 && hd >= 64 && t * group > (hd == 128 ? 16 : 32);
+}
 
 // Splits of the keys: as many CTAs as the GPU holds at once.
 int splits_of(int sms, int t, int kh, int group, int hd) {

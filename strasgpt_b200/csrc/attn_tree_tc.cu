@@ -310,6 +310,40 @@ __device__ __forceinline__ void parts(float x0, float x1, uint32_t* p) {
   }
 }
 
+// Two fp32 operations in one instruction.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack(float x, float y) {
+  f32x2 v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+  return v;
+}
+__device__ __forceinline__ void unpack(f32x2 v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+// What cutting both values to bf16 leaves.
+__device__ __forceinline__ f32x2 rest2(f32x2 v) {
+  float x, y;
+  unpack(v, x, y);
+  const f32x2 cut = pack(__uint_as_float(__float_as_uint(x) & 0xFFFF0000u),
+                         __uint_as_float(__float_as_uint(y) & 0xFFFF0000u));
+  return fma2(cut, pack(-1.f, -1.f), v);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float v;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
+  return v;
+}
+
 // Byte of 16-byte group c (8 entries) of row r in a tile of `rows` rows.
 __device__ __forceinline__ uint32_t at_sw128(int rows, int r, int c) {
   return (uint32_t)((c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
@@ -656,25 +690,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       fence_after();
       float keep = 1.f;
-      // Four partial maxima and sums: chains of 16, not of 64.
-      float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, sum4[4] = {0.f, 0.f, 0.f, 0.f};
+      // Partial maxima and sums: short chains.
+      float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      f32x2 sum2[2] = {0, 0};
       // P of 32 keys: this thread's scores -> its columns of the region.
       // `all`: none of the tile's keys is behind the last.
       auto probabilities = [&](const uint32_t* s, int c, float shift, auto all) {
         uint32_t p[C::kPParts][16];
+        const f32x2 scale2 = pack(scale, scale), shift2 = pack(-shift, -shift);
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
-          float x0 = ex2(fmaf(__uint_as_float(s[j]), scale, -shift));
-          float x1 = ex2(fmaf(__uint_as_float(s[j + 1]), scale, -shift));
+          float x0, x1;
+          unpack(fma2(pack(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), scale2, shift2), x0,
+                 x1);
+          x0 = ex2(x0);
+          x1 = ex2(x1);
           if constexpr (!decltype(all)::value) {
             if (c * 32 + j >= keys) x0 = 0.f;
             if (c * 32 + j + 1 >= keys) x1 = 0.f;
           }
-          sum4[j / 2 % 4] += x0 + x1;
-          uint32_t e[C::kPParts];
-          parts<C::kPParts>(x0, x1, e);
+          f32x2 x = pack(x0, x1);
+          sum2[j / 2 % 2] = add2(sum2[j / 2 % 2], x);
+          // The parts as in parts<N>().
 #pragma unroll
-          for (int y = 0; y < C::kPParts; y++) p[y][j / 2] = e[y];
+          for (int y = 0; y < C::kPParts; y++) {
+            unpack(x, x0, x1);
+            p[y][j / 2] = C::kPParts == 2 && y == 1 ? bf16x2(x0, x1) : upper(x0, x1);
+            if (y + 1 < C::kPParts) x = rest2(x);
+          }
         }
 #pragma unroll
         for (int y = 0; y < C::kPParts; y++)
@@ -682,9 +725,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       auto largest = [&](const uint32_t* s, int c, auto all) {
 #pragma unroll
-        for (int j = 0; j < 32; j++)
-          if (decltype(all)::value || c * 32 + j < keys)
-            top4[j % 4] = fmaxf(top4[j % 4], __uint_as_float(s[j]));
+        for (int j = 0; j < 32; j += 2) {
+          float x = __uint_as_float(s[j]), y = __uint_as_float(s[j + 1]);
+          if constexpr (!decltype(all)::value) {
+            if (c * 32 + j >= keys) x = -INFINITY;
+            if (c * 32 + j + 1 >= keys) y = -INFINITY;
+          }
+          top4[j / 2 % 4] = max3(top4[j / 2 % 4], x, y);
+        }
       };
       const std::true_type full;
       const std::false_type part;
@@ -760,7 +808,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         else
           tile(part);
       }
-      l = l * keep + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
+      float even, odd;
+      unpack(add2(sum2[0], sum2[1]), even, odd);
+      l = l * keep + (even + odd);
       tmem_wait_st();
       fence_before();
       mbar_arrive(saddr(&p_full[b]));
