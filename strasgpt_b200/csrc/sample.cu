@@ -69,6 +69,7 @@ struct SampleArgs {
   float* prob;
   int* kept;
   int vec;                       // rows can be read 16 bytes at a time
+  int pending;                   // only the rows that k_sample_rows left
 };
 
 struct Entry {
@@ -189,6 +190,183 @@ __device__ __forceinline__ u64 block_sort(u64 v, int n, u64* x) {
       v = larger == (v > o) ? v : o;
     }
   return v;
+}
+
+// The choice of a row from its n <= kThreads entries that can be kept, one
+// block's work. mark: this thread's entry, its key over INT_MAX - index (0
+// behind the last). `few` and `order` hold kThreads words, `wsum` kWarps.
+template <typename W>
+__device__ __forceinline__ void finish(const SampleArgs& a, int row, u64 mark, int n, int k,
+                                       float p, double min_w, float u, W weight, u64* few,
+                                       u64* order, double* wsum, int* found, unsigned* fill) {
+  // Sorted, entry `tid` of the order is thread tid's.
+  const int tid = threadIdx.x;
+  const bool real = tid < n;
+  const u64 v = block_sort(mark, n, order);
+  double w = real ? weight(of_key((unsigned)(v >> 32))) : 0.0;
+  bool stays = real && tid < k;
+  double mass;
+  const double upto_w = block_prefix(stays ? w : 0.0, wsum, &mass);
+  if (p < 1.f) stays = stays && (tid == 0 || upto_w - w < (double)p * mass);
+  stays = stays && w >= min_w;
+  const int kept = __syncthreads_count(stays);
+  // What stays, by index.
+  double* weights = reinterpret_cast<double*>(few);
+  weights[tid] = w;
+  const u64 byi = block_sort(stays ? (u64)(unsigned)v << 32 | (unsigned)tid : 0, n, order);
+  __syncthreads();
+  w = tid < kept ? weights[(unsigned)byi] : 0.0;
+  double total;
+  const double run = block_prefix(w, wsum, &total);
+  const double target = u > 0.f ? (double)u * total : 0.0;
+  if (tid == 0) {
+    *found = kThreads;
+    *fill = 0;
+  }
+  __syncthreads();
+  if (w > 0) {
+    if (run > target) atomicMin(found, tid);
+    atomicMax(fill, tid);
+  }
+  __syncthreads();
+  if (tid == min(*found, (int)*fill)) {
+    a.token[row] = INT_MAX - (int)(unsigned)(byi >> 32);
+    if (a.prob) a.prob[row] = (float)(w / total);
+    if (a.kept) a.kept[row] = kept;
+  }
+}
+
+// Many rows under top-k: a block per row reads it twice, once for the largest
+// logits of 1024 groups (two a thread), whose k-th largest bounds the row's,
+// and once, from L2, for the entries above that bound, at most kThreads. No
+// block waits for another. A row that this does not serve (no top-k, or too
+// many entries left, or infinite logits) gets the token kPending and is the
+// cluster kernel's.
+constexpr int kPending = -2;
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) k_sample_rows(SampleArgs a) {
+  __shared__ u64 few[kThreads], order[kThreads], wred[kWarps];
+  __shared__ double wsum[kWarps];
+  __shared__ float wtop[kWarps], wleast[kWarps];
+  __shared__ unsigned count[kBins], fill, bin;
+  __shared__ int found;
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  sg::pdl_trigger();
+  sg::pdl_wait();
+  const float T_ = a.temperature ? a.temperature[row] : 1.f;
+  const int k = a.top_k[row];
+  const float p = a.top_p ? a.top_p[row] : 1.f;
+  const float min_p = a.min_p ? a.min_p[row] : 0.f;
+  const bool greedy = !(T_ > 0.f) || k == 1 || p <= 0.f;
+  if (!greedy && (k <= 0 || k > kThreads || k >= a.vocab)) {
+    if (tid == 0) a.token[row] = kPending;
+    return;
+  }
+  const T* src = static_cast<const T*>(a.logits) + row * a.ld;
+  constexpr int V = 16 / sizeof(T);
+  const int nv = a.vec ? a.vocab / V : 0;
+  // f(logit, index) for all of the row; a NaN or -inf fails its comparisons.
+  auto each = [&](auto f) {
+#pragma unroll 4
+    for (int v = tid; v < nv; v += kThreads) {
+      const uint4 r = reinterpret_cast<const uint4*>(src)[v];
+      T e[V];
+      memcpy(e, &r, 16);
+#pragma unroll
+      for (int j = 0; j < V; j++) f(load_f(e[j]), v * V + j);
+    }
+    for (int i = nv * V + tid; i < a.vocab; i += kThreads) f(load_f(src[i]), i);
+  };
+  float top[2] = {-INFINITY, -INFINITY};
+  each([&](float x, int i) { top[i & 1] = fmaxf(top[i & 1], x); });
+  top[0] += 0.f;  // -0 is 0
+  top[1] += 0.f;
+  float M = fmaxf(top[0], top[1]);
+  // The smallest of the groups' largest that are there.
+  float least = fminf(top[0] > -INFINITY ? top[0] : INFINITY, top[1] > -INFINITY ? top[1] : INFINITY);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
+    least = fminf(least, __shfl_xor_sync(0xFFFFFFFFu, least, o));
+  }
+  if (lane == 0) {
+    wtop[warp] = M;
+    wleast[warp] = least;
+  }
+  count[tid] = 0;
+  if (tid == 0) {
+    fill = 0;
+    bin = kBins;
+    found = INT_MAX;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWarps; w++) {
+    M = fmaxf(M, wtop[w]);
+    least = fminf(least, wleast[w]);
+  }
+  if (M == -INFINITY) {          // nothing but -inf and NaN
+    if (tid == 0) {
+      a.token[row] = -1;
+      if (a.prob) a.prob[row] = 0.f;
+      if (a.kept) a.kept[row] = 0;
+    }
+    return;
+  }
+  if (greedy) {
+    // The largest, at its lowest index.
+    int first = INT_MAX;
+    each([&](float x, int i) { first = x == M ? min(first, i) : first; });
+    if (first < INT_MAX) atomicMin(&found, first);
+    __syncthreads();
+    if (tid == 0) {
+      a.token[row] = found;
+      if (a.prob) a.prob[row] = 1.f;
+      if (a.kept) a.kept[row] = 1;
+    }
+    return;
+  }
+  if (M == INFINITY) {
+    if (tid == 0) a.token[row] = kPending;
+    return;
+  }
+  // The bin of the k-th largest group, and a logit just below that bin.
+  const float bins_per = fminf((kBins - 1) / (M - least), 1e37f);
+#pragma unroll
+  for (int g = 0; g < 2; g++)
+    if (top[g] > -INFINITY)
+      atomicAdd(&count[(int)fminf((M - top[g]) * bins_per, (float)(kBins - 1))], 1u);
+  __syncthreads();
+  u64 all;
+  const u64 upto = block_prefix((u64)count[tid], wred, &all);
+  if (upto >= (u64)k) atomicMin(&bin, (unsigned)tid);
+  __syncthreads();
+  // Fewer groups than k: no bound. The last bin ends at the smallest group.
+  const float floor =
+      bin == kBins ? -FLT_MAX
+                   : bin == kBins - 1
+                         ? least
+                         : __double2float_rd((double)M - (bin + 1.01) / (double)bins_per -
+                                             1e-6 * (fabs((double)M) + (double)(M - least)));
+  each([&](float x, int i) {
+    if (x >= floor) {
+      const unsigned at = atomicAdd(&fill, 1u);
+      if (at < kThreads) few[at] = ((u64)key_of(x + 0.f) << 32) | (unsigned)(INT_MAX - i);
+    }
+  });
+  __syncthreads();
+  const unsigned n = fill;
+  __syncthreads();               // before `fill` serves the choice
+  if (n > kThreads) {
+    if (tid == 0) a.token[row] = kPending;
+    return;
+  }
+  const double scale = 1.4426950408889634 / (double)T_;
+  const double min_w = min_p > 0.f ? fmin((double)min_p, 1.0) : 0.0;
+  finish(a, row, tid < (int)n ? few[tid] : 0, (int)n, k, p, min_w, a.u[row],
+         [&](float x) { return exp2(((double)x - (double)M) * scale); }, few, order, wsum, &found,
+         &fill);
 }
 
 template <typename T>
@@ -713,6 +891,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleArgs a) {
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int row = blockIdx.x / ranks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (a.pending) {
+    sg::pdl_trigger();
+    sg::pdl_wait();
+    if (a.token[row] != kPending) return;
+  }
   cluster.barrier_arrive();  // waited for before the first access to another CTA
   if (threadIdx.x < 256) sh->table[threadIdx.x] = exp2(threadIdx.x / 256.0);
   sg::pdl_trigger();
@@ -878,40 +1061,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleArgs a) {
       // thread tid's.
       if (rank > 0) return;
       const int tid = threadIdx.x;
-      const bool real = tid < (int)all;
-      const u64 v = block_sort(real ? sh->few[tid] : 0, (int)all, sh->order);
-      double w = real ? r.weight(of_key((unsigned)(v >> 32))) : 0.0;
-      bool stays = real && tid < k_;
-      double mass;
-      const double upto_w = block_prefix(stays ? w : 0.0, sh->wsum, &mass);
-      if (p_ < 1.f) stays = stays && (tid == 0 || upto_w - w < (double)p_ * mass);
-      stays = stays && w >= min_w;
-      const int kept = __syncthreads_count(stays);
-      // What stays, by index.
-      double* weights = reinterpret_cast<double*>(sh->few);
-      weights[tid] = w;
-      const u64 byi =
-          block_sort(stays ? (u64)(unsigned)v << 32 | (unsigned)tid : 0, (int)all, sh->order);
-      __syncthreads();
-      w = tid < kept ? weights[(unsigned)byi] : 0.0;
-      double total;
-      const double run = block_prefix(w, sh->wsum, &total);
-      const double target = u_ > 0.f ? (double)u_ * total : 0.0;
-      if (tid == 0) {
-        sh->found = kThreads;
-        sh->fill = 0;
-      }
-      __syncthreads();
-      if (w > 0) {
-        if (run > target) atomicMin(&sh->found, tid);
-        atomicMax(&sh->fill, tid);
-      }
-      __syncthreads();
-      if (tid == min(sh->found, (int)sh->fill)) {
-        a.token[row] = INT_MAX - (int)(unsigned)(byi >> 32);
-        if (a.prob) a.prob[row] = (float)(w / total);
-        if (a.kept) a.kept[row] = kept;
-      }
+      finish(a, row, tid < (int)all ? sh->few[tid] : 0, (int)all, k_, p_, min_w, u_,
+             [&](float x) { return r.weight(x); }, sh->few, sh->order, sh->wsum, &sh->found,
+             &sh->fill);
       return;
     }
     r.histogram();
@@ -1003,12 +1155,20 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleArgs a) {
   }
 }
 
+// From this many rows on, where a top-k is given, k_sample_rows goes first.
+constexpr int kManyRows = 32;
+
 template <typename T>
-cudaError_t launch(const SampleArgs& a, int rows, int cluster, int dev, cudaStream_t s) {
+cudaError_t launch(SampleArgs a, int rows, int cluster, int dev, cudaStream_t s) {
   static std::atomic<size_t> allowed[sg::kDevices];
   const size_t smem = sizeof(Shared) + (size_t)a.per * sizeof(T);
-  const cudaError_t e = sg::allow_smem(k_sample<T>, smem, dev, allowed);
+  cudaError_t e = sg::allow_smem(k_sample<T>, smem, dev, allowed);
   if (e != cudaSuccess) return e;
+  a.pending = a.top_k && rows >= kManyRows;
+  if (a.pending) {
+    e = sg::try_launch(k_sample_rows<T>, dim3((unsigned)rows), dim3(kThreads), 0, 1, s, a);
+    if (e != cudaSuccess) return e;
+  }
   return sg::try_launch(k_sample<T>, dim3((unsigned)(rows * cluster)), dim3(kThreads), smem,
                         cluster, s, a);
 }
