@@ -469,12 +469,15 @@ struct Row {
   __device__ u64 in_units(double w, int unit) const {
     return (u64)__double_as_longlong(fma(w, pow2(unit), 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
   }
-  // Adds the weight of x, f bins from M, to bin b.
-  __device__ void add(int b, float x, float f, int unit) {
+  // The weight of x, f bins from M, in a bin's unit.
+  __device__ unsigned units(float x, float f, int unit) const {
     int e;
     const double v = power(x, &e);
     const unsigned w = (unsigned)__double2loint(shifted(v, e + unit) + 4503599627370496.0);
-    if (!(f < last) || w == 0) return;
+    return f < last ? w : 0u;
+  }
+  __device__ void add(int b, unsigned w) {
+    if (w == 0) return;
     atomicAdd(&sh->lo[b], w & 0xFFFFu);
     atomicAdd(&sh->hi[b], w >> 16);
   }
@@ -491,18 +494,25 @@ struct Row {
       const float f = pos(x);
       const int b = bin_at(f);
       atomicAdd(&sh->count[b], 1u);
-      add(b, x, f, unit_of(b));
+      add(b, units(x, f, unit_of(b)));
     });
     gather_histogram();
   }
   // The masses alone, of all of the row.
   __device__ void histogram_of_all() {
     clear();
-#pragma unroll 2
-    for (int i = c0; i < c1; i++) {
-      const float x = load_f(xs[i]), f = pos(x);
-      const int b = bin_at(f);
-      add(b, x, f, unit_of(b));
+    // Four entries' weights side by side, then their additions.
+    for (int i = c0; i < c1; i += 4) {
+      unsigned w[4];
+      int b[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float x = i + j < c1 ? load_f(xs[i + j]) : -INFINITY, f = pos(x);
+        b[j] = bin_at(f);
+        w[j] = units(x, f, unit_of(b[j]));
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++) add(b[j], w[j]);
     }
     gather_histogram();
   }
@@ -694,7 +704,7 @@ struct Row {
       auto divide = [&](float x, float f) {
         const int d = bin_at((f - from) * kBins);
         atomicAdd(&sh->count[d], 1u);
-        add(d, x, f, unit);
+        add(d, units(x, f, unit));
       };
       if (listed) {
         each([&](float x, int) {
@@ -806,7 +816,7 @@ struct Row {
         if (!in_set(x)) return;
         const int d = (int)((kmax - key_of(x)) >> shift);
         atomicAdd(&sh->count[d], 1u);
-        add(d, x, pos(x), unit);
+        add(d, units(x, pos(x), unit));
       });
       gather_histogram();
       find_sub_bin(by_mass, target, k, count, base, mass, step);
@@ -1157,6 +1167,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleArgs a) {
 
 // From this many rows on, where a top-k is given, k_sample_rows goes first.
 constexpr int kManyRows = 32;
+// A slice that leaves room for two CTAs on an SM.
+constexpr int kSliceBytes = 78 * 1024;
 
 template <typename T>
 cudaError_t launch(SampleArgs a, int rows, int cluster, int dev, cudaStream_t s) {
@@ -1202,9 +1214,17 @@ extern "C" int strasgpt_k_sample(const void* logits, int type, long long ld, int
       if (const char* why = sg::not_on_device(p, dev)) return sg::refuse(me, why);
 
   // Eight CTAs a row; fewer for a small vocabulary, whose slices would cost
-  // more in exchanges than they save in reading.
+  // more in exchanges than they save in reading, and for as many rows as
+  // still give every SM a CTA, as long as slices leave room for two on an SM
+  // (128 rows of 32003 fp32 logits under top-p: 49 us with 2 a row, 113 us
+  // with 8; 64 rows: 37 us with 4, 61 us with 8, 47 us with 2).
   int cluster = kMaxCluster;
-  while (cluster > 1 && (vocab + cluster - 1) / cluster < 2048) cluster /= 2;
+  while (cluster > 1) {
+    const int half = cluster / 2, slice = (vocab + half - 1) / half;
+    const bool small = (vocab + cluster - 1) / cluster < 2048;
+    if (!small && ((long long)rows * half < sms || slice * size > kSliceBytes)) break;
+    cluster = half;
+  }
   SampleArgs a;
   a.logits = logits; a.ld = ld; a.vocab = vocab;
   a.per = ((vocab + cluster - 1) / cluster + 7) & ~7;
