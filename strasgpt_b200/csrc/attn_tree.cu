@@ -23,6 +23,7 @@
 // attn_tree_tc.cu's (see on_tc).
 #include "attn_tree.h"
 
+#include <limits.h>
 #include <math.h>
 
 #include <algorithm>
@@ -799,6 +800,8 @@ const char* bad_shape(int t, int kh, int group, int hd) {
   if (t > STRASGPT_ATTN_TREE_MAX) return "more than 1024 drafted tokens";
   if (group > 128 || kh > 65535) return "more than 128 q heads per kv head, or 65535 kv heads";
   if (hd != 32 && hd != 64 && hd != 128) return "head_dim must be 32, 64 or 128";
+  // k_merge has a block per row.
+  if ((long long)t * kh * group > INT_MAX) return "more than 2^31 - 1 rows of q heads";
   return nullptr;
 }
 

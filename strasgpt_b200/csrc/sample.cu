@@ -342,13 +342,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(SampleArgs a) {
   const u64 upto = block_prefix((u64)count[tid], wred, &all);
   if (upto >= (u64)k) atomicMin(&bin, (unsigned)tid);
   __syncthreads();
-  // Fewer groups than k: no bound. The last bin ends at the smallest group.
-  const float floor =
-      bin == kBins ? -FLT_MAX
-                   : bin == kBins - 1
-                         ? least
-                         : __double2float_rd((double)M - (bin + 1.01) / (double)bins_per -
-                                             1e-6 * (fabs((double)M) + (double)(M - least)));
+  // Fewer groups than k: no bound but -inf's. The last bin ends at the
+  // smallest group. (A range beyond fp32 has one bin and no bound either.)
+  const float floor = fmaxf(
+      -FLT_MAX, bin == kBins ? -FLT_MAX
+                : bin == kBins - 1
+                    ? least
+                    : __double2float_rd((double)M - (bin + 1.01) / (double)bins_per -
+                                        1e-6 * (fabs((double)M) + (double)(M - least))));
   each([&](float x, int i) {
     if (x >= floor) {
       const unsigned at = atomicAdd(&fill, 1u);

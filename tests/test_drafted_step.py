@@ -400,6 +400,64 @@ def test_tree_offsets_beyond_32_bits(cuda):
         del k, v
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [F32, BF16])
+@pytest.mark.parametrize("t,g,hd", [(9, 4, 128), (17, 1, 128), (33, 1, 64), (256, 1, 64),
+                                    (2, 128, 128), (1, 128, 32)])
+def test_tree_caches_that_end_with_the_tree(cuda, type_, t, g, hd):
+    """No row behind the drafted ones, few or none before them: caches shorter
+    than a tile of keys, and the length cut to what the cache holds."""
+    torch = cuda
+    for n in (0, 1, 62, 64):
+        q, k, v = inputs(torch, t, 2, g, hd, n + t, type_, t + n)
+        m = tree_mask(t, 4)
+        want, reach, top = tree_reference(torch, q, k, v, n, m)
+        got = run_tree(torch, q, k, v, n, m, type_)
+        err = (got.double() - want).abs()
+        assert (err <= tree_tolerance(want, reach, top, n + t, hd, type_)).all()
+        cut = run_tree(torch, q, k, v, 2 ** 31 - 1, m, type_)
+        assert torch.equal(cut, got)
+        if n == 0:
+            assert torch.equal(run_tree(torch, q, k, v, -5, m, type_), got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [F32, BF16])
+@pytest.mark.parametrize("t,hd", [(24, 128), (20, 64), (3, 128)])
+def test_tree_two_graphs_at_once(cuda, type_, t, hd):
+    """Two captured calls with workspaces of their own, replayed on two streams
+    at the same time, the lengths changed between replays."""
+    torch = cuda
+    L, kh, g, ctx = runtime.lib(), 2, 4, 4000
+    sides = []
+    for seed in (1, 2):
+        q, k, v = inputs(torch, t, kh, g, hd, ctx, type_, seed)
+        m = tree_mask(t, seed)
+        size = L.strasgpt_k_attn_tree_workspace(t, kh, g, hd)
+        x = dict(q=q, k=k, v=v, m=m, words=mask_words(torch, m), att=torch.zeros_like(q),
+                 n=torch.zeros(1, dtype=torch.int32, device="cuda"),
+                 work=torch.full((size // 4 + 1,), float("nan"), device="cuda"),
+                 stream=torch.cuda.Stream(), graph=torch.cuda.CUDAGraph())
+        torch.cuda.synchronize()
+        with torch.cuda.graph(x["graph"], stream=x["stream"]):
+            assert L.strasgpt_k_attn_tree(
+                q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), type_, t, kh, g, hd, ctx,
+                x["n"].data_ptr(), x["words"].data_ptr(), x["att"].data_ptr(), q.stride(0),
+                x["work"].data_ptr(), size, torch.cuda.current_stream().cuda_stream) == 0
+        sides.append(x)
+    for lengths in ((3900, 1), (0, 3333), (640, 641)):
+        for x, n in zip(sides, lengths):
+            x["n"].fill_(n)
+        torch.cuda.synchronize()
+        for _ in range(10):
+            for x in sides:
+                with torch.cuda.stream(x["stream"]):
+                    x["graph"].replay()
+        torch.cuda.synchronize()
+        for x, n in zip(sides, lengths):
+            assert torch.equal(x["att"], run_tree(torch, x["q"], x["k"], x["v"], n, x["m"], type_))
+
+
 # --------------------------------------------------------------------------
 # sample
 # --------------------------------------------------------------------------
@@ -643,6 +701,126 @@ def test_sample_parameters_differ_by_row_and_replays_agree(cuda):
             assert (got.cpu().numpy() == w).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab", [(32, 1), (33, 60), (40, 700), (47, 5003), (64, 40001),
+                                        (36, 201088)])
+def test_sample_many_rows_under_top_k(cuda, type_, rows, vocab):
+    """From 32 rows on a top-k row may be a block's own: here with rows among
+    them that are not (no top-k, one above 512, one of the whole vocabulary)."""
+    torch = cuda
+    rng = np.random.RandomState(rows)
+    ks = [0, 1, 2, 50, 300, 511, 512, 513, 2000, vocab - 1, vocab, -4]
+    for i, f in enumerate([dict(), dict(top_p=0.9), dict(min_p=0.02),
+                           dict(top_p=0.99, min_p=0.001)]):
+        x = logits(torch, rows, vocab, type_, 40 + i)
+        check_sample(torch, x, heat=rng.choice([0.0, 0.3, 1.0, 1.6], rows).astype(np.float32),
+                     top_k=rng.choice(ks, rows).astype(np.int32),
+                     u=rng.uniform(0, 1, rows).astype(np.float32), **f)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [F32, BF16])
+@pytest.mark.parametrize("vocab", [600, 9001])
+def test_sample_many_rows_masked_and_odd_values(cuda, type_, vocab):
+    torch = cuda
+    inf, nan = float("inf"), float("nan")
+    x = logits(torch, 36, vocab, type_, 6)
+    low, high = torch.finfo(x.dtype).min, torch.finfo(x.dtype).max
+    x[0] = -inf
+    x[1] = nan
+    x[2] = -inf
+    x[2, 123] = low
+    x[3, ::2] = -inf
+    x[4, 1::2] = low
+    x[5] = low
+    x[6, 17] = inf
+    x[6, 400:403] = inf
+    x[7, ::3] = nan
+    x[8, :-1] = -inf
+    x[9, 1:] = -inf
+    x[10] = 1.25                                 # all equal: more than a block holds
+    x[11, 100:] = -inf                           # fewer entries than some k
+    x[12] = -inf                                 # the widest range there is, and masked ones
+    x[12, 5], x[12, 50:60], x[12, 70] = high, 1.0, low
+    x[13] = 0.0
+    x[13, ::2] = -0.0
+    x[14, 1:] = x[14, 1:] * 2.0 ** -20 + 1       # all but one nearly equal
+    x[15, 0] = high                              # far above the others
+    x[16] = -inf
+    x[16, 3] = inf                               # one infinity, nothing else
+    rng = np.random.RandomState(8)
+    for k in (1, 2, 40, 300, 512):
+        for heat in (1.0, 1e-3, 1e30):
+            for f in (dict(), dict(top_p=0.7), dict(min_p=0.3)):
+                check_sample(torch, x, heat=heat, top_k=k,
+                             u=rng.uniform(0, 1, 36).astype(np.float32), **f)
+    token, prob, kept = run_sample(torch, x, u=0.3, heat=float("inf"), top_k=300)
+    assert token[1] == -1 and kept[11] == 100 and abs(prob[11] - 0.01) < 1e-8
+    assert kept[12] == 12 and abs(prob[12] * 12 - 1) < 1e-6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [F32, BF16])
+def test_sample_many_rows_of_a_wider_matrix(cuda, type_):
+    torch = cuda
+    for start, vocab, ld in ((1, 4099, 4111), (8, 4096, 4120), (3, 129, 1000)):
+        big = torch.full((35 * ld + 8,), float("inf"), device="cuda", dtype=dtype(torch, type_))
+        x = logits(torch, 35, vocab, type_, ld)
+        view = big[start:start + 35 * ld].view(35, ld)[:, :vocab]
+        view.copy_(x)
+        check_sample(torch, view, top_k=30, top_p=0.9, u=0.77, ld=ld)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab", [(160, 2050), (40, 8200), (80, 16500), (160, 16500),
+                                        (150, 39900), (150, 39945), (75, 80001)])
+def test_sample_rows_that_fill_the_gpu(cuda, type_, rows, vocab):
+    """Rows of one, two, four and eight CTAs, slices up to the longest that
+    two CTAs on an SM leave room for."""
+    torch = cuda
+    rng = np.random.RandomState(rows + vocab)
+    for i, f in enumerate([dict(top_p=0.95), dict(top_p=0.6, min_p=0.01), dict()]):
+        x = logits(torch, rows, vocab, type_, i)
+        check_sample(torch, x, heat=rng.uniform(0.3, 1.6, rows).astype(np.float32),
+                     u=rng.uniform(0, 1, rows).astype(np.float32), **f)
+
+
+@pytest.mark.gpu
+def test_sample_calls_at_once(cuda):
+    """Many rows with a block each on one stream, a few rows on another, at
+    the same time: what each gives alone."""
+    torch = cuda
+    a, b = logits(torch, 64, 50000, BF16, 1), logits(torch, 9, 128256, F32, 2)
+    ka = dict(top_k=50, top_p=0.9, u=0.35)
+    kb = dict(top_p=0.9, u=0.8)
+    one, two = check_sample(torch, a, **ka), check_sample(torch, b, **kb)
+    L = runtime.lib()
+
+    def prepare(x, k, p, u):
+        n = x.shape[0]
+        full = lambda v, dt: torch.full((n,), v, dtype=dt, device="cuda")  # noqa: E731
+        out = (full(-7, torch.int32), full(0, torch.float32), full(-7, torch.int32))
+        keep = (full(k, torch.int32), full(p, torch.float32), full(u, torch.float32))
+        call = lambda s: L.strasgpt_k_sample(  # noqa: E731
+            x.data_ptr(), F32 if x.dtype == torch.float32 else BF16, x.shape[1], n, x.shape[1],
+            None, keep[0].data_ptr(), keep[1].data_ptr(), None, keep[2].data_ptr(),
+            *[o.data_ptr() for o in out], s.cuda_stream)
+        return call, out, keep
+
+    ca, oa, _ka = prepare(a, 50, 0.9, 0.35)
+    cb, ob, _kb = prepare(b, 0, 0.9, 0.8)
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        assert ca(sa) == 0 and cb(sb) == 0
+    torch.cuda.synchronize()
+    for out, want in ((oa, one), (ob, two)):
+        for got, w in zip(out, want):
+            assert (got.cpu().numpy() == w).all()
+
+
 # --------------------------------------------------------------------------
 # together
 # --------------------------------------------------------------------------
@@ -774,7 +952,8 @@ def test_rope_refuses(capfd, change, words):
     (dict(cached=None), "null"), (dict(mask=None), "null"), (dict(att=None), "null"),
     (dict(q=FAKE + 4), "16-byte"), (dict(k=FAKE + 8), "16-byte"), (dict(ldq=1026), "16-byte"),
     (dict(att=FAKE + 8), "16-byte"), (dict(cached=FAKE + 2), "aligned"),
-    (dict(mask=FAKE + 4), "aligned"), (dict(), ""),
+    (dict(mask=FAKE + 4), "aligned"),
+    (dict(t=1024, kh=65535, g=128, ctx=4000, ld=1 << 30), "rows of q heads"), (dict(), ""),
 ])
 def test_tree_refuses(capfd, change, words):
     a = dict(type_=F32, t=8, kh=2, g=4, hd=128, ctx=64, ldq=1024, ldo=1024, q=FAKE, k=FAKE, v=FAKE,
@@ -790,7 +969,8 @@ def test_tree_refuses(capfd, change, words):
 
 def test_tree_workspace_refuses(capfd):
     f = runtime.lib().strasgpt_k_attn_tree_workspace
-    for shape in ((-1, 1, 1, 64), (1, 0, 1, 64), (1, 1, 200, 64), (1, 1, 1, 65), (2000, 1, 1, 64)):
+    for shape in ((-1, 1, 1, 64), (1, 0, 1, 64), (1, 1, 200, 64), (1, 1, 1, 65), (2000, 1, 1, 64),
+                  (1024, 65535, 128, 32)):
         assert f(*shape) == 0
         assert "[StrasGPT] Error" in capfd.readouterr().err
 
