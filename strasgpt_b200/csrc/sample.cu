@@ -91,6 +91,10 @@ struct alignas(16) Shared {
       u64 few[kThreads];         // the row's entries that the bound leaves,
       u64 order[kThreads];       // when they are few: key, index
     };
+    struct {
+      u64 gather_mass[kBins];    // a share of the bins from every CTA
+      unsigned gather_count[kBins];
+    };
   };
   union {
     float maxima[kMaxCluster * kGroups];  // the groups' largest logits
@@ -440,20 +444,19 @@ struct Row {
   // The weights of bin b are at most 2^-e: their unit is 2^-(e + kUnit).
   __device__ int unit_of(int b) const { return kUnit + whole((float)b * octaves); }
 
-  // exp((x - M) / T) as (v, e): v 2^e, with 1 <= v < 2 or nearly so. 2^t with
-  // t in units of 1/256 taken apart by adding 1.5 * 2^44, a cubic for the
-  // rest (|r ln 2| < 1.4e-3, the next term is below 1.5e-13). No branches, so
-  // that a loop's weights overlap.
-  __device__ double power(float x, int* e) const {
-    const double t = ((double)x - (double)M) * scale;
+  // exp((x - M) / T) as v p 2^e, with 1 <= v < 2 and p nearly 1. 2^t with t in
+  // units of 1/256 taken apart by adding 1.5 * 2^44, a cubic for the rest
+  // (|r ln 2| < 1.4e-3, the next term is below 1.5e-13). No branches, so that a
+  // loop's weights overlap.
+  __device__ double power(float x, double* p, int* e) const {
+    const double d = (double)x - (double)M;
     const double magic = 6755399441055744.0 / 256;
-    const double z = t + magic;
+    const double z = fma(d, scale, magic);
     const int n = __double2loint(z);
-    const double r = t - (z - magic);
-    const double p = fma(fma(fma(r, 0.05550410866482158, 0.2402265069591007), r,
-                             0.6931471805599453), r, 1.0);
+    const double r = fma(d, scale, magic - z);
+    *p = fma(fma(fma(r, 0.05550410866482158, 0.2402265069591007), r, 0.6931471805599453), r, 1.0);
     *e = n >> 8;
-    return sh->table[n & 255] * p;
+    return sh->table[n & 255];
   }
   __device__ static double shifted(double v, int e) {
     return __hiloint2double(__double2hiint(v) + e * (1 << 20), __double2loint(v));
@@ -461,8 +464,9 @@ struct Row {
   // The weight; 0 below 2^-1000 (and for -inf and NaN).
   __device__ double weight(float x) const {
     int e;
-    const double v = power(x, &e);
-    return pos(x) < last ? shifted(v, e) : 0.0;
+    double p;
+    const double v = power(x, &p, &e);
+    return pos(x) < last ? shifted(v * p, e) : 0.0;
   }
   // A weight in units of 2^-unit, rounded: adding 2^52 leaves the nearest
   // integer in the low 52 bits. (A rounding of the bin's border may let a
@@ -473,8 +477,9 @@ struct Row {
   // The weight of x, f bins from M, in a bin's unit.
   __device__ unsigned units(float x, float f, int unit) const {
     int e;
-    const double v = power(x, &e);
-    const unsigned w = (unsigned)__double2loint(shifted(v, e + unit) + 4503599627370496.0);
+    double p;
+    const double v = power(x, &p, &e);
+    const unsigned w = (unsigned)__double2loint(fma(shifted(v, e + unit), p, 4503599627370496.0));
     return f < last ? w : 0u;
   }
   __device__ void add(int b, unsigned w) {
@@ -509,8 +514,10 @@ struct Row {
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         const float x = i + j < c1 ? load_f(xs[i + j]) : -INFINITY, f = pos(x);
-        b[j] = bin_at(f);
-        w[j] = units(x, f, unit_of(b[j]));
+        // bin_at and unit_of, without a conversion.
+        const float z = __fadd_rd(fminf(f, (float)(kBins - 1)), 8388608.f);
+        b[j] = __float_as_int(z) & 0x7FFFFF;
+        w[j] = units(x, f, kUnit + whole((z - 8388608.f) * octaves));
       }
 #pragma unroll
       for (int j = 0; j < 4; j++) add(b[j], w[j]);
@@ -518,16 +525,24 @@ struct Row {
     gather_histogram();
   }
   // The slices' histograms become the row's, in every CTA: each adds up its
-  // share of the bins and hands it to all, a thread per bin and CTA.
+  // share of the bins and hands it to all. A warp reads, and writes, one other
+  // CTA's neighbouring bins.
   __device__ void gather_histogram() {
     cluster.sync();
-    const int b = rank * (kBins / ranks) + threadIdx.x / ranks;
-    Shared* o = cluster.map_shared_rank(sh, threadIdx.x % ranks);
+    const int share = kBins / ranks, at = threadIdx.x & (share - 1), b = rank * share + at;
+    Shared* o = cluster.map_shared_rank(sh, threadIdx.x / share);
     unsigned c = o->count[b];
     u64 m = join(o->lo[b], o->hi[b]);
-    for (int d = 1; d < ranks; d *= 2) {
-      c += __shfl_xor_sync(0xFFFFFFFFu, c, d);
-      m += __shfl_xor_sync(0xFFFFFFFFu, m, d);
+    if (ranks > 1) {
+      sh->gather_count[threadIdx.x] = c;
+      sh->gather_mass[threadIdx.x] = m;
+      __syncthreads();
+      c = 0;
+      m = 0;
+      for (int r = 0; r < ranks; r++) {
+        c += sh->gather_count[r * share + at];
+        m += sh->gather_mass[r * share + at];
+      }
     }
     o->gcount[b] = c;
     o->gmass[b] = m;
