@@ -378,6 +378,7 @@ template <typename T>
 struct Row {
   Shared* sh;
   const T* xs;                   // this CTA's slice
+  int n;                         // its entries
   cg::cluster_group cluster;
   int rank, ranks;
   int start, per;                // the slice's first index, a slice's length
@@ -391,6 +392,25 @@ struct Row {
   float last;                    // bins from M to where weights are 0
 
   __device__ float at(int i) const { return clean(load_f(xs[i])); }
+
+  // f(four logits, place of the first) for all of the slice, in any order;
+  // behind the last, -inf.
+  template <typename F>
+  __device__ __forceinline__ void fours(F f) const {
+    constexpr int V = 16 / sizeof(T);
+    for (int v = threadIdx.x; v * V < n; v += kThreads) {
+      const uint4 r = reinterpret_cast<const uint4*>(xs)[v];
+      T e[V];
+      memcpy(e, &r, 16);
+#pragma unroll
+      for (int h = 0; h < V; h += 4) {
+        float x[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] = v * V + h + j < n ? load_f(e[h + j]) : -INFINITY;
+        f(x, v * V + h);
+      }
+    }
+  }
 
   // Drops the entries below `least` (and -inf) and returns how many stay. Up
   // to kKept of them are listed, so that the threads get equal shares;
@@ -508,20 +528,20 @@ struct Row {
   __device__ void histogram_of_all() {
     clear();
     // Four entries' weights side by side, then their additions.
-    for (int i = c0; i < c1; i += 4) {
+    fours([&](const float* x, int) {
       unsigned w[4];
       int b[4];
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const float x = i + j < c1 ? load_f(xs[i + j]) : -INFINITY, f = pos(x);
+        const float f = pos(x[j]);
         // bin_at and unit_of, without a conversion.
         const float z = __fadd_rd(fminf(f, (float)(kBins - 1)), 8388608.f);
         b[j] = __float_as_int(z) & 0x7FFFFF;
-        w[j] = units(x, f, kUnit + whole((z - 8388608.f) * octaves));
+        w[j] = units(x[j], f, kUnit + whole((z - 8388608.f) * octaves));
       }
 #pragma unroll
       for (int j = 0; j < 4; j++) add(b[j], w[j]);
-    }
+    });
     gather_histogram();
   }
   // The slices' histograms become the row's, in every CTA: each adds up its
@@ -730,16 +750,18 @@ struct Row {
         });
       } else {
         // The bin's entries are listed for the last look at them.
-#pragma unroll 4
-        for (int i = c0; i < c1; i++) {
-          const float x = load_f(xs[i]), f = pos(x);
-          above += f < from;
-          if (f >= from && f < to && x >= floor) {
-            divide(x, f);
-            const unsigned p = atomicAdd(&sh->fill, 1u);
-            if (p < kKept) sh->kept[p] = (unsigned short)i;
+        fours([&](const float* x, int i) {
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const float f = pos(x[j]);
+            above += f < from;
+            if (f >= from && f < to && x[j] >= floor) {
+              divide(x[j], f);
+              const unsigned p = atomicAdd(&sh->fill, 1u);
+              if (p < kKept) sh->kept[p] = (unsigned short)(i + j);
+            }
           }
-        }
+        });
       }
       gather_histogram();
       own = sh->fill;
@@ -1010,7 +1032,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleArgs a) {
   }
 
   const int chunk = ((a.per + kThreads - 1) / kThreads) | 1;  // odd: no bank conflicts
-  Row<T> r{sh, xs, cluster, rank, ranks, start, a.per};
+  Row<T> r{sh, xs, n, cluster, rank, ranks, start, a.per};
   r.c0 = min((int)threadIdx.x * chunk, n);
   r.c1 = min(r.c0 + chunk, n);
   if (top == INFINITY) {
