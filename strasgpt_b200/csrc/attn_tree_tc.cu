@@ -567,36 +567,47 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (ok) {
             const uint8_t* from = gbase + (ring - base) + (u % kRing) * C::kUnit;
             uint8_t* to = gbase + (is_v ? C::kTile : 0);
-            constexpr int kItems = kKeys * (HD / 8);
-#pragma unroll 3
-            for (int x = id; x < kItems; x += kLoaders) {
-              const int r = x / (HD / 8), c = x % (HD / 8);
-              float4 f = make_float4(0.f, 0.f, 0.f, 0.f), g = f;
-              if (r < rows) {  // zeros behind the last key
-                f = *reinterpret_cast<const float4*>(from + x * 32);
-                g = *reinterpret_cast<const float4*>(from + x * 32 + 16);
-              }
-              float e[8] = {f.x, f.y, f.z, f.w, g.x, g.y, g.z, g.w};
-              uint8_t* at = to + at_sw128(kKeys, r, c);
+            // A warp takes four rows at a time, eight lanes each: rows r and
+            // r + 4 in half a warp, which with the swizzle have all banks.
+#pragma unroll 1
+            for (int it = warp - 10; it < kKeys / 4; it += kLoadWarps) {
+              const int r = (it >> 1) * 8 + (it & 1) * 2 + (lane >> 4) + ((lane >> 3) & 1) * 4;
+              float4 v[HD / 32];
 #pragma unroll
-              for (int p = 0; p < 3; p++) {
-                *reinterpret_cast<uint4*>(at + p * C::kPart) =
-                    make_uint4(upper(e[0], e[1]), upper(e[2], e[3]), upper(e[4], e[5]),
-                               upper(e[6], e[7]));
+              for (int j = 0; j < HD / 32; j++)
+                v[j] = r < rows ? *reinterpret_cast<const float4*>(from + r * HD * 4 + j * 128 +
+                                                                   (lane & 7) * 16)
+                                : make_float4(0.f, 0.f, 0.f, 0.f);  // behind the last key
+              uint8_t* at = to + r * 128 + (lane & 1) * 8;
 #pragma unroll
-                for (int j = 0; j < 8; j++) e[j] = rest(e[j]);
+              for (int j = 0; j < HD / 32; j++) {
+                uint8_t* p = at + (j >> 1) * kKeys * 128 +
+                             ((((j & 1) * 4 + ((lane & 7) >> 1)) ^ (r & 7)) << 4);
+                f32x2 x = pack(v[j].x, v[j].y), y = pack(v[j].z, v[j].w);
+#pragma unroll
+                for (int q = 0; q < 3; q++) {
+                  float x0, x1, y0, y1;
+                  unpack(x, x0, x1);
+                  unpack(y, y0, y1);
+                  *reinterpret_cast<uint2*>(p + q * C::kPart) =
+                      make_uint2(upper(x0, x1), upper(y0, y1));
+                  if (q < 2) {
+                    x = rest2(x);
+                    y = rest2(y);
+                  }
+                }
               }
             }
             fence_operands();
             mbar_arrive(saddr(is_v ? &v_full[0] : &k_full[0]));
           }
           mbar_arrive(saddr(&raw_empty[u % kRing]));
-          // The first warp refills the buffer of the unit before, which the
+          // The last warp refills the buffer of the unit before, which the
           // others are done with by now as a rule.
-          if (warp == 10 && u > 0 && u - 1 + kRing < units) {
+          if (warp == 15 && u > 0 && u - 1 + kRing < units) {
             ok = ok && warp_wait(saddr(&raw_empty[(u - 1) % kRing]), ((u - 1) / kRing) & 1,
                                  &failed);
-            if (id == 0 && ok) fetch(u - 1 + kRing);
+            if (one && ok) fetch(u - 1 + kRing);
             __syncwarp();
           }
         }
