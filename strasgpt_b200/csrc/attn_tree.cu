@@ -17,10 +17,12 @@
 // and carries the probabilities as two bf16 parts, so that the only rounding
 // to bf16 is that of the result.
 //
-// What bounds it: the cache's bytes with up to 16 rows a kv head (90 us for
-// 8 heads of 128000 bf16 keys of 128 entries, 5.8 TB/s; 238 us, 4.4 TB/s, in
-// fp32), mma.sync above; from 17 or 33 rows on the cached keys are
-// attn_tree_tc.cu's (see on_tc).
+// What bounds it: the cache's bytes with up to 16 rows a kv head in bf16 (90
+// us for 8 heads of 128000 keys of 128 entries, 5.8 TB/s); mma.sync in fp32
+// (238 us, 4.4 TB/s: its three products take 174 us of that, as the slope from
+// 32 to 64 rows says) and above; from 17 or 33 rows on the cached keys are
+// attn_tree_tc.cu's (see on_tc). Short caches are latency: 9 us for one token
+// over 613 keys, both kernels.
 #include "attn_tree.h"
 
 #include <limits.h>
@@ -728,11 +730,11 @@ Shape shape_of(int rows) {
 // Whether the cached keys go to tcgen05 (attn_tree_tc.cu): where mma.sync, not
 // the cache's bytes, is what bounds this file's kernel. Measured with 8 kv
 // heads, us here / there:
-//   head_dim 128, 16 rows: bf16 128000 keys 92 / 92, 8000 13.5 / 15.4;
-//                          fp32 128000 keys 245 / 335
-//                 32 rows: bf16 119 / 92, 19.1 / 16.3; fp32 431 / 337
-//   head_dim 64,  32 rows: bf16 77 / 70, 11.4 / 13.2; fp32 191 / 241
-//                 48 rows: bf16 121 / 71, 14.2 / 13.6; fp32 338 / 241
+//   head_dim 128, 16 rows: bf16 128000 keys 92 / 91, 8000 14.0 / 15.6;
+//                          fp32 128000 keys 244 / 295, 8000 29 / 32
+//                 32 rows: bf16 119 / 93, 19.0 / 16.5; fp32 409 / 301, 40 / 33
+//   head_dim 64,  32 rows: bf16 76 / 69, 11.3 / 13.3; fp32 190 / 211, 22 / 23
+//                 48 rows: bf16 120 / 69, 14.2 / 13.6; fp32 338 / 212, 32 / 23
 // Not for many drafted tokens, whose own keys the merge reads one by one, and
 // not for head_dim 32.
 bool on_tc(int t, int group, int hd) {

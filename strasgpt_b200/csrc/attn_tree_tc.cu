@@ -2,32 +2,43 @@
 //
 // A CTA has 128 rows (drafted token, q head) of one kv head and a share of
 // the cached keys, which all of its rows see. Sixteen warps: two warpgroups
-// of softmax, one thread per row, that take the key tiles in turn; two warps
-// that issue the matrix instructions, one Q K^T and one P V, so that neither
-// waits for what the other waits for; six that bring in keys and values. Per tile of 64 keys: S = Q K^T into tensor memory; its warpgroup
-// reads S, subtracts the running maximum and writes P = 2^(S - m) over it, as
-// bf16 parts; then O (+)= P V in tensor memory. Each warpgroup has its own
-// maximum, sum and output, joined at the end, so that one's softmax runs
-// under the other's matrix instructions.
+// of softmax, one thread per row, that take the key tiles in turn; a warp
+// that issues Q K^T and one that issues P V, so that neither waits for what
+// the other waits for; six that bring in keys and values. Per tile of 64
+// keys: S = Q K^T into tensor memory; its warpgroup reads S, subtracts the
+// running maximum and writes P = 2^(S - m) over it, as bf16 parts; then
+// O (+)= P V in tensor memory. Each warpgroup has its own maximum, sum and
+// output, joined at the end, so that one's softmax runs under the other's
+// matrix instructions.
 //
-// bf16: O stays in tensor memory. A new maximum rescales it only when it is
-// 2^8 above the one that P is relative to (P is at most 2^8 then), which
-// happens in the first few tiles as a rule. fp32: the tensor cores' sums are
-// cut, not rounded, so each tile's O starts from zero and is added, scaled,
-// to the warpgroup's registers.
+// bf16: K and V by TMA, a warp each; Q in shared memory (128 entries) or
+// tensor memory (64); O stays in tensor memory. A new maximum rescales it
+// only when it is 2^8 above the one that P is relative to (P is at most 2^8
+// then), which happens in the first few tiles as a rule.
+// fp32: rows by bulk copies into a ring, from which six warps write their
+// parts. The tensor cores' sums are cut, not rounded, so each tile's O starts
+// from zero and is added, scaled, to the warpgroup's registers.
 //
-// Q and P are operands in tensor memory: read from shared memory, Q alone
-// would take two thirds of its bandwidth at 64 keys a tile. Keys and values
-// lie in shared memory as rows of 64 head entries (128 bytes, 128-byte
+// P, and fp32's Q, are operands in tensor memory: read from shared memory, Q
+// alone would take two thirds of its bandwidth at 64 keys a tile. Keys and
+// values lie in shared memory as rows of 64 head entries (128 bytes, 128-byte
 // swizzle): K-major for Q K^T, the same rows MN-major for P V.
 //
 // Precision. bf16: operands as they are, P as two bf16 parts (2^-17). fp32:
 // every operand as three bf16 parts of 8 bits each, all 24 of them, and the six
 // products that matter (the others are below 2^-24).
 //
-// Bound, in cycles per key and SM: the cache's bytes 23 (bf16, one row tile;
-// fp32 46; row tiles of the same keys share what L2 holds), exp2 8, issue of
-// the softmax 11, matrix instructions 12 (bf16) or 48 (fp32's six products).
+// Measured, 8 kv heads of head_dim 128: 256 rows over 65500 bf16 keys 97 us
+// (2.8 TB/s of cache, 710 TFLOP/s), over 32768 fp32 keys 170 us (1.6 TB/s,
+// 200 TFLOP/s); 32 rows over 128000 keys 93 us (5.6 TB/s) and 301 us (3.5
+// TB/s). What bounds 128 rows and more: bf16, 0.7 us per tile, the matrix
+// instructions (0.4 us: 32 cycles per 16 entries of Q K^T from tensor memory,
+// 48 from shared memory, 64 per 16 keys and part of P V) and the hand-overs
+// between them and the softmax; fp32, 2.9 us per tile, the six warps that make
+// parts (0.9 us for 64 rows, and as much again in waiting and handing over),
+// while the matrix instructions take 1.6. Two fp16 parts of scaled rows and
+// half the matrix instructions were slower (226 us): the rows' largest values
+// cost those warps more than the third part.
 #include "attn_tree.h"
 
 #include <cuda.h>
@@ -644,10 +655,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < kBatch; j++)
             *reinterpret_cast<uint4*>(gbase + (q_at - base) + at_sw128(kRows, r, c * kBatch + j)) =
                 x[j];
-          continue;
         }
+        // 16 entries at a time, 8 columns a part.
 #pragma unroll
-        for (int h = 0; h < kBatch * kVec / 16; h++) {  // 16 entries, 8 columns a part
+        for (int h = 0; h < (C::kQShared ? 0 : kBatch * kVec / 16); h++) {
           uint32_t e[C::kParts][8];
           if constexpr (kF32) {
 #pragma unroll

@@ -27,8 +27,19 @@
 // the bin in which a filter's border lies (a count for top-k, a mass for
 // top-p); the entries of that bin, a few as a rule, are exchanged and ranked
 // among themselves. A bin with more entries than kList is divided again, by
-// distance and then by key, until few or only equal ones are left. Where top-k's bound leaves at
-// most kThreads entries of the row, one CTA sorts those and does the rest.
+// distance and then by key, until few or only equal ones are left. Where
+// top-k's bound leaves at most kThreads entries of the row, one CTA sorts
+// those and does the rest. Many rows under top-k: see k_sample_rows.
+//
+// What bounds it, measured: one row of 128256 fp32 logits under top-k 50 takes
+// 12 us, a chain of reading, two exchanges between CTAs, a sort. 64 rows of
+// 151936 under top-p 0.95, 97 us: two rounds of CTAs, 31 us each, of which the
+// histogram's 64-bit weights and shared-memory additions are 10 us (0.5 cycles
+// an entry and SM), four exchanges 11, the division of the border's bin 4, the
+// reading 3. 256 rows of 201088 bf16 logits under top-k 200, 56 us (1.8 TB/s;
+// 16 us of bytes): two reads, the second from L2, and a sort per row. Slices
+// read again from L2 instead of kept in shared memory were slower at every
+// size (64 rows of 151936: 129 us).
 #include <cooperative_groups.h>
 #include <float.h>
 
@@ -1203,18 +1214,21 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleArgs a) {
   }
 }
 
-// From this many rows on, where a top-k is given, k_sample_rows goes first.
-constexpr int kManyRows = 32;
 // A slice that leaves room for two CTAs on an SM.
 constexpr int kSliceBytes = 78 * 1024;
 
 template <typename T>
-cudaError_t launch(SampleArgs a, int rows, int cluster, int dev, cudaStream_t s) {
+cudaError_t launch(SampleArgs a, int rows, int cluster, int sms, int dev, cudaStream_t s) {
   static std::atomic<size_t> allowed[sg::kDevices];
   const size_t smem = sizeof(Shared) + (size_t)a.per * sizeof(T);
   cudaError_t e = sg::allow_smem(k_sample<T>, smem, dev, allowed);
   if (e != cudaSuccess) return e;
-  a.pending = a.top_k && rows >= kManyRows;
+  // Where a top-k is given and the GPU does not hold all clusters at once (two
+  // CTAs on an SM), k_sample_rows goes first: 128256 fp32 logits under top-k 50
+  // and top-p, 48 rows 22 us, 128 rows 33 us, against 28 and 67 with clusters
+  // only; 32 rows 21 against 19. Where it finds no top-k in any row it costs
+  // 10 us (64 rows 85 against 75).
+  a.pending = a.top_k && rows * cluster > 2 * sms;
   if (a.pending) {
     e = sg::try_launch(k_sample_rows<T>, dim3((unsigned)rows), dim3(kThreads), 0, 1, s, a);
     if (e != cudaSuccess) return e;
@@ -1270,8 +1284,8 @@ extern "C" int strasgpt_k_sample(const void* logits, int type, long long ld, int
   a.token = token; a.prob = prob; a.kept = kept;
   a.vec = sg::aligned(logits, 16) && (rows == 1 || ld * size % 16 == 0);
   const cudaStream_t s = (cudaStream_t)stream;
-  const cudaError_t e = type == STRASGPT_F32 ? launch<float>(a, rows, cluster, dev, s)
-                                             : launch<uint16_t>(a, rows, cluster, dev, s);
+  const cudaError_t e = type == STRASGPT_F32 ? launch<float>(a, rows, cluster, sms, dev, s)
+                                             : launch<uint16_t>(a, rows, cluster, sms, dev, s);
   if (e != cudaSuccess) return sg::refuse_cuda(me, "launch", e);
   return 0;
 }

@@ -703,11 +703,12 @@ def test_sample_parameters_differ_by_row_and_replays_agree(cuda):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("type_", [F32, BF16])
-@pytest.mark.parametrize("rows,vocab", [(32, 1), (33, 60), (40, 700), (47, 5003), (64, 40001),
-                                        (36, 201088)])
+@pytest.mark.parametrize("rows,vocab", [(300, 1), (301, 60), (330, 700), (299, 5003),
+                                        (150, 40001), (40, 201088), (40, 700)])
 def test_sample_many_rows_under_top_k(cuda, type_, rows, vocab):
-    """From 32 rows on a top-k row may be a block's own: here with rows among
-    them that are not (no top-k, one above 512, one of the whole vocabulary)."""
+    """More rows than the GPU holds clusters: a top-k row may be a block's own;
+    here with rows among them that are not (no top-k, one above 512, one of the
+    whole vocabulary)."""
     torch = cuda
     rng = np.random.RandomState(rows)
     ks = [0, 1, 2, 50, 300, 511, 512, 513, 2000, vocab - 1, vocab, -4]
@@ -749,12 +750,13 @@ def test_sample_many_rows_masked_and_odd_values(cuda, type_, vocab):
     x[15, 0] = high                              # far above the others
     x[16] = -inf
     x[16, 3] = inf                               # one infinity, nothing else
+    x = x[:20].repeat(15, 1)                     # more rows than clusters at once
     rng = np.random.RandomState(8)
     for k in (1, 2, 40, 300, 512):
         for heat in (1.0, 1e-3, 1e30):
             for f in (dict(), dict(top_p=0.7), dict(min_p=0.3)):
                 check_sample(torch, x, heat=heat, top_k=k,
-                             u=rng.uniform(0, 1, 36).astype(np.float32), **f)
+                             u=rng.uniform(0, 1, 300).astype(np.float32), **f)
     token, prob, kept = run_sample(torch, x, u=0.3, heat=float("inf"), top_k=300)
     assert token[1] == -1 and kept[11] == 100 and abs(prob[11] - 0.01) < 1e-8
     assert kept[12] == 12 and abs(prob[12] * 12 - 1) < 1e-6
@@ -765,9 +767,9 @@ def test_sample_many_rows_masked_and_odd_values(cuda, type_, vocab):
 def test_sample_many_rows_of_a_wider_matrix(cuda, type_):
     torch = cuda
     for start, vocab, ld in ((1, 4099, 4111), (8, 4096, 4120), (3, 129, 1000)):
-        big = torch.full((35 * ld + 8,), float("inf"), device="cuda", dtype=dtype(torch, type_))
-        x = logits(torch, 35, vocab, type_, ld)
-        view = big[start:start + 35 * ld].view(35, ld)[:, :vocab]
+        big = torch.full((300 * ld + 8,), float("inf"), device="cuda", dtype=dtype(torch, type_))
+        x = logits(torch, 300, vocab, type_, ld)
+        view = big[start:start + 300 * ld].view(300, ld)[:, :vocab]
         view.copy_(x)
         check_sample(torch, view, top_k=30, top_p=0.9, u=0.77, ld=ld)
 
@@ -792,7 +794,7 @@ def test_sample_calls_at_once(cuda):
     """Many rows with a block each on one stream, a few rows on another, at
     the same time: what each gives alone."""
     torch = cuda
-    a, b = logits(torch, 64, 50000, BF16, 1), logits(torch, 9, 128256, F32, 2)
+    a, b = logits(torch, 150, 50000, BF16, 1), logits(torch, 9, 128256, F32, 2)
     ka = dict(top_k=50, top_p=0.9, u=0.35)
     kb = dict(top_p=0.9, u=0.8)
     one, two = check_sample(torch, a, **ka), check_sample(torch, b, **kb)
