@@ -33,10 +33,10 @@
 //
 // What bounds it, measured: one row of 128256 fp32 logits under top-k 50 takes
 // 12 us, a chain of reading, two exchanges between CTAs, a sort. 64 rows of
-// 151936 under top-p 0.95, 97 us: two rounds of CTAs, 31 us each, of which the
+// 151936 under top-p 0.95, 87 us: two rounds of CTAs, 31 us each, of which the
 // histogram's 64-bit weights and shared-memory additions are 10 us (0.5 cycles
 // an entry and SM), four exchanges 11, the division of the border's bin 4, the
-// reading 3. 256 rows of 201088 bf16 logits under top-k 200, 56 us (1.8 TB/s;
+// reading 3. 256 rows of 201088 bf16 logits under top-k 200, 53 us (1.9 TB/s;
 // 16 us of bytes): two reads, the second from L2, and a sort per row. Slices
 // read again from L2 instead of kept in shared memory were slower at every
 // size (64 rows of 151936: 129 us).
@@ -253,10 +253,10 @@ __device__ __forceinline__ void finish(const SampleArgs& a, int row, u64 mark, i
 
 // Many rows under top-k: a block per row reads it twice, once for the largest
 // logits of 1024 groups (two a thread), whose k-th largest bounds the row's,
-// and once, from L2, for the entries above that bound, at most kThreads. No
-// block waits for another. A row that this does not serve (no top-k, or too
-// many entries left, or infinite logits) gets the token kPending and is the
-// cluster kernel's.
+// and once, in part from L2, for the entries above that bound, at most
+// kThreads. No block waits for another. A row that this does not serve (no
+// top-k up to kThreads, too many entries left, infinite logits) gets the token
+// kPending and is the cluster kernel's.
 constexpr int kPending = -2;
 
 template <typename T>
@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(SampleArgs a) {
   const float p = a.top_p ? a.top_p[row] : 1.f;
   const float min_p = a.min_p ? a.min_p[row] : 0.f;
   const bool greedy = !(T_ > 0.f) || k == 1 || p <= 0.f;
-  if (!greedy && (k <= 0 || k > kThreads || k >= a.vocab)) {
+  if (k <= 0 || k > kThreads || k >= a.vocab) {
     if (tid == 0) a.token[row] = kPending;
     return;
   }
@@ -282,9 +282,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(SampleArgs a) {
   constexpr int V = 16 / sizeof(T);
   const int nv = a.vec ? a.vocab / V : 0;
   // f(logit, index) for all of the row; a NaN or -inf fails its comparisons.
-  auto each = [&](auto f) {
+  // The second time from the end: what was read last is in L2 (256 rows of
+  // 201088 bf16, 56.5 -> 53.4 us).
+  auto each = [&](bool back, auto f) {
+    const int number = nv > tid ? (nv - 1 - tid) / kThreads + 1 : 0;
+    const int step = back ? -kThreads : kThreads;
+    int v = back ? tid + (number - 1) * kThreads : tid;
 #pragma unroll 4
-    for (int v = tid; v < nv; v += kThreads) {
+    for (int left = number; left > 0; left--, v += step) {
       const uint4 r = reinterpret_cast<const uint4*>(src)[v];
       T e[V];
       memcpy(e, &r, 16);
@@ -294,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(SampleArgs a) {
     for (int i = nv * V + tid; i < a.vocab; i += kThreads) f(load_f(src[i]), i);
   };
   float top[2] = {-INFINITY, -INFINITY};
-  each([&](float x, int i) { top[i & 1] = fmaxf(top[i & 1], x); });
+  each(false, [&](float x, int i) { top[i & 1] = fmaxf(top[i & 1], x); });
   top[0] += 0.f;  // -0 is 0
   top[1] += 0.f;
   float M = fmaxf(top[0], top[1]);
@@ -332,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(SampleArgs a) {
   if (greedy) {
     // The largest, at its lowest index.
     int first = INT_MAX;
-    each([&](float x, int i) { first = x == M ? min(first, i) : first; });
+    each(true, [&](float x, int i) { first = x == M ? min(first, i) : first; });
     if (first < INT_MAX) atomicMin(&found, first);
     __syncthreads();
     if (tid == 0) {
@@ -365,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample_rows(SampleArgs a) {
                     ? least
                     : __double2float_rd((double)M - (bin + 1.01) / (double)bins_per -
                                         1e-6 * (fabs((double)M) + (double)(M - least))));
-  each([&](float x, int i) {
+  each(true, [&](float x, int i) {
     if (x >= floor) {
       const unsigned at = atomicAdd(&fill, 1u);
       if (at < kThreads) few[at] = ((u64)key_of(x + 0.f) << 32) | (unsigned)(INT_MAX - i);
@@ -1226,8 +1231,8 @@ cudaError_t launch(SampleArgs a, int rows, int cluster, int sms, int dev, cudaSt
   // Where a top-k is given and the GPU does not hold all clusters at once (two
   // CTAs on an SM), k_sample_rows goes first: 128256 fp32 logits under top-k 50
   // and top-p, 48 rows 22 us, 128 rows 33 us, against 28 and 67 with clusters
-  // only; 32 rows 21 against 19. Where it finds no top-k in any row it costs
-  // 10 us (64 rows 85 against 75).
+  // only; 32 rows 21 against 19. A row without a top-k is not its own, greedy
+  // ones neither: one block would read all of it.
   a.pending = a.top_k && rows * cluster > 2 * sms;
   if (a.pending) {
     e = sg::try_launch(k_sample_rows<T>, dim3((unsigned)rows), dim3(kThreads), 0, 1, s, a);
