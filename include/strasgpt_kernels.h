@@ -2,9 +2,9 @@
 // that manage their own device buffers. All pointers are DEVICE pointers;
 // `stream` is a cudaStream_t (NULL: the legacy default stream). Each call
 // only enqueues work; it returns 0, or dies with "[StrasGPT] Error ..." on an
-// invalid shape (or, where it says so, returns -1). None of these has a counterpart in the reference API: they
-// expose the pieces of transformer_predict_chunk (source/transformer.c:
-// 1186-1602) one at a time.
+// invalid shape (or, where it says so, returns -1). None of these has a
+// counterpart in the reference API: they expose the pieces of
+// transformer_predict_chunk (source/transformer.c:1186-1602) one at a time.
 #ifndef STRASGPT_KERNELS_H
 #define STRASGPT_KERNELS_H
 
@@ -180,9 +180,10 @@ int strasgpt_k_attn_tree(const void* q, long long ldq, const void* k_cache,
 // of all that remain (u not above 0: the first, u not below 1: the last; an
 // entry whose w is 0 in 64 bits is never drawn). Weights and sums are held in
 // 64 bits, weights to 2^-42 of themselves. prob (NULL: not wanted) gets the
-// token's share of the remaining mass, kept (NULL) how many entries remained. NaN logits count as
-// -inf, which are never taken; a row of nothing else gets token -1, prob 0,
-// kept 0. vocab is at most STRASGPT_SAMPLE_MAX_VOCAB. The result does not
+// token's share of the remaining mass, kept (NULL) how many entries remained.
+// NaN logits count as -inf, which are never taken; a row of nothing else gets
+// token -1, prob 0, kept 0. Where logits are +inf, those weigh 1 and all
+// others 0. vocab is at most STRASGPT_SAMPLE_MAX_VOCAB. The result does not
 // depend on timing: the same inputs give the same bits.
 #define STRASGPT_SAMPLE_MAX_VOCAB 360448
 int strasgpt_k_sample(const void* logits, int type, long long ld, int rows,

@@ -170,7 +170,7 @@ extern "C" int strasgpt_k_rope(const void* x, long long x_token_stride, long lon
   if (rope->dim < 2 || rope->dim % 2 || rope->dim > head_dim || rope->dim > 2 * kMaxPairs)
     return sg::refuse(me, "the turned part must be even, 2 to min(head_dim, 512) entries");
   if (!(rope->theta > 0) || !isfinite(rope->theta)) return sg::refuse(me, "theta must be positive");
-  if (!isfinite(rope->magnitude)) return sg::refuse(me, "magnitude must be finite");
+  if (!isfinite((float)rope->magnitude)) return sg::refuse(me, "magnitude must be finite");
   if (rope->scaling < STRASGPT_ROPE_NONE || rope->scaling > STRASGPT_ROPE_BANDS)
     return sg::refuse(me, "unknown scaling");
   if (rope->scaling != STRASGPT_ROPE_NONE && (!(rope->factor > 0) || !isfinite(rope->factor)))

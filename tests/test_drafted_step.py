@@ -402,6 +402,75 @@ def test_tree_offsets_beyond_32_bits(cuda):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("type_", [F32, BF16])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_tree_many_rows_one_split_and_wide_rows(cuda, type_, hd):
+    """As above where the cached keys have a kernel of their own: one split per
+    kv head, q and att as parts of wider rows."""
+    torch = cuda
+    t, kh, g, n = 40, 160, 1, 200
+    q0, k, v = inputs(torch, t, kh, g, hd, 250, type_, 6)
+    wide = torch.full((t, kh * g * hd + 64), float("nan"), device="cuda", dtype=q0.dtype)
+    wide[:, 32:-32] = q0.view(t, -1)
+    q = wide[:, 32:-32].view(t, kh * g, hd)
+    out = torch.full((t, kh * g * hd + 48), 7.0, device="cuda").to(q0.dtype)
+    att = out[:, 16:-32].view(t, kh * g, hd)
+    m = tree_mask(t, 1)
+    run_tree(torch, q, k, v, n, m, type_, att=att)
+    want, reach, top = tree_reference(torch, q, k, v, n, m)
+    err = (att.double() - want).abs()
+    assert (err <= tree_tolerance(want, reach, top, n + t, hd, type_)).all()
+    assert (out[:, :16] == 7).all() and (out[:, -32:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [F32, BF16])
+def test_tree_many_rows_with_offsets_beyond_32_bits(cuda, type_):
+    """The same caches of more than 2^31 entries as above, for more rows per kv
+    head."""
+    torch = cuda
+    t, g, hd = 5, 4, 128
+    for kh, ctx, n in ((5, 3_500_000, 90), (1, 17_000_016, 17_000_000)):
+        k = torch.zeros(kh, ctx, hd, device="cuda", dtype=dtype(torch, type_))
+        v = torch.zeros_like(k)
+        q, k2, v2 = inputs(torch, t, kh, g, hd, 64, type_, 11)
+        k[:, n + t - 64:n + t] = k2
+        v[:, n + t - 64:n + t] = 1000 * v2
+        m = tree_mask(t, 6)
+        got = run_tree(torch, q, k, v, n, m, type_).double()
+        zeros = n + t - 64
+        want = torch.zeros(t, kh * g, hd, dtype=torch.float64, device="cuda")
+        for h in range(kh * g):
+            for i in range(t):
+                see = torch.cat([torch.ones(64 - t, dtype=torch.bool),
+                                 torch.from_numpy(m[i])]).cuda()
+                s = k2[h // g][see].double() @ q[i, h].double() / hd ** 0.5
+                w = torch.exp(s)
+                want[i, h] = w @ (1000 * v2)[h // g][see].double() / (w.sum() + zeros)
+        scale = want.abs().max()
+        assert scale > 0
+        assert ((got - want).abs() <= B * want.abs() + 2.0 ** -12 * scale).all()
+        del k, v
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [F32, BF16])
+@pytest.mark.parametrize("scale", [1e-12, 1e12])
+@pytest.mark.parametrize("t", [3, 24])
+def test_tree_large_and_small_numbers(cuda, type_, t, scale):
+    """Keys and values far from 1, queries that bring the scores back: nothing
+    overflows or vanishes on the way."""
+    torch = cuda
+    q, k, v = inputs(torch, t, 2, 4, 128, 700, type_, 9)
+    q, k, v = q / scale, k * scale, v * scale ** 2
+    m = tree_mask(t, 3)
+    want, reach, top = tree_reference(torch, q, k, v, 600, m)
+    got = run_tree(torch, q, k, v, 600, m, type_)
+    err = (got.double() - want).abs()
+    assert (err <= tree_tolerance(want, reach, top, 600 + t, 128, type_)).all(), err.max().item()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [F32, BF16])
 @pytest.mark.parametrize("t,g,hd", [(9, 4, 128), (17, 1, 128), (33, 1, 64), (256, 1, 64),
                                     (2, 128, 128), (1, 128, 32)])
 def test_tree_caches_that_end_with_the_tree(cuda, type_, t, g, hd):
@@ -922,6 +991,7 @@ def refused(capfd, status, words):
     (dict(rope=dict(dim=130)), "turned part"), (dict(rope=dict(theta=0.0)), "theta"),
     (dict(rope=dict(theta=float("nan"))), "theta"),
     (dict(rope=dict(magnitude=float("inf"))), "magnitude"),
+    (dict(rope=dict(magnitude=1e300)), "magnitude"),
     (dict(rope=dict(scaling=3)), "unknown scaling"),
     (dict(rope=dict(scaling=1, factor=0.0)), "factor"),
     (dict(rope=dict(scaling=2, factor=2.0, low=4.0, high=4.0)), "bands"),
