@@ -18,11 +18,12 @@
 // to bf16 is that of the result.
 //
 // What bounds it: the cache's bytes with up to 16 rows a kv head in bf16 (90
-// us for 8 heads of 128000 keys of 128 entries, 5.8 TB/s); mma.sync in fp32
-// (238 us, 4.4 TB/s: its three products take 174 us of that, as the slope from
-// 32 to 64 rows says) and above; from 17 or 33 rows on the cached keys are
-// attn_tree_tc.cu's (see on_tc). Short caches are latency: 9 us for one token
-// over 613 keys, both kernels.
+// us for 8 heads of 128000 keys of 128 entries, 5.8 TB/s) and up to 4 in fp32
+// (190 us, 5.5 TB/s, by FMAs: k_tree_few); mma.sync in fp32 with 16 (244 us:
+// its three products take 174 us of that, as the slope from 32 to 64 rows
+// says) and above; from 17 or 33 rows on the cached keys are attn_tree_tc.cu's
+// (see on_tc). Short caches are latency: 7.4 us for one token over 613 keys,
+// both kernels.
 #include "attn_tree.h"
 
 #include <limits.h>
@@ -122,6 +123,56 @@ struct Tile {
   static constexpr size_t kBytes = (size_t)kStages * kStage;
 };
 
+// The tiles of a split: the cached keys, then the drafted ones. A tile holds
+// keys of one kind, never of both.
+template <typename T, int HD, int THREADS>
+struct Walk {
+  using L = Tile<T, HD>;
+  const T *k, *v;                // of the kv head
+  int t, n, old_tiles, tile0, tile1;
+  uint32_t smem;
+
+  // The cache's length is read on the device (a captured call serves every
+  // later length); one outside the cache is cut to it.
+  __device__ Walk(const TreeArgs& a, int split, int head, const void* stages) {
+    t = a.t;
+    n = sg::tree_cached(a);
+    old_tiles = (n + L::kKeys - 1) / L::kKeys;
+    const int tiles = old_tiles + (t + L::kKeys - 1) / L::kKeys;
+    const int per = (tiles + a.splits - 1) / a.splits;
+    tile0 = split * per;
+    tile1 = min(tiles, tile0 + per);
+    k = static_cast<const T*>(a.k) + (size_t)head * a.ctx * HD;
+    v = static_cast<const T*>(a.v) + (size_t)head * a.ctx * HD;
+    smem = saddr(stages);
+  }
+  // First cache row of a tile and its rows.
+  __device__ void extent(int tile, int& row, int& rows) const {
+    const bool old = tile < old_tiles;
+    const int k0 = (old ? tile : tile - old_tiles) * L::kKeys;
+    row = old ? k0 : n + k0;
+    rows = min(L::kKeys, (old ? n : t) - k0);
+  }
+  __device__ void fetch(int tile) const {
+    if (tile < tile1) {
+      int row, rows;
+      extent(tile, row, rows);
+      const uint32_t ks = smem + (tile - tile0) % kStages * L::kStage;
+      const uint32_t vs = ks + L::kKeys * L::kKRow;
+      constexpr int kVecs = HD * (int)sizeof(T) / 16;
+#pragma unroll 8
+      for (int i = threadIdx.x; i < L::kKeys * kVecs; i += THREADS) {
+        const int r = i / kVecs, x = i % kVecs;
+        const int bytes = r < rows ? 16 : 0;  // rows behind the last key are zeros
+        const size_t at = (size_t)(row + (r < rows ? r : 0)) * HD + x * (16 / sizeof(T));
+        cp_async16(ks + r * L::kKRow + x * 16, k + at, bytes);
+        cp_async16(vs + r * L::kVRow + x * 16, v + at, bytes);
+      }
+    }
+    cp_async_commit();
+  }
+};
+
 // MW warps side by side in rows (16 each), KW in keys.
 template <typename T, int HD, int MW, int KW>
 __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(TreeArgs a) {
@@ -142,45 +193,11 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Tree
   sg::pdl_trigger();
   sg::pdl_wait();
 
-  // The cache's length is read on the device (a captured call serves every
-  // later length); one outside the cache is cut to it.
-  const int n = sg::tree_cached(a);
-  const int old_tiles = (n + kKeys - 1) / kKeys;
-  const int tiles = old_tiles + (a.t + kKeys - 1) / kKeys;
-  const int per = (tiles + a.splits - 1) / a.splits;
-  const int tile0 = split * per, tile1 = min(tiles, tile0 + per);
+  const Walk<T, HD, kThreads> walk(a, split, head, smem);
+  const int n = walk.n, old_tiles = walk.old_tiles, tile0 = walk.tile0, tile1 = walk.tile1;
   if (tile0 >= tile1) return;
-
-  const T* kbase = static_cast<const T*>(a.k) + (size_t)head * a.ctx * HD;
-  const T* vbase = static_cast<const T*>(a.v) + (size_t)head * a.ctx * HD;
-  // First cache row of a tile and its rows: a tile holds cached keys or
-  // drafted ones, never both.
-  auto extent = [&](int tile, int& row, int& rows) {
-    const bool old = tile < old_tiles;
-    const int k0 = (old ? tile : tile - old_tiles) * kKeys;
-    row = old ? k0 : n + k0;
-    rows = min(kKeys, (old ? n : a.t) - k0);
-  };
-  auto fetch = [&](int tile) {
-    if (tile < tile1) {
-      int row, rows;
-      extent(tile, row, rows);
-      const uint32_t ks = saddr(smem) + (tile - tile0) % kStages * L::kStage;
-      const uint32_t vs = ks + kKeys * L::kKRow;
-      constexpr int kVecs = HD * (int)sizeof(T) / 16;
-#pragma unroll 8
-      for (int i = threadIdx.x; i < kKeys * kVecs; i += kThreads) {
-        const int r = i / kVecs, x = i % kVecs;
-        const int bytes = r < rows ? 16 : 0;  // rows behind the last key are zeros
-        const size_t at = (size_t)(row + (r < rows ? r : 0)) * HD + x * (16 / sizeof(T));
-        cp_async16(ks + r * L::kKRow + x * 16, kbase + at, bytes);
-        cp_async16(vs + r * L::kVRow + x * 16, vbase + at, bytes);
-      }
-    }
-    cp_async_commit();
-  };
 #pragma unroll
-  for (int s = 0; s < kStages - 1; s++) fetch(tile0 + s);
+  for (int s = 0; s < kStages - 1; s++) walk.fetch(tile0 + s);
 
   // This lane's rows g8 and g8 + 8 of the warp's 16.
   const int rA = r0 + 16 * mw + g8, rB = rA + 8;
@@ -231,9 +248,9 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Tree
   for (int tile = tile0; tile < tile1; tile++) {
     cp_async_wait<kStages - 2>();
     __syncthreads();
-    fetch(tile + kStages - 1);  // into the buffer that the last tile left
+    walk.fetch(tile + kStages - 1);  // into the buffer that the last tile left
     int row, rows;
-    extent(tile, row, rows);
+    walk.extent(tile, row, rows);
     const bool old = tile < old_tiles;
     const unsigned char* ks = smem + (tile - tile0) % kStages * L::kStage;
     const unsigned char* vs = ks + kKeys * L::kKRow;
@@ -565,6 +582,176 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Tree
   }
 }
 
+// Up to kFewRows rows a kv head, fp32, head_dim 128: FMAs. Most of a matrix
+// instruction's 16 rows would be empty, and three products of each bound
+// k_tree: 4 rows over 8 x 128000 keys take 238 us there, 190 here (5.5 TB/s),
+// over 8 x 500 9.4 and 7.9. (With shorter heads a key's softmax outweighs its
+// products: 64 entries 111 there, 128 here.) A warp takes 8 keys at a time;
+// four lanes share a key's scores, each having a quarter of the entries of key
+// and queries, then every lane has 4 entries of the outputs.
+constexpr int kFewRows = 4, kFewWarps = 4, kFewHeadDim = 128;
+
+__global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(TreeArgs a) {
+  constexpr int HD = kFewHeadDim;
+  using L = Tile<float, HD>;
+  constexpr int kWarpKeys = L::kKeys / kFewWarps, kQ = HD / 16, kO = HD / 32;
+  static_assert(kWarpKeys == 8, "a warp's keys of a tile are one step");
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, c4 = lane & 3;
+  const int split = blockIdx.x, head = blockIdx.y, R = a.t * a.group;
+  sg::pdl_trigger();
+  sg::pdl_wait();
+  const Walk<float, HD, 32 * kFewWarps> walk(a, split, head, smem);
+  if (walk.tile0 >= walk.tile1) return;
+#pragma unroll
+  for (int s = 0; s < kStages - 1; s++) walk.fetch(walk.tile0 + s);
+
+  // Scores in units of log2, so that the softmax is exp2.
+  const float scale = 1.4426950408889634f / sqrtf((float)HD);
+  float4 q[kFewRows][kQ];
+  float m[kFewRows], l[kFewRows], o[kFewRows][kO];
+#pragma unroll
+  for (int r = 0; r < kFewRows; r++) {
+    const int row = r < R ? r : 0, tok = row / a.group;
+    const float* from = static_cast<const float*>(a.q) + tok * a.ldq +
+                        (size_t)(head * a.group + row - tok * a.group) * HD + 4 * c4;
+#pragma unroll
+    for (int j = 0; j < kQ; j++) {
+      q[r][j] = *reinterpret_cast<const float4*>(from + 16 * j);
+      q[r][j].x *= scale;
+      q[r][j].y *= scale;
+      q[r][j].z *= scale;
+      q[r][j].w *= scale;
+    }
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kO; i++) o[r][i] = 0.f;
+  }
+
+  for (int tile = walk.tile0; tile < walk.tile1; tile++) {
+    cp_async_wait<kStages - 2>();
+    __syncthreads();
+    walk.fetch(tile + kStages - 1);  // into the buffer that the last tile left
+    int row, rows;
+    walk.extent(tile, row, rows);
+    const bool old = tile < walk.old_tiles;
+    const unsigned char* ks = smem + (tile - walk.tile0) % kStages * L::kStage;
+    const unsigned char* vs = ks + L::kKeys * L::kKRow;
+    const int k0 = warp * kWarpKeys;  // the warp's first key in the tile
+    if (k0 < rows) {
+      float s[kFewRows][2];
+#pragma unroll
+      for (int r = 0; r < kFewRows; r++) s[r][0] = s[r][1] = 0.f;
+      const unsigned char* kp = ks + (k0 + g8) * L::kKRow + c4 * 16;
+#pragma unroll
+      for (int j = 0; j < kQ; j++) {
+        const float4 x = *reinterpret_cast<const float4*>(kp + j * 64);
+#pragma unroll
+        for (int r = 0; r < kFewRows; r++) {
+          s[r][0] = fmaf(q[r][j].x, x.x, s[r][0]);
+          s[r][1] = fmaf(q[r][j].y, x.y, s[r][1]);
+          s[r][0] = fmaf(q[r][j].z, x.z, s[r][0]);
+          s[r][1] = fmaf(q[r][j].w, x.w, s[r][1]);
+        }
+      }
+      float p[kFewRows], top[kFewRows];
+#pragma unroll
+      for (int r = 0; r < kFewRows; r++) {
+        p[r] = s[r][0] + s[r][1];
+        p[r] += __shfl_xor_sync(0xFFFFFFFFu, p[r], 1);
+        p[r] += __shfl_xor_sync(0xFFFFFFFFu, p[r], 2);
+        bool in = k0 + g8 < rows && r < R;
+        if (!old && in) {
+          const int j = row - walk.n + k0 + g8;  // drafted index
+          in = a.mask[(size_t)(r / a.group) * a.words + (j >> 6)] >> (j & 63) & 1;
+        }
+        if (!in) p[r] = -INFINITY;
+        top[r] = fmaxf(p[r], __shfl_xor_sync(0xFFFFFFFFu, p[r], 4));
+        top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 8));
+        top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 16));
+      }
+#pragma unroll
+      for (int r = 0; r < kFewRows; r++) {
+        if (top[r] > m[r]) {  // the same in all lanes
+          const float f = exp2f(m[r] - top[r]);
+          m[r] = top[r];
+          l[r] *= f;
+#pragma unroll
+          for (int i = 0; i < kO; i++) o[r][i] *= f;
+        }
+        // A row that has seen no key yet keeps m = -inf and zeros.
+        p[r] = exp2f(p[r] - (m[r] == -INFINITY ? 0.f : m[r]));
+        l[r] += p[r];
+      }
+      const unsigned char* vp = vs + k0 * L::kVRow + lane * kO * 4;
+#pragma unroll
+      for (int kk = 0; kk < 8; kk++) {
+        const float4 v4 = *reinterpret_cast<const float4*>(vp + kk * L::kVRow);
+        const float x[kO] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+        for (int r = 0; r < kFewRows; r++) {
+          const float w = __shfl_sync(0xFFFFFFFFu, p[r], 4 * kk);
+          // A drafted row that is hidden may hold anything; cached ones are
+          // seen by all.
+          if (old || w != 0.f) {
+#pragma unroll
+            for (int i = 0; i < kO; i++) o[r][i] = fmaf(w, x[i], o[r][i]);
+          }
+        }
+      }
+    }
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+
+  // The warps' parts are joined in shared memory, a row by each warp.
+  float* part = reinterpret_cast<float*>(smem);  // [warp][row][HD + 2]
+  static_assert(kFewWarps * kFewRows * (HD + 2) * 4 <= (int)L::kBytes, "join fits the tiles");
+  static_assert(kFewWarps == kFewRows, "a warp per row");
+#pragma unroll
+  for (int r = 0; r < kFewRows; r++) {
+    l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 4);
+    l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 8);
+    l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 16);
+    float* to = part + (warp * kFewRows + r) * (HD + 2);
+#pragma unroll
+    for (int i = 0; i < kO; i++) to[lane * kO + i] = o[r][i];
+    if (lane == 0) {
+      to[HD] = m[r];
+      to[HD + 1] = l[r];
+    }
+  }
+  __syncthreads();
+  if (warp >= R) return;
+  float all = -INFINITY, sum = 0.f, out[kO];
+#pragma unroll
+  for (int i = 0; i < kO; i++) out[i] = 0.f;
+#pragma unroll
+  for (int w = 0; w < kFewWarps; w++)
+    all = fmaxf(all, part[(w * kFewRows + warp) * (HD + 2) + HD]);
+#pragma unroll
+  for (int w = 0; w < kFewWarps; w++) {
+    const float* from = part + (w * kFewRows + warp) * (HD + 2);
+    const float f = all == -INFINITY ? 0.f : exp2f(from[HD] - all);
+    sum += from[HD + 1] * f;
+#pragma unroll
+    for (int i = 0; i < kO; i++) out[i] = fmaf(from[lane * kO + i], f, out[i]);
+  }
+  // One split: the row is complete (one without keys is zeros). Else its part
+  // goes to the workspace.
+  const bool whole = a.splits == 1;
+  const float f = whole ? (sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum)) : 1.f;
+  const int tok = warp / a.group;
+  const size_t at = ((size_t)split * a.kh + head) * R + warp;
+  if (!whole && lane == 0) a.ml[at] = make_float2(all, sum);
+  float* to = whole ? static_cast<float*>(a.att) + tok * a.ldo +
+                          (size_t)(head * a.group + warp - tok * a.group) * HD
+                    : a.part + at * HD;
+#pragma unroll
+  for (int i = 0; i < kO; i++) to[lane * kO + i] = out[i] * f;
+}
+
 // A block joins the parts of one row: sixteen groups of eight lanes, a lane
 // having HD / 8 entries of the head, take the parts in turn, each with a
 // running maximum of its own, so that a row's loads are all on their way at
@@ -757,6 +944,17 @@ size_t workspace_of(int splits, int t, int kh, int group, int hd) {
   return (size_t)splits * kh * t * group * (hd + 2) * sizeof(float);
 }
 
+cudaError_t launch_few(const TreeArgs& a, int dev, cudaStream_t s) {
+  static std::atomic<size_t> allowed[sg::kDevices];
+  using L = Tile<float, kFewHeadDim>;
+  cudaError_t e = sg::allow_smem(k_tree_few, L::kBytes, dev, allowed);
+  if (e != cudaSuccess) return e;
+  e = sg::try_launch(k_tree_few, dim3(a.splits, a.kh), dim3(32 * kFewWarps), L::kBytes, 1, s, a);
+  if (e != cudaSuccess || a.splits == 1) return e;
+  return sg::try_launch(k_merge<float, kFewHeadDim, false>, dim3(a.t * a.group * a.kh),
+                        dim3(kMergeThreads), 0, 1, s, a, L::kKeys);
+}
+
 template <typename T, int HD, int MW, int KW>
 cudaError_t launch_shape(const TreeArgs& a, int dev, cudaStream_t s) {
   static std::atomic<size_t> allowed[sg::kDevices];
@@ -783,6 +981,8 @@ cudaError_t launch_hd(const TreeArgs& a, int dev, cudaStream_t s) {
                             0, 1, s, a, sg::tree_tc_keys());
     }
   }
+  if constexpr (sizeof(T) == 4 && HD == kFewHeadDim)
+    if (a.t * a.group <= kFewRows) return launch_few(a, dev, s);
   const Shape f = shape_of(a.t * a.group);
   if (f.mw == 1) return launch_shape<T, HD, 1, 4>(a, dev, s);
   if (f.mw == 2) return launch_shape<T, HD, 2, 2>(a, dev, s);

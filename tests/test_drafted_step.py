@@ -402,6 +402,38 @@ def test_tree_offsets_beyond_32_bits(cuda):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("type_", [F32, BF16])
+@pytest.mark.parametrize("t,kh,g", [(4, 1, 1), (3, 2, 1), (2, 3, 2), (1, 8, 3), (1, 1, 4),
+                                    (4, 320, 1), (5, 2, 1)])
+@pytest.mark.parametrize("n", [0, 7, 31, 33, 500, 4097])
+def test_tree_few_rows(cuda, type_, t, kh, g, n):
+    """Up to four rows per kv head (and five), some drafted rows hidden from
+    all and not finite; the last token sees nothing where nothing is cached."""
+    torch = cuda
+    hd = 128
+    if kh > 100:
+        n = min(n, 500)
+    q, k, v = inputs(torch, t, kh, g, hd, n + t + 9, type_, 7 * t + n)
+    m = tree_mask(t, n)
+    clean = k.clone(), v.clone()
+    if t > 1:
+        m[:, 0] = False
+        m[-1] = False
+        k[:, n], v[:, n] = float("nan"), float("inf")
+    k[:, n + t:], v[:, n + t:] = float("inf"), float("nan")
+    want, reach, top = tree_reference(torch, q, *clean, n, m)
+    got = run_tree(torch, q, k, v, n, m, type_)
+    err = (got.double() - want).abs()
+    assert (err <= tree_tolerance(want, reach, top, n + t, hd, type_)).all(), err.max().item()
+    if n == 0 and t > 1:
+        assert (got[-1] == 0).all()
+    if t > 1:
+        m[1, 0] = True                     # now the second token sees it
+        got = run_tree(torch, q, k, v, n, m, type_)
+        assert got[1].isnan().all() and not got[2:].isnan().any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [F32, BF16])
 @pytest.mark.parametrize("hd", [64, 128])
 def test_tree_many_rows_one_split_and_wide_rows(cuda, type_, hd):
     """As above where the cached keys have a kernel of their own: one split per
