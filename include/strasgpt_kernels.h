@@ -146,8 +146,10 @@ int strasgpt_k_rope(const void* x, long long x_token_stride,
 // 0..*cached - 1 of the caches are seen by every token, rows *cached + j are
 // the drafted tokens' own: token i sees j where bit j % 64 of
 // mask[i * ((t + 63) / 64) + j / 64] is set (its own bit included, or it does
-// not see itself). Scores are q.k / sqrt(head_dim); sums, maxima and
-// probabilities are held in 32 bits. A token that sees nothing gets zeros.
+// not see itself). Scores are q.k / sqrt(head_dim); sums and maxima are held
+// in 32 bits. Products keep 21 bits of each fp32 operand at least; bf16 ones
+// are exact, the probabilities that multiply bf16 values keep 17 bits. A token
+// that sees nothing gets zeros.
 // Rows that a token does not see, and rows behind the last, may hold anything
 // (infinities and NaN too). *cached is read on the device and cut to
 // 0..ctx - t. head_dim 32, 64 or 128; group 1..128; q, the caches, att, their
