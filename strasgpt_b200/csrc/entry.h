@@ -4,6 +4,7 @@
 #pragma once
 
 #include <atomic>
+#include <mutex>
 
 #include "common.cuh"
 
@@ -61,11 +62,17 @@ inline const char* current_device(int* dev, int* sms) {
   return nullptr;
 }
 
-// Raises `kernel`'s dynamic shared memory limit to `bytes`, once per kernel
-// and device (`done` belongs to the kernel: one flag per device).
+// Raises `kernel`'s dynamic shared memory limit to `bytes`, and never lowers it
+// (`done` belongs to the kernel: the limit on each device). Callers may ask
+// for different sizes from several threads: reading the limit, setting it and
+// noting it are one step under the lock.
+inline std::mutex smem_lock;
+
 template <typename K>
 inline cudaError_t allow_smem(K kernel, size_t bytes, int dev, std::atomic<size_t>* done) {
   if (done[dev].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
+  const std::lock_guard<std::mutex> hold(smem_lock);
+  if (done[dev].load(std::memory_order_relaxed) >= bytes) return cudaSuccess;
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (e == cudaSuccess) done[dev].store(bytes, std::memory_order_release);
