@@ -403,7 +403,8 @@ struct Row {
   float floor;                   // entries below are out
   float M;
   double scale;                  // log2(e) / T
-  float bins_per;                // histogram bins per unit of logit
+  float shrink;                  // distances are measured times this
+  float bins_per;                // histogram bins per unit of that
   float octaves;                 // octaves of weight per bin
   float last;                    // bins from M to where weights are 0
 
@@ -471,7 +472,8 @@ struct Row {
 
   // Distance from M in bins (-inf and NaN: FLT_MAX). Every step is monotone,
   // so larger logits come first whatever the roundings.
-  __device__ float pos(float x) const { return fminf((M - x) * bins_per, FLT_MAX); }
+  __device__ float distance(float x) const { return fmaf(x, -shrink, M * shrink); }
+  __device__ float pos(float x) const { return fminf(distance(x) * bins_per, FLT_MAX); }
   // The integer below, by adding 2^23 rounded down.
   __device__ static int whole(float f) { return __float_as_int(__fadd_rd(f, 8388608.f)) & 0x7FFFFF; }
   // Histogram bin; the last one is open to below.
@@ -1073,8 +1075,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleArgs a) {
   // The bins share what is within kReach octaves of the largest weight, or
   // down to the smallest logit if that is nearer. (Bins in 32 bits: all CTAs
   // compute the same ones, and any monotone ones do.)
-  const float bits = (float)fmin(r.scale, 1e37);
-  const float range = fminf(kReach / bits, (r.M - least) * 1.00001f);
+  // Distances that fp32 might not hold are measured as quarters: then no step
+  // below overflows, whatever the temperature. (M - x is one rounding either
+  // way; a quarter is exact but for a denormal M, whose distance rounds to 0.)
+  r.shrink = r.M - least <= FLT_MAX / 4 ? 1.f : 0.25f;
+  const float bits = (float)fmin(r.scale / r.shrink, 1e37);
+  const float range = fminf(kReach / bits, r.distance(least) * 1.00001f);
   r.bins_per = fminf((kBins - 1) / range, 1e37f);
   r.octaves = fminf(bits / r.bins_per, 2.0f * kReach / kBins);
   r.last = fminf(1000.f / (bits / r.bins_per), 1e38f);
@@ -1102,8 +1108,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleArgs a) {
       // Everything down to that bin's end stays.
       const int b = (int)sh->bbin;
       if (b < kBins - 1)
-        least_kept = __double2float_rd((double)r.M - (b + 1.01) / (double)r.bins_per -
-                                       1e-6 * (fabs((double)r.M) + range));
+        least_kept = __double2float_rd((double)r.M -
+                                       (b + 1.01) / ((double)r.bins_per * r.shrink) -
+                                       1e-6 * (fabs((double)r.M) + (double)range / r.shrink));
     }
     const unsigned mine = r.bound(least_kept);
     // How many of the row are left; this slice's go to CTA 0 if it has few.

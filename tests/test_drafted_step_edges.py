@@ -6,7 +6,9 @@ import os
 import subprocess
 import sys
 
+import numpy as np
 import pytest
+from test_drafted_step import BF16, F32, check_sample, dtype
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -40,3 +42,36 @@ assert status == [0] * 400, status
     for _ in range(2):
         subprocess.run([sys.executable, "-c", program], cwd=ROOT, check=True, timeout=300,
                        env=dict(os.environ, PYTHONPATH=ROOT))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [F32, BF16])
+@pytest.mark.parametrize("vocab", [70, 3001, 40000])
+@pytest.mark.parametrize("rows", [7, 300])
+def test_sample_distances_beyond_fp32(cuda, type_, vocab, rows):
+    """Logits whose distance from the largest overflows fp32, at temperatures
+    that give them a weight all the same: the largest and the lowest value of
+    the type; masks of the lowest value under ordinary logits. With few rows
+    (clusters) and with many (under top-k, a block each)."""
+    torch = cuda
+    inf = float("inf")
+    x = torch.full((7, vocab), -inf, device="cuda", dtype=dtype(torch, type_))
+    low, high = torch.finfo(x.dtype).min, torch.finfo(x.dtype).max
+    x[0, 5], x[0, 50:60], x[0, 69] = high, 1.0, low
+    x[1, 0:3] = torch.tensor([low, 1.0, high])
+    x[2] = low
+    x[2, 11:40] = torch.arange(29, device="cuda") / 4
+    x[3] = 2e38
+    x[3, ::2] = -2e38
+    x[4, ::3] = high
+    x[4, 1::3] = low
+    x[5] = torch.linspace(low / 2, high / 2, vocab, device="cuda")   # the difference just fits
+    x[6] = torch.linspace(float(low) * 0.9, float(high) * 0.9, vocab, device="cuda",
+                          dtype=torch.float64).to(x.dtype)
+    x = x.repeat((rows + 6) // 7, 1)[:rows]
+    rng = np.random.RandomState(vocab)
+    for heat in (inf, 1e38, 3e38, 2e37, 1e36, 1.0):
+        for f in (dict(), dict(top_k=2), dict(top_k=40, top_p=0.97), dict(top_p=0.7),
+                  dict(min_p=0.01), dict(top_k=300, min_p=0.3)):
+            check_sample(torch, x, heat=heat, u=rng.uniform(0.01, 0.99, rows).astype(np.float32),
+                         **f)
