@@ -207,6 +207,12 @@ __device__ __forceinline__ u64 block_sort(u64 v, int n, u64* x) {
   return v;
 }
 
+// Where the running mass has to be exceeded. u at or above 1 takes the last
+// entry with a weight, which roundings of the sums must not decide.
+__device__ __forceinline__ double draw_at(float u, double total) {
+  return u < 1.f ? (u > 0.f ? (double)u * total : 0.0) : u == u ? (double)INFINITY : 0.0;
+}
+
 // The choice of a row from its n <= kThreads entries that can be kept, one
 // block's work. mark: this thread's entry, its key over INT_MAX - index (0
 // behind the last). `few` and `order` hold kThreads words, `wsum` kWarps.
@@ -233,7 +239,7 @@ __device__ __forceinline__ void finish(const SampleArgs& a, int row, u64 mark, i
   w = tid < kept ? weights[(unsigned)byi] : 0.0;
   double total;
   const double run = block_prefix(w, wsum, &total);
-  const double target = u > 0.f ? (double)u * total : 0.0;
+  const double target = draw_at(u, total);
   if (tid == 0) {
     *found = kThreads;
     *fill = 0;
@@ -403,6 +409,7 @@ struct Row {
   float floor;                   // entries below are out
   float M;
   double scale;                  // log2(e) / T
+  bool ends;                     // u near 0, or not below 1: the smallest weight counts
   float shrink;                  // distances are measured times this
   float bins_per;                // histogram bins per unit of that
   float octaves;                 // octaves of weight per bin
@@ -703,8 +710,8 @@ struct Row {
   }
 
   // The prefix of the order that a filter keeps: its last entry (key and
-  // index) and its mass. tail: the border lies among entries of weight 0; all
-  // others are kept, and `zeros` of those. sums: sh->before_mass and
+  // index) and its mass. tail: the border lies among entries whose weight the
+  // histogram rounds to 0; all others are kept, and `zeros` of those. sums: sh->before_mass and
   // sh->before_count say what is kept of each slice.
   struct Cut {
     unsigned key;
@@ -726,7 +733,7 @@ struct Row {
     const double step = pow2(-unit), base = sh->bbase;
     unsigned count = sh->bcount, number = sh->gcount[bin];
     u64 mass = 0;                         // within the bin, before its border
-    if (!by_mass && bin == kBins - 1 && sh->gmass[bin] == 0) {
+    if (!by_mass && bin == kBins - 1 && sh->gmass[bin] == 0 && !ends) {
       cut.tail = true;
       cut.zeros = k - count;
       cut.mass = base;
@@ -1070,6 +1077,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleArgs a) {
   }
   r.M = top;
   r.listed = false;
+  // What the histogram rounds to 0, below 2^-104 of the largest weight, comes
+  // to less than 2^-85 in all: only a u outside [2^-50, 1) can draw it.
+  r.ends = !(u_ >= 0x1p-50f && u_ < 1.f);
   r.floor = -FLT_MAX;
   r.scale = 1.4426950408889634 / (double)T_;
   // The bins share what is within kReach octaves of the largest weight, or
@@ -1180,7 +1190,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleArgs a) {
     if (numbers) block_prefix((u64)number, sh->wred, numbers);
     return total;
   };
-  const bool known = cut.sums;  // what each slice keeps
+  const bool known = cut.sums && !r.ends;  // what each slice keeps
   if (!known) {
     u64 numbers;
     const double total = add_up(&numbers);
@@ -1200,7 +1210,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleArgs a) {
   }
   // The slice in which the running mass exceeds u total; the last with any
   // if none (u at or above 1).
-  const double target = u_ > 0.f ? (double)u_ * total : 0.0;
+  const double target = draw_at(u_, total);
   double run = 0, before = 0;
   int owner = -1;
   for (int q = 0; q < ranks; q++) {

@@ -8,7 +8,7 @@ import sys
 
 import numpy as np
 import pytest
-from test_drafted_step import BF16, F32, check_sample, dtype
+from test_drafted_step import BF16, F32, H, check_sample, dtype, run_sample, sample_row
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -44,6 +44,20 @@ assert status == [0] * 400, status
                        env=dict(os.environ, PYTHONPATH=ROOT))
 
 
+def check_tiny(torch, x, period, u, heat=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """check_sample where probabilities may be below what fp32 holds: half a
+    step of fp32 is 2^-150 there, whatever the value. Rows of x repeat after
+    `period`."""
+    f32 = lambda v: float(np.float32(v))  # noqa: E731
+    token, prob, kept = run_sample(torch, x, u=u, heat=heat, top_k=top_k, top_p=top_p, min_p=min_p)
+    wants = [sample_row(row, f32(heat), top_k, f32(top_p), f32(min_p), f32(u))
+             for row in x[:period].double().cpu().numpy()]
+    for r in range(x.shape[0]):
+        want = wants[r % period]
+        assert (token[r], kept[r]) == (want[0], want[2]), (r, token[r], kept[r], want)
+        assert abs(prob[r] - want[1]) <= 4 * H * want[1] + 2.0 ** -150
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("type_", [F32, BF16])
 @pytest.mark.parametrize("vocab", [70, 3001, 40000])
@@ -75,3 +89,31 @@ def test_sample_distances_beyond_fp32(cuda, type_, vocab, rows):
                   dict(min_p=0.01), dict(top_k=300, min_p=0.3)):
             check_sample(torch, x, heat=heat, u=rng.uniform(0.01, 0.99, rows).astype(np.float32),
                          **f)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [F32, BF16])
+@pytest.mark.parametrize("rows", [6, 312])
+@pytest.mark.parametrize("vocab", [600, 9001, 128256])
+def test_sample_ends_of_u_take_the_smallest_weights(cuda, type_, rows, vocab):
+    """u of 0 takes the first entry that remains and u of 1 the last, however
+    little they weigh beside the largest one (2^-100 to 2^-900), under each
+    filter, with few rows and many."""
+    torch = cuda
+    if rows > 6 and vocab > 9001:
+        rows = 60                                # more than the GPU holds clusters
+    gen = torch.Generator(device="cuda").manual_seed(vocab)
+    x = -300 + 60 * torch.randn(6, vocab, device="cuda", generator=gen).clamp(-4, 4)
+    x[0] = -600.0                                # thousands of equal tiny weights
+    x[1, : vocab // 2] = -72.5                   # 2^-104.6
+    x[2] = -float("inf")
+    x[2, ::7] = -100.0
+    x[3, vocab - 1], x[3, 0] = -620.0, -620.0
+    x[4, 1:40] = torch.arange(39, device="cuda") / -2
+    x[:, vocab // 2] = 0.0
+    x[:, vocab // 2 + 3] = -0.25
+    x = x.to(dtype(torch, type_)).repeat((rows + 5) // 6, 1)[:rows]
+    for f in (dict(), dict(top_k=30), dict(top_k=vocab // 2), dict(top_k=513), dict(min_p=1e-35),
+              dict(top_k=vocab - 1), dict(top_p=0.9), dict(top_k=520, top_p=0.9999999)):
+        for u in (0.0, -1.0, 1e-38, 1e-28, 1e-20, 0.4, 1 - 2.0 ** -24, 1.0, 2.0):
+            check_tiny(torch, x, 6, u, **f)
