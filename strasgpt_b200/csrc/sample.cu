@@ -413,7 +413,8 @@ struct Row {
   float shrink;                  // distances are measured times this
   float bins_per;                // histogram bins per unit of that
   float octaves;                 // octaves of weight per bin
-  float last;                    // bins from M to where weights are 0
+  float last;                    // bins from M to where a bin's unit is far above the weights
+  float gone;                    // logits up to here weigh less than e^-749, 0 in 64 bits
 
   __device__ float at(int i) const { return clean(load_f(xs[i])); }
 
@@ -506,12 +507,13 @@ struct Row {
   __device__ static double shifted(double v, int e) {
     return __hiloint2double(__double2hiint(v) + e * (1 << 20), __double2loint(v));
   }
-  // The weight; 0 below 2^-1000 (and for -inf and NaN).
+  // The weight; 0 where 64 bits round it to 0 (and for -inf and NaN). The last
+  // factor makes the subnormal ones.
   __device__ double weight(float x) const {
     int e;
     double p;
     const double v = power(x, &p, &e);
-    return pos(x) < last ? shifted(v * p, e) : 0.0;
+    return x > gone ? shifted(v * p, e + 128) * 0x1p-128 : 0.0;
   }
   // A weight in units of 2^-unit, rounded: adding 2^52 leaves the nearest
   // integer in the low 52 bits. (A rounding of the bin's border may let a
@@ -519,7 +521,8 @@ struct Row {
   __device__ u64 in_units(double w, int unit) const {
     return (u64)__double_as_longlong(fma(w, pow2(unit), 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
   }
-  // The weight of x, f bins from M, in a bin's unit.
+  // The weight of x, f bins from M, in a bin's unit (0 far below the bins'
+  // units).
   __device__ unsigned units(float x, float f, int unit) const {
     int e;
     double p;
@@ -1094,6 +1097,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleArgs a) {
   r.bins_per = fminf((kBins - 1) / range, 1e37f);
   r.octaves = fminf(bits / r.bins_per, 2.0f * kReach / kBins);
   r.last = fminf(1000.f / (bits / r.bins_per), 1e38f);
+  r.gone = fminf(__double2float_rd((double)r.M - 749.0 * (double)T_), of_key(key_of(r.M) - 1));
   const double min_w = m_ > 0.f ? fmin((double)m_, 1.0) : 0.0;
   // A logit just below M + T ln(w).
   auto logit_of = [&](double w) {

@@ -117,3 +117,26 @@ def test_sample_ends_of_u_take_the_smallest_weights(cuda, type_, rows, vocab):
               dict(top_k=vocab - 1), dict(top_p=0.9), dict(top_k=520, top_p=0.9999999)):
         for u in (0.0, -1.0, 1e-38, 1e-28, 1e-20, 0.4, 1 - 2.0 ** -24, 1.0, 2.0):
             check_tiny(torch, x, 6, u, **f)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [F32, BF16])
+@pytest.mark.parametrize("rows", [5, 320])
+def test_sample_smallest_weights(cuda, type_, rows):
+    """Weights down to the smallest number that 64 bits hold (2^-1074, at 744.4
+    below the largest logit) can be drawn: u of 0 takes the first entry that
+    has one."""
+    torch = cuda
+    vocab = 5000
+    x = torch.full((5, vocab), -900.0, device="cuda", dtype=dtype(torch, type_))
+    x[:, 4321] = 0.0
+    x[0, 77], x[0, 4400] = -700.0, -1.0          # 2^-1010
+    x[1, 40:60] = -740.0                         # 2^-1068
+    x[2, 1000] = -744.0                          # 2^-1074 times 1.4
+    x[2, 999] = -748.0                           # rounds to 0
+    x[3, ::5] = -720.0
+    x[4, 4990] = -743.0                          # behind the largest
+    x = x.repeat((rows + 4) // 5, 1)[:rows]
+    for f in (dict(), dict(top_k=30), dict(top_k=2000), dict(min_p=1e-40), dict(top_p=0.9)):
+        for u in (0.0, 1e-30, 0.5, 1.0):
+            check_tiny(torch, x, 5, u, **f)
