@@ -185,8 +185,9 @@ int strasgpt_k_attn_tree(const void* q, long long ldq, const void* k_cache,
 // token's share of the remaining mass, kept (NULL) how many entries remained.
 // NaN logits count as -inf, which are never taken; a row of nothing else gets
 // token -1, prob 0, kept 0. Where logits are +inf, those weigh 1 and all
-// others 0. vocab is at most STRASGPT_SAMPLE_MAX_VOCAB. The result does not
-// depend on timing: the same inputs give the same bits.
+// others 0. vocab is at most STRASGPT_SAMPLE_MAX_VOCAB. token, prob and kept
+// share no memory with each other or the inputs. The result does not depend on
+// timing: the same inputs give the same bits.
 #define STRASGPT_SAMPLE_MAX_VOCAB 360448
 int strasgpt_k_sample(const void* logits, int type, long long ld, int rows,
                       int vocab, const float* temperature, const int* top_k,

@@ -38,6 +38,12 @@ inline const char* not_on_device(const void* p, int dev) {
 
 inline bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
+// Whether `bytes` from p and `bytes` from q on share any.
+inline bool overlap(const void* p, const void* q, size_t bytes) {
+  const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
+  return a < b ? b - a < bytes : a - b < bytes;
+}
+
 // Device index below this bound: per-device set-up is remembered by index.
 constexpr int kDevices = 64;
 

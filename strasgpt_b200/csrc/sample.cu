@@ -1283,6 +1283,12 @@ extern "C" int strasgpt_k_sample(const void* logits, int type, long long ld, int
                         (const void*)min_p, (const void*)u, (const void*)token,
                         (const void*)prob, (const void*)kept})
     if (!sg::aligned(p, 4)) return sg::refuse(me, "a buffer is not aligned to its entries");
+  // A token also says which kernel a row is left to, while filters are read.
+  const void* const by_row[] = {token, prob, kept, temperature, top_k, top_p, min_p, u};
+  for (int i = 0; i < 3; i++)
+    for (int j = i + 1; j < 8; j++)
+      if (by_row[i] && by_row[j] && sg::overlap(by_row[i], by_row[j], (size_t)rows * 4))
+        return sg::refuse(me, "token, prob and kept must not share memory with each other or the inputs");
   int dev = 0, sms = 0;
   if (const char* why = sg::current_device(&dev, &sms)) return sg::refuse(me, why);
   for (const void* p : {logits, (const void*)temperature, (const void*)top_k, (const void*)top_p,

@@ -8,7 +8,9 @@ import sys
 
 import numpy as np
 import pytest
-from test_drafted_step import BF16, F32, H, check_sample, dtype, run_sample, sample_row
+from strasgpt_b200 import runtime
+from test_drafted_step import (BF16, F32, FAKE, H, check_sample, dtype, run_sample,
+                               sample_row)
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -140,3 +142,18 @@ def test_sample_smallest_weights(cuda, type_, rows):
     for f in (dict(), dict(top_k=30), dict(top_k=2000), dict(min_p=1e-40), dict(top_p=0.9)):
         for u in (0.0, 1e-30, 0.5, 1.0):
             check_tiny(torch, x, 5, u, **f)
+
+
+@pytest.mark.parametrize("one,other,apart,shared", [
+    ("token", "k", 0, True), ("token", "u", 4, True), ("prob", "u", 0, True),
+    ("kept", "token", -4, True), ("prob", "heat", 8, True), ("kept", "p", -8, True),
+    ("token", "m", 12, False), ("prob", "kept", -12, False), ("heat", "u", 0, False)])
+def test_sample_refuses_shared_outputs(capfd, one, other, apart, shared):
+    """The outputs of three rows, a few bytes before or behind another array.
+    (Inputs may be one array; what passes is refused as no device memory.)"""
+    names = ("heat", "k", "p", "m", "u", "token", "prob", "kept")
+    at = {n: (2 + i) * FAKE for i, n in enumerate(names)}
+    at[one] = at[other] + apart
+    status = runtime.lib().strasgpt_k_sample(FAKE, F32, 100, 3, 100, *[at[n] for n in names], None)
+    err = capfd.readouterr().err
+    assert status == -1 and ("share memory" in err) == shared, err
