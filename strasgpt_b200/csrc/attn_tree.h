@@ -32,4 +32,12 @@ cudaError_t tree_tc(const TreeArgs& a, bool f32, int head_dim, int dev, cudaStre
 // Keys per tile: what a split's share is a multiple of.
 int tree_tc_keys();
 
+// Tiles i = 0, 1, ... go to a ring of `stages`, tile i to stage i % stages, and
+// each fill of a stage completes a phase of its barrier. The parity of the
+// phase that stage s's last fill completes, when `asked` > s tiles were asked
+// for: a wait on it ends when that fill has landed, and not at an older one.
+__host__ __device__ constexpr unsigned tree_last_parity(int asked, int s, int stages) {
+  return (unsigned)((asked - 1 - s) / stages) & 1u;
+}
+
 }  // namespace sg

@@ -72,3 +72,32 @@ int main() {
   return 0;
 }
 """)
+
+
+def test_last_fill_of_a_stage_is_waited_for(tmp_path):
+    """A barrier's wait on a parity ends when the phase that is under way has
+    the other one. For every number of tiles and stages the wait for a stage's
+    last fill lasts while that fill is on its way, and ends once it has landed."""
+    run_program(tmp_path, r"""
+#include "attn_tree.h"
+#include <cstdio>
+int main() {
+  for (int stages = 1; stages <= 8; stages++)
+    for (int asked = 1; asked <= 5 * stages + 3; asked++)
+      for (int s = 0; s < stages && s < asked; s++) {
+        int fills = 0;
+        for (int i = s; i < asked; i += stages) fills++;
+        const unsigned parity = sg::tree_last_parity(asked, s, stages);
+        for (int landed = fills - 1; landed <= fills; landed++) {
+          const unsigned under_way = (unsigned)landed & 1;   // phases count from 0
+          const bool ends = under_way != parity;
+          if (ends != (landed == fills)) {
+            printf("%d stages, %d tiles, stage %d: %d of %d landed, wait %s\n", stages, asked, s,
+                   landed, fills, ends ? "ends" : "lasts");
+            return 1;
+          }
+        }
+      }
+  return 0;
+}
+""")
