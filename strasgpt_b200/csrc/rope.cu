@@ -201,23 +201,27 @@ extern "C" int strasgpt_k_rope(const void* x, long long x_token_stride, long lon
   a.yt = y_token_stride; a.yh = y_head_stride;
   a.t = t; a.heads = heads; a.hd = head_dim; a.dim = rope->dim;
   a.magnitude = (float)rope->magnitude;
-  const double two_pi = 6.283185307179586476925;
   const int half = rope->dim / 2;
-  // f_j = theta^(-2 j / dim) as a running product: 255 roundings of 2^-53 at
-  // most, far below what the fp32 sine keeps.
-  const double ratio = pow(rope->theta, -2.0 / rope->dim);
-  double f = 1.0;
+  // f_j = theta^(-2 j / dim) as a running product in 64-bit mantissas: at most
+  // 255 roundings and as many times the ratio's own, 2^-55 in all, so that a
+  // pair's turns per position are off by their last rounding to 64 bits (2^-53)
+  // and no more, which is what counts at far positions. (In doubles the
+  // product was off by up to 2^-46: 4e-6 radians at position 2^31 for 512
+  // entries and theta 2.)
+  const long double per_turn = 1 / 6.283185307179586476925286766559L;
+  const long double ratio = powl(rope->theta, -2.0L / rope->dim);
+  const long double stretched =
+      rope->scaling == STRASGPT_ROPE_NONE ? per_turn : per_turn / rope->factor;
+  long double f = 1;
   for (int j = 0; j < half; j++, f *= ratio) {
-    double g = f;
-    if (rope->scaling == STRASGPT_ROPE_LINEAR) {
-      g = f / rope->factor;
-    } else if (rope->scaling == STRASGPT_ROPE_BANDS) {
-      const double turns = rope->original * f / two_pi;
-      double keep = (turns - rope->low) / (rope->high - rope->low);
+    long double turns = stretched;
+    if (rope->scaling == STRASGPT_ROPE_BANDS) {
+      long double keep = (rope->original * f * per_turn - rope->low) /
+                         ((long double)rope->high - rope->low);
       keep = keep < 0 ? 0 : keep > 1 ? 1 : keep;
-      g = f * (keep + (1 - keep) / rope->factor);
+      turns = keep * per_turn + (1 - keep) * stretched;
     }
-    a.turns[j] = g / two_pi;
+    a.turns[j] = (double)(f * turns);
   }
 
   // 16-byte accesses where every run of their entries starts on 16 bytes; for

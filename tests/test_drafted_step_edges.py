@@ -46,6 +46,49 @@ assert status == [0] * 400, status
                        env=dict(os.environ, PYTHONPATH=ROOT))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [0, 1])
+@pytest.mark.parametrize("dim,theta,scaling", [(512, 1e4, "none"), (512, 2.0, "none"),
+                                               (256, 5e5, "linear"), (512, 1e3, "bands"),
+                                               (128, 1e4, "none")])
+def test_rope_far_positions(cuda, interleaved, dim, theta, scaling):
+    """Positions up to the largest int, against angles with 64-bit mantissas.
+    The turns per position and their product with the position are rounded to
+    64 bits, 2^-53 of the turns each: 2^-52 |pos| f radians on top of the bound
+    for near positions."""
+    torch = cuda
+    ld = np.longdouble
+    kind = dict(none=dict(), linear=dict(scaling=runtime.ROPE_LINEAR, factor=3.0),
+                bands=dict(scaling=runtime.ROPE_BANDS, factor=8.0, original=8192))[scaling]
+    r = runtime.Rope(dim, theta=theta, interleaved=interleaved, **kind)
+    pos = np.array([2 ** 31 - 1, -2 ** 31, 2 ** 30 + 12345, 2 ** 29 - 7, 100000007, 2 ** 24 + 1, 1])
+    f = ld(theta) ** (-ld(2) * np.arange(dim // 2, dtype=ld) / ld(dim))
+    two_pi = 8 * np.arctan(ld(1))
+    if scaling == "linear":
+        f = f / ld(3)
+    if scaling == "bands":
+        keep = np.clip((8192 * f / two_pi - 1) / ld(3), 0, 1)
+        f = f * (keep + (1 - keep) / ld(8))
+    turns = pos.astype(ld)[:, None] * (f / two_pi)
+    angle = ((turns - np.rint(turns)) * two_pi).astype(np.float64)
+    c, s = np.cos(angle)[:, None], np.sin(angle)[:, None]
+    gen = torch.Generator(device="cuda").manual_seed(dim)
+    x = torch.randn(len(pos), 3, dim, device="cuda", generator=gen)
+    y = torch.full_like(x, float("nan"))
+    where = torch.from_numpy(pos).to(torch.int32).cuda()
+    assert runtime.lib().strasgpt_k_rope(
+        x.data_ptr(), 3 * dim, dim, y.data_ptr(), 3 * dim, dim, F32, len(pos), 3, dim,
+        where.data_ptr(), r, torch.cuda.current_stream().cuda_stream) == 0
+    one, two = ((slice(0, dim, 2), slice(1, dim, 2)) if interleaved
+                else (slice(0, dim // 2), slice(dim // 2, dim)))
+    a, b = (x.double().cpu().numpy()[..., i] for i in (one, two))
+    got = y.double().cpu().numpy()
+    tol = (16 * H + 2.0 ** -52 * np.abs(pos)[:, None] * f.astype(np.float64))[:, None]
+    tol = tol * (np.abs(a) + np.abs(b))
+    assert (np.abs(got[..., one] - (a * c - b * s)) <= tol).all()
+    assert (np.abs(got[..., two] - (a * s + b * c)) <= tol).all()
+
+
 def check_tiny(torch, x, period, u, heat=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """check_sample where probabilities may be below what fp32 holds: half a
     step of fp32 is 2^-150 there, whatever the value. Rows of x repeat after
