@@ -129,7 +129,7 @@ typedef struct strasgpt_rope {
 // position pos[i] (any int: tokens may share a position, a negative one turns
 // back) and written to y + i * y_token_stride + h * y_head_stride; entries
 // behind the first rope->dim are copied. Angles are computed in 64 bits, the
-// rest in 32. y is x with the same strides (in place), or shares no memory
+// rest in 32 (frequencies of 1e298 turns and more are refused). y is x with the same strides (in place), or shares no memory
 // with x's rows; rows of y must not overlap. With the strides of a layer's
 // cache ([kv_heads][ctx][head_dim]: head_dim and ctx * head_dim) it appends
 // keys. t 0 does nothing.

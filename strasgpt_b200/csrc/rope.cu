@@ -190,11 +190,6 @@ extern "C" int strasgpt_k_rope(const void* x, long long x_token_stride, long lon
   const size_t size = type == STRASGPT_F32 ? 4 : 2;
   if (!sg::aligned(x, size) || !sg::aligned(y, size) || !sg::aligned(pos, 4))
     return sg::refuse(me, "a buffer is not aligned to its entries");
-  int dev = 0, sms = 0;
-  if (const char* why = sg::current_device(&dev, &sms)) return sg::refuse(me, why);
-  for (const void* p : {x, (const void*)y, (const void*)pos})
-    if (const char* why = sg::not_on_device(p, dev)) return sg::refuse(me, why);
-
   RopeArgs a;
   a.x = x; a.y = y; a.pos = pos;
   a.xt = x_token_stride; a.xh = x_head_stride;
@@ -222,7 +217,13 @@ extern "C" int strasgpt_k_rope(const void* x, long long x_token_stride, long lon
       turns = keep * per_turn + (1 - keep) * stretched;
     }
     a.turns[j] = (double)(f * turns);
+    // Times any position it must stay within 64 bits.
+    if (!(fabs(a.turns[j]) < 1e298)) return sg::refuse(me, "frequencies beyond 64 bits");
   }
+  int dev = 0, sms = 0;
+  if (const char* why = sg::current_device(&dev, &sms)) return sg::refuse(me, why);
+  for (const void* p : {x, (const void*)y, (const void*)pos})
+    if (const char* why = sg::not_on_device(p, dev)) return sg::refuse(me, why);
 
   // 16-byte accesses where every run of their entries starts on 16 bytes; for
   // adjacent pairs, else, an access per pair where pairs start on their size;

@@ -200,3 +200,18 @@ def test_sample_refuses_shared_outputs(capfd, one, other, apart, shared):
     status = runtime.lib().strasgpt_k_sample(FAKE, F32, 100, 3, 100, *[at[n] for n in names], None)
     err = capfd.readouterr().err
     assert status == -1 and ("share memory" in err) == shared, err
+
+
+@pytest.mark.parametrize("kind,far", [
+    (dict(dim=512, theta=5e-324), True), (dict(dim=64, theta=1e-300, scaling=1, factor=1e-100), True),
+    (dict(dim=64, theta=1e4, scaling=1, factor=5e-324), True),
+    (dict(dim=64, theta=1e4, scaling=2, factor=1e-300, original=10), True),
+    (dict(dim=512, theta=1e-290), False), (dict(dim=512, theta=1.7e308), False),
+    (dict(dim=2, theta=5e-324), False), (dict(dim=64, theta=1e4, scaling=1, factor=1e300), False)])
+def test_rope_refuses_frequencies_beyond_64_bits(capfd, kind, far):
+    """Parameters whose angles would not be finite numbers at every position.
+    (What passes is refused as no device memory.)"""
+    status = runtime.lib().strasgpt_k_rope(FAKE, 512, 512, 2 * FAKE, 512, 512, F32, 4, 1, 512,
+                                           FAKE, runtime.Rope(**kind), None)
+    err = capfd.readouterr().err
+    assert status == -1 and ("beyond 64 bits" in err) == far, err
