@@ -89,6 +89,38 @@ def test_rope_far_positions(cuda, interleaved, dim, theta, scaling):
     assert (np.abs(got[..., two] - (a * s + b * c)) <= tol).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("theta,dim", [(1e4, 128), (5e5, 64), (1e4, 6)])
+def test_rope_sines_keep_their_bits(cuda, theta, dim):
+    """Pairs (1, 0) become (cosine, sine). Near whole and half turns the sine
+    is small, near quarters the cosine, and each is right relative to itself:
+    sincospif to 2 steps (4 h), the correction's sum and the products (by 1, 0
+    and the magnitude 1) to half a step each (2 h), the correction itself to
+    2^-23 steps; and to the 64-bit angle's own error, 2^-52 |pos| f."""
+    torch = cuda
+    t = 4096
+    rng = np.random.RandomState(dim)
+    pos = np.concatenate([np.arange(t // 2), rng.randint(-2 ** 21, 2 ** 21, t - t // 2)])
+    ld = np.longdouble
+    two_pi = 8 * np.arctan(ld(1))
+    f = ld(theta) ** (-ld(2) * np.arange(dim // 2, dtype=ld) / ld(dim))
+    turns = pos.astype(ld)[:, None] * (f / two_pi)
+    angle = (turns - np.rint(turns)) * two_pi
+    x = torch.zeros(t, 1, dim, device="cuda")
+    x[..., :dim // 2] = 1.0
+    y = torch.full_like(x, float("nan"))
+    where = torch.from_numpy(pos).to(torch.int32).cuda()
+    assert runtime.lib().strasgpt_k_rope(
+        x.data_ptr(), dim, dim, y.data_ptr(), dim, dim, F32, t, 1, dim, where.data_ptr(),
+        runtime.Rope(dim, theta=theta), torch.cuda.current_stream().cuda_stream) == 0
+    got = y[:, 0].double().cpu().numpy()
+    for part, want in ((got[:, :dim // 2], np.cos(angle)), (got[:, dim // 2:], np.sin(angle))):
+        err = np.abs(part - want)
+        tol = (6 + 2.0 ** -20) * H * np.abs(want) + 2.0 ** -46 * H + 2.0 ** -52 * np.abs(
+            pos)[:, None] * f
+        assert (err <= tol).all(), float((err - tol).max())
+
+
 def check_tiny(torch, x, period, u, heat=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """check_sample where probabilities may be below what fp32 holds: half a
     step of fp32 is 2^-150 there, whatever the value. Rows of x repeat after
