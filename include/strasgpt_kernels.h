@@ -93,11 +93,13 @@ int strasgpt_k_matvec_noalloc(const float* x, const uint16_t* norm_w,
 // device memory of the current device; `type` is STRASGPT_F32 (float) or
 // STRASGPT_BF16 (uint16_t) for every buffer given as void*; strides count
 // entries. They allocate nothing, keep nothing between calls, and can be
-// captured into a CUDA graph. Each returns 0 once its work is enqueued; an
+// captured into a CUDA graph, which keeps the addresses and numbers of the
+// call and reads what is in device memory (positions, lengths, masks, filters,
+// random numbers) at each replay. Each returns 0 once its work is enqueued; an
 // invalid argument, a buffer that is not on the current device or a failed
 // launch returns -1 with a "[StrasGPT] Error ..." message on stderr and
-// enqueues nothing. What is in device memory (positions, lengths, masks,
-// filters) cannot be refused: each says what it does with any value.
+// enqueues nothing. What is in device memory cannot be refused: each says what
+// it does with any value.
 #define STRASGPT_F32  0
 #define STRASGPT_BF16 1
 
@@ -132,7 +134,10 @@ typedef struct strasgpt_rope {
 // rest in 32 (frequencies of 1e298 turns and more are refused). y is x with the same strides (in place), or shares no memory
 // with x's rows; rows of y must not overlap. With the strides of a layer's
 // cache ([kv_heads][ctx][head_dim]: head_dim and ctx * head_dim) it appends
-// keys. t 0 does nothing.
+// keys. y is an address: a captured call writes the same cache rows at every
+// replay. Where a graph is to serve other lengths, as strasgpt_k_attn_tree's
+// does, let it write to a buffer and copy the rows into the cache outside the
+// graph (or capture again, or update the node). t 0 does nothing.
 int strasgpt_k_rope(const void* x, long long x_token_stride,
                     long long x_head_stride, void* y, long long y_token_stride,
                     long long y_head_stride, int type, int t, int heads,

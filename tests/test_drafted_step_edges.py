@@ -9,8 +9,8 @@ import sys
 import numpy as np
 import pytest
 from strasgpt_b200 import runtime
-from test_drafted_step import (BF16, F32, FAKE, H, check_sample, dtype, run_sample,
-                               sample_row)
+from test_drafted_step import (BF16, F32, FAKE, H, check_rope, check_sample, dtype, mask_words,
+                               run_sample, sample_row, tree_mask, tree_reference, tree_tolerance)
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -247,3 +247,129 @@ def test_rope_refuses_frequencies_beyond_64_bits(capfd, kind, far):
                                            FAKE, runtime.Rope(**kind), None)
     err = capfd.readouterr().err
     assert status == -1 and ("beyond 64 bits" in err) == far, err
+
+
+# --------------------------------------------------------------------------
+# captured steps
+# --------------------------------------------------------------------------
+class Step:
+    """A step over drafted tokens on buffers of its own: q turned in place, k
+    and v rows into the caches, attention, a head's logits, a token each."""
+    T, KH, G, HD, CTX, VOCAB = 19, 2, 4, 64, 512, 2048
+
+    def __init__(self, torch):
+        self.torch, self.L = torch, runtime.lib()
+        t, kh, hd, ctx, qh = self.T, self.KH, self.HD, self.CTX, self.KH * self.G
+        self.gen = torch.Generator(device="cuda").manual_seed(5)
+        self.rows = torch.zeros(t, qh + 2 * kh, hd, device="cuda")
+        self.turned = torch.zeros(t, kh, hd, device="cuda")
+        self.k, self.v = (torch.randn(kh, ctx, hd, device="cuda", generator=self.gen)
+                          for _ in range(2))
+        self.w = torch.randn(self.VOCAB, qh * hd, device="cuda",
+                             generator=self.gen).to(torch.bfloat16)
+        self.cached = torch.zeros(1, dtype=torch.int32, device="cuda")
+        self.pos = torch.zeros(t, dtype=torch.int32, device="cuda")
+        self.mask = tree_mask(t, 13)
+        self.words = mask_words(torch, self.mask)
+        self.att = torch.zeros(t, qh, hd, device="cuda")
+        self.logits = torch.zeros(t, self.VOCAB, device="cuda")
+        self.u = torch.zeros(t, device="cuda")
+        self.token = torch.zeros(t, dtype=torch.int32, device="cuda")
+        self.size = self.L.strasgpt_k_attn_tree_workspace(t, kh, self.G, hd)
+        self.work = torch.zeros(self.size, dtype=torch.uint8, device="cuda")
+        self.rope = runtime.Rope(hd, theta=500000.0)
+        self.side = torch.cuda.Stream()
+
+    def turn(self, n):
+        """q in place, k into the cache rows from n on (None: a buffer)."""
+        s, qh, t = self.torch.cuda.current_stream().cuda_stream, self.KH * self.G, self.T
+        ld, hd = self.rows.stride(0), self.HD
+        to, yt, yh = ((self.turned, self.turned.stride(0), hd) if n is None
+                      else (self.k[:, n:], hd, self.CTX * hd))
+        assert self.L.strasgpt_k_rope(self.rows[:, qh:].data_ptr(), ld, hd, to.data_ptr(), yt, yh,
+                                      F32, t, self.KH, hd, self.pos.data_ptr(), self.rope, s) == 0
+        assert self.L.strasgpt_k_rope(self.rows.data_ptr(), ld, hd, self.rows.data_ptr(), ld, hd,
+                                      F32, t, qh, hd, self.pos.data_ptr(), self.rope, s) == 0
+
+    def values(self, n):
+        self.v[:, n:n + self.T].copy_(self.rows[:, -self.KH:].transpose(0, 1))
+
+    def answer(self):
+        s, d = self.torch.cuda.current_stream().cuda_stream, self.att.stride(0)
+        assert self.L.strasgpt_k_attn_tree(
+            self.rows.data_ptr(), self.rows.stride(0), self.k.data_ptr(), self.v.data_ptr(), F32,
+            self.T, self.KH, self.G, self.HD, self.CTX, self.cached.data_ptr(),
+            self.words.data_ptr(), self.att.data_ptr(), d, self.work.data_ptr(), self.size, s) == 0
+        assert self.L.strasgpt_k_gemm_simt(self.att.data_ptr(), d, self.w.data_ptr(), d, self.T,
+                                           self.VOCAB, self.logits.data_ptr(), self.VOCAB, 0,
+                                           s) == 0
+        assert self.L.strasgpt_k_sample(self.logits.data_ptr(), F32, self.VOCAB, self.T,
+                                        self.VOCAB, None, None, None, None, self.u.data_ptr(),
+                                        self.token.data_ptr(), None, None, s) == 0
+
+    def capture(self, *parts):
+        graph = self.torch.cuda.CUDAGraph()
+        self.torch.cuda.synchronize()
+        with self.torch.cuda.graph(graph, stream=self.side):
+            for part in parts:
+                part()
+        return graph
+
+    def new_inputs(self, n):
+        """On the side stream, for a step at length n; a copy for check()."""
+        self.rows.normal_(generator=self.gen)
+        self.u.uniform_(generator=self.gen)
+        self.cached.fill_(n)
+        self.pos.copy_(self.torch.from_numpy(n + self.mask.sum(1) - 1))
+        self.token.fill_(-7)
+        self.att.fill_(float("nan"))
+        self.before = [x.clone() for x in (self.rows, self.k, self.v)]
+
+    def check(self, n):
+        self.torch.cuda.synchronize()
+        torch, t, qh, kh = self.torch, self.T, self.KH * self.G, self.KH
+        rows, k, v = self.before
+        check_rope(torch, self.rows[:, :qh], rows[:, :qh], self.pos, self.rope, F32)
+        check_rope(torch, self.k[:, n:n + t].transpose(0, 1), rows[:, qh:qh + kh], self.pos,
+                   self.rope, F32)
+        v[:, n:n + t] = rows[:, qh + kh:].transpose(0, 1)
+        k[:, n:n + t] = self.k[:, n:n + t]
+        assert torch.equal(self.k, k) and torch.equal(self.v, v)   # and nothing else
+        want, reach, top = tree_reference(torch, self.rows[:, :qh], k, v, n, self.mask)
+        err = (self.att.double() - want).abs()
+        assert (err <= tree_tolerance(want, reach, top, n + t, self.HD, F32)).all()
+        for i, row in enumerate(self.logits.double().cpu().numpy()):
+            assert self.token[i] == sample_row(row, 1.0, 0, 1.0, 0.0, float(self.u[i]))[0]
+
+
+@pytest.mark.gpu
+def test_a_captured_step_is_replayed(cuda):
+    """The whole step in one graph, replayed for other inputs of the same
+    length; captured again for another length, whose rows it then writes."""
+    torch = cuda
+    step = Step(torch)
+    for n in (333, 40):
+        graph = step.capture(lambda: step.turn(n), lambda: step.values(n), step.answer)
+        for _ in range(3):
+            with torch.cuda.stream(step.side):
+                step.new_inputs(n)
+                graph.replay()
+            step.check(n)
+
+
+@pytest.mark.gpu
+def test_captured_parts_serve_every_length(cuda):
+    """Rotation into a buffer is one graph, attention to token another; between
+    their replays the keys and values go to the rows behind the cached ones by
+    copies that are not captured. The length moves on, back and to the end."""
+    torch = cuda
+    step = Step(torch)
+    turn, answer = step.capture(lambda: step.turn(None)), step.capture(step.answer)
+    for n in (333, 338, 0, 7, step.CTX - step.T):
+        with torch.cuda.stream(step.side):
+            step.new_inputs(n)
+            turn.replay()
+            step.k[:, n:n + step.T].copy_(step.turned.transpose(0, 1))
+            step.values(n)
+            answer.replay()
+        step.check(n)
