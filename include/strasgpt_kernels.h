@@ -96,10 +96,12 @@ int strasgpt_k_matvec_noalloc(const float* x, const uint16_t* norm_w,
 // captured into a CUDA graph, which keeps the addresses and numbers of the
 // call and reads what is in device memory (positions, lengths, masks, filters,
 // random numbers) at each replay. Each returns 0 once its work is enqueued; an
-// invalid argument, a buffer that is not on the current device or a failed
-// launch returns -1 with a "[StrasGPT] Error ..." message on stderr and
-// enqueues nothing. What is in device memory cannot be refused: each says what
-// it does with any value.
+// invalid argument or a buffer that is not on the current device returns -1
+// with a "[StrasGPT] Error ..." message on stderr and enqueues nothing. A
+// launch that fails returns -1 with a message too; attention and sampling may
+// be two launches, of which the first is then enqueued: outputs and workspace
+// hold nothing of use. What is in device memory cannot be refused: each says
+// what it does with any value.
 #define STRASGPT_F32  0
 #define STRASGPT_BF16 1
 
