@@ -188,7 +188,9 @@ int strasgpt_k_attn_tree(const void* q, long long ldq, const void* k_cache,
 // one, in index order, at which the running sum of w exceeds u times the sum
 // of all that remain (u not above 0: the first, u not below 1: the last; an
 // entry whose w is 0 in 64 bits is never drawn). Weights and sums are held in
-// 64 bits, weights to 2^-42 of themselves. prob (NULL: not wanted) gets the
+// 64 bits, weights to 2^-42 of themselves; where top_p's border, or the mass
+// of what the filters leave, is summed over a whole row, to 2^-30, which counts
+// where a border lies that close to an entry's end. prob (NULL: not wanted) gets the
 // token's share of the remaining mass, kept (NULL) how many entries remained.
 // NaN logits count as -inf, which are never taken; a row of nothing else gets
 // token -1, prob 0, kept 0. Where logits are +inf, those weigh 1 and all

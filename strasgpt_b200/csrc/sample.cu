@@ -12,9 +12,14 @@
 // hundred thousand tokens by more than many of them weigh. Sums that atomics
 // gather are integers, in a unit of 2^-31 of the largest weight that can be
 // in their bin of the histogram (two 16-bit halves of up to 45056 entries fit
-// 32-bit sums; the roundings, to nearest, stay below 1e-11 of a row's mass in
-// the mean), and all others are added in a fixed order: the same row gives
-// the same bits whatever the order of CTAs and threads.
+// 32-bit sums), and all others are added in a fixed order: the same row gives
+// the same bits whatever the order of CTAs and threads. A bin is less than 0.3
+// octaves wide and its unit's power of two at most one octave above its largest
+// weight, so a weight is rounded, to nearest, by at most 2^-30.7 of itself
+// (below 2^-72 of the largest one: by 2^-104). Different weights' roundings
+// mostly cancel; equal logits, as bf16 rows have by the thousand, round alike,
+// and move a border by up to that much of the mass before it: 2e-4 of an entry
+// in a flat row of 360448. Entries ranked next to a border have kFine bits more.
 //
 // A row is a thread-block cluster, each CTA holding a slice of it in shared
 // memory: logits are read from HBM once, whatever the filters then need.
