@@ -158,8 +158,9 @@ int strasgpt_k_rope(const void* x, long long x_token_stride,
 // are exact, the probabilities that multiply bf16 values keep 17 bits. A token
 // that sees nothing gets zeros.
 // Rows that a token does not see, and rows behind the last, may hold anything
-// (infinities and NaN too). *cached is read on the device and cut to
-// 0..ctx - t. head_dim 32, 64 or 128; group 1..128; q, the caches, att, their
+// (infinities and NaN too). att is q with ldo = ldq (in place), or shares no memory
+// with what is read. *cached is read on the device and cut to 0..ctx - t.
+// head_dim 32, 64 or 128; group 1..128; q, the caches, att, their
 // rows and the workspace are 16-byte aligned.
 //
 // The workspace has strasgpt_k_attn_tree_workspace(t, kv_heads, group,
@@ -190,13 +191,13 @@ int strasgpt_k_attn_tree(const void* q, long long ldq, const void* k_cache,
 // entry whose w is 0 in 64 bits is never drawn). Weights and sums are held in
 // 64 bits, weights to 2^-42 of themselves; where top_p's border, or the mass
 // of what the filters leave, is summed over a whole row, to 2^-30, which counts
-// where a border lies that close to an entry's end. prob (NULL: not wanted) gets the
-// token's share of the remaining mass, kept (NULL) how many entries remained.
-// NaN logits count as -inf, which are never taken; a row of nothing else gets
-// token -1, prob 0, kept 0. Where logits are +inf, those weigh 1 and all
-// others 0. vocab is at most STRASGPT_SAMPLE_MAX_VOCAB. token, prob and kept
-// share no memory with each other or the inputs. The result does not depend on
-// timing: the same inputs give the same bits.
+// where a border lies that close to an entry's end. prob (NULL: not wanted)
+// gets the token's share of the remaining mass, kept (NULL) how many entries
+// remained. NaN logits count as -inf, which are never taken; a row of nothing
+// else gets token -1, prob 0, kept 0. Where logits are +inf, those weigh 1 and
+// all others 0. vocab is at most STRASGPT_SAMPLE_MAX_VOCAB. token, prob and
+// kept share no memory with each other or the inputs. The result does not
+// depend on timing: the same inputs give the same bits.
 #define STRASGPT_SAMPLE_MAX_VOCAB 360448
 int strasgpt_k_sample(const void* logits, int type, long long ld, int rows,
                       int vocab, const float* temperature, const int* top_k,

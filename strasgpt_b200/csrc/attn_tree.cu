@@ -1044,6 +1044,8 @@ int strasgpt_k_attn_tree(const void* q, long long ldq, const void* k_cache, cons
   if (!sg::aligned(q, 16) || !sg::aligned(k_cache, 16) || !sg::aligned(v_cache, 16) ||
       !sg::aligned(att, 16) || (t > 1 && (ldq * size % 16 || ldo * size % 16)))
     return sg::refuse(me, "q, the caches, att and their rows must be 16-byte aligned");
+  if (q == att && t > 1 && ldq != ldo)
+    return sg::refuse(me, "in place, q and att must have the same strides");
   if (!sg::aligned(cached, 4) || !sg::aligned(mask, 8))
     return sg::refuse(me, "a buffer is not aligned to its entries");
   int dev = 0, sms = 0;

@@ -9,8 +9,9 @@ import sys
 import numpy as np
 import pytest
 from strasgpt_b200 import runtime
-from test_drafted_step import (BF16, F32, FAKE, H, check_rope, check_sample, dtype, mask_words,
-                               run_sample, sample_row, tree_mask, tree_reference, tree_tolerance)
+from test_drafted_step import (BF16, F32, FAKE, H, check_rope, check_sample, dtype, inputs,
+                               mask_words, run_sample, run_tree, sample_row, tree_mask,
+                               tree_reference, tree_tolerance)
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -247,6 +248,35 @@ def test_rope_refuses_frequencies_beyond_64_bits(capfd, kind, far):
                                            FAKE, runtime.Rope(**kind), None)
     err = capfd.readouterr().err
     assert status == -1 and ("beyond 64 bits" in err) == far, err
+
+
+# (t, kv heads, q heads on each, head_dim, cached) -> every kernel of the
+# attention, with and without splits of the keys.
+SHAPES = [(1, 2, 4, 128, 700), (4, 320, 1, 128, 100), (3, 2, 5, 128, 700), (6, 2, 4, 64, 1000),
+          (20, 320, 1, 64, 90), (9, 2, 8, 32, 500), (3, 320, 2, 32, 45), (70, 2, 1, 32, 300),
+          (24, 2, 4, 128, 900), (40, 160, 1, 64, 200), (260, 1, 1, 128, 400)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [F32, BF16])
+@pytest.mark.parametrize("t,kh,g,hd,n", SHAPES)
+def test_tree_in_place(cuda, type_, t, kh, g, hd, n):
+    """The outputs over the queries: what another buffer gets."""
+    torch = cuda
+    q, k, v = inputs(torch, t, kh, g, hd, n + t + 3, type_, t)
+    m = tree_mask(t, n)
+    want = run_tree(torch, q, k, v, n, m, type_)
+    same = q.clone()
+    assert torch.equal(run_tree(torch, same, k, v, n, m, type_, att=same), want)
+
+
+@pytest.mark.parametrize("ldo,words", [(1024, "device"), (1536, "in place")])
+def test_tree_refuses_other_strides_in_place(capfd, ldo, words):
+    status = runtime.lib().strasgpt_k_attn_tree(
+        FAKE, 1024, 2 * FAKE, 3 * FAKE, F32, 8, 2, 4, 128, 64, FAKE, FAKE, FAKE, ldo, FAKE,
+        1 << 40, None)
+    err = capfd.readouterr().err
+    assert status == -1 and words in err.lower(), err
 
 
 # --------------------------------------------------------------------------
