@@ -158,7 +158,10 @@ int strasgpt_k_rope(const void* x, long long x_token_stride,
 // are exact, the probabilities that multiply bf16 values keep 17 bits. A token
 // that sees nothing gets zeros.
 // Rows that a token does not see, and rows behind the last, may hold anything
-// (infinities and NaN too). att is q with ldo = ldq (in place), or shares no memory
+// (infinities and NaN too). Rows that it sees hold finite numbers: an infinity
+// or NaN among them leaves that token's outputs of the q heads on that kv head
+// unspecified (infinite, NaN, or as if the row were not there, by the number of
+// rows), and no others. att is q with ldo = ldq (in place), or shares no memory
 // with what is read. *cached is read on the device and cut to 0..ctx - t.
 // head_dim 32, 64 or 128; group 1..128; q, the caches, att, their
 // rows and the workspace are 16-byte aligned.

@@ -279,6 +279,37 @@ def test_tree_refuses_other_strides_in_place(capfd, ldo, words):
     assert status == -1 and words in err.lower(), err
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [F32, BF16])
+@pytest.mark.parametrize("t,kh,g,hd,n", SHAPES)
+def test_tree_infinite_cached_rows_stay_in_their_head(cuda, type_, t, kh, g, hd, n):
+    """Infinities and NaN in rows that all tokens see: nothing is said of the q
+    heads on that kv head, all others have the same bits."""
+    torch = cuda
+    kh = max(kh, 2)
+    q, k, v = inputs(torch, t, kh, g, hd, n + t + 3, type_, t)
+    m = tree_mask(t, n)
+    want = run_tree(torch, q, k, v, n, m, type_).view(t, kh, g, hd)
+    k[1, 5], k[1, n - 1, 3] = float("inf"), -float("inf")
+    v[1, 17], v[1, n // 2, 0] = float("nan"), float("inf")
+    got = run_tree(torch, q, k, v, n, m, type_).view(t, kh, g, hd)
+    others = [h for h in range(kh) if h != 1]
+    assert torch.equal(got[:, others], want[:, others])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [F32, BF16])
+@pytest.mark.parametrize("t,kh,g,hd,n", SHAPES)
+def test_tree_repeats_itself(cuda, type_, t, kh, g, hd, n):
+    """The same call, the same bits."""
+    torch = cuda
+    q, k, v = inputs(torch, t, kh, g, hd, n + t + 3, type_, t)
+    m = tree_mask(t, n)
+    want = run_tree(torch, q, k, v, n, m, type_)
+    for _ in range(3):
+        assert torch.equal(run_tree(torch, q, k, v, n, m, type_), want)
+
+
 # --------------------------------------------------------------------------
 # captured steps
 # --------------------------------------------------------------------------
