@@ -113,21 +113,29 @@ __device__ __forceinline__ bool finite_bf16x8(uint4 v) {
 // paddings make every fragment load below free of bank conflicts: 16 bytes
 // shift ldmatrix rows (bf16) and the fp32 value rows 2c apart by two 16-byte
 // groups; 64 bytes put neighbouring fp32 key rows on opposite banks.
-template <typename T, int HD>
+//
+// CTAs of up to four warps are two to an SM, and their tiles must leave room:
+// with head_dim 32, where a row's padding is as much as half of it, that takes
+// half the keys (16 rows over 8 x 128000 keys: fp32 92 -> 85 us, bf16 54 -> 54;
+// over 8 x 4000: 11.0 -> 9.2, 8.4 -> 7.9). Larger CTAs have an SM each.
+constexpr size_t kSmSmem = 228 * 1024, kCtaReserved = 1024;
+
+template <typename T, int HD, int WARPS>
 struct Tile {
   static constexpr bool kF32 = sizeof(T) == 4;
-  static constexpr int kKeys = (kF32 ? 4096 : 8192) / HD;
+  static constexpr int kKeys = (kF32 ? 4096 : 8192) / HD / (WARPS <= 4 && HD == 32 ? 2 : 1);
   static constexpr int kKRow = HD * (int)sizeof(T) + (kF32 ? 64 : 16);
   static constexpr int kVRow = HD * (int)sizeof(T) + 16;
   static constexpr int kStage = kKeys * (kKRow + kVRow);
   static constexpr size_t kBytes = (size_t)kStages * kStage;
+  static_assert((WARPS <= 4 ? 2 : 1) * (kBytes + kCtaReserved) <= kSmSmem, "the CTAs of an SM fit");
 };
 
 // The tiles of a split: the cached keys, then the drafted ones. A tile holds
 // keys of one kind, never of both.
 template <typename T, int HD, int THREADS>
 struct Walk {
-  using L = Tile<T, HD>;
+  using L = Tile<T, HD, THREADS / 32>;
   const T *k, *v;                // of the kv head
   int t, n, old_tiles, tile0, tile1;
   uint32_t smem;
@@ -176,7 +184,7 @@ struct Walk {
 // MW warps side by side in rows (16 each), KW in keys.
 template <typename T, int HD, int MW, int KW>
 __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(TreeArgs a) {
-  using L = Tile<T, HD>;
+  using L = Tile<T, HD, MW * KW>;
   constexpr bool kF32 = L::kF32;
   constexpr int kThreads = 32 * MW * KW;
   constexpr int kRows = 16 * MW;
@@ -593,7 +601,7 @@ constexpr int kFewRows = 4, kFewWarps = 4, kFewHeadDim = 128;
 
 __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(TreeArgs a) {
   constexpr int HD = kFewHeadDim;
-  using L = Tile<float, HD>;
+  using L = Tile<float, HD, kFewWarps>;
   constexpr int kWarpKeys = L::kKeys / kFewWarps, kQ = HD / 16, kO = HD / 32;
   static_assert(kWarpKeys == 8, "a warp's keys of a tile are one step");
   extern __shared__ __align__(16) unsigned char smem[];
@@ -946,7 +954,7 @@ size_t workspace_of(int splits, int t, int kh, int group, int hd) {
 
 cudaError_t launch_few(const TreeArgs& a, int dev, cudaStream_t s) {
   static std::atomic<size_t> allowed[sg::kDevices];
-  using L = Tile<float, kFewHeadDim>;
+  using L = Tile<float, kFewHeadDim, kFewWarps>;
   cudaError_t e = sg::allow_smem(k_tree_few, L::kBytes, dev, allowed);
   if (e != cudaSuccess) return e;
   e = sg::try_launch(k_tree_few, dim3(a.splits, a.kh), dim3(32 * kFewWarps), L::kBytes, 1, s, a);
@@ -958,7 +966,8 @@ cudaError_t launch_few(const TreeArgs& a, int dev, cudaStream_t s) {
 template <typename T, int HD, int MW, int KW>
 cudaError_t launch_shape(const TreeArgs& a, int dev, cudaStream_t s) {
   static std::atomic<size_t> allowed[sg::kDevices];
-  constexpr size_t bytes = Tile<T, HD>::kBytes;
+  using L = Tile<T, HD, MW * KW>;
+  constexpr size_t bytes = L::kBytes;
   cudaError_t e = sg::allow_smem(k_tree<T, HD, MW, KW>, bytes, dev, allowed);
   if (e != cudaSuccess) return e;
   const int rows = a.t * a.group;
@@ -967,7 +976,7 @@ cudaError_t launch_shape(const TreeArgs& a, int dev, cudaStream_t s) {
                      dim3(32 * MW * KW), bytes, 1, s, a);
   if (e != cudaSuccess || a.splits == 1) return e;
   return sg::try_launch(k_merge<T, HD, false>, dim3(rows * a.kh), dim3(kMergeThreads), 0, 1, s, a,
-                        Tile<T, HD>::kKeys);
+                        L::kKeys);
 }
 
 template <typename T, int HD>
