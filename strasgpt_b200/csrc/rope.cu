@@ -10,8 +10,8 @@
 // (fp32 rows) what its rounding left, less than 2^-23, to first order. That
 // correction and the magnitude, as two fp32 values, come to one rounding.
 //
-// What bounds it: bytes (each entry read and written once) for a chunk, one
-// launch for a token. A block has a run of items (two a thread), loads them
+// What bounds it: bytes (each entry read and written once) for a chunk of fp32,
+// instruction issue (73 % of cycles) for one of bf16, one launch for a token. A block has a run of items (two a thread), loads them
 // first, and computes the sines of their tokens, once for all heads, in
 // shared memory while they are on their way: the sines' 64-bit part costs a
 // multiply per pair and token instead of one per entry. Measured on a B200:

@@ -41,10 +41,11 @@
 // 151936 under top-p 0.95, 87 us: two rounds of CTAs, 31 us each, of which the
 // histogram's 64-bit weights and shared-memory additions are 10 us (0.5 cycles
 // an entry and SM), four exchanges 11, the division of the border's bin 4, the
-// reading 3. 256 rows of 201088 bf16 logits under top-k 200, 53 us (1.9 TB/s;
-// 16 us of bytes): two reads, the second from L2, and a sort per row. Slices
-// read again from L2 instead of kept in shared memory were slower at every
-// size (64 rows of 151936: 129 us).
+// reading 3 (of the other 25 us a part is the launch in front, k_sample_rows;
+// they were not taken apart further). 256 rows of 201088 bf16 logits under
+// top-k 200, 53 us (1.9 TB/s; 16 us of bytes): two reads, the second from L2,
+// and a sort per row. Slices read again from L2 instead of kept in shared
+// memory were slower at every size (64 rows of 151936: 129 us).
 #include <cooperative_groups.h>
 #include <float.h>
 
