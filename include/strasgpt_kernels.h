@@ -133,10 +133,10 @@ typedef struct strasgpt_rope {
 // position pos[i] (any int: tokens may share a position, a negative one turns
 // back) and written to y + i * y_token_stride + h * y_head_stride; entries
 // behind the first rope->dim are copied. Angles are computed in 64 bits, the
-// rest in 32 (frequencies of 1e298 turns and more are refused). y is x with the same strides (in place), or shares no memory
-// with x's rows; rows of y must not overlap. With the strides of a layer's
-// cache ([kv_heads][ctx][head_dim]: head_dim and ctx * head_dim) it appends
-// keys. y is an address: a captured call writes the same cache rows at every
+// rest in 32 (frequencies of 1e298 turns and more are refused). y is x with the
+// same strides (in place), or shares no memory with x's rows; rows of y must
+// not overlap. With the strides of a layer's cache ([kv_heads][ctx][head_dim]:
+// head_dim and ctx * head_dim) it appends keys. y is an address: a captured call writes the same cache rows at every
 // replay. Where a graph is to serve other lengths, as strasgpt_k_attn_tree's
 // does, let it write to a buffer and copy the rows into the cache outside the
 // graph (or capture again, or update the node). t 0 does nothing.
@@ -157,14 +157,15 @@ int strasgpt_k_rope(const void* x, long long x_token_stride,
 // in 32 bits. Products keep 21 bits of each fp32 operand at least; bf16 ones
 // are exact, the probabilities that multiply bf16 values keep 17 bits. A token
 // that sees nothing gets zeros.
+//
 // Rows that a token does not see, and rows behind the last, may hold anything
 // (infinities and NaN too). Rows that it sees hold finite numbers: an infinity
 // or NaN among them leaves that token's outputs of the q heads on that kv head
 // unspecified (infinite, NaN, or as if the row were not there, by the number of
 // rows), and no others. att is q with ldo = ldq (in place), or shares no memory
 // with what is read. *cached is read on the device and cut to 0..ctx - t.
-// head_dim 32, 64 or 128; group 1..128; q, the caches, att, their
-// rows and the workspace are 16-byte aligned.
+// head_dim 32, 64 or 128; group 1..128; q, the caches, att, their rows and the
+// workspace are 16-byte aligned.
 //
 // The workspace has strasgpt_k_attn_tree_workspace(t, kv_heads, group,
 // head_dim) bytes (asked on the same device; 0: may be NULL). Its contents

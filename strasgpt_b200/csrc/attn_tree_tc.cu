@@ -33,9 +33,9 @@
 // 200 TFLOP/s); 32 rows over 128000 keys 93 us (5.6 TB/s) and 301 us (3.5
 // TB/s), in short runs; calls one after another for a second take 118, 201 and
 // (bf16) 113 us. What bounds 128 rows and more: bf16, 0.7 us per tile, the
-// matrix instructions (0.4 us: 32 cycles per 16 entries of Q K^T from tensor memory,
-// 48 from shared memory, 64 per 16 keys and part of P V) and the hand-overs
-// between them and the softmax; fp32, 2.9 us per tile, the six warps that make
+// matrix instructions (0.4 us: 32 cycles per 16 entries of Q K^T from tensor
+// memory, 48 from shared memory, 64 per 16 keys and part of P V) and the
+// hand-overs between them and the softmax; fp32, 2.9 us per tile, the six warps that make
 // parts (0.9 us for 64 rows, and as much again in waiting and handing over),
 // while the matrix instructions take 1.6. Two fp16 parts of scaled rows and
 // half the matrix instructions were slower (226 us): the rows' largest values

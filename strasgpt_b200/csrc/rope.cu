@@ -11,10 +11,11 @@
 // correction and the magnitude, as two fp32 values, come to one rounding.
 //
 // What bounds it: bytes (each entry read and written once) for a chunk of fp32,
-// instruction issue (73 % of cycles) for one of bf16, one launch for a token. A block has a run of items (two a thread), loads them
-// first, and computes the sines of their tokens, once for all heads, in
-// shared memory while they are on their way: the sines' 64-bit part costs a
-// multiply per pair and token instead of one per entry. Measured on a B200:
+// instruction issue (73 % of cycles) for one of bf16, one launch for a token.
+// A block has a run of items (two a thread), loads them first, and computes
+// the sines of their tokens, once for all heads, in shared memory while they
+// are on their way: the sines' 64-bit part costs a multiply per pair and token
+// instead of one per entry. Measured on a B200:
 // 1.8 us for one token of 40 heads of 128 fp32 entries, 4.5 us (3.7 TB/s) for
 // 2048 tokens of 8 such heads into a cache, 44 us (3.8 TB/s; a plain copy of
 // as many contiguous bytes takes 33) for 8191 tokens of 40 heads of 128 bf16
@@ -209,11 +210,11 @@ extern "C" int strasgpt_k_rope(const void* x, long long x_token_stride, long lon
   a.magnitude_rest = (float)(rope->magnitude - a.magnitude);
   const int half = rope->dim / 2;
   // f_j = theta^(-2 j / dim) as a running product in 64-bit mantissas: at most
-  // 255 roundings and as many times the ratio's own, 2^-55 in all, so that a
-  // pair's turns per position are off by their last rounding to 64 bits (2^-53)
-  // and no more, which is what counts at far positions. (In doubles the
-  // product was off by up to 2^-46: 4e-6 radians at position 2^31 for 512
-  // entries and theta 2.)
+  // 255 roundings of 2^-64 and as many times the ratio's own (2^-63), 2^-54 in
+  // all, so that a pair's turns per position are off by little more than their
+  // last rounding to 64 bits (2^-53), which is what counts at far positions.
+  // (In doubles the product was off by up to 2^-46: 4e-6 radians at position
+  // 2^31 for 512 entries and theta 2.)
   const long double per_turn = 1 / 6.283185307179586476925286766559L;
   const long double ratio = powl(rope->theta, -2.0L / rope->dim);
   const long double stretched =

@@ -720,8 +720,8 @@ struct Row {
 
   // The prefix of the order that a filter keeps: its last entry (key and
   // index) and its mass. tail: the border lies among entries whose weight the
-  // histogram rounds to 0; all others are kept, and `zeros` of those. sums: sh->before_mass and
-  // sh->before_count say what is kept of each slice.
+  // histogram rounds to 0; all others are kept, and `zeros` of those. sums:
+  // sh->before_mass and sh->before_count say what is kept of each slice.
   struct Cut {
     unsigned key;
     int idx;
@@ -1294,7 +1294,8 @@ extern "C" int strasgpt_k_sample(const void* logits, int type, long long ld, int
   for (int i = 0; i < 3; i++)
     for (int j = i + 1; j < 8; j++)
       if (by_row[i] && by_row[j] && sg::overlap(by_row[i], by_row[j], (size_t)rows * 4))
-        return sg::refuse(me, "token, prob and kept must not share memory with each other or the inputs");
+        return sg::refuse(me, "token, prob and kept must not share memory with each other or the "
+                              "inputs");
   int dev = 0, sms = 0;
   if (const char* why = sg::current_device(&dev, &sms)) return sg::refuse(me, why);
   for (const void* p : {logits, (const void*)temperature, (const void*)top_k, (const void*)top_p,

@@ -54,9 +54,9 @@ assert status == [0] * 400, status
                                                (128, 1e4, "none")])
 def test_rope_far_positions(cuda, interleaved, dim, theta, scaling):
     """Positions up to the largest int, against angles with 64-bit mantissas.
-    The turns per position and their product with the position are rounded to
-    64 bits, 2^-53 of the turns each: 2^-52 |pos| f radians on top of the bound
-    for near positions."""
+    The turns per position are off by 2^-54 of themselves (a running product)
+    and rounded to 64 bits, as is their product with the position, 2^-53 each:
+    1.25 2^-52 |pos| f radians on top of the bound for near positions."""
     torch = cuda
     ld = np.longdouble
     kind = dict(none=dict(), linear=dict(scaling=runtime.ROPE_LINEAR, factor=3.0),
@@ -84,7 +84,7 @@ def test_rope_far_positions(cuda, interleaved, dim, theta, scaling):
                 else (slice(0, dim // 2), slice(dim // 2, dim)))
     a, b = (x.double().cpu().numpy()[..., i] for i in (one, two))
     got = y.double().cpu().numpy()
-    tol = (16 * H + 2.0 ** -52 * np.abs(pos)[:, None] * f.astype(np.float64))[:, None]
+    tol = (16 * H + 1.25 * 2.0 ** -52 * np.abs(pos)[:, None] * f.astype(np.float64))[:, None]
     tol = tol * (np.abs(a) + np.abs(b))
     assert (np.abs(got[..., one] - (a * c - b * s)) <= tol).all()
     assert (np.abs(got[..., two] - (a * s + b * c)) <= tol).all()
@@ -97,7 +97,7 @@ def test_rope_sines_keep_their_bits(cuda, theta, dim):
     is small, near quarters the cosine, and each is right relative to itself:
     sincospif to 2 steps (4 h), the correction's sum and the products (by 1, 0
     and the magnitude 1) to half a step each (2 h), the correction itself to
-    2^-23 steps; and to the 64-bit angle's own error, 2^-52 |pos| f."""
+    2^-23 steps; and to the 64-bit angle's own error, 1.25 2^-52 |pos| f."""
     torch = cuda
     t = 4096
     rng = np.random.RandomState(dim)
@@ -117,8 +117,8 @@ def test_rope_sines_keep_their_bits(cuda, theta, dim):
     got = y[:, 0].double().cpu().numpy()
     for part, want in ((got[:, :dim // 2], np.cos(angle)), (got[:, dim // 2:], np.sin(angle))):
         err = np.abs(part - want)
-        tol = (6 + 2.0 ** -20) * H * np.abs(want) + 2.0 ** -46 * H + 2.0 ** -52 * np.abs(
-            pos)[:, None] * f
+        tol = ((6 + 2.0 ** -20) * H * np.abs(want) + 2.0 ** -46 * H
+               + 1.25 * 2.0 ** -52 * np.abs(pos)[:, None] * f)
         assert (err <= tol).all(), float((err - tol).max())
 
 
