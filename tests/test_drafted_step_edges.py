@@ -236,7 +236,8 @@ def test_sample_refuses_shared_outputs(capfd, one, other, apart, shared):
 
 
 @pytest.mark.parametrize("kind,far", [
-    (dict(dim=512, theta=5e-324), True), (dict(dim=64, theta=1e-300, scaling=1, factor=1e-100), True),
+    (dict(dim=512, theta=5e-324), True),
+    (dict(dim=64, theta=1e-300, scaling=1, factor=1e-100), True),
     (dict(dim=64, theta=1e4, scaling=1, factor=5e-324), True),
     (dict(dim=64, theta=1e4, scaling=2, factor=1e-300, original=10), True),
     (dict(dim=512, theta=1e-290), False), (dict(dim=512, theta=1.7e308), False),
