@@ -148,9 +148,8 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, unsigned parity) {
       : "memory");
   return ok != 0;
 }
-// Bounded wait for what was issued, whatever has failed. Not inlined: with its
-// loops in the loaders' code 256 rows over 65500 bf16 keys took 129 us for 115.
-__device__ __noinline__ void mbar_drain(uint32_t bar, unsigned parity) {
+// Bounded wait for what was issued, whatever has failed.
+__device__ __forceinline__ void mbar_drain(uint32_t bar, unsigned parity) {
   const unsigned long long t0 = now_ns();
   while (!mbar_try_wait(bar, parity) && now_ns() - t0 < kTimeoutNs) {
   }
@@ -544,10 +543,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           // Nothing is on its way when the CTA ends, whatever has failed: the
           // last tile asked for in each stage is waited for (those before it
-          // were, before it was asked for).
-#pragma unroll 1
-          for (int s = 0; s < kStages && s < asked; s++)
-            mbar_drain(saddr(&full[s]), tree_last_parity(asked, s, kStages));
+          // were, before it was asked for), by a lane each: a loop over the
+          // stages made 256 rows over 65500 bf16 keys 129 us for 115.
+          if (lane < kStages && lane < asked)
+            mbar_drain(saddr(&full[lane]), tree_last_parity(asked, lane, kStages));
+          __syncwarp();
         };
         if (warp == 10) load(&k_map, kbase, false, k_full, k_empty);
         if (warp == 11) load(&v_map, vbase, true, v_full, v_empty);
@@ -634,9 +634,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         // After a failure units may still be on their way: their memory is
         // this CTA's until they have landed. (The last warp has waited for
         // all of them otherwise.)
-        if (warp == 15 && !ok)
-          for (int x = 0; x < kRing && x < asked; x++)
-            mbar_drain(saddr(&raw_full[x]), tree_last_parity(asked, x, kRing));
+        if (warp == 15 && !ok && lane < kRing && lane < asked)
+          mbar_drain(saddr(&raw_full[lane]), tree_last_parity(asked, lane, kRing));
+        __syncwarp();
       }
     }
   } else {
