@@ -31,8 +31,8 @@
 // Measured, 8 kv heads of head_dim 128: 256 rows over 65500 bf16 keys 97 us
 // (2.8 TB/s of cache, 710 TFLOP/s), over 32768 fp32 keys 170 us (1.6 TB/s,
 // 200 TFLOP/s); 32 rows over 128000 keys 93 us (5.6 TB/s) and 301 us (3.5
-// TB/s), in short runs; calls one after another for a second take 118, 201 and
-// (bf16) 113 us. What bounds 128 rows and more: bf16, 0.7 us per tile, the
+// TB/s), in short runs; calls one after another for a second take 115, 198 and
+// (bf16) 110 us. What bounds 128 rows and more: bf16, 0.7 us per tile, the
 // matrix instructions (0.4 us: 32 cycles per 16 entries of Q K^T from tensor
 // memory, 48 from shared memory, 64 per 16 keys and part of P V) and the
 // hand-overs between them and the softmax; fp32, 2.9 us per tile, the six warps that make
