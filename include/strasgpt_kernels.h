@@ -208,6 +208,76 @@ int strasgpt_k_sample(const void* logits, int type, long long ld, int rows,
                       const float* top_p, const float* min_p, const float* u,
                       int* token, float* prob, int* kept, void* stream);
 
+// --- A step of a batch of requests ------------------------------------------
+// The entry points below serve a batch of requests at once: positions on
+// several axes (images and video among the text), an adapter of its own for
+// each request, attention behind a prefix that all requests share. What is
+// said above of a step over drafted tokens holds for them: device memory of
+// the current device, STRASGPT_F32 or STRASGPT_BF16 buffers, nothing allocated
+// or kept between calls, captured calls that read device memory anew at each
+// replay, -1 with a message and nothing enqueued for what is refused.
+
+// How the dim / 2 turned pairs of a head are shared out among axes, such as
+// time, height and width:
+//   STRASGPT_AXES_RUNS   the first section[0] pairs are axis 0's, the next
+//                        section[1] axis 1's, and so on
+//   STRASGPT_AXES_DEALT  one pair to each axis in turn; an axis that has its
+//                        section[i] pairs is passed over
+#define STRASGPT_AXES_RUNS  0
+#define STRASGPT_AXES_DEALT 1
+#define STRASGPT_ROPE_AXES_MAX 4
+typedef struct strasgpt_rope_axes {
+  int axes;      // 1..STRASGPT_ROPE_AXES_MAX
+  int section[STRASGPT_ROPE_AXES_MAX];  // pairs of each axis, dim / 2 in all; 0: none
+  int order;     // STRASGPT_AXES_*
+  int separate;  // 0: pair j turns by f_j, whatever its axis. 1: each axis counts
+                 // its own pairs from 0, and its m-th turns by
+                 // f = theta^(-m / section), stretched as rope->scaling says
+} strasgpt_rope_axes_t;
+
+// strasgpt_k_rope for tokens that have a position on each of several axes: pair
+// j, which is axis a's, turns by the angle of position
+// pos[a * pos_axis_stride + i * pos_token_stride] (strides not negative; 0:
+// positions that axes, or tokens, share). All else is as there: with one axis,
+// or the same position on all of them and separate 0, the results are the same
+// bits.
+int strasgpt_k_rope_axes(const void* x, long long x_token_stride,
+                         long long x_head_stride, void* y,
+                         long long y_token_stride, long long y_head_stride,
+                         int type, int t, int heads, int head_dim,
+                         const int* pos, long long pos_axis_stride,
+                         long long pos_token_stride, const strasgpt_rope_t* rope,
+                         const strasgpt_rope_axes_t* axes, void* stream);
+
+// Low-rank adapters of a batch's requests, beside a projection that all of its
+// m tokens share. Token i (k entries at x + i * ldx) has adapter
+// d = adapter[i]: A = a + d * rank * k ([rank][k], as a weight matrix) and
+// B = b + d * n * rank ([n][rank]), bf16 both. With
+//   v = base_i + scale[d] B (A x_i)      (n entries; scale NULL: 1)
+// where base_i (at base + i * ldb; NULL: zeros) is the token's row of the
+// shared projection, out_i (at out + i * ldo) gets, by epi,
+//   STRASGPT_EPI_STORE   v
+//   STRASGPT_EPI_ADD     out_i + v (the projection's output onto a residual)
+//   STRASGPT_EPI_SWIGLU  silu(v_2f) v_2f+1, f < n / 2: base and B have gate and
+//                        up rows interleaved as in strasgpt_k_gemm_tc
+// A token whose adapter[i] is not in 0..adapters - 1 has none: v = base_i, and
+// nothing of a, b or x is read for it. Any tokens of a call may have any
+// adapters; neighbours that share one share its products. Adapters of a lower
+// rank are padded with zeros.
+//
+// x, base and out have the type `type`; A x and all sums are held in 32 bits,
+// out is rounded once. A token's result does not depend on the other tokens of
+// the call, except for the order in which sums are taken (by m). rank is a
+// multiple of 8, at most STRASGPT_LORA_MAX_RANK, k a multiple of 8; x, its
+// rows, a and b are 16-byte aligned. base may be out (STRASGPT_EPI_STORE, the
+// same stride); else out shares no memory with what is read. m 0 does nothing.
+#define STRASGPT_LORA_MAX_RANK 128
+int strasgpt_k_lora(const void* x, long long ldx, const uint16_t* a,
+                    const uint16_t* b, int type, int m, int k, int n, int rank,
+                    int adapters, const int* adapter, const float* scale,
+                    const void* base, long long ldb, void* out, long long ldo,
+                    int epi, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,4 +1,5 @@
-// strasgpt_k_rope: rotary positions given per token.
+// strasgpt_k_rope, strasgpt_k_rope_axes: rotary positions given per token, or
+// per token and axis.
 //
 // Entry pair j of a head turns by the angle pos f_j (f_j: include/
 // strasgpt_kernels.h):
@@ -47,6 +48,18 @@ struct RopeArgs {
   double turns[kMaxPairs];   // f_j / 2 pi
 };
 
+// Several axes: pair j turns by the position of its axis.
+struct AxesArgs : RopeArgs {
+  long long pa, pt;          // axis and token strides of pos
+  uint8_t axis[kMaxPairs];
+};
+
+// Position that turns pair j of a token.
+__device__ __forceinline__ int position(const RopeArgs& a, int token, int) { return a.pos[token]; }
+__device__ __forceinline__ int position(const AxesArgs& a, int token, int j) {
+  return a.pos[a.axis[j] * a.pa + token * a.pt];
+}
+
 // V entries as one access.
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec {
@@ -75,8 +88,8 @@ constexpr int blocks_of(Layout l) { return l == kHalves ? 4 : 6; }
 
 // An item is the pairs of one access, or V entries behind the turned ones,
 // which are copied.
-template <typename T, int V, Layout LAYOUT>
-__global__ void __launch_bounds__(kThreads, blocks_of(LAYOUT)) k_rope(const __grid_constant__ RopeArgs a) {
+template <typename T, int V, Layout LAYOUT, typename Args>
+__global__ void __launch_bounds__(kThreads, blocks_of(LAYOUT)) k_rope(const __grid_constant__ Args a) {
   constexpr int kPairs = LAYOUT == kAdjacent ? V / 2 : V;  // of an item
   constexpr bool kTwo = LAYOUT != kAdjacent;               // two accesses
   __shared__ float2 cs[kSinesMax];
@@ -114,7 +127,7 @@ __global__ void __launch_bounds__(kThreads, blocks_of(LAYOUT)) k_rope(const __gr
   }
   for (int i = threadIdx.x; i < nt * half; i += kThreads) {
     const int token = i / half, j = i - token * half;
-    const double turns = (double)a.pos[t0 + token] * a.turns[j];
+    const double turns = (double)position(a, t0 + token, j) * a.turns[j];
     const double half_turns = 2.0 * (turns - rint(turns));
     const float near = (float)half_turns;
     float s, c, s_rest = 0.f, c_rest = 0.f;
@@ -151,11 +164,11 @@ __global__ void __launch_bounds__(kThreads, blocks_of(LAYOUT)) k_rope(const __gr
   }
 }
 
-template <typename T, int V>
-cudaError_t launch(const RopeArgs& a, bool interleaved, dim3 grid, cudaStream_t s) {
+template <typename T, int V, typename Args>
+cudaError_t launch(const Args& a, bool interleaved, dim3 grid, cudaStream_t s) {
   constexpr Layout kPaired = V > 1 ? kAdjacent : kSingle;
-  return interleaved ? sg::try_launch(k_rope<T, V, kPaired>, grid, kThreads, 0, 1, s, a)
-                     : sg::try_launch(k_rope<T, V, kHalves>, grid, kThreads, 0, 1, s, a);
+  return interleaved ? sg::try_launch(k_rope<T, V, kPaired, Args>, grid, kThreads, 0, 1, s, a)
+                     : sg::try_launch(k_rope<T, V, kHalves, Args>, grid, kThreads, 0, 1, s, a);
 }
 
 // Whether rows of `hd` entries at i st + j sh (i < t, j < heads) share no
@@ -167,30 +180,68 @@ bool rows_apart(long long t, long long st, long long heads, long long sh, long l
   return st >= (heads - 1) * sh + hd || sh >= (t - 1) * st + hd;
 }
 
-}  // namespace
-
-extern "C" int strasgpt_k_rope(const void* x, long long x_token_stride, long long x_head_stride,
-                               void* y, long long y_token_stride, long long y_head_stride,
-                               int type, int t, int heads, int head_dim, const int* pos,
-                               const strasgpt_rope_t* rope, void* stream) {
-  const char* const me = "strasgpt_k_rope";
-  if (type != STRASGPT_F32 && type != STRASGPT_BF16) return sg::refuse(me, "unknown type");
-  if (t < 0 || heads <= 0 || head_dim <= 0) return sg::refuse(me, "empty shape");
-  if (heads > 65535 || head_dim > 65536) return sg::refuse(me, "too many heads or entries");
-  if (!rope) return sg::refuse(me, "null parameters");
+// Why the parameters are refused, or NULL.
+const char* bad_parameters(const strasgpt_rope_t* rope, int head_dim) {
+  if (!rope) return "null parameters";
   if (rope->dim < 2 || rope->dim % 2 || rope->dim > head_dim || rope->dim > 2 * kMaxPairs)
-    return sg::refuse(me, "the turned part must be even, 2 to min(head_dim, 512) entries");
-  if (!(rope->theta > 0) || !isfinite(rope->theta)) return sg::refuse(me, "theta must be positive");
-  if (!isfinite((float)rope->magnitude)) return sg::refuse(me, "magnitude must be finite");
+    return "the turned part must be even, 2 to min(head_dim, 512) entries";
+  if (!(rope->theta > 0) || !isfinite(rope->theta)) return "theta must be positive";
+  if (!isfinite((float)rope->magnitude)) return "magnitude must be finite";
   if (rope->scaling < STRASGPT_ROPE_NONE || rope->scaling > STRASGPT_ROPE_BANDS)
-    return sg::refuse(me, "unknown scaling");
+    return "unknown scaling";
   if (rope->scaling != STRASGPT_ROPE_NONE && (!(rope->factor > 0) || !isfinite(rope->factor)))
-    return sg::refuse(me, "factor must be positive");
+    return "factor must be positive";
   if (rope->scaling == STRASGPT_ROPE_BANDS &&
       (!(rope->low < rope->high) || !isfinite(rope->low) || !isfinite(rope->high) ||
        rope->original <= 0))
-    return sg::refuse(me, "bands need low < high and a positive original length");
-  if (t == 0) return 0;
+    return "bands need low < high and a positive original length";
+  return nullptr;
+}
+
+// Turns per position of `count` pairs, f_m = theta^(-m / count), m = 0, 1, ...,
+// to turns[at(m)], and whether all of them, times any position, stay within 64
+// bits.
+//
+// f_m is a running product in 64-bit mantissas: at most 255 roundings of 2^-64
+// and as many times the ratio's own (2^-63), 2^-54 in all, so that a pair's
+// turns per position are off by little more than their last rounding to 64
+// bits (2^-53), which is what counts at far positions. (In doubles the product
+// was off by up to 2^-46: 4e-6 radians at position 2^31 for 512 entries and
+// theta 2.)
+template <typename At>
+bool turns_of(const strasgpt_rope_t& rope, int count, double* turns, At at) {
+  const long double per_turn = 1 / 6.283185307179586476925286766559L;
+  const long double ratio = powl(rope.theta, -2.0L / (2 * count));
+  const long double stretched =
+      rope.scaling == STRASGPT_ROPE_NONE ? per_turn : per_turn / rope.factor;
+  long double f = 1;
+  for (int m = 0; m < count; m++, f *= ratio) {
+    long double t = stretched;
+    if (rope.scaling == STRASGPT_ROPE_BANDS) {
+      long double keep = (rope.original * f * per_turn - rope.low) /
+                         ((long double)rope.high - rope.low);
+      keep = keep < 0 ? 0 : keep > 1 ? 1 : keep;
+      t = keep * per_turn + (1 - keep) * stretched;
+    }
+    turns[at(m)] = (double)(f * t);
+    if (!(fabs(turns[at(m)]) < 1e298)) return false;
+  }
+  return true;
+}
+
+// Both entry points: checks, and the launch for arguments `a` whose positions
+// and frequencies are set by `fill(a)` (which says why it refuses, or NULL).
+template <typename Args, typename Fill>
+int turn(const char* me, const void* x, long long x_token_stride, long long x_head_stride, void* y,
+         long long y_token_stride, long long y_head_stride, int type, int t, int heads,
+         int head_dim, const int* pos, const strasgpt_rope_t* rope, void* stream, Fill fill) {
+  if (type != STRASGPT_F32 && type != STRASGPT_BF16) return sg::refuse(me, "unknown type");
+  if (t < 0 || heads <= 0 || head_dim <= 0) return sg::refuse(me, "empty shape");
+  if (heads > 65535 || head_dim > 65536) return sg::refuse(me, "too many heads or entries");
+  if (const char* why = bad_parameters(rope, head_dim)) return sg::refuse(me, why);
+  Args a;
+  const char* const why_not = fill(a);
+  if (t == 0) return why_not ? sg::refuse(me, why_not) : 0;
   if (!x || !y || !pos) return sg::refuse(me, "null buffer");
   if (x_token_stride < 0 || x_head_stride < 0) return sg::refuse(me, "negative stride");
   if (!rows_apart(t, y_token_stride, heads, y_head_stride, head_dim))
@@ -201,7 +252,7 @@ extern "C" int strasgpt_k_rope(const void* x, long long x_token_stride, long lon
   const size_t size = type == STRASGPT_F32 ? 4 : 2;
   if (!sg::aligned(x, size) || !sg::aligned(y, size) || !sg::aligned(pos, 4))
     return sg::refuse(me, "a buffer is not aligned to its entries");
-  RopeArgs a;
+  if (why_not) return sg::refuse(me, why_not);
   a.x = x; a.y = y; a.pos = pos;
   a.xt = x_token_stride; a.xh = x_head_stride;
   a.yt = y_token_stride; a.yh = y_head_stride;
@@ -209,29 +260,6 @@ extern "C" int strasgpt_k_rope(const void* x, long long x_token_stride, long lon
   a.magnitude = (float)rope->magnitude;
   a.magnitude_rest = (float)(rope->magnitude - a.magnitude);
   const int half = rope->dim / 2;
-  // f_j = theta^(-2 j / dim) as a running product in 64-bit mantissas: at most
-  // 255 roundings of 2^-64 and as many times the ratio's own (2^-63), 2^-54 in
-  // all, so that a pair's turns per position are off by little more than their
-  // last rounding to 64 bits (2^-53), which is what counts at far positions.
-  // (In doubles the product was off by up to 2^-46: 4e-6 radians at position
-  // 2^31 for 512 entries and theta 2.)
-  const long double per_turn = 1 / 6.283185307179586476925286766559L;
-  const long double ratio = powl(rope->theta, -2.0L / rope->dim);
-  const long double stretched =
-      rope->scaling == STRASGPT_ROPE_NONE ? per_turn : per_turn / rope->factor;
-  long double f = 1;
-  for (int j = 0; j < half; j++, f *= ratio) {
-    long double turns = stretched;
-    if (rope->scaling == STRASGPT_ROPE_BANDS) {
-      long double keep = (rope->original * f * per_turn - rope->low) /
-                         ((long double)rope->high - rope->low);
-      keep = keep < 0 ? 0 : keep > 1 ? 1 : keep;
-      turns = keep * per_turn + (1 - keep) * stretched;
-    }
-    a.turns[j] = (double)(f * turns);
-    // Times any position it must stay within 64 bits.
-    if (!(fabs(a.turns[j]) < 1e298)) return sg::refuse(me, "frequencies beyond 64 bits");
-  }
   int dev = 0, sms = 0;
   if (const char* why = sg::current_device(&dev, &sms)) return sg::refuse(me, why);
   for (const void* p : {x, (const void*)y, (const void*)pos})
@@ -271,3 +299,65 @@ extern "C" int strasgpt_k_rope(const void* x, long long x_token_stride, long lon
   if (e != cudaSuccess) return sg::refuse_cuda(me, "launch", e);
   return 0;
 }
+
+const char* const kTooFast = "frequencies beyond 64 bits";
+
+}  // namespace
+
+extern "C" {
+
+int strasgpt_k_rope(const void* x, long long x_token_stride, long long x_head_stride, void* y,
+                    long long y_token_stride, long long y_head_stride, int type, int t, int heads,
+                    int head_dim, const int* pos, const strasgpt_rope_t* rope, void* stream) {
+  return turn<RopeArgs>("strasgpt_k_rope", x, x_token_stride, x_head_stride, y, y_token_stride,
+                        y_head_stride, type, t, heads, head_dim, pos, rope, stream,
+                        [&](RopeArgs& a) -> const char* {
+                          if (t == 0) return nullptr;
+                          return turns_of(*rope, rope->dim / 2, a.turns, [](int m) { return m; })
+                                     ? nullptr
+                                     : kTooFast;
+                        });
+}
+
+int strasgpt_k_rope_axes(const void* x, long long x_token_stride, long long x_head_stride, void* y,
+                         long long y_token_stride, long long y_head_stride, int type, int t,
+                         int heads, int head_dim, const int* pos, long long pos_axis_stride,
+                         long long pos_token_stride, const strasgpt_rope_t* rope,
+                         const strasgpt_rope_axes_t* axes, void* stream) {
+  return turn<AxesArgs>(
+      "strasgpt_k_rope_axes", x, x_token_stride, x_head_stride, y, y_token_stride, y_head_stride,
+      type, t, heads, head_dim, pos, rope, stream, [&](AxesArgs& a) -> const char* {
+        if (!axes) return "null axes";
+        const int n = axes->axes, half = rope->dim / 2;
+        if (n < 1 || n > STRASGPT_ROPE_AXES_MAX) return "1 to 4 axes";
+        if (axes->order != STRASGPT_AXES_RUNS && axes->order != STRASGPT_AXES_DEALT)
+          return "unknown order of the axes";
+        long long sum = 0;
+        for (int i = 0; i < n; i++) {
+          if (axes->section[i] < 0) return "a section of fewer than 0 pairs";
+          sum += axes->section[i];
+        }
+        if (sum != half) return "the sections must add up to the turned pairs";
+        if (pos_axis_stride < 0 || pos_token_stride < 0) return "negative stride of pos";
+        a.pa = pos_axis_stride;
+        a.pt = pos_token_stride;
+        // Pair of every axis's m-th.
+        uint8_t pair[STRASGPT_ROPE_AXES_MAX][kMaxPairs];
+        int given[STRASGPT_ROPE_AXES_MAX] = {};
+        for (int j = 0, i = 0; j < half; j++) {
+          while (given[i] == axes->section[i]) i = (i + 1) % n;
+          a.axis[j] = (uint8_t)i;
+          pair[i][given[i]++] = (uint8_t)j;
+          if (axes->order == STRASGPT_AXES_DEALT) i = (i + 1) % n;
+        }
+        if (!axes->separate)
+          return turns_of(*rope, half, a.turns, [](int m) { return m; }) ? nullptr : kTooFast;
+        for (int i = 0; i < n; i++)
+          if (axes->section[i] &&
+              !turns_of(*rope, axes->section[i], a.turns, [&](int m) { return pair[i][m]; }))
+            return kTooFast;
+        return nullptr;
+      });
+}
+
+}  // extern "C"

@@ -80,6 +80,22 @@ class Rope(ctypes.Structure):
                          high, magnitude)
 
 
+AXES_RUNS, AXES_DEALT = 0, 1  # STRASGPT_AXES_*
+ROPE_AXES_MAX = 4  # STRASGPT_ROPE_AXES_MAX
+
+
+class RopeAxes(ctypes.Structure):
+    """strasgpt_rope_axes_t (include/strasgpt_kernels.h): RopeAxes([24, 20, 20])."""
+    _fields_ = [("axes", ctypes.c_int), ("section", ctypes.c_int * ROPE_AXES_MAX),
+                ("order", ctypes.c_int), ("separate", ctypes.c_int)]
+
+    def __init__(self, sections, order=AXES_RUNS, separate=0):
+        if not 1 <= len(sections) <= ROPE_AXES_MAX:
+            raise ValueError(f"1 to {ROPE_AXES_MAX} axes")
+        super().__init__(len(sections), (ctypes.c_int * ROPE_AXES_MAX)(*sections), order,
+                         separate)
+
+
 def lib() -> ctypes.CDLL:
     """Load libstrasgpt.so (raises if it was not built)."""
     global _lib
@@ -135,6 +151,13 @@ def lib() -> ctypes.CDLL:
     L.strasgpt_k_rope.restype = i32
     L.strasgpt_k_rope.argtypes = [vp, i64, i64, vp, i64, i64, i32, i32, i32, i32, vp,
                                   ctypes.POINTER(Rope), vp]
+    L.strasgpt_k_rope_axes.restype = i32
+    L.strasgpt_k_rope_axes.argtypes = [vp, i64, i64, vp, i64, i64, i32, i32, i32, i32, vp,
+                                       i64, i64, ctypes.POINTER(Rope),
+                                       ctypes.POINTER(RopeAxes), vp]
+    L.strasgpt_k_lora.restype = i32
+    L.strasgpt_k_lora.argtypes = [vp, i64, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, vp,
+                                  i64, vp, i64, i32, vp]
     L.strasgpt_k_attn_tree_workspace.restype = sz
     L.strasgpt_k_attn_tree_workspace.argtypes = [i32, i32, i32, i32]
     L.strasgpt_k_attn_tree.restype = i32
