@@ -278,6 +278,45 @@ int strasgpt_k_lora(const void* x, long long ldx, const uint16_t* a,
                     const void* base, long long ldb, void* out, long long ldo,
                     int epi, void* stream);
 
+// GQA attention of a batch of requests behind one prefix that all of them
+// share: the prefix's keys are read once for the whole batch. q holds `tokens`
+// rows, att gets the outputs, both as in strasgpt_k_attn_tree; rows first[r] to
+// first[r + 1] - 1 are request r's new tokens, at most t of them (first NULL: t
+// each). The prefix is rows 0..*prefix - 1 of k_prefix and v_prefix
+// [kv_heads][prefix_ctx][head_dim], seen by every token. Behind it each request
+// has rows of its own, rows[r] of them, in its cache [kv_heads][ctx][head_dim]
+// at k_cache + r * request_stride (and v_cache): the last are its new tokens',
+// in order, and token j of c sees rows 0..rows[r] - c + j. (Fewer rows than new
+// tokens: the first of them see the prefix alone.) Scores, precision and what a
+// token that sees nothing gets are strasgpt_k_attn_tree's, and so is what rows
+// that a token does not see may hold.
+//
+// A row of q outside first[0]..first[requests] - 1 is of no request: its row of
+// att stays as it is. *prefix, rows and first are read on the device; *prefix
+// is cut to 0..prefix_ctx, rows[r] to 0..ctx, and of a request's tokens those
+// among the `tokens` rows, t at most, are taken. With a first that decreases,
+// or that gives a request more than t tokens, outputs of the rows it is wrong
+// about are unspecified. att may be q (ldo = ldq), or shares no memory with
+// what is read. head_dim 32, 64 or 128; group 1..128; t at most
+// STRASGPT_ATTN_SHARED_MAX; buffers and rows 16-byte aligned. No requests, or
+// no tokens: does nothing.
+//
+// The workspace has strasgpt_k_attn_shared_workspace(type, requests, t, tokens,
+// kv_heads, group, head_dim) bytes, and is as strasgpt_k_attn_tree's.
+#define STRASGPT_ATTN_SHARED_MAX 1024
+size_t strasgpt_k_attn_shared_workspace(int type, int requests, int t,
+                                        int tokens, int kv_heads, int group,
+                                        int head_dim);
+int strasgpt_k_attn_shared(const void* q, long long ldq, const void* k_prefix,
+                           const void* v_prefix, int prefix_ctx,
+                           const int* prefix, const void* k_cache,
+                           const void* v_cache, long long request_stride,
+                           int ctx, const int* rows, const int* first, int type,
+                           int requests, int t, int tokens, int kv_heads,
+                           int group, int head_dim, void* att, long long ldo,
+                           void* workspace, size_t workspace_bytes,
+                           void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,5 +1,6 @@
 // strasgpt_k_attn_tree: GQA attention of a tree of drafted tokens over the
-// cache that ends with the tree's own rows.
+// cache that ends with the tree's own rows; strasgpt_k_attn_shared: of a batch
+// of requests over a prefix that all share and over caches of their own.
 //
 // Drafted token i and head h attend to the cached keys 0..n-1 and to the
 // drafted keys j (cache row n + j) whose bit j is set in row i of the mask:
@@ -30,6 +31,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 extern "C" {
 #include "strasgpt_kernels.h"
@@ -131,6 +133,62 @@ struct Tile {
   static_assert((WARPS <= 4 ? 2 : 1) * (kBytes + kCtaReserved) <= kSmSmem, "the CTAs of an SM fit");
 };
 
+// A CTA's tokens and split.
+struct Rows {
+  int token0, t;        // first token and tokens (of the tree, of a request)
+  int r0;               // first row of the CTA, of t * group
+  int split;
+  int cached, drafted;  // keys that all rows see, and those behind them
+  int late;             // request: token i sees its drafted keys 0..i - late
+  size_t cache;         // entries before the request's cache
+
+  __device__ Rows(const TreeArgs& a, int tile_rows) {
+    token0 = 0;
+    t = a.t;
+    split = blockIdx.x;
+    r0 = blockIdx.z * tile_rows;
+    cached = sg::tree_cached(a);
+    drafted = a.drafted;
+    late = 0;
+    cache = 0;
+  }
+  // Whatever stands in device memory, tokens and cache rows are among those
+  // that the call names.
+  __device__ Rows(const sg::BatchArgs& a, int tile_rows) {
+    split = blockIdx.x % a.splits;
+    const int request = blockIdx.x / a.splits / a.tiles;
+    r0 = blockIdx.x / a.splits % a.tiles * tile_rows;
+    const int from = a.first ? a.first[request] : min((long long)request * a.most, (long long)a.t);
+    const int to = a.first ? a.first[request + 1] : min((request + 1ll) * a.most, (long long)a.t);
+    token0 = min(max(from, 0), a.t);
+    t = min(max(min(to, a.t) - token0, 0), a.most);
+    const int n = min(max(a.rows[request], 0), a.ctx);
+    cached = max(n - t, 0);
+    drafted = n - cached;
+    late = t - drafted;
+    cache = (size_t)request * a.stride;
+  }
+};
+
+// Which of the 64 drafted keys from j0 (a multiple of 8, below a word's end)
+// token i sees, as bits.
+__device__ __forceinline__ u64 seen_of(const TreeArgs& a, const Rows&, int i, int j0) {
+  return a.mask[(size_t)i * a.words + (j0 >> 6)] >> (j0 & 63);
+}
+__device__ __forceinline__ u64 seen_of(const sg::BatchArgs&, const Rows& r, int i, int j0) {
+  const int count = i - r.late - j0 + 1;
+  return count >= 64 ? ~0ull : count > 0 ? (1ull << count) - 1 : 0;
+}
+// Where a row's part lies.
+__device__ __forceinline__ size_t part_of(const TreeArgs& a, const Rows& r, int head, int row) {
+  return ((size_t)r.split * a.kh + head) * a.t * a.group + row;
+}
+__device__ __forceinline__ size_t part_of(const sg::BatchArgs& a, const Rows& r, int head,
+                                          int row) {
+  return ((size_t)(a.split0 + r.split) * a.kh + head) * a.t * a.group +
+         (size_t)r.token0 * a.group + row;
+}
+
 // The tiles of a split: the cached keys, then the drafted ones. A tile holds
 // keys of one kind, never of both.
 template <typename T, int HD, int THREADS>
@@ -140,18 +198,18 @@ struct Walk {
   int t, n, old_tiles, tile0, tile1;
   uint32_t smem;
 
-  // The cache's length is read on the device (a captured call serves every
-  // later length); one outside the cache is cut to it.
-  __device__ Walk(const TreeArgs& a, int split, int head, const void* stages) {
-    t = a.t;
-    n = sg::tree_cached(a);
+  // (The cache's length is read on the device: a captured call serves every
+  // later length.)
+  __device__ Walk(const TreeArgs& a, const Rows& r, int head, const void* stages) {
+    t = r.drafted;
+    n = r.cached;
     old_tiles = (n + L::kKeys - 1) / L::kKeys;
     const int tiles = old_tiles + (t + L::kKeys - 1) / L::kKeys;
     const int per = (tiles + a.splits - 1) / a.splits;
-    tile0 = split * per;
+    tile0 = r.split * per;
     tile1 = min(tiles, tile0 + per);
-    k = static_cast<const T*>(a.k) + (size_t)head * a.ctx * HD;
-    v = static_cast<const T*>(a.v) + (size_t)head * a.ctx * HD;
+    k = static_cast<const T*>(a.k) + r.cache + (size_t)head * a.ctx * HD;
+    v = static_cast<const T*>(a.v) + r.cache + (size_t)head * a.ctx * HD;
     smem = saddr(stages);
   }
   // First cache row of a tile and its rows.
@@ -182,10 +240,10 @@ struct Walk {
 };
 
 // MW warps side by side in rows (16 each), KW in keys.
-template <typename T, int HD, int MW, int KW>
-__global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(TreeArgs a) {
+template <typename T, int HD, int MW, int KW, typename Args>
+__global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Args a) {
   using L = Tile<T, HD, MW * KW>;
-  constexpr bool kF32 = L::kF32;
+  constexpr bool kF32 = L::kF32, kBatch = std::is_same<Args, sg::BatchArgs>::value;
   constexpr int kThreads = 32 * MW * KW;
   constexpr int kRows = 16 * MW;
   constexpr int kKeys = L::kKeys, kWarpKeys = kKeys / KW;
@@ -196,14 +254,21 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Tree
   extern __shared__ __align__(16) unsigned char smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, c4 = lane & 3;
   const int mw = warp % MW, kw = warp / MW;
-  const int split = blockIdx.x, head = blockIdx.y, r0 = blockIdx.z * kRows;
-  const int R = a.t * a.group;
+  const int head = blockIdx.y;
   sg::pdl_trigger();
   sg::pdl_wait();
 
-  const Walk<T, HD, kThreads> walk(a, split, head, smem);
+  const Rows rows_of(a, kRows);
+  const int R = rows_of.t * a.group, r0 = rows_of.r0;
+  const Walk<T, HD, kThreads> walk(a, rows_of, head, smem);
   const int n = walk.n, old_tiles = walk.old_tiles, tile0 = walk.tile0, tile1 = walk.tile1;
-  if (tile0 >= tile1) return;
+  if (r0 >= R) return;
+  if (tile0 >= tile1) {
+    if constexpr (kBatch)
+      for (int r = r0 + threadIdx.x; r < min(R, r0 + kRows); r += kThreads)
+        a.ml[part_of(a, rows_of, head, r)] = make_float2(-INFINITY, 0.f);
+    return;
+  }
 #pragma unroll
   for (int s = 0; s < kStages - 1; s++) walk.fetch(tile0 + s);
 
@@ -211,9 +276,9 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Tree
   const int rA = r0 + 16 * mw + g8, rB = rA + 8;
   const int tA = rA / a.group, tB = rB / a.group;
   const bool inA = rA < R, inB = rB < R;
-  const T* qA = static_cast<const T*>(a.q) + (inA ? tA : 0) * a.ldq +
+  const T* qA = static_cast<const T*>(a.q) + (rows_of.token0 + (inA ? tA : 0)) * a.ldq +
                 (size_t)(head * a.group + (inA ? rA - tA * a.group : 0)) * HD;
-  const T* qB = static_cast<const T*>(a.q) + (inB ? tB : 0) * a.ldq +
+  const T* qB = static_cast<const T*>(a.q) + (rows_of.token0 + (inB ? tB : 0)) * a.ldq +
                 (size_t)(head * a.group + (inB ? rB - tB * a.group : 0)) * HD;
   // Scores in units of log2, so that the softmax is exp2.
   const float scale = 1.4426950408889634f / sqrtf((float)HD);
@@ -341,8 +406,8 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Tree
       // What the rows may see: all cached keys, or the mask's bits.
       if (!old) {
         const int j0 = row - n + k0;  // drafted index, a multiple of 8
-        const u64 wA = inA ? a.mask[(size_t)tA * a.words + (j0 >> 6)] >> (j0 & 63) : 0;
-        const u64 wB = inB ? a.mask[(size_t)tB * a.words + (j0 >> 6)] >> (j0 & 63) : 0;
+        const u64 wA = inA ? seen_of(a, rows_of, tA, j0) : 0;
+        const u64 wB = inB ? seen_of(a, rows_of, tB, j0) : 0;
 #pragma unroll
         for (int i = 0; i < kN8; i++)
 #pragma unroll
@@ -553,14 +618,14 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Tree
 
   // One split: the rows are complete (a row without keys is zeros). Else the
   // parts go to the workspace as they are, in 32 bits.
-  const bool whole = a.splits == 1;
+  const bool whole = !kBatch && a.whole && a.splits == 1;
 #pragma unroll
   for (int half = 0; half < 2; half++) {
     const int r = half ? rB : rA, tok = half ? tB : tA;
     if (r >= R) continue;
     const float m = half ? mB : mA, l = half ? lB : lA;
     const float f = whole ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
-    const size_t at = ((size_t)split * a.kh + head) * R + r;
+    const size_t at = part_of(a, rows_of, head, r);
     if (!whole && c4 == 0) a.ml[at] = make_float2(m, l);
     T* out = static_cast<T*>(a.att) + tok * a.ldo +
              (size_t)(head * a.group + r - tok * a.group) * HD;
@@ -599,18 +664,28 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Tree
 // and queries, then every lane has 4 entries of the outputs.
 constexpr int kFewRows = 4, kFewWarps = 4, kFewHeadDim = 128;
 
-__global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(TreeArgs a) {
+template <typename Args>
+__global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(Args a) {
   constexpr int HD = kFewHeadDim;
+  constexpr bool kBatch = std::is_same<Args, sg::BatchArgs>::value;
   using L = Tile<float, HD, kFewWarps>;
   constexpr int kWarpKeys = L::kKeys / kFewWarps, kQ = HD / 16, kO = HD / 32;
   static_assert(kWarpKeys == 8, "a warp's keys of a tile are one step");
   extern __shared__ __align__(16) unsigned char smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, c4 = lane & 3;
-  const int split = blockIdx.x, head = blockIdx.y, R = a.t * a.group;
+  const int head = blockIdx.y;
   sg::pdl_trigger();
   sg::pdl_wait();
-  const Walk<float, HD, 32 * kFewWarps> walk(a, split, head, smem);
-  if (walk.tile0 >= walk.tile1) return;
+  const Rows rows_of(a, kFewRows);
+  const int R = rows_of.t * a.group;
+  const Walk<float, HD, 32 * kFewWarps> walk(a, rows_of, head, smem);
+  if (R == 0) return;
+  if (walk.tile0 >= walk.tile1) {
+    if constexpr (kBatch)
+      if (threadIdx.x < R)
+        a.ml[part_of(a, rows_of, head, threadIdx.x)] = make_float2(-INFINITY, 0.f);
+    return;
+  }
 #pragma unroll
   for (int s = 0; s < kStages - 1; s++) walk.fetch(walk.tile0 + s);
 
@@ -621,7 +696,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(TreeArgs a) {
 #pragma unroll
   for (int r = 0; r < kFewRows; r++) {
     const int row = r < R ? r : 0, tok = row / a.group;
-    const float* from = static_cast<const float*>(a.q) + tok * a.ldq +
+    const float* from = static_cast<const float*>(a.q) + (rows_of.token0 + tok) * a.ldq +
                         (size_t)(head * a.group + row - tok * a.group) * HD + 4 * c4;
 #pragma unroll
     for (int j = 0; j < kQ; j++) {
@@ -671,8 +746,8 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(TreeArgs a) {
         p[r] += __shfl_xor_sync(0xFFFFFFFFu, p[r], 2);
         bool in = k0 + g8 < rows && r < R;
         if (!old && in) {
-          const int j = row - walk.n + k0 + g8;  // drafted index
-          in = a.mask[(size_t)(r / a.group) * a.words + (j >> 6)] >> (j & 63) & 1;
+          const int j = row - walk.n + k0;  // drafted index of the warp's first key
+          in = seen_of(a, rows_of, r / a.group, j) >> g8 & 1;
         }
         if (!in) p[r] = -INFINITY;
         top[r] = fmaxf(p[r], __shfl_xor_sync(0xFFFFFFFFu, p[r], 4));
@@ -748,10 +823,10 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(TreeArgs a) {
   }
   // One split: the row is complete (one without keys is zeros). Else its part
   // goes to the workspace.
-  const bool whole = a.splits == 1;
+  const bool whole = !kBatch && a.whole && a.splits == 1;
   const float f = whole ? (sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum)) : 1.f;
   const int tok = warp / a.group;
-  const size_t at = ((size_t)split * a.kh + head) * R + warp;
+  const size_t at = part_of(a, rows_of, head, warp);
   if (!whole && lane == 0) a.ml[at] = make_float2(all, sum);
   float* to = whole ? static_cast<float*>(a.att) + tok * a.ldo +
                           (size_t)(head * a.group + warp - tok * a.group) * HD
@@ -771,8 +846,17 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(TreeArgs a) {
 // it does not see are not even read.
 constexpr int kMergeThreads = 128, kMergeGroups = kMergeThreads / 8;
 
-template <typename T, int HD, bool DRAFTED>
-__global__ void __launch_bounds__(kMergeThreads) k_merge(TreeArgs a, int keys_per_tile) {
+//
+// BATCH: the parts of the prefix, then each request's own; rows of no request
+// stay as they are.
+struct BatchMerge : TreeArgs {   // of the prefix
+  int own_splits, requests, most;
+  const int* first;
+};
+
+template <typename T, int HD, bool DRAFTED, bool BATCH = false>
+__global__ void __launch_bounds__(kMergeThreads)
+    k_merge(std::conditional_t<BATCH, BatchMerge, TreeArgs> a, int keys_per_tile) {
   constexpr int V = HD / 8;  // entries per lane
   constexpr bool kF32 = sizeof(T) == 4;
   __shared__ float warp_o[kMergeThreads / 32][HD];
@@ -784,11 +868,18 @@ __global__ void __launch_bounds__(kMergeThreads) k_merge(TreeArgs a, int keys_pe
   sg::pdl_wait();
   const int n = sg::tree_cached(a);
   const int tiles = (n + keys_per_tile - 1) / keys_per_tile +
-                    (DRAFTED ? 0 : (a.t + keys_per_tile - 1) / keys_per_tile);
+                    (DRAFTED ? 0 : (a.drafted + keys_per_tile - 1) / keys_per_tile);
   const int per = (tiles + a.splits - 1) / a.splits;
   const int parts = tiles ? (tiles + per - 1) / per : 0;
+  int own = 0;
   const int head = row / R, r = row - head * R, tok = r / a.group;
   const size_t at = (size_t)(head * a.group + r - tok * a.group) * HD;
+  if constexpr (BATCH) {
+    own = a.own_splits;
+    if (a.first ? tok < a.first[0] || tok >= a.first[a.requests]
+                : tok >= (long long)a.requests * a.most)
+      return;
+  }
   auto read = [&](const T* p, float* x) {
     if constexpr (kF32) {
 #pragma unroll
@@ -862,8 +953,10 @@ __global__ void __launch_bounds__(kMergeThreads) k_merge(TreeArgs a, int keys_pe
   }
   const size_t step = (size_t)a.kh * R;
 #pragma unroll 2
-  for (int s = group; s < parts; s += kMergeGroups) {
+  for (int i = group; i < parts + own; i += kMergeGroups) {
+    const int s = i < parts ? i : a.splits + i - parts;
     const float2 p = a.ml[s * step + row];
+    if (BATCH && i >= parts && p.y == 0.f) continue;  // no keys: nothing was written
     const float* from = a.part + (s * step + row) * HD + e0;
     float x[V];
 #pragma unroll
@@ -936,11 +1029,12 @@ bool on_tc(int t, int group, int hd) {
   return t <= 256 && hd >= 64 && t * group > (hd == 128 ? 16 : 32);
 }
 
+// The same for the keys of a shared prefix, which every row sees.
+bool prefix_on_tc(int rows, int hd) { return hd >= 64 && rows > (hd == 128 ? 16 : 32); }
+
 // Splits of the keys: as many CTAs as the GPU holds at once.
-int splits_of(int sms, int t, int kh, int group, int hd) {
-  const int rows = t * group;
+int splits_of(int sms, int rows, int kh, bool tc) {
   const Shape s = shape_of(rows);
-  const bool tc = on_tc(t, group, hd);
   const int resident = sms * (!tc && s.mw * s.kw <= 4 ? 2 : 1);
   const int tile = tc ? sg::kTreeTcRows : 16 * s.mw;
   const long long others = (long long)kh * ((rows + tile - 1) / tile);
@@ -952,51 +1046,92 @@ size_t workspace_of(int splits, int t, int kh, int group, int hd) {
   return (size_t)splits * kh * t * group * (hd + 2) * sizeof(float);
 }
 
-cudaError_t launch_few(const TreeArgs& a, int dev, cudaStream_t s) {
-  static std::atomic<size_t> allowed[sg::kDevices];
-  using L = Tile<float, kFewHeadDim, kFewWarps>;
-  cudaError_t e = sg::allow_smem(k_tree_few, L::kBytes, dev, allowed);
-  if (e != cudaSuccess) return e;
-  e = sg::try_launch(k_tree_few, dim3(a.splits, a.kh), dim3(32 * kFewWarps), L::kBytes, 1, s, a);
-  if (e != cudaSuccess || a.splits == 1) return e;
-  return sg::try_launch(k_merge<float, kFewHeadDim, false>, dim3(a.t * a.group * a.kh),
-                        dim3(kMergeThreads), 0, 1, s, a, L::kKeys);
+// CTAs for the splits and row tiles of a tree, and of a batch.
+dim3 grid_of(const TreeArgs& a, int tile_rows) {
+  return dim3(a.splits, a.kh, (a.t * a.group + tile_rows - 1) / tile_rows);
+}
+dim3 grid_of(const sg::BatchArgs& a, int) {
+  return dim3((unsigned)a.splits * a.tiles * a.requests, a.kh);
 }
 
-template <typename T, int HD, int MW, int KW>
-cudaError_t launch_shape(const TreeArgs& a, int dev, cudaStream_t s) {
+template <typename Args>
+cudaError_t launch_few(const Args& a, int dev, cudaStream_t s) {
   static std::atomic<size_t> allowed[sg::kDevices];
-  using L = Tile<T, HD, MW * KW>;
-  constexpr size_t bytes = L::kBytes;
-  cudaError_t e = sg::allow_smem(k_tree<T, HD, MW, KW>, bytes, dev, allowed);
+  using L = Tile<float, kFewHeadDim, kFewWarps>;
+  const cudaError_t e = sg::allow_smem(k_tree_few<Args>, L::kBytes, dev, allowed);
   if (e != cudaSuccess) return e;
-  const int rows = a.t * a.group;
-  e = sg::try_launch(k_tree<T, HD, MW, KW>,
-                     dim3(a.splits, a.kh, (rows + 16 * MW - 1) / (16 * MW)),
-                     dim3(32 * MW * KW), bytes, 1, s, a);
-  if (e != cudaSuccess || a.splits == 1) return e;
-  return sg::try_launch(k_merge<T, HD, false>, dim3(rows * a.kh), dim3(kMergeThreads), 0, 1, s, a,
-                        L::kKeys);
+  return sg::try_launch(k_tree_few<Args>, grid_of(a, kFewRows), dim3(32 * kFewWarps), L::kBytes, 1,
+                        s, a);
+}
+
+template <typename T, int HD, int MW, int KW, typename Args>
+cudaError_t launch_shape(const Args& a, int dev, cudaStream_t s) {
+  static std::atomic<size_t> allowed[sg::kDevices];
+  constexpr size_t bytes = Tile<T, HD, MW * KW>::kBytes;
+  const cudaError_t e = sg::allow_smem(k_tree<T, HD, MW, KW, Args>, bytes, dev, allowed);
+  if (e != cudaSuccess) return e;
+  return sg::try_launch(k_tree<T, HD, MW, KW, Args>, grid_of(a, 16 * MW), dim3(32 * MW * KW), bytes,
+                        1, s, a);
+}
+
+// This file's kernels for `rows` rows of a kv head (of a tree, of a request);
+// *keys: of a tile of theirs.
+template <typename T, int HD, typename Args>
+cudaError_t launch_mma(const Args& a, int rows, int* keys, int dev, cudaStream_t s) {
+  if constexpr (sizeof(T) == 4 && HD == kFewHeadDim)
+    if (rows <= kFewRows) {
+      *keys = Tile<float, HD, kFewWarps>::kKeys;
+      return launch_few(a, dev, s);
+    }
+  const Shape f = shape_of(rows);
+  *keys = f.mw * f.kw <= 4 ? Tile<T, HD, 4>::kKeys : Tile<T, HD, 8>::kKeys;
+  if (f.mw == 1) return launch_shape<T, HD, 1, 4>(a, dev, s);
+  if (f.mw == 2) return launch_shape<T, HD, 2, 2>(a, dev, s);
+  if (f.mw == 4) return launch_shape<T, HD, 4, 1>(a, dev, s);
+  return launch_shape<T, HD, 8, 1>(a, dev, s);
 }
 
 template <typename T, int HD>
 cudaError_t launch_hd(const TreeArgs& a, int dev, cudaStream_t s) {
+  const dim3 rows(a.t * a.group * a.kh);
   if (on_tc(a.t, a.group, HD)) {
     if constexpr (HD >= 64) {
       constexpr bool kF32 = sizeof(T) == 4;
       const cudaError_t e = sg::tree_tc(a, kF32, HD, dev, s);
       if (e != cudaSuccess) return e;
-      return sg::try_launch(k_merge<T, HD, true>, dim3(a.t * a.group * a.kh), dim3(kMergeThreads),
-                            0, 1, s, a, sg::tree_tc_keys());
+      return sg::try_launch(k_merge<T, HD, true>, rows, dim3(kMergeThreads), 0, 1, s, a,
+                            sg::tree_tc_keys());
     }
   }
-  if constexpr (sizeof(T) == 4 && HD == kFewHeadDim)
-    if (a.t * a.group <= kFewRows) return launch_few(a, dev, s);
-  const Shape f = shape_of(a.t * a.group);
-  if (f.mw == 1) return launch_shape<T, HD, 1, 4>(a, dev, s);
-  if (f.mw == 2) return launch_shape<T, HD, 2, 2>(a, dev, s);
-  if (f.mw == 4) return launch_shape<T, HD, 4, 1>(a, dev, s);
-  return launch_shape<T, HD, 8, 1>(a, dev, s);
+  int keys = 0;
+  const cudaError_t e = launch_mma<T, HD>(a, a.t * a.group, &keys, dev, s);
+  if (e != cudaSuccess || a.splits == 1) return e;
+  return sg::try_launch(k_merge<T, HD, false>, rows, dim3(kMergeThreads), 0, 1, s, a, keys);
+}
+
+// Behind a shared prefix: parts of the prefix for all rows, parts of each
+// request's own keys, and their joins.
+template <typename T, int HD>
+cudaError_t launch_shared(const TreeArgs& p, const sg::BatchArgs& own, int dev, cudaStream_t s) {
+  int keys = 0, none = 0;
+  cudaError_t e;
+  if (prefix_on_tc(p.t * p.group, HD)) {
+    if constexpr (HD >= 64) e = sg::tree_tc(p, sizeof(T) == 4, HD, dev, s);
+    keys = sg::tree_tc_keys();
+  } else {
+    e = launch_mma<T, HD>(p, p.t * p.group, &keys, dev, s);
+  }
+  if (e != cudaSuccess) return e;
+  e = launch_mma<T, HD>(own, own.most * own.group, &none, dev, s);
+  if (e != cudaSuccess) return e;
+  BatchMerge m;
+  static_cast<TreeArgs&>(m) = p;
+  m.own_splits = own.splits;
+  m.requests = own.requests;
+  m.most = own.most;
+  m.first = own.first;
+  return sg::try_launch(k_merge<T, HD, false, true>, dim3(p.t * p.group * p.kh), dim3(kMergeThreads),
+                        0, 1, s, m, keys);
 }
 
 template <typename T>
@@ -1016,6 +1151,38 @@ const char* bad_shape(int t, int kh, int group, int hd) {
   return nullptr;
 }
 
+// How a batch is split: its prefix, and the requests' own keys.
+struct Batch {
+  int splits, own_splits, tiles;
+  size_t bytes;
+};
+Batch batch_of(int sms, int requests, int t, int tokens, int kh, int group, int hd) {
+  Batch b;
+  b.splits = splits_of(sms, tokens * group, kh, prefix_on_tc(tokens * group, hd));
+  const Shape s = shape_of(t * group);
+  b.tiles = (t * group + 16 * s.mw - 1) / (16 * s.mw);
+  const int resident = sms * (s.mw * s.kw <= 4 ? 2 : 1);
+  const long long others = (long long)requests * kh * b.tiles;
+  b.own_splits = (int)std::max(1ll, std::min((long long)kMaxSplits, resident / others));
+  b.bytes = (size_t)(b.splits + b.own_splits) * kh * tokens * group * (hd + 2) * sizeof(float);
+  return b;
+}
+
+const char* bad_batch(int type, int requests, int t, int tokens, int kh, int group, int hd) {
+  if (type != STRASGPT_F32 && type != STRASGPT_BF16) return "unknown type";
+  if (requests < 0 || t <= 0 || tokens < 0 || kh <= 0 || group <= 0) return "empty shape";
+  if (t > STRASGPT_ATTN_SHARED_MAX) return "more than 1024 new tokens of a request";
+  if (group > 128 || kh > 65535) return "more than 128 q heads per kv head, or 65535 kv heads";
+  if (hd != 32 && hd != 64 && hd != 128) return "head_dim must be 32, 64 or 128";
+  // k_merge has a block per row, the prefix's kernels one per 16 rows or more
+  // along z, the requests' ones a block per request, split and tile.
+  if ((long long)tokens * kh * group > INT_MAX) return "more than 2^31 - 1 rows of q heads";
+  if ((long long)tokens * group > 65535ll * 64) return "more than 4194240 rows of a kv head";
+  if ((long long)requests * t * group > INT_MAX / kMaxSplits)
+    return "more than 2^23 - 1 rows of all requests' most tokens";
+  return nullptr;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1031,9 +1198,8 @@ size_t strasgpt_k_attn_tree_workspace(int t, int kv_heads, int group, int head_d
     sg::refuse(me, why);
     return 0;
   }
-  return t ? workspace_of(splits_of(sms, t, kv_heads, group, head_dim), t, kv_heads, group,
-                          head_dim)
-           : 0;
+  const int splits = splits_of(sms, t * group, kv_heads, on_tc(t, group, head_dim));
+  return t ? workspace_of(splits, t, kv_heads, group, head_dim) : 0;
 }
 
 int strasgpt_k_attn_tree(const void* q, long long ldq, const void* k_cache, const void* v_cache,
@@ -1062,7 +1228,7 @@ int strasgpt_k_attn_tree(const void* q, long long ldq, const void* k_cache, cons
   for (const void* p : {q, k_cache, v_cache, (const void*)cached, (const void*)mask,
                         (const void*)att})
     if (const char* why = sg::not_on_device(p, dev)) return sg::refuse(me, why);
-  const int splits = splits_of(sms, t, kv_heads, group, head_dim);
+  const int splits = splits_of(sms, t * group, kv_heads, on_tc(t, group, head_dim));
   const size_t need = workspace_of(splits, t, kv_heads, group, head_dim);
   if (need) {
     if (!workspace || workspace_bytes < need)
@@ -1073,7 +1239,9 @@ int strasgpt_k_attn_tree(const void* q, long long ldq, const void* k_cache, cons
   TreeArgs a;
   a.q = q; a.k = k_cache; a.v = v_cache; a.att = att;
   a.ldq = ldq; a.ldo = ldo;
-  a.t = t; a.kh = kv_heads; a.group = group; a.ctx = ctx; a.words = (t + 63) / 64;
+  a.t = a.drafted = t;
+  a.kh = kv_heads; a.group = group; a.ctx = ctx; a.words = (t + 63) / 64;
+  a.whole = true;
   a.cached = cached; a.mask = (const u64*)mask;
   a.splits = splits;
   a.part = (float*)workspace;
@@ -1081,6 +1249,90 @@ int strasgpt_k_attn_tree(const void* q, long long ldq, const void* k_cache, cons
   const cudaStream_t s = (cudaStream_t)stream;
   const cudaError_t e = type == STRASGPT_F32 ? launch_type<float>(a, head_dim, dev, s)
                                              : launch_type<uint16_t>(a, head_dim, dev, s);
+  if (e != cudaSuccess) return sg::refuse_cuda(me, "launch", e);
+  return 0;
+}
+
+size_t strasgpt_k_attn_shared_workspace(int type, int requests, int t, int tokens, int kv_heads,
+                                        int group, int head_dim) {
+  const char* const me = "strasgpt_k_attn_shared_workspace";
+  if (const char* why = bad_batch(type, requests, t, tokens, kv_heads, group, head_dim)) {
+    sg::refuse(me, why);
+    return 0;
+  }
+  int dev = 0, sms = 0;
+  if (const char* why = sg::current_device(&dev, &sms)) {
+    sg::refuse(me, why);
+    return 0;
+  }
+  if (requests == 0 || tokens == 0) return 0;
+  return batch_of(sms, requests, t, tokens, kv_heads, group, head_dim).bytes;
+}
+
+int strasgpt_k_attn_shared(const void* q, long long ldq, const void* k_prefix,
+                           const void* v_prefix, int prefix_ctx, const int* prefix,
+                           const void* k_cache, const void* v_cache, long long request_stride,
+                           int ctx, const int* rows, const int* first, int type, int requests,
+                           int t, int tokens, int kv_heads, int group, int head_dim, void* att,
+                           long long ldo, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* const me = "strasgpt_k_attn_shared";
+  if (const char* why = bad_batch(type, requests, t, tokens, kv_heads, group, head_dim))
+    return sg::refuse(me, why);
+  if (prefix_ctx < 1 || ctx < 1) return sg::refuse(me, "a cache without rows");
+  const long long row = (long long)kv_heads * group * head_dim;
+  if (tokens > 1 && (ldq < row || ldo < row)) return sg::refuse(me, "rows of q or att overlap");
+  if (request_stride < 0) return sg::refuse(me, "negative stride");
+  if (requests == 0 || tokens == 0) return 0;
+  if (!q || !k_prefix || !v_prefix || !prefix || !k_cache || !v_cache || !rows || !att)
+    return sg::refuse(me, "null buffer");
+  const size_t size = type == STRASGPT_F32 ? 4 : 2;
+  if (!sg::aligned(q, 16) || !sg::aligned(k_prefix, 16) || !sg::aligned(v_prefix, 16) ||
+      !sg::aligned(k_cache, 16) || !sg::aligned(v_cache, 16) || !sg::aligned(att, 16) ||
+      (tokens > 1 && (ldq * size % 16 || ldo * size % 16)) ||
+      (requests > 1 && request_stride * size % 16))
+    return sg::refuse(me, "q, the caches, att and their rows must be 16-byte aligned");
+  if (q == att && tokens > 1 && ldq != ldo)
+    return sg::refuse(me, "in place, q and att must have the same strides");
+  if (!sg::aligned(prefix, 4) || !sg::aligned(rows, 4) || !sg::aligned(first, 4))
+    return sg::refuse(me, "a buffer is not aligned to its entries");
+  int dev = 0, sms = 0;
+  if (const char* why = sg::current_device(&dev, &sms)) return sg::refuse(me, why);
+  const Batch b = batch_of(sms, requests, t, tokens, kv_heads, group, head_dim);
+  if (!workspace || workspace_bytes < b.bytes)
+    return sg::refuse(me, "the workspace is smaller than strasgpt_k_attn_shared_workspace says");
+  if (!sg::aligned(workspace, 16)) return sg::refuse(me, "workspace must be 16-byte aligned");
+  for (const void* p : {q, k_prefix, v_prefix, (const void*)prefix, k_cache, v_cache,
+                        (const void*)rows, (const void*)first, (const void*)att,
+                        (const void*)workspace})
+    if (p)
+      if (const char* why = sg::not_on_device(p, dev)) return sg::refuse(me, why);
+  TreeArgs a = {};
+  a.q = q; a.k = k_prefix; a.v = v_prefix; a.att = att;
+  a.ldq = ldq; a.ldo = ldo;
+  a.t = tokens; a.kh = kv_heads; a.group = group; a.ctx = prefix_ctx;
+  a.cached = prefix;
+  a.splits = b.splits;
+  a.part = (float*)workspace;
+  a.ml = (float2*)(a.part + (size_t)(b.splits + b.own_splits) * kv_heads * tokens * group *
+                                head_dim);
+  sg::BatchArgs own = {};
+  static_cast<TreeArgs&>(own) = a;
+  own.k = k_cache; own.v = v_cache; own.ctx = ctx;
+  own.splits = b.own_splits;
+  own.requests = requests; own.most = t; own.first = first; own.rows = rows;
+  own.stride = request_stride;
+  own.tiles = b.tiles;
+  own.split0 = b.splits;
+  const cudaStream_t s = (cudaStream_t)stream;
+  cudaError_t e;
+  if (type == STRASGPT_F32)
+    e = head_dim == 128  ? launch_shared<float, 128>(a, own, dev, s)
+        : head_dim == 64 ? launch_shared<float, 64>(a, own, dev, s)
+                         : launch_shared<float, 32>(a, own, dev, s);
+  else
+    e = head_dim == 128  ? launch_shared<uint16_t, 128>(a, own, dev, s)
+        : head_dim == 64 ? launch_shared<uint16_t, 64>(a, own, dev, s)
+                         : launch_shared<uint16_t, 32>(a, own, dev, s);
   if (e != cudaSuccess) return sg::refuse_cuda(me, "launch", e);
   return 0;
 }

@@ -1,5 +1,6 @@
-// What the two kernels behind strasgpt_k_attn_tree share: attn_tree.cu (the
-// entry point, few rows per kv head) and attn_tree_tc.cu (many).
+// What the kernels behind strasgpt_k_attn_tree and strasgpt_k_attn_shared share:
+// attn_tree.cu (the entry points, few rows per kv head) and attn_tree_tc.cu
+// (many).
 #pragma once
 
 #include "entry.h"
@@ -13,17 +14,31 @@ struct TreeArgs {
   void* att;
   long long ldq, ldo;
   int t, kh, group, ctx, words;
+  int drafted;     // keys behind the cached ones that the mask is about: t, or 0
   const int* cached;
   const unsigned long long* mask;
   int splits;
   float* part;     // [splits][kh][t * group][HD] outputs before division
   float2* ml;      // [splits][kh][t * group] running maximum (base 2) and sum
+  bool whole;      // one split writes att; else, and always where not set, parts
 };
 
 // Cached keys, cut to what the cache holds.
 __device__ __forceinline__ int tree_cached(const TreeArgs& a) {
-  return min(max(*a.cached, 0), a.ctx - a.t);
+  return min(max(*a.cached, 0), a.ctx - a.drafted);
 }
+
+// A batch of requests whose t tokens are in all, each request's next to one
+// another: k, v and ctx are the requests' own caches', and a request's tokens
+// see each other in order.
+struct BatchArgs : TreeArgs {
+  int requests, most;        // most: of a request's tokens
+  const int* first;          // [requests + 1], or NULL: most each
+  const int* rows;           // [requests]: of its cache, its tokens' included
+  long long stride;          // entries from one request's cache to the next's
+  int tiles;                 // row tiles of a request
+  int split0;                // parts of the prefix come before the requests' own
+};
 
 // The cached keys [0, *cached) on the fifth-generation tensor cores, 128 rows
 // per CTA; the drafted ones are k_merge's. head_dim 64 or 128.

@@ -158,6 +158,11 @@ def lib() -> ctypes.CDLL:
     L.strasgpt_k_lora.restype = i32
     L.strasgpt_k_lora.argtypes = [vp, i64, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, vp,
                                   i64, vp, i64, i32, vp]
+    L.strasgpt_k_attn_shared_workspace.restype = sz
+    L.strasgpt_k_attn_shared_workspace.argtypes = [i32, i32, i32, i32, i32, i32, i32]
+    L.strasgpt_k_attn_shared.restype = i32
+    L.strasgpt_k_attn_shared.argtypes = [vp, i64, vp, vp, i32, vp, vp, vp, i64, i32, vp, vp,
+                                         i32, i32, i32, i32, i32, i32, i32, vp, i64, vp, sz, vp]
     L.strasgpt_k_attn_tree_workspace.restype = sz
     L.strasgpt_k_attn_tree_workspace.argtypes = [i32, i32, i32, i32]
     L.strasgpt_k_attn_tree.restype = i32
