@@ -5,11 +5,14 @@ Tolerance, with h = 2^-24 (half a step of fp32) and b = 2^-8 (of bf16). A matrix
 instruction cuts its sums: 2 h of the sum of the products' sizes each. For a
 token, |A||x| (of a rank) and |B||s| stand for those sums.
 
-A x. fp32 rows: products are exact (three parts of 8 bits); 32 entries take six
-instructions from zero, 12 h; the warp's steps, at most k / 512 + 1, are added
-with roundings of h, then up to 8 warps' and 8 CTAs' sums, and the scale:
-(12 + k / 512 + 18) h. bf16 rows: products as they are, two instructions a step
-in one sum: (4 (k / 512 + 1) + 17) h.
+A x. fp32 rows: products are exact (three parts of 8 bits). Up to 256 tokens, 32
+entries take six instructions from zero, 12 h; a warp's steps, at most k / 1024 + 1,
+are added with roundings of h. More tokens: two instructions per 32 entries in one sum
+of the large parts over at most k / 16 + 64 entries, 4 h (k / 512 + 2), and the small
+parts' (2^-7 of them, twice as many): 5 h (k / 512 + 2) in all. Then up to 8 warps' and
+8 CTAs' sums, and the scale, 17 h: below (12 + 5 (k / 512 + 2) + 17) h. bf16 rows:
+products as they are, four instructions per 64 entries in one sum, 4 h (k / 512 + 2)
+as well: the same bound.
 B s. s as three parts (fp32; exact) or two (2^-17): rank / 16 steps, three
 instructions each: 6 (rank / 16 + 1) h, and 2^-16 for two parts.
 Then big and small sums, base and ADD's old value are added: 3 h of their sizes.
@@ -41,8 +44,7 @@ def reference(torch, x, a, b, adapter, scale, base, out, epi, type_):
     d, n, r = b.shape
     v = torch.zeros(m, n, dtype=torch.float64, device="cuda") if base is None else base.double()
     size, err = v.abs(), torch.zeros_like(v)
-    steps = k / 512 + 1
-    first = (12 + steps + 17) * H if type_ == F32 else (4 * steps + 17) * H
+    first = (12 + 5 * (k / 512 + 2) + 17) * H
     second = 6 * (r / 16 + 1) * H + (2.0 ** -16 if type_ == BF16 else 0)
     for i in range(d):
         of = torch.nonzero(adapter == i)[:, 0]
