@@ -133,31 +133,26 @@ struct Tile {
   static_assert((WARPS <= 4 ? 2 : 1) * (kBytes + kCtaReserved) <= kSmSmem, "the CTAs of an SM fit");
 };
 
-// A CTA's tokens and split.
+// A CTA's tokens: of the tree, or of one request.
 struct Rows {
-  int token0, t;        // first token and tokens (of the tree, of a request)
+  int token0, t;        // first token and tokens
   int r0;               // first row of the CTA, of t * group
-  int split;
   int cached, drafted;  // keys that all rows see, and those behind them
   int late;             // request: token i sees its drafted keys 0..i - late
-  size_t cache;         // entries before the request's cache
 
+  __device__ Rows() {}
   __device__ Rows(const TreeArgs& a, int tile_rows) {
     token0 = 0;
     t = a.t;
-    split = blockIdx.x;
     r0 = blockIdx.z * tile_rows;
     cached = sg::tree_cached(a);
     drafted = a.drafted;
     late = 0;
-    cache = 0;
   }
   // Whatever stands in device memory, tokens and cache rows are among those
   // that the call names.
-  __device__ Rows(const sg::BatchArgs& a, int tile_rows) {
-    split = blockIdx.x % a.splits;
-    const int request = blockIdx.x / a.splits / a.tiles;
-    r0 = blockIdx.x / a.splits % a.tiles * tile_rows;
+  __device__ Rows(const sg::BatchArgs& a, int request, int first_row) {
+    r0 = first_row;
     const int from = a.first ? a.first[request] : min((long long)request * a.most, (long long)a.t);
     const int to = a.first ? a.first[request + 1] : min((request + 1ll) * a.most, (long long)a.t);
     token0 = min(max(from, 0), a.t);
@@ -166,7 +161,6 @@ struct Rows {
     cached = max(n - t, 0);
     drafted = n - cached;
     late = t - drafted;
-    cache = (size_t)request * a.stride;
   }
 };
 
@@ -179,67 +173,241 @@ __device__ __forceinline__ u64 seen_of(const sg::BatchArgs&, const Rows& r, int 
   const int count = i - r.late - j0 + 1;
   return count >= 64 ? ~0ull : count > 0 ? (1ull << count) - 1 : 0;
 }
-// Where a row's part lies.
-__device__ __forceinline__ size_t part_of(const TreeArgs& a, const Rows& r, int head, int row) {
-  return ((size_t)r.split * a.kh + head) * a.t * a.group + row;
-}
-__device__ __forceinline__ size_t part_of(const sg::BatchArgs& a, const Rows& r, int head,
-                                          int row) {
-  return ((size_t)(a.split0 + r.split) * a.kh + head) * a.t * a.group +
-         (size_t)r.token0 * a.group + row;
+// `rows` cache rows from `row` on to a stage, zeros behind them.
+template <typename T, int HD, int THREADS>
+__device__ __forceinline__ void load_tile(const T* k, const T* v, int row, int rows, uint32_t ks) {
+  using L = Tile<T, HD, THREADS / 32>;
+  const uint32_t vs = ks + L::kKeys * L::kKRow;
+  constexpr int kVecs = HD * (int)sizeof(T) / 16;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < L::kKeys * kVecs; i += THREADS) {
+    const int r = i / kVecs, x = i % kVecs;
+    const int bytes = r < rows ? 16 : 0;
+    const size_t at = (size_t)(row + (r < rows ? r : 0)) * HD + x * (16 / sizeof(T));
+    cp_async16(ks + r * L::kKRow + x * 16, k + at, bytes);
+    cp_async16(vs + r * L::kVRow + x * 16, v + at, bytes);
+  }
 }
 
 // The tiles of a split: the cached keys, then the drafted ones. A tile holds
 // keys of one kind, never of both.
-template <typename T, int HD, int THREADS>
+template <typename T, int HD, int THREADS, int ROWS>
 struct Walk {
   using L = Tile<T, HD, THREADS / 32>;
   const T *k, *v;                // of the kv head
-  int t, n, old_tiles, tile0, tile1;
+  Rows r;
+  int n, old_tiles, tile0, tile1;
   uint32_t smem;
 
   // (The cache's length is read on the device: a captured call serves every
   // later length.)
-  __device__ Walk(const TreeArgs& a, const Rows& r, int head, const void* stages) {
-    t = r.drafted;
+  __device__ Walk(const TreeArgs& a, const void* stages) : r(a, ROWS) {
     n = r.cached;
     old_tiles = (n + L::kKeys - 1) / L::kKeys;
-    const int tiles = old_tiles + (t + L::kKeys - 1) / L::kKeys;
+    const int tiles = old_tiles + (r.drafted + L::kKeys - 1) / L::kKeys;
     const int per = (tiles + a.splits - 1) / a.splits;
-    tile0 = r.split * per;
+    tile0 = blockIdx.x * per;
     tile1 = min(tiles, tile0 + per);
-    k = static_cast<const T*>(a.k) + r.cache + (size_t)head * a.ctx * HD;
-    v = static_cast<const T*>(a.v) + r.cache + (size_t)head * a.ctx * HD;
+    k = static_cast<const T*>(a.k) + (size_t)blockIdx.y * a.ctx * HD;
+    v = static_cast<const T*>(a.v) + (size_t)blockIdx.y * a.ctx * HD;
     smem = saddr(stages);
   }
-  // First cache row of a tile and its rows.
-  __device__ void extent(int tile, int& row, int& rows) const {
+  __device__ int count() const { return max(0, tile1 - tile0); }
+  __device__ const Rows& rows(int) const { return r; }
+  __device__ int head(int) const { return blockIdx.y; }
+  // Tile i of the split: first cache row and rows.
+  __device__ void extent(int i, int& row, int& rows) const {
+    const int tile = tile0 + i;
     const bool old = tile < old_tiles;
     const int k0 = (old ? tile : tile - old_tiles) * L::kKeys;
     row = old ? k0 : n + k0;
-    rows = min(L::kKeys, (old ? n : t) - k0);
+    rows = min(L::kKeys, (old ? n : r.drafted) - k0);
   }
-  __device__ void fetch(int tile) const {
-    if (tile < tile1) {
+  // Its rows, and its first key's drafted index, negative if it holds cached ones.
+  __device__ void keys(int i, int& rows, int& j0) const {
+    int row;
+    extent(i, row, rows);
+    j0 = tile0 + i < old_tiles ? -1 : row - n;
+  }
+  __device__ bool last(int i) const { return tile0 + i + 1 >= tile1; }
+  __device__ void fetch(int i) const {
+    if (tile0 + i < tile1) {
       int row, rows;
-      extent(tile, row, rows);
-      const uint32_t ks = smem + (tile - tile0) % kStages * L::kStage;
-      const uint32_t vs = ks + L::kKeys * L::kKRow;
-      constexpr int kVecs = HD * (int)sizeof(T) / 16;
-#pragma unroll 8
-      for (int i = threadIdx.x; i < L::kKeys * kVecs; i += THREADS) {
-        const int r = i / kVecs, x = i % kVecs;
-        const int bytes = r < rows ? 16 : 0;  // rows behind the last key are zeros
-        const size_t at = (size_t)(row + (r < rows ? r : 0)) * HD + x * (16 / sizeof(T));
-        cp_async16(ks + r * L::kKRow + x * 16, k + at, bytes);
-        cp_async16(vs + r * L::kVRow + x * 16, v + at, bytes);
-      }
+      extent(i, row, rows);
+      load_tile<T, HD, THREADS>(k, v, row, rows, smem + i % kStages * L::kStage);
     }
     cp_async_commit();
+  }
+  __device__ int parts(int) const { return 0; }
+  // Where the part of row r (of t * group) lies.
+  __device__ size_t part(const TreeArgs& a, const Rows&, int head, int, int r) const {
+    return ((size_t)blockIdx.x * a.kh + head) * a.t * a.group + r;
+  }
+};
+
+// A batch: the tiles of all requests, kv heads and row tiles, in this order, are
+// shared out evenly, a run to each CTA, whose fetches go on from one (request, head,
+// row tile) to the next. Each of these has a tile at least, which may be empty, if
+// there are rows.
+//
+// Its parts: that of the run with its first tile lies with its rows, those of the
+// runs that go on with it lie by CTA; which they are is noted for each row.
+//
+// One thread looks ahead and notes what the others need of a tile.
+template <typename T, int HD, int THREADS, int ROWS>
+struct Stream {
+  using L = Tile<T, HD, THREADS / 32>;
+  struct Note {
+    size_t base;       // entries before the cache of the tile's request and head
+    int row, rows;     // first cache row, rows
+    int j0;            // first key's drafted index, or -1
+    int head, token0, t, r0, late;
+    int parts;         // runs over the (request, head, row tile); 0: not its first tile
+    int last;          // of it, or of this CTA's
+  };
+  static constexpr int kNotes = 4;  // two tiles ahead, and one that is written
+  struct Shared {
+    Note notes[kNotes];
+    Rows r;
+    int request, head, z, tile, tiles, old_tiles;
+    long long at, per, end;  // the next tile's number; a CTA's tiles; the last's number + 1
+    long long sums[THREADS / 32];
+  };
+  const sg::BatchArgs& a;
+  Shared& s;
+  uint32_t smem;
+  int tiles_;
+
+  static __device__ int key_tiles(const Rows& r) {
+    return max(1, (r.cached + L::kKeys - 1) / L::kKeys + (r.drafted + L::kKeys - 1) / L::kKeys);
+  }
+  static __device__ int row_tiles(const sg::BatchArgs& a, const Rows& r) {
+    return (r.t * a.group + ROWS - 1) / ROWS;
+  }
+  __device__ void enter(int request) {
+    s.request = request;
+    s.r = Rows(a, request, 0);
+    s.old_tiles = (s.r.cached + L::kKeys - 1) / L::kKeys;
+    s.tiles = key_tiles(s.r);
+  }
+  // Notes the next tile, as this CTA's i-th.
+  __device__ void look_ahead(int i) {
+    if (s.at >= s.end) return;
+    Note& n = s.notes[i % kNotes];
+    const bool old = s.tile < s.old_tiles;
+    const int k0 = (old ? s.tile : s.tile - s.old_tiles) * L::kKeys;
+    n.base = (size_t)s.request * a.stride + (size_t)s.head * a.ctx * HD;
+    n.row = old ? k0 : s.r.cached + k0;
+    n.rows = max(0, min(L::kKeys, (old ? s.r.cached : s.r.drafted) - k0));
+    n.j0 = old ? -1 : k0;
+    n.head = s.head;
+    n.token0 = s.r.token0;
+    n.t = s.r.t;
+    n.r0 = s.z * ROWS;
+    n.late = s.r.late;
+    n.parts = s.tile ? 0 : (int)((s.at + s.tiles - 1) / s.per - blockIdx.x + 1);
+    s.at++;
+    s.tile++;
+    n.last = s.tile == s.tiles || s.at == s.end;
+    if (s.tile < s.tiles || s.at == s.end) return;
+    s.tile = 0;
+    if (++s.z < row_tiles(a, s.r)) return;
+    s.z = 0;
+    if (++s.head < a.kh) return;
+    s.head = 0;
+    // (There is one: there are tiles left.)
+    do enter(s.request + 1);
+    while (s.r.t == 0);
+  }
+
+  __device__ Stream(const sg::BatchArgs& args, Shared& shared, const void* stages)
+      : a(args), s(shared) {
+    smem = saddr(stages);
+    // Every thread counts the tiles of some requests in a row; the one that has
+    // this CTA's first tile's finds it.
+    const int each = (a.requests + THREADS - 1) / THREADS, lane = threadIdx.x & 31;
+    const int from = threadIdx.x * each, to = min(a.requests, from + each);
+    auto tiles_of = [&](int request) {
+      const Rows r(a, request, 0);
+      return (long long)key_tiles(r) * row_tiles(a, r) * a.kh;
+    };
+    long long mine = 0;
+    for (int r = from; r < to; r++) mine += tiles_of(r);
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const long long x = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    if (lane == 31) s.sums[threadIdx.x >> 5] = upto;
+    __syncthreads();
+    long long before = upto - mine, all = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; w++) {
+      if (w < (int)(threadIdx.x >> 5)) before += s.sums[w];
+      all += s.sums[w];
+    }
+    const long long per = max(1ll, (all + gridDim.x - 1) / gridDim.x), at = per * blockIdx.x;
+    tiles_ = (int)max(0ll, min(per, all - at));
+    if (tiles_ && at >= before && at < before + mine) {
+      long long left = at - before;
+      int r = from;
+      for (long long n; left >= (n = tiles_of(r)); r++) left -= n;
+      enter(r);
+      const int rows = row_tiles(a, s.r);
+      s.tile = (int)(left % s.tiles);
+      left /= s.tiles;
+      s.z = (int)(left % rows);
+      s.head = (int)(left / rows);
+      s.at = at;
+      s.per = per;
+      s.end = at + tiles_;
+      for (int i = 0; i < kNotes - 1; i++) look_ahead(i);
+    }
+    __syncthreads();
+  }
+  __device__ int count() const { return tiles_; }
+  __device__ Rows rows(int i) const {
+    const Note& n = s.notes[i % kNotes];
+    Rows r;
+    r.token0 = n.token0;
+    r.t = n.t;
+    r.r0 = n.r0;
+    r.late = n.late;
+    return r;
+  }
+  __device__ int head(int i) const { return s.notes[i % kNotes].head; }
+  __device__ void keys(int i, int& rows, int& j0) const {
+    rows = s.notes[i % kNotes].rows;
+    j0 = s.notes[i % kNotes].j0;
+  }
+  __device__ bool last(int i) const { return s.notes[i % kNotes].last; }
+  // Asks for tile i, if there is one (it is noted). Between two calls is a barrier.
+  __device__ void fetch(int i) {
+    if (i < tiles_) {
+      const Note& n = s.notes[i % kNotes];
+      load_tile<T, HD, THREADS>(static_cast<const T*>(a.k) + n.base,
+                                static_cast<const T*>(a.v) + n.base, n.row, n.rows,
+                                smem + i % kStages * L::kStage);
+      if (i >= kStages - 1 && threadIdx.x == 0) look_ahead(i + 1);
+    }
+    cp_async_commit();
+  }
+  __device__ int parts(int i) const { return s.notes[i % kNotes].parts; }
+  // Where the part of row r of these lies; the first run notes who goes on.
+  __device__ size_t part(const sg::BatchArgs& a, const Rows& rows, int head, int parts, int r) const {
+    const size_t all = (size_t)a.t * a.group, row = head * all + (size_t)rows.token0 * a.group + r;
+    if (!parts) return (a.split0 + 1) * a.kh * all + (size_t)blockIdx.x * ROWS + (r - rows.r0);
+    a.where[row] = make_int2(blockIdx.x, parts * 128 + r - rows.r0);
+    return a.split0 * a.kh * all + row;
   }
 };
 
 // MW warps side by side in rows (16 each), KW in keys.
+template <typename T, int HD, int THREADS, int ROWS, typename Args>
+using Walker = std::conditional_t<std::is_same<Args, sg::BatchArgs>::value,
+                                  Stream<T, HD, THREADS, ROWS>, Walk<T, HD, THREADS, ROWS>>;
+
 template <typename T, int HD, int MW, int KW, typename Args>
 __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Args a) {
   using L = Tile<T, HD, MW * KW>;
@@ -254,24 +422,28 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Args
   extern __shared__ __align__(16) unsigned char smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, c4 = lane & 3;
   const int mw = warp % MW, kw = warp / MW;
-  const int head = blockIdx.y;
   sg::pdl_trigger();
   sg::pdl_wait();
 
-  const Rows rows_of(a, kRows);
-  const int R = rows_of.t * a.group, r0 = rows_of.r0;
-  const Walk<T, HD, kThreads> walk(a, rows_of, head, smem);
-  const int n = walk.n, old_tiles = walk.old_tiles, tile0 = walk.tile0, tile1 = walk.tile1;
-  if (r0 >= R) return;
-  if (tile0 >= tile1) {
-    if constexpr (kBatch)
-      for (int r = r0 + threadIdx.x; r < min(R, r0 + kRows); r += kThreads)
-        a.ml[part_of(a, rows_of, head, r)] = make_float2(-INFINITY, 0.f);
-    return;
-  }
+  using W = Walker<T, HD, kThreads, kRows, Args>;
+  auto start = [&] {
+    if constexpr (kBatch) {
+      __shared__ typename W::Shared shared;
+      return W(a, shared, smem);
+    } else {
+      return W(a, smem);
+    }
+  };
+  W walk = start();
+  if (walk.count() == 0) return;
 #pragma unroll
-  for (int s = 0; s < kStages - 1; s++) walk.fetch(tile0 + s);
+  for (int s = 0; s < kStages - 1; s++) walk.fetch(s);
 
+  int at = 0;  // tiles gone through
+  do {
+  const Rows rows_of = walk.rows(at);
+  const int head = walk.head(at), R = rows_of.t * a.group, r0 = rows_of.r0;
+  const int parts = walk.parts(at);
   // This lane's rows g8 and g8 + 8 of the warp's 16.
   const int rA = r0 + 16 * mw + g8, rB = rA + 8;
   const int tA = rA / a.group, tB = rB / a.group;
@@ -318,14 +490,15 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Args
   for (int i = 0; i < kOut; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float mA = -INFINITY, mB = -INFINITY, lA = 0.f, lB = 0.f;
 
-  for (int tile = tile0; tile < tile1; tile++) {
+  for (bool more = true; more; at++) {
     cp_async_wait<kStages - 2>();
     __syncthreads();
-    walk.fetch(tile + kStages - 1);  // into the buffer that the last tile left
-    int row, rows;
-    walk.extent(tile, row, rows);
-    const bool old = tile < old_tiles;
-    const unsigned char* ks = smem + (tile - tile0) % kStages * L::kStage;
+    walk.fetch(at + kStages - 1);  // into the buffer that the last tile left
+    int rows, first;
+    walk.keys(at, rows, first);
+    more = !walk.last(at);
+    const bool old = first < 0;
+    const unsigned char* ks = smem + at % kStages * L::kStage;
     const unsigned char* vs = ks + kKeys * L::kKRow;
     // A drafted value row with an infinity or NaN may be hidden from some of
     // the rows: 0 * NaN in a matrix instruction would reach them. Such a tile
@@ -405,7 +578,7 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Args
 
       // What the rows may see: all cached keys, or the mask's bits.
       if (!old) {
-        const int j0 = row - n + k0;  // drafted index, a multiple of 8
+        const int j0 = first + k0;  // drafted index, a multiple of 8
         const u64 wA = inA ? seen_of(a, rows_of, tA, j0) : 0;
         const u64 wB = inB ? seen_of(a, rows_of, tB, j0) : 0;
 #pragma unroll
@@ -562,18 +735,19 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Args
       }
     }
   }
-  cp_async_wait<0>();
+  if constexpr (!kBatch) cp_async_wait<0>();
   lA += __shfl_xor_sync(0xFFFFFFFFu, lA, 1);
   lA += __shfl_xor_sync(0xFFFFFFFFu, lA, 2);
   lB += __shfl_xor_sync(0xFFFFFFFFu, lB, 1);
   lB += __shfl_xor_sync(0xFFFFFFFFu, lB, 2);
 
   // The key warps' parts of the rows are joined in shared memory, warps of
-  // the upper half into the lower one.
+  // the upper half into the lower one, in the last tile's place (tiles behind it
+  // may be on their way).
   if constexpr (KW > 1) {
     constexpr int kLane = kOut * 4 + 4;  // values a lane hands over
-    float* x = reinterpret_cast<float*>(smem);
-    static_assert((size_t)MW * (KW / 2) * 32 * kLane * 4 <= L::kBytes, "join fits the tiles");
+    float* x = reinterpret_cast<float*>(smem + (kBatch ? (at - 1) % kStages * L::kStage : 0));
+    static_assert((size_t)MW * (KW / 2) * 32 * kLane * 4 <= L::kStage, "join fits a tile");
 #pragma unroll
     for (int half = KW / 2; half > 0; half /= 2) {
       __syncthreads();
@@ -613,8 +787,8 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Args
         }
       }
     }
-    if (kw > 0) return;
   }
+  if (kw == 0) {
 
   // One split: the rows are complete (a row without keys is zeros). Else the
   // parts go to the workspace as they are, in 32 bits.
@@ -625,7 +799,7 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Args
     if (r >= R) continue;
     const float m = half ? mB : mA, l = half ? lB : lA;
     const float f = whole ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
-    const size_t at = part_of(a, rows_of, head, r);
+    const size_t at = walk.part(a, rows_of, head, parts, r);
     if (!whole && c4 == 0) a.ml[at] = make_float2(m, l);
     T* out = static_cast<T*>(a.att) + tok * a.ldo +
              (size_t)(head * a.group + r - tok * a.group) * HD;
@@ -653,6 +827,8 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Args
       }
     }
   }
+  }
+  } while (kBatch && at < walk.count());
 }
 
 // Up to kFewRows rows a kv head, fp32, head_dim 128: FMAs. Most of a matrix
@@ -673,22 +849,26 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(Args a) {
   static_assert(kWarpKeys == 8, "a warp's keys of a tile are one step");
   extern __shared__ __align__(16) unsigned char smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, c4 = lane & 3;
-  const int head = blockIdx.y;
   sg::pdl_trigger();
   sg::pdl_wait();
-  const Rows rows_of(a, kFewRows);
-  const int R = rows_of.t * a.group;
-  const Walk<float, HD, 32 * kFewWarps> walk(a, rows_of, head, smem);
-  if (R == 0) return;
-  if (walk.tile0 >= walk.tile1) {
-    if constexpr (kBatch)
-      if (threadIdx.x < R)
-        a.ml[part_of(a, rows_of, head, threadIdx.x)] = make_float2(-INFINITY, 0.f);
-    return;
-  }
+  using W = Walker<float, HD, 32 * kFewWarps, kFewRows, Args>;
+  auto start = [&] {
+    if constexpr (kBatch) {
+      __shared__ typename W::Shared shared;
+      return W(a, shared, smem);
+    } else {
+      return W(a, smem);
+    }
+  };
+  W walk = start();
+  if (walk.count() == 0) return;
 #pragma unroll
-  for (int s = 0; s < kStages - 1; s++) walk.fetch(walk.tile0 + s);
+  for (int s = 0; s < kStages - 1; s++) walk.fetch(s);
 
+  int at = 0;  // tiles gone through
+  do {
+  const Rows rows_of = walk.rows(at);
+  const int head = walk.head(at), R = rows_of.t * a.group, parts = walk.parts(at);
   // Scores in units of log2, so that the softmax is exp2.
   const float scale = 1.4426950408889634f / sqrtf((float)HD);
   float4 q[kFewRows][kQ];
@@ -712,14 +892,15 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(Args a) {
     for (int i = 0; i < kO; i++) o[r][i] = 0.f;
   }
 
-  for (int tile = walk.tile0; tile < walk.tile1; tile++) {
+  for (bool more = true; more; at++) {
     cp_async_wait<kStages - 2>();
     __syncthreads();
-    walk.fetch(tile + kStages - 1);  // into the buffer that the last tile left
-    int row, rows;
-    walk.extent(tile, row, rows);
-    const bool old = tile < walk.old_tiles;
-    const unsigned char* ks = smem + (tile - walk.tile0) % kStages * L::kStage;
+    walk.fetch(at + kStages - 1);  // into the buffer that the last tile left
+    int rows, first;
+    walk.keys(at, rows, first);
+    more = !walk.last(at);
+    const bool old = first < 0;
+    const unsigned char* ks = smem + at % kStages * L::kStage;
     const unsigned char* vs = ks + L::kKeys * L::kKRow;
     const int k0 = warp * kWarpKeys;  // the warp's first key in the tile
     if (k0 < rows) {
@@ -746,8 +927,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(Args a) {
         p[r] += __shfl_xor_sync(0xFFFFFFFFu, p[r], 2);
         bool in = k0 + g8 < rows && r < R;
         if (!old && in) {
-          const int j = row - walk.n + k0;  // drafted index of the warp's first key
-          in = seen_of(a, rows_of, r / a.group, j) >> g8 & 1;
+          in = seen_of(a, rows_of, r / a.group, first + k0) >> g8 & 1;
         }
         if (!in) p[r] = -INFINITY;
         top[r] = fmaxf(p[r], __shfl_xor_sync(0xFFFFFFFFu, p[r], 4));
@@ -785,12 +965,14 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(Args a) {
       }
     }
   }
-  cp_async_wait<0>();
+  if constexpr (!kBatch) cp_async_wait<0>();
   __syncthreads();
 
-  // The warps' parts are joined in shared memory, a row by each warp.
-  float* part = reinterpret_cast<float*>(smem);  // [warp][row][HD + 2]
-  static_assert(kFewWarps * kFewRows * (HD + 2) * 4 <= (int)L::kBytes, "join fits the tiles");
+  // The warps' parts are joined in shared memory, a row by each warp, in the last
+  // tile's place.
+  float* part =  // [warp][row][HD + 2]
+      reinterpret_cast<float*>(smem + (kBatch ? (at - 1) % kStages * L::kStage : 0));
+  static_assert(kFewWarps * kFewRows * (HD + 2) * 4 <= (int)L::kStage, "join fits a tile");
   static_assert(kFewWarps == kFewRows, "a warp per row");
 #pragma unroll
   for (int r = 0; r < kFewRows; r++) {
@@ -806,7 +988,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(Args a) {
     }
   }
   __syncthreads();
-  if (warp >= R) return;
+  if (warp < R) {
   float all = -INFINITY, sum = 0.f, out[kO];
 #pragma unroll
   for (int i = 0; i < kO; i++) out[i] = 0.f;
@@ -826,13 +1008,15 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(Args a) {
   const bool whole = !kBatch && a.whole && a.splits == 1;
   const float f = whole ? (sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum)) : 1.f;
   const int tok = warp / a.group;
-  const size_t at = part_of(a, rows_of, head, warp);
+  const size_t at = walk.part(a, rows_of, head, parts, warp);
   if (!whole && lane == 0) a.ml[at] = make_float2(all, sum);
   float* to = whole ? static_cast<float*>(a.att) + tok * a.ldo +
                           (size_t)(head * a.group + warp - tok * a.group) * HD
                     : a.part + at * HD;
 #pragma unroll
   for (int i = 0; i < kO; i++) to[lane * kO + i] = out[i] * f;
+  }
+  } while (kBatch && at < walk.count());
 }
 
 // A block joins the parts of one row: sixteen groups of eight lanes, a lane
@@ -846,17 +1030,8 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(Args a) {
 // it does not see are not even read.
 constexpr int kMergeThreads = 128, kMergeGroups = kMergeThreads / 8;
 
-//
-// BATCH: the parts of the prefix, then each request's own; rows of no request
-// stay as they are.
-struct BatchMerge : TreeArgs {   // of the prefix
-  int own_splits, requests, most;
-  const int* first;
-};
-
-template <typename T, int HD, bool DRAFTED, bool BATCH = false>
-__global__ void __launch_bounds__(kMergeThreads)
-    k_merge(std::conditional_t<BATCH, BatchMerge, TreeArgs> a, int keys_per_tile) {
+template <typename T, int HD, bool DRAFTED>
+__global__ void __launch_bounds__(kMergeThreads) k_merge(TreeArgs a, int keys_per_tile) {
   constexpr int V = HD / 8;  // entries per lane
   constexpr bool kF32 = sizeof(T) == 4;
   __shared__ float warp_o[kMergeThreads / 32][HD];
@@ -871,15 +1046,8 @@ __global__ void __launch_bounds__(kMergeThreads)
                     (DRAFTED ? 0 : (a.drafted + keys_per_tile - 1) / keys_per_tile);
   const int per = (tiles + a.splits - 1) / a.splits;
   const int parts = tiles ? (tiles + per - 1) / per : 0;
-  int own = 0;
   const int head = row / R, r = row - head * R, tok = r / a.group;
   const size_t at = (size_t)(head * a.group + r - tok * a.group) * HD;
-  if constexpr (BATCH) {
-    own = a.own_splits;
-    if (a.first ? tok < a.first[0] || tok >= a.first[a.requests]
-                : tok >= (long long)a.requests * a.most)
-      return;
-  }
   auto read = [&](const T* p, float* x) {
     if constexpr (kF32) {
 #pragma unroll
@@ -953,10 +1121,8 @@ __global__ void __launch_bounds__(kMergeThreads)
   }
   const size_t step = (size_t)a.kh * R;
 #pragma unroll 2
-  for (int i = group; i < parts + own; i += kMergeGroups) {
-    const int s = i < parts ? i : a.splits + i - parts;
+  for (int s = group; s < parts; s += kMergeGroups) {
     const float2 p = a.ml[s * step + row];
-    if (BATCH && i >= parts && p.y == 0.f) continue;  // no keys: nothing was written
     const float* from = a.part + (s * step + row) * HD + e0;
     float x[V];
 #pragma unroll
@@ -1004,6 +1170,108 @@ __global__ void __launch_bounds__(kMergeThreads)
     asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(*to) : "f"(out));
 }
 
+// A batch's parts: those of the prefix, that of the run with the row's first own
+// tile, those of the runs that go on with it. WARPS of a block share a row, a run of
+// its parts each: a lane has a part's maximum and sum, then HD / 32 entries of the
+// outputs. Rows of no request stay as they are.
+struct JoinArgs : TreeArgs {   // of the prefix
+  const int2* where;
+  int ctas, rows;              // of the requests' own tiles: CTAs, and rows of one
+  int requests, most;
+  const int* first;
+};
+constexpr int kJoinWarps = 4;
+constexpr int kJoinFew = 4096;  // rows for which a block each is on its way at once
+
+template <typename T, int HD, int WARPS>
+__global__ void __launch_bounds__(32 * kJoinWarps) k_join(JoinArgs a, int keys_per_tile) {
+  constexpr int V = HD / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part_of = warp % WARPS;
+  const size_t all = (size_t)a.t * a.group;
+  const long long row = (long long)blockIdx.x * (kJoinWarps / WARPS) + warp / WARPS;
+  sg::pdl_trigger();
+  sg::pdl_wait();
+  const int head = (int)(row / all), r = (int)(row - head * all), tok = r / a.group;
+  const bool in = head < a.kh && (a.first ? tok >= a.first[0] && tok < a.first[a.requests]
+                                          : tok < (long long)a.requests * a.most);
+  if (WARPS == 1 && !in) return;
+  float m = -INFINITY, l = 0.f, o[V];
+#pragma unroll
+  for (int i = 0; i < V; i++) o[i] = 0.f;
+  if (in) {
+    const int tiles = (sg::tree_cached(a) + keys_per_tile - 1) / keys_per_tile;
+    const int per = (tiles + a.splits - 1) / a.splits, prefix = tiles ? (tiles + per - 1) / per : 0;
+    // (Within the workspace, whatever stands there.)
+    const int2 w = a.where[row];
+    const int cta = min(max(w.x, 0), a.ctas - 1), place = min(w.y & 127, a.rows - 1);
+    const int parts = prefix + min(max(w.y >> 7, 1), a.ctas - cta);
+    auto index = [&](int i) {
+      return i <= prefix ? (size_t)(i < prefix ? i : a.splits) * a.kh * all + row
+                         : (size_t)(a.splits + 1) * a.kh * all +
+                               (size_t)(cta + i - prefix) * a.rows + place;
+    };
+    const int share = (parts + WARPS - 1) / WARPS, end = min(parts, (part_of + 1) * share);
+    for (int from = part_of * share; from < end; from += 32) {
+      const int n = min(32, end - from);
+      const float2 p = lane < n ? a.ml[index(from + lane)] : make_float2(-INFINITY, 0.f);
+      const float next = fmaxf(m, sg::warp_max(p.x));
+      const float f = next == -INFINITY ? 1.f : exp2f(m - next);
+      const float g = next == -INFINITY || p.y == 0.f ? 0.f : exp2f(p.x - next);
+      m = next;
+      l = l * f + sg::warp_sum(p.y == 0.f ? 0.f : p.y * g);
+#pragma unroll
+      for (int i = 0; i < V; i++) o[i] *= f;
+#pragma unroll 4
+      for (int j = 0; j < n; j++) {
+        const float weight = __shfl_sync(0xFFFFFFFFu, g, j);
+        if (weight == 0.f) continue;  // no keys, or too far below: may hold anything
+        const float* x = a.part + index(from + j) * HD + lane * V;
+        if constexpr (V == 4) {
+          const float4 y = *reinterpret_cast<const float4*>(x);
+          o[0] = fmaf(weight, y.x, o[0]); o[1] = fmaf(weight, y.y, o[1]);
+          o[2] = fmaf(weight, y.z, o[2]); o[3] = fmaf(weight, y.w, o[3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; i++) o[i] = fmaf(weight, x[i], o[i]);
+        }
+      }
+    }
+  }
+  if constexpr (WARPS > 1) {
+    __shared__ float outs[kJoinWarps][HD];
+    __shared__ float2 sums[kJoinWarps];
+#pragma unroll
+    for (int i = 0; i < V; i++) outs[warp][lane * V + i] = o[i];
+    if (lane == 0) sums[warp] = make_float2(m, l);
+    __syncthreads();
+    if (part_of || !in) return;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) top = fmaxf(top, sums[warp + w].x);
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; i++) o[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) {
+      const float f = top == -INFINITY ? 0.f : exp2f(sums[warp + w].x - top);
+      l += sums[warp + w].y * f;
+#pragma unroll
+      for (int i = 0; i < V; i++) o[i] = fmaf(outs[warp + w][lane * V + i], f, o[i]);
+    }
+  }
+  // A row without keys is zeros.
+  const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  T* to = static_cast<T*>(a.att) + tok * a.ldo + (size_t)(head * a.group + r - tok * a.group) * HD +
+          lane * V;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < V; i++) to[i] = o[i] * f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i++) asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(to[i]) : "f"(o[i] * f));
+  }
+}
+
 // Rows of a kv head -> warps in rows and in keys.
 struct Shape {
   int mw, kw;
@@ -1029,7 +1297,12 @@ bool on_tc(int t, int group, int hd) {
   return t <= 256 && hd >= 64 && t * group > (hd == 128 ? 16 : 32);
 }
 
-// The same for the keys of a shared prefix, which every row sees.
+// Rows of a tile of requests' rows.
+int own_rows(int hd, bool f32, int rows) {
+  return f32 && hd == kFewHeadDim && rows <= kFewRows ? kFewRows : 16 * shape_of(rows).mw;
+}
+
+// Whether a shared prefix's keys, which every row sees, go to tcgen05.
 bool prefix_on_tc(int rows, int hd) { return hd >= 64 && rows > (hd == 128 ? 16 : 32); }
 
 // Splits of the keys: as many CTAs as the GPU holds at once.
@@ -1046,13 +1319,11 @@ size_t workspace_of(int splits, int t, int kh, int group, int hd) {
   return (size_t)splits * kh * t * group * (hd + 2) * sizeof(float);
 }
 
-// CTAs for the splits and row tiles of a tree, and of a batch.
+// CTAs for the splits and row tiles of a tree; of a batch.
 dim3 grid_of(const TreeArgs& a, int tile_rows) {
   return dim3(a.splits, a.kh, (a.t * a.group + tile_rows - 1) / tile_rows);
 }
-dim3 grid_of(const sg::BatchArgs& a, int) {
-  return dim3((unsigned)a.splits * a.tiles * a.requests, a.kh);
-}
+dim3 grid_of(const sg::BatchArgs& a, int) { return dim3(a.ctas); }
 
 template <typename Args>
 cudaError_t launch_few(const Args& a, int dev, cudaStream_t s) {
@@ -1124,14 +1395,20 @@ cudaError_t launch_shared(const TreeArgs& p, const sg::BatchArgs& own, int dev, 
   if (e != cudaSuccess) return e;
   e = launch_mma<T, HD>(own, own.most * own.group, &none, dev, s);
   if (e != cudaSuccess) return e;
-  BatchMerge m;
-  static_cast<TreeArgs&>(m) = p;
-  m.own_splits = own.splits;
-  m.requests = own.requests;
-  m.most = own.most;
-  m.first = own.first;
-  return sg::try_launch(k_merge<T, HD, false, true>, dim3(p.t * p.group * p.kh), dim3(kMergeThreads),
-                        0, 1, s, m, keys);
+  JoinArgs j;
+  static_cast<TreeArgs&>(j) = p;
+  j.where = own.where;
+  j.ctas = own.ctas;
+  j.rows = own_rows(HD, sizeof(T) == 4, own.most * own.group);
+  j.requests = own.requests;
+  j.most = own.most;
+  j.first = own.first;
+  const long long rows = (long long)p.t * p.group * p.kh;
+  if (rows <= kJoinFew)
+    return sg::try_launch(k_join<T, HD, kJoinWarps>, dim3((unsigned)rows), dim3(32 * kJoinWarps), 0,
+                          1, s, j, keys);
+  return sg::try_launch(k_join<T, HD, 1>, dim3((unsigned)((rows + kJoinWarps - 1) / kJoinWarps)),
+                        dim3(32 * kJoinWarps), 0, 1, s, j, keys);
 }
 
 template <typename T>
@@ -1151,20 +1428,35 @@ const char* bad_shape(int t, int kh, int group, int hd) {
   return nullptr;
 }
 
-// How a batch is split: its prefix, and the requests' own keys.
+// How a batch is split: its prefix, and the requests' own keys; its workspace.
 struct Batch {
-  int splits, own_splits, tiles;
-  size_t bytes;
+  int splits, ctas;
+  size_t parts, where, bytes;  // parts; bytes before the notes where they lie, and in all
 };
-Batch batch_of(int sms, int requests, int t, int tokens, int kh, int group, int hd) {
+Batch batch_of(int sms, int type, int t, int tokens, int kh, int group, int hd) {
   Batch b;
-  b.splits = splits_of(sms, tokens * group, kh, prefix_on_tc(tokens * group, hd));
+  const size_t rows = (size_t)kh * tokens * group;
+  const bool tc = prefix_on_tc(tokens * group, hd);
+  b.splits = splits_of(sms, tokens * group, kh, tc);
+  if (tc) {
+    // One CTA to an SM: whole rounds of them, in units of a tile's time, for a
+    // prefix of 128 tiles (its length is not known here); a CTA's start and end cost
+    // as much as six.
+    const long long units = (long long)kh * ((tokens * group + sg::kTreeTcRows - 1) / sg::kTreeTcRows);
+    double best = 1e30;
+    for (int n = 1; n <= 16; n++) {
+      const double cost = (double)((units * n + sms - 1) / sms) * (128.0 / n + 6);
+      if (cost < best) {
+        best = cost;
+        b.splits = n;
+      }
+    }
+  }
   const Shape s = shape_of(t * group);
-  b.tiles = (t * group + 16 * s.mw - 1) / (16 * s.mw);
-  const int resident = sms * (s.mw * s.kw <= 4 ? 2 : 1);
-  const long long others = (long long)requests * kh * b.tiles;
-  b.own_splits = (int)std::max(1ll, std::min((long long)kMaxSplits, resident / others));
-  b.bytes = (size_t)(b.splits + b.own_splits) * kh * tokens * group * (hd + 2) * sizeof(float);
+  b.ctas = sms * (s.mw * s.kw <= 4 ? 2 : 1);
+  b.parts = (b.splits + 1) * rows + (size_t)b.ctas * own_rows(hd, type == STRASGPT_F32, t * group);
+  b.where = b.parts * (hd + 2) * sizeof(float);
+  b.bytes = b.where + rows * sizeof(int2);
   return b;
 }
 
@@ -1174,12 +1466,11 @@ const char* bad_batch(int type, int requests, int t, int tokens, int kh, int gro
   if (t > STRASGPT_ATTN_SHARED_MAX) return "more than 1024 new tokens of a request";
   if (group > 128 || kh > 65535) return "more than 128 q heads per kv head, or 65535 kv heads";
   if (hd != 32 && hd != 64 && hd != 128) return "head_dim must be 32, 64 or 128";
-  // k_merge has a block per row, the prefix's kernels one per 16 rows or more
-  // along z, the requests' ones a block per request, split and tile.
+  // k_join has a block per row, the prefix's kernels one per 16 rows or more along
+  // z.
   if ((long long)tokens * kh * group > INT_MAX) return "more than 2^31 - 1 rows of q heads";
   if ((long long)tokens * group > 65535ll * 64) return "more than 4194240 rows of a kv head";
-  if ((long long)requests * t * group > INT_MAX / kMaxSplits)
-    return "more than 2^23 - 1 rows of all requests' most tokens";
+  if (requests >= 1 << 30) return "more than 2^30 - 1 requests";
   return nullptr;
 }
 
@@ -1266,7 +1557,7 @@ size_t strasgpt_k_attn_shared_workspace(int type, int requests, int t, int token
     return 0;
   }
   if (requests == 0 || tokens == 0) return 0;
-  return batch_of(sms, requests, t, tokens, kv_heads, group, head_dim).bytes;
+  return batch_of(sms, type, t, tokens, kv_heads, group, head_dim).bytes;
 }
 
 int strasgpt_k_attn_shared(const void* q, long long ldq, const void* k_prefix,
@@ -1297,7 +1588,7 @@ int strasgpt_k_attn_shared(const void* q, long long ldq, const void* k_prefix,
     return sg::refuse(me, "a buffer is not aligned to its entries");
   int dev = 0, sms = 0;
   if (const char* why = sg::current_device(&dev, &sms)) return sg::refuse(me, why);
-  const Batch b = batch_of(sms, requests, t, tokens, kv_heads, group, head_dim);
+  const Batch b = batch_of(sms, type, t, tokens, kv_heads, group, head_dim);
   if (!workspace || workspace_bytes < b.bytes)
     return sg::refuse(me, "the workspace is smaller than strasgpt_k_attn_shared_workspace says");
   if (!sg::aligned(workspace, 16)) return sg::refuse(me, "workspace must be 16-byte aligned");
@@ -1313,16 +1604,15 @@ int strasgpt_k_attn_shared(const void* q, long long ldq, const void* k_prefix,
   a.cached = prefix;
   a.splits = b.splits;
   a.part = (float*)workspace;
-  a.ml = (float2*)(a.part + (size_t)(b.splits + b.own_splits) * kv_heads * tokens * group *
-                                head_dim);
+  a.ml = (float2*)(a.part + b.parts * head_dim);
   sg::BatchArgs own = {};
   static_cast<TreeArgs&>(own) = a;
   own.k = k_cache; own.v = v_cache; own.ctx = ctx;
-  own.splits = b.own_splits;
   own.requests = requests; own.most = t; own.first = first; own.rows = rows;
   own.stride = request_stride;
-  own.tiles = b.tiles;
+  own.ctas = b.ctas;
   own.split0 = b.splits;
+  own.where = (int2*)((char*)workspace + b.where);
   const cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e;
   if (type == STRASGPT_F32)

@@ -36,8 +36,9 @@ struct BatchArgs : TreeArgs {
   const int* first;          // [requests + 1], or NULL: most each
   const int* rows;           // [requests]: of its cache, its tokens' included
   long long stride;          // entries from one request's cache to the next's
-  int tiles;                 // row tiles of a request
+  int ctas;                  // that share the requests' tiles
   int split0;                // parts of the prefix come before the requests' own
+  int2* where;               // [kh][t * group]: which CTAs a row's own parts are of
 };
 
 // The cached keys [0, *cached) on the fifth-generation tensor cores, 128 rows

@@ -262,7 +262,7 @@ GOOD = dict(type_=F32, requests=3, t=2, tokens=6, kh=2, g=4, hd=128, pctx=64, ct
     (dict(t=1025), "1024 new"), (dict(g=129, ldq=1 << 20, ldo=1 << 20), "more than 128"),
     (dict(hd=96), "head_dim"), (dict(pctx=0), "without rows"), (dict(ctx=0), "without rows"),
     (dict(tokens=1 << 29), "2^31"), (dict(tokens=1 << 20, g=4, kh=1, t=1024), "4194240"),
-    (dict(requests=1 << 20, t=1024), "2^23"),
+    (dict(requests=1 << 30), "2^30"),
     (dict(ldq=1023), "overlap"), (dict(ldo=512), "overlap"), (dict(stride=-8), "negative"),
     *[({name: None}, "null") for name in ("q", "kp", "vp", "prefix", "k", "v", "rows", "att")],
     *[({name: FAKE + 8}, "16-byte") for name in ("q", "kp", "vp", "k", "v", "att")],
