@@ -422,8 +422,11 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Args
   extern __shared__ __align__(16) unsigned char smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, c4 = lane & 3;
   const int mw = warp % MW, kw = warp / MW;
+  // A batch's own tiles follow its prefix's, which they do not need: they start as
+  // that one's CTAs leave room. It lets them once all before it is complete, and is
+  // waited for at the end: this kernel is complete when both are.
+  if constexpr (!kBatch) sg::pdl_wait();
   sg::pdl_trigger();
-  sg::pdl_wait();
 
   using W = Walker<T, HD, kThreads, kRows, Args>;
   auto start = [&] {
@@ -435,7 +438,10 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Args
     }
   };
   W walk = start();
-  if (walk.count() == 0) return;
+  if (walk.count() == 0) {
+    if constexpr (kBatch) sg::pdl_wait();
+    return;
+  }
 #pragma unroll
   for (int s = 0; s < kStages - 1; s++) walk.fetch(s);
 
@@ -829,6 +835,7 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Args
   }
   }
   } while (kBatch && at < walk.count());
+  if constexpr (kBatch) sg::pdl_wait();
 }
 
 // Up to kFewRows rows a kv head, fp32, head_dim 128: FMAs. Most of a matrix
@@ -849,8 +856,8 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(Args a) {
   static_assert(kWarpKeys == 8, "a warp's keys of a tile are one step");
   extern __shared__ __align__(16) unsigned char smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, c4 = lane & 3;
+  if constexpr (!kBatch) sg::pdl_wait();  // (see k_tree)
   sg::pdl_trigger();
-  sg::pdl_wait();
   using W = Walker<float, HD, 32 * kFewWarps, kFewRows, Args>;
   auto start = [&] {
     if constexpr (kBatch) {
@@ -861,7 +868,10 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(Args a) {
     }
   };
   W walk = start();
-  if (walk.count() == 0) return;
+  if (walk.count() == 0) {
+    if constexpr (kBatch) sg::pdl_wait();
+    return;
+  }
 #pragma unroll
   for (int s = 0; s < kStages - 1; s++) walk.fetch(s);
 
@@ -1017,6 +1027,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(Args a) {
   for (int i = 0; i < kO; i++) to[lane * kO + i] = out[i] * f;
   }
   } while (kBatch && at < walk.count());
+  if constexpr (kBatch) sg::pdl_wait();
 }
 
 // A block joins the parts of one row: sixteen groups of eight lanes, a lane

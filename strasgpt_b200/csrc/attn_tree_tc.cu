@@ -376,7 +376,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int failed;
   __shared__ float2 ml[kRows];  // of the second warpgroup
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // The same in all lanes, and known to be: what the matrix instructions and TMA are
+  // given stays in uniform registers.
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t base = (saddr(raw) + 1023u) & ~1023u;
   uint8_t* const gbase = raw + (base - saddr(raw));
   auto k_tile = [&](int s) { return base + s * 2 * C::kTile; };
@@ -384,8 +386,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t q_at = base + kStages * 2 * C::kTile;
   const int split = blockIdx.x, head = blockIdx.y, r0 = blockIdx.z * kRows;
   const int R = a.t * a.group;
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();  // a batch's own tiles need what came before this kernel, not this kernel
   const int n = tree_cached(a);
   const int tiles = (n + kKeys - 1) / kKeys, per = (tiles + a.splits - 1) / a.splits;
   const int tile0 = split * per, nt = min(tiles, tile0 + per) - tile0;
@@ -425,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncthreads();
   fence_after();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, tmem_slot, 0);
 
   // 512 threads of 128 registers: 2 x 128 x 208 + 2 x 128 x 48 make as many.
   if (warp >= 8) {

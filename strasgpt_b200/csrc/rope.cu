@@ -37,6 +37,26 @@ constexpr int kMaxPairs = 256;    // dim <= 512
 constexpr int kUnroll = 2;        // items in flight per thread
 constexpr int kSinesMax = 2048;   // (token, pair) sines of a block: 16 KB
 
+// Division of numbers below 2^31 by d, 1..2^30, as a product: with 2^(b - 1) < d <=
+// 2^b and mul = floor(2^(31 + b) / d) + 1, mul d is above 2^(31 + b) by 2^b at most,
+// which n < 2^31 does not carry into the quotient. (A division by a number that is
+// not known beforehand takes some 30 instructions, three of them an item, where
+// instructions are what counts: 8191 tokens of 32 heads of 80 bf16 entries 23.9 ->
+// DIV us.)
+struct Divisor {
+  unsigned d, mul, shift;
+  Divisor() = default;
+  explicit Divisor(unsigned by) : d(by) {
+    unsigned b = 0;
+    while ((1u << b) < by) b++;
+    mul = (unsigned)((1ull << (31 + b)) / by + 1);
+    shift = b - 1;  // (by 1: not used)
+  }
+};
+__device__ __forceinline__ int divide(int n, const Divisor& by) {
+  return by.d == 1 ? n : (int)(__umulhi((unsigned)n, by.mul) >> by.shift);
+}
+
 struct RopeArgs {
   const void* x;
   void* y;
@@ -44,6 +64,7 @@ struct RopeArgs {
   const int* pos;
   int t, heads, hd, dim;
   int per_block;             // items of a block
+  Divisor token_items, head_items, token_pairs;  // items of a token, of a head; pairs
   float magnitude, magnitude_rest;  // their sum, to 48 bits
   double turns[kMaxPairs];   // f_j / 2 pi
 };
@@ -115,8 +136,8 @@ __global__ void __launch_bounds__(kThreads, blocks_of(LAYOUT)) k_rope(const __gr
   for (int u = 0; u < kUnroll; u++) {
     const int i = threadIdx.x + u * kThreads;
     if (i >= items) break;
-    const int token = (skip + i) / per_token, place = skip + i - token * per_token;
-    const int h = place / per_head, v = place - h * per_head;
+    const int token = divide(skip + i, a.token_items), place = skip + i - token * per_token;
+    const int h = divide(place, a.head_items), v = place - h * per_head;
     const bool turn = v < turned;
     const int at = !turn ? a.dim + (v - turned) * V : LAYOUT == kSingle ? 2 * v : v * V;
     const T* from = x + (t0 + token) * a.xt + h * a.xh + at;
@@ -126,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, blocks_of(LAYOUT)) k_rope(const __gr
     pair[u] = turn ? token * half + v : -1;
   }
   for (int i = threadIdx.x; i < nt * half; i += kThreads) {
-    const int token = i / half, j = i - token * half;
+    const int token = divide(i, a.token_pairs), j = i - token * half;
     const double turns = (double)position(a, t0 + token, j) * a.turns[j];
     const double half_turns = 2.0 * (turns - rint(turns));
     const float near = (float)half_turns;
@@ -284,7 +305,10 @@ int turn(const char* me, const void* x, long long x_token_stride, long long x_he
   const long long room = (kSinesMax / half - 2) * per_token;
   a.per_block = (int)(room < per_block ? room : per_block);
   const long long blocks = (all + a.per_block - 1) / a.per_block;
-  if (per_token > INT_MAX / 2 || blocks > INT_MAX) return sg::refuse(me, "too many entries");
+  if (per_token > 1 << 30 || blocks > INT_MAX) return sg::refuse(me, "too many entries");
+  a.token_items = Divisor((unsigned)per_token);
+  a.head_items = Divisor((unsigned)per_head);
+  a.token_pairs = Divisor((unsigned)half);
   const dim3 grid((unsigned)blocks);
   const cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e;
