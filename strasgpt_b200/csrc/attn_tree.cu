@@ -85,6 +85,29 @@ __device__ __forceinline__ void mma_tf32(float* d, const uint32_t* a, uint32_t b
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Two fp32 operations in one instruction.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float x, float y) {
+  f32x2 v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+  return v;
+}
+__device__ __forceinline__ float2 unpack2(f32x2 v) {
+  float2 x;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x.x), "=f"(x.y) : "l"(v));
+  return x;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 v;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+
 // x = hi + lo with hi its upper 19 bits (a tf32 value) and lo the exact
 // remainder cut to tf32: 21 bits of x at least.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
@@ -179,7 +202,21 @@ __device__ __forceinline__ void load_tile(const T* k, const T* v, int row, int r
   using L = Tile<T, HD, THREADS / 32>;
   const uint32_t vs = ks + L::kKeys * L::kKRow;
   constexpr int kVecs = HD * (int)sizeof(T) / 16;
-#pragma unroll 8
+  if (rows == L::kKeys && THREADS % kVecs == 0) {
+    // A thread's accesses are a fixed distance apart.
+    constexpr int kStep = THREADS / kVecs < 1 ? 1 : THREADS / kVecs;
+    const int r = threadIdx.x / kVecs, x = threadIdx.x % kVecs;
+    const size_t at = (size_t)(row + r) * HD + x * (16 / sizeof(T));
+    const T *from_k = k + at, *from_v = v + at;
+    const uint32_t to_k = ks + r * L::kKRow + x * 16, to_v = vs + r * L::kVRow + x * 16;
+#pragma unroll
+    for (int i = 0; i < L::kKeys; i += kStep) {
+      cp_async16(to_k + i * L::kKRow, from_k + (size_t)i * HD, 16);
+      cp_async16(to_v + i * L::kVRow, from_v + (size_t)i * HD, 16);
+    }
+    return;
+  }
+#pragma unroll 4
   for (int i = threadIdx.x; i < L::kKeys * kVecs; i += THREADS) {
     const int r = i / kVecs, x = i % kVecs;
     const int bytes = r < rows ? 16 : 0;
@@ -881,8 +918,9 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(Args a) {
   const int head = walk.head(at), R = rows_of.t * a.group, parts = walk.parts(at);
   // Scores in units of log2, so that the softmax is exp2.
   const float scale = 1.4426950408889634f / sqrtf((float)HD);
-  float4 q[kFewRows][kQ];
-  float m[kFewRows], l[kFewRows], o[kFewRows][kO];
+  ulonglong2 q[kFewRows][kQ];
+  float m[kFewRows], l[kFewRows];
+  f32x2 o[kFewRows][kO / 2];
 #pragma unroll
   for (int r = 0; r < kFewRows; r++) {
     const int row = r < R ? r : 0, tok = row / a.group;
@@ -890,16 +928,14 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(Args a) {
                         (size_t)(head * a.group + row - tok * a.group) * HD + 4 * c4;
 #pragma unroll
     for (int j = 0; j < kQ; j++) {
-      q[r][j] = *reinterpret_cast<const float4*>(from + 16 * j);
-      q[r][j].x *= scale;
-      q[r][j].y *= scale;
-      q[r][j].z *= scale;
-      q[r][j].w *= scale;
+      const float4 x = *reinterpret_cast<const float4*>(from + 16 * j);
+      q[r][j].x = pack2(x.x * scale, x.y * scale);
+      q[r][j].y = pack2(x.z * scale, x.w * scale);
     }
     m[r] = -INFINITY;
     l[r] = 0.f;
 #pragma unroll
-    for (int i = 0; i < kO; i++) o[r][i] = 0.f;
+    for (int i = 0; i < kO / 2; i++) o[r][i] = 0;
   }
 
   for (bool more = true; more; at++) {
@@ -914,25 +950,24 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(Args a) {
     const unsigned char* vs = ks + L::kKeys * L::kKRow;
     const int k0 = warp * kWarpKeys;  // the warp's first key in the tile
     if (k0 < rows) {
-      float s[kFewRows][2];
+      f32x2 s[kFewRows];
 #pragma unroll
-      for (int r = 0; r < kFewRows; r++) s[r][0] = s[r][1] = 0.f;
+      for (int r = 0; r < kFewRows; r++) s[r] = 0;
       const unsigned char* kp = ks + (k0 + g8) * L::kKRow + c4 * 16;
 #pragma unroll
       for (int j = 0; j < kQ; j++) {
-        const float4 x = *reinterpret_cast<const float4*>(kp + j * 64);
+        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(kp + j * 64);
 #pragma unroll
         for (int r = 0; r < kFewRows; r++) {
-          s[r][0] = fmaf(q[r][j].x, x.x, s[r][0]);
-          s[r][1] = fmaf(q[r][j].y, x.y, s[r][1]);
-          s[r][0] = fmaf(q[r][j].z, x.z, s[r][0]);
-          s[r][1] = fmaf(q[r][j].w, x.w, s[r][1]);
+          s[r] = fma2(q[r][j].x, x.x, s[r]);
+          s[r] = fma2(q[r][j].y, x.y, s[r]);
         }
       }
       float p[kFewRows], top[kFewRows];
 #pragma unroll
       for (int r = 0; r < kFewRows; r++) {
-        p[r] = s[r][0] + s[r][1];
+        const float2 both = unpack2(s[r]);
+        p[r] = both.x + both.y;
         p[r] += __shfl_xor_sync(0xFFFFFFFFu, p[r], 1);
         p[r] += __shfl_xor_sync(0xFFFFFFFFu, p[r], 2);
         bool in = k0 + g8 < rows && r < R;
@@ -951,7 +986,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(Args a) {
           m[r] = top[r];
           l[r] *= f;
 #pragma unroll
-          for (int i = 0; i < kO; i++) o[r][i] *= f;
+          for (int i = 0; i < kO / 2; i++) o[r][i] = mul2(pack2(f, f), o[r][i]);
         }
         // A row that has seen no key yet keeps m = -inf and zeros.
         p[r] = exp2f(p[r] - (m[r] == -INFINITY ? 0.f : m[r]));
@@ -960,16 +995,15 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(Args a) {
       const unsigned char* vp = vs + k0 * L::kVRow + lane * kO * 4;
 #pragma unroll
       for (int kk = 0; kk < 8; kk++) {
-        const float4 v4 = *reinterpret_cast<const float4*>(vp + kk * L::kVRow);
-        const float x[kO] = {v4.x, v4.y, v4.z, v4.w};
+        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(vp + kk * L::kVRow);
 #pragma unroll
         for (int r = 0; r < kFewRows; r++) {
           const float w = __shfl_sync(0xFFFFFFFFu, p[r], 4 * kk);
           // A drafted row that is hidden may hold anything; cached ones are
           // seen by all.
           if (old || w != 0.f) {
-#pragma unroll
-            for (int i = 0; i < kO; i++) o[r][i] = fmaf(w, x[i], o[r][i]);
+            o[r][0] = fma2(pack2(w, w), x.x, o[r][0]);
+            o[r][1] = fma2(pack2(w, w), x.y, o[r][1]);
           }
         }
       }
@@ -991,7 +1025,8 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(Args a) {
     l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 16);
     float* to = part + (warp * kFewRows + r) * (HD + 2);
 #pragma unroll
-    for (int i = 0; i < kO; i++) to[lane * kO + i] = o[r][i];
+    for (int i = 0; i < kO / 2; i++)
+      *reinterpret_cast<float2*>(to + lane * kO + 2 * i) = unpack2(o[r][i]);
     if (lane == 0) {
       to[HD] = m[r];
       to[HD + 1] = l[r];
