@@ -1065,6 +1065,313 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(Args a) {
   if constexpr (kBatch) sg::pdl_wait();
 }
 
+// 2^x; results below 2^-126 are 0.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The transpose of an 8 x 8 matrix of 16-bit values, a row to four lanes.
+__device__ __forceinline__ uint32_t transpose(uint32_t v) {
+  uint32_t t;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(t) : "r"(v));
+  return t;
+}
+
+// A batch's own tiles, bf16, up to 8 NT rows a request and kv head: the keys are the
+// 16 rows of matrix instructions, the queries their columns, so that one token of
+// eight heads fills what k_tree's 16 rows would leave half empty, and the scores come
+// out as the weights go in. Rows rescale only when a score is 2^8 above what their
+// weights are relative to. A warp has a quarter of a tile's keys, 32 at a time.
+//   S^T = K Q^T;  O^T += V^T P^T
+constexpr int kOwnWarps = 4;
+
+template <int HD, int NT>
+__global__ void __launch_bounds__(32 * kOwnWarps, 2) k_own(sg::BatchArgs a) {
+  constexpr int kThreads = 32 * kOwnWarps, kRows = 8 * NT;
+  using L = Tile<uint16_t, HD, kOwnWarps>;
+  constexpr int kKeys = L::kKeys, kWarpKeys = kKeys / kOwnWarps;
+  constexpr int kStep = NT > 2 || kWarpKeys < 32 ? 16 : 32, kGroups = kStep / 16;
+  constexpr int kQ = HD / 16;  // k steps of the scores, row tiles of the outputs
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, c4 = lane & 3;
+  sg::pdl_trigger();  // (see k_tree)
+  using W = Stream<uint16_t, HD, kThreads, kRows>;
+  __shared__ typename W::Shared shared;
+  W walk(a, shared, smem);
+  if (walk.count() == 0) {
+    sg::pdl_wait();
+    return;
+  }
+#pragma unroll
+  for (int s = 0; s < kStages - 1; s++) walk.fetch(s);
+  const float scale = 1.4426950408889634f / sqrtf((float)HD);  // scores in units of log2
+
+  int at = 0;  // tiles gone through
+  do {
+    const Rows rows_of = walk.rows(at);
+    const int head = walk.head(at), R = rows_of.t * a.group, r0 = rows_of.r0;
+    const int parts = walk.parts(at);
+    auto query = [&](int r) {  // of row r of the request
+      const int tok = r / a.group;
+      return static_cast<const uint16_t*>(a.q) + (rows_of.token0 + tok) * a.ldq +
+             (size_t)(head * a.group + r - tok * a.group) * HD;
+    };
+    uint32_t q[NT][kQ][2];
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+      const int r = r0 + 8 * j + g8;
+      const uint16_t* const from = query(r < R ? r : r0) + 2 * c4;
+#pragma unroll
+      for (int k = 0; k < kQ; k++)
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+          q[j][k][h] = r < R ? *reinterpret_cast<const uint32_t*>(from + 16 * k + 8 * h) : 0u;
+    }
+    // This lane's rows 8 j + 2 c4 + e: their last drafted key, maximum and (this
+    // lane's keys') sum; outputs 16 i + g8 + 8 h of them.
+    int last[NT][2];
+    float m[NT][2], l[NT][2], o[NT][kQ][4];
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int r = r0 + 8 * j + 2 * c4 + e;
+        last[j][e] = r < R ? r / a.group - rows_of.late : -1;
+        m[j][e] = -INFINITY;
+        l[j][e] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < kQ; i++) o[j][i][0] = o[j][i][1] = o[j][i][2] = o[j][i][3] = 0.f;
+    }
+
+    for (bool more = true; more; at++) {
+      cp_async_wait<kStages - 2>();
+      __syncthreads();
+      walk.fetch(at + kStages - 1);  // into the buffer that the last tile left
+      int rows, first;
+      walk.keys(at, rows, first);
+      more = !walk.last(at);
+      const unsigned char* ks = smem + at % kStages * L::kStage;
+      const unsigned char* vs = ks + kKeys * L::kKRow;
+      // As in k_tree: an infinity or NaN in a value row that some rows do not see.
+      bool slow = false;
+      if (first >= 0) {
+        bool bad = false;
+        constexpr int kVecs = HD * 2 / 16;
+        for (int i = threadIdx.x; i < kKeys * kVecs; i += kThreads)
+          bad = bad || !finite_bf16x8(*reinterpret_cast<const uint4*>(
+                           vs + i / kVecs * L::kVRow + i % kVecs * 16));
+        slow = __syncthreads_or(bad);
+      }
+#pragma unroll 1
+      for (int ch = 0; ch < kWarpKeys; ch += kStep) {
+        const int k0 = warp * kWarpKeys + ch;  // first key of the step in the tile
+        if (k0 >= rows) break;
+        float s[NT][kGroups][4];
+        const uint32_t kp = saddr(ks) + (k0 + (lane & 15)) * L::kKRow + (lane >> 4) * 16;
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+          for (int b = 0; b < kGroups; b++) s[j][b][0] = s[j][b][1] = s[j][b][2] = s[j][b][3] = 0.f;
+#pragma unroll
+        for (int k = 0; k < kQ; k++)
+#pragma unroll
+          for (int b = 0; b < kGroups; b++) {
+            uint32_t x[4];
+            ldsm4(kp + b * 16 * L::kKRow + k * 32, x);
+#pragma unroll
+            for (int j = 0; j < NT; j++) mma_bf16(s[j][b], x, q[j][k][0], q[j][k][1]);
+          }
+        // What the rows do not see.
+        if (first >= 0 || k0 + kStep > rows) {
+#pragma unroll
+          for (int b = 0; b < kGroups; b++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+              const int key = k0 + 16 * b + g8 + 8 * (x >> 1);
+#pragma unroll
+              for (int j = 0; j < NT; j++)
+                if (key >= rows || (first >= 0 && first + key > last[j][x & 1]))
+                  s[j][b][x] = -INFINITY;
+            }
+        }
+        // A new maximum, for all lanes of a row.
+        float top[NT][2];
+        bool higher = false;
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            float x = fmaxf(s[j][0][e], s[j][0][2 + e]);
+#pragma unroll
+            for (int b = 1; b < kGroups; b++) x = fmaxf(x, fmaxf(s[j][b][e], s[j][b][2 + e]));
+            top[j][e] = x * scale;
+            higher = higher || top[j][e] > m[j][e] + 8.f;
+          }
+        if (__any_sync(0xFFFFFFFFu, higher)) {
+#pragma unroll
+          for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              float x = top[j][e];
+#pragma unroll
+              for (int d = 4; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, d));
+              const float next = fmaxf(m[j][e], x);
+              // A row that has seen no key yet keeps m = -inf and zeros.
+              const float f = next == -INFINITY ? 1.f : ex2(m[j][e] - next);
+              m[j][e] = next;
+              l[j][e] *= f;
+#pragma unroll
+              for (int i = 0; i < kQ; i++) {
+                o[j][i][e] *= f;
+                o[j][i][2 + e] *= f;
+              }
+            }
+        }
+        // Weights, as two bf16 parts; transposed, they are operands.
+        uint32_t ph[NT][kGroups][2], pl[NT][kGroups][2];
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+          const float z0 = m[j][0] == -INFINITY ? 0.f : m[j][0];
+          const float z1 = m[j][1] == -INFINITY ? 0.f : m[j][1];
+#pragma unroll
+          for (int b = 0; b < kGroups; b++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              float& x = s[j][b][2 * h];
+              float& y = s[j][b][2 * h + 1];
+              x = ex2(fmaf(x, scale, -z0));
+              y = ex2(fmaf(y, scale, -z1));
+              l[j][0] += x;
+              l[j][1] += y;
+              uint32_t hi, lo;
+              split_bf16(x, y, hi, lo);
+              ph[j][b][h] = transpose(hi);
+              pl[j][b][h] = transpose(lo);
+            }
+        }
+        if (slow) {
+          // Key by key, weights of exactly 0 left out.
+          for (int kk = 0; kk < kStep && k0 + kk < rows; kk++) {
+            const uint16_t* const row =
+                reinterpret_cast<const uint16_t*>(vs + (k0 + kk) * L::kVRow) + g8;
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+              float w[2] = {0.f, 0.f};
+#pragma unroll
+              for (int b = 0; b < kGroups; b++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                  if (kk / 8 == 2 * b + h) {
+                    w[0] = s[j][b][2 * h];
+                    w[1] = s[j][b][2 * h + 1];
+                  }
+              const int from = kk % 8 * 4 + c4;
+              w[0] = __shfl_sync(0xFFFFFFFFu, w[0], from);
+              w[1] = __shfl_sync(0xFFFFFFFFu, w[1], from);
+#pragma unroll
+              for (int i = 0; i < kQ; i++)
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+                  if (w[x & 1] != 0.f)
+                    o[j][i][x] = fmaf(w[x & 1], sg::bf16_to_f32(row[16 * i + 8 * (x >> 1)]), o[j][i][x]);
+            }
+          }
+          continue;
+        }
+        const uint32_t vp = saddr(vs) + (k0 + (lane & 7) + (lane >> 4) * 8) * L::kVRow +
+                            ((lane >> 3) & 1) * 16;
+#pragma unroll
+        for (int b = 0; b < kGroups; b++)
+#pragma unroll
+          for (int i = 0; i < kQ; i++) {
+            uint32_t x[4];
+            ldsm4t(vp + b * 16 * L::kVRow + i * 32, x);
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+              mma_bf16(o[j][i], x, pl[j][b][0], pl[j][b][1]);
+              mma_bf16(o[j][i], x, ph[j][b][0], ph[j][b][1]);
+            }
+          }
+      }
+    }
+
+    // The warps' parts are joined in shared memory, in the last tile's place (tiles
+    // behind it may be on their way), those of the upper half into the lower.
+#pragma unroll
+    for (int j = 0; j < NT; j++)
+#pragma unroll
+      for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2) l[j][e] += __shfl_xor_sync(0xFFFFFFFFu, l[j][e], d);
+    constexpr int kLane = NT * (4 * kQ + 4);  // values a lane hands over
+    static_assert(kOwnWarps / 2 * 32 * kLane * 4 <= L::kStage, "join fits a tile");
+    float* const x = reinterpret_cast<float*>(smem + (at - 1) % kStages * L::kStage);
+#pragma unroll
+    for (int half = kOwnWarps / 2; half > 0; half /= 2) {
+      constexpr int kApart = kOwnWarps / 2 * 32;
+      __syncthreads();
+      // [value][warp][lane]: lanes side by side.
+      if (warp >= half && warp < 2 * half) {
+        float* p = x + (warp - half) * 32 + lane;
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+#pragma unroll
+          for (int i = 0; i < kQ; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++, p += kApart) *p = o[j][i][e];
+#pragma unroll
+          for (int e = 0; e < 2; e++, p += 2 * kApart) {
+            p[0] = m[j][e];
+            p[kApart] = l[j][e];
+          }
+        }
+      }
+      __syncthreads();
+      if (warp < half) {
+        const float* p = x + warp * 32 + lane;
+#pragma unroll
+        for (int j = 0; j < NT; j++, p += (4 * kQ + 4) * kApart) {
+          float f[2], g[2];
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const float m2 = p[(4 * kQ + 2 * e) * kApart], l2 = p[(4 * kQ + 2 * e + 1) * kApart];
+            const float next = fmaxf(m[j][e], m2);
+            f[e] = next == -INFINITY ? 0.f : ex2(m[j][e] - next);
+            g[e] = next == -INFINITY ? 0.f : ex2(m2 - next);
+            m[j][e] = next;
+            l[j][e] = l[j][e] * f[e] + l2 * g[e];
+          }
+#pragma unroll
+          for (int i = 0; i < kQ; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              o[j][i][e] = o[j][i][e] * f[e & 1] + p[(4 * i + e) * kApart] * g[e & 1];
+        }
+      }
+    }
+    if (warp == 0) {
+#pragma unroll
+      for (int j = 0; j < NT; j++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const int r = r0 + 8 * j + 2 * c4 + e;
+          if (r >= R) continue;
+          const size_t to = walk.part(a, rows_of, head, parts, r);
+          if (g8 == 0) a.ml[to] = make_float2(m[j][e], l[j][e]);
+          float* const part = a.part + to * HD + g8;
+#pragma unroll
+          for (int i = 0; i < kQ; i++) {
+            part[16 * i] = o[j][i][e];
+            part[16 * i + 8] = o[j][i][2 + e];
+          }
+        }
+    }
+  } while (at < walk.count());
+  sg::pdl_wait();
+}
+
 // A block joins the parts of one row: sixteen groups of eight lanes, a lane
 // having HD / 8 entries of the head, take the parts in turn, each with a
 // running maximum of its own, so that a row's loads are all on their way at
@@ -1344,8 +1651,16 @@ bool on_tc(int t, int group, int hd) {
 }
 
 // Rows of a tile of requests' rows.
+// Tiles of eight rows of k_own that take a request's `rows`; 0: none does.
+int own_tiles(int hd, int rows) {
+  if (rows <= 8) return 1;
+  if (rows <= 16) return 2;
+  return hd > 64 || rows > 48 ? 0 : rows <= 32 ? 4 : 6;
+}
 int own_rows(int hd, bool f32, int rows) {
-  return f32 && hd == kFewHeadDim && rows <= kFewRows ? kFewRows : 16 * shape_of(rows).mw;
+  if (f32 && hd == kFewHeadDim && rows <= kFewRows) return kFewRows;
+  const int tiles = f32 ? 0 : own_tiles(hd, rows);
+  return tiles ? 8 * tiles : 16 * shape_of(rows).mw;
 }
 
 // Whether a shared prefix's keys, which every row sees, go to tcgen05.
@@ -1426,11 +1741,40 @@ cudaError_t launch_hd(const TreeArgs& a, int dev, cudaStream_t s) {
   return sg::try_launch(k_merge<T, HD, false>, rows, dim3(kMergeThreads), 0, 1, s, a, keys);
 }
 
+template <int HD, int NT>
+cudaError_t launch_own_as(const sg::BatchArgs& a, int dev, cudaStream_t s) {
+  static std::atomic<size_t> allowed[sg::kDevices];
+  constexpr size_t bytes = Tile<uint16_t, HD, kOwnWarps>::kBytes;
+  const cudaError_t e = sg::allow_smem(k_own<HD, NT>, bytes, dev, allowed);
+  if (e != cudaSuccess) return e;
+  return sg::try_launch(k_own<HD, NT>, dim3(a.ctas), dim3(32 * kOwnWarps), bytes, 1, s, a);
+}
+
+// A batch's own tiles.
+template <typename T, int HD>
+cudaError_t launch_own(const sg::BatchArgs& a, int dev, cudaStream_t s) {
+  const int rows = a.most * a.group;
+  if constexpr (sizeof(T) == 2) {
+    switch (own_tiles(HD, rows)) {
+      case 1: return launch_own_as<HD, 1>(a, dev, s);
+      case 2: return launch_own_as<HD, 2>(a, dev, s);
+    }
+    if constexpr (HD <= 64) {
+      switch (own_tiles(HD, rows)) {
+        case 4: return launch_own_as<HD, 4>(a, dev, s);
+        case 6: return launch_own_as<HD, 6>(a, dev, s);
+      }
+    }
+  }
+  int none = 0;
+  return launch_mma<T, HD>(a, rows, &none, dev, s);
+}
+
 // Behind a shared prefix: parts of the prefix for all rows, parts of each
 // request's own keys, and their joins.
 template <typename T, int HD>
 cudaError_t launch_shared(const TreeArgs& p, const sg::BatchArgs& own, int dev, cudaStream_t s) {
-  int keys = 0, none = 0;
+  int keys = 0;
   cudaError_t e;
   if (prefix_on_tc(p.t * p.group, HD)) {
     if constexpr (HD >= 64) e = sg::tree_tc(p, sizeof(T) == 4, HD, dev, s);
@@ -1439,7 +1783,7 @@ cudaError_t launch_shared(const TreeArgs& p, const sg::BatchArgs& own, int dev, 
     e = launch_mma<T, HD>(p, p.t * p.group, &keys, dev, s);
   }
   if (e != cudaSuccess) return e;
-  e = launch_mma<T, HD>(own, own.most * own.group, &none, dev, s);
+  e = launch_own<T, HD>(own, dev, s);
   if (e != cudaSuccess) return e;
   JoinArgs j;
   static_cast<TreeArgs&>(j) = p;
@@ -1498,8 +1842,10 @@ Batch batch_of(int sms, int type, int t, int tokens, int kh, int group, int hd) 
       }
     }
   }
+  // As many CTAs as an SM takes (k_own has four warps).
   const Shape s = shape_of(t * group);
-  b.ctas = sms * (s.mw * s.kw <= 4 ? 2 : 1);
+  const bool own = type == STRASGPT_BF16 && own_tiles(hd, t * group) > 0;
+  b.ctas = sms * (own || s.mw * s.kw <= kOwnWarps ? 2 : 1);
   b.parts = (b.splits + 1) * rows + (size_t)b.ctas * own_rows(hd, type == STRASGPT_F32, t * group);
   b.where = b.parts * (hd + 2) * sizeof(float);
   b.bytes = b.where + rows * sizeof(int2);
