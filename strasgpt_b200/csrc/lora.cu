@@ -24,11 +24,12 @@
 // parts and the small ones, and added with rounding. A x is held in 32 bits, and is
 // three parts (fp32 rows) or two (bf16 rows: 2^-17 of it, where the result has 2^-9).
 //
-// Measured on a B200: 4.0 us for one token of 2048 x 2048, rank 8; 11 us for 61
-// tokens, most with an adapter of rank 16 of their own, on 4096 x 6144 (latency: the
-// adapters are 20 MB); 47 us for 2047 fp32 tokens of six prompts, rank 32, on 4096 x
-// 4096 (2.2 TB/s); 170 us for 4001 bf16 tokens, rank 64, on 4096 x 28672 with SwiGLU
-// (2.3 TB/s). What bounds the last two is noted at k_lora_many.
+// Measured on a B200: 3.8 us for one token of 2048 x 2048, rank 8; 7.7 us for 61
+// tokens, most with one of 48 adapters of rank 16, on 4096 x 6144 (latency: a read of
+// A, the cluster's sums and a read of B, one after the other); 46 us for 2047 fp32
+// tokens of six prompts, rank 32, on 4096 x 4096 (2.2 TB/s); 149 us for 4001 bf16
+// tokens, rank 64, on 4096 x 28672 with SwiGLU (2.6 TB/s). What bounds the last two is
+// noted at k_lora_many.
 #include "entry.h"
 
 #include <cuda.h>
@@ -101,9 +102,19 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void cluster_sync() {
+__device__ __forceinline__ void cluster_arrive() {
   asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+}
+// This CTA has started: the others may write to its shared memory.
+__device__ __forceinline__ void cluster_started() {
+  asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  cluster_arrive();
+  cluster_wait();
 }
 // Stores v to p's place in the shared memory of the cluster's CTA `to`.
 __device__ __forceinline__ void store_to(const float* p, uint32_t to, float v) {
@@ -287,6 +298,7 @@ __global__ void __launch_bounds__(kThreads, U <= 2 ? 2 : 1) k_lora_few(const Lor
   const int id = me < p.m ? adapter(me) : -2, d = adapter(token);
   const int earlier = __syncthreads_count(me < token && id == d);
   if (earlier % kGroup) return;  // the same in all CTAs of the cluster
+  cluster_started();
   const unsigned peers = __ballot_sync(0xFFFFFFFFu, me >= token && id == d);
   if (lane == 0) before[warp] = __popc(peers);
   __syncthreads();
@@ -389,6 +401,7 @@ __global__ void __launch_bounds__(kThreads, U <= 2 ? 2 : 1) k_lora_few(const Lor
     }
   }
   __syncthreads();
+  cluster_wait();
   // The warps' sums, to all CTAs; then the CTAs' sums.
   if (d >= 0)
     for (int e = me; e < count * p.rank; e += kThreads) {
@@ -780,7 +793,8 @@ struct Place {
 
 // Calls f(first token, tokens, adapter or -1) for each of this cluster's items: an
 // item is a run of one adapter in a tile of p.tokens tokens, and each cluster has
-// every clusters-th. All threads of the cluster's CTAs take part.
+// every clusters-th. All threads of the cluster's CTAs take part, and have arrived at
+// the cluster's barrier.
 template <typename F>
 __device__ __forceinline__ void each_item(const LoraArgs& p, unsigned* starts, int* before, F f) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, clusters = gridDim.x / kCluster;
@@ -793,7 +807,8 @@ __device__ __forceinline__ void each_item(const LoraArgs& p, unsigned* starts, i
 #pragma unroll 1
   for (int w0 = 0; w0 < p.m;) {
     const int wn = min(32 * kChunks, p.m - w0), chunks = (wn + 31) / 32;
-    if (w0) cluster_sync();  // all are done with the last ones
+    if (w0) cluster_arrive();
+    cluster_wait();  // all are there, and done with the last ones
     // Each CTA looks over every kCluster-th chunk for all of them.
 #pragma unroll 1
     for (int c = warp * kCluster + cta; c < chunks; c += kManyThreads / 32 * kCluster) {
@@ -867,6 +882,7 @@ __global__ void __launch_bounds__(kManyThreads, P == 1 ? 2 : 1)
   const bool worker = warp < kWarps, loader = !worker && warp < kWarps + 2;
   const int side_of = worker ? warp >> 2 : warp & 1;  // its stages: even, odd ones
   const uint32_t cta = cluster_rank(), s_at = (saddr(raw) + 1023u) & ~1023u;
+  cluster_started();
   uint8_t* const operand = raw + (s_at - saddr(raw));
   const uint32_t ring_at = s_at + l.operand + side_of * l.stages * l.stage;
   uint8_t* const ring = operand + l.operand + side_of * l.stages * l.stage;
