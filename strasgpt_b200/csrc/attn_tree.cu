@@ -23,8 +23,18 @@
 // (190 us, 5.5 TB/s, by FMAs: k_tree_few); mma.sync in fp32 with 16 (244 us:
 // its three products take 174 us of that, as the slope from 32 to 64 rows
 // says) and above; from 17 or 33 rows on the cached keys are attn_tree_tc.cu's
-// (see on_tc). Short caches are latency: 7.4 us for one token over 613 keys,
+// (see on_tc). Short caches are latency: 7.0 us for one token over 613 keys,
 // both kernels.
+//
+// Behind a shared prefix: the prefix is read once for all requests' rows, by the
+// kernels above (on_tc's from 16 rows a kv head on); the requests' own keys, tiles of
+// rows by tiles of keys, are shared out evenly over as many CTAs as the GPU holds,
+// which start as the prefix's leave room; k_join adds up both. Measured, 8 kv heads:
+// 64 requests of four heads of 128 bf16 entries, up to 1021 rows each behind 32768,
+// 90 us (prefix 47, own rows 41, alone: 4.9 TB/s; join 11); 48 in fp32, 700 behind
+// 8191, 107 us (50, 58, 8); 31 requests with up to six drafted tokens of eight heads of
+// 64 bf16 entries, 2000 behind 16001, 117 us (66, 57, 10); 16 prompts of up to 96
+// tokens behind 8192 rows 210 us (173, 32, 27); two requests behind 613 rows 11 us.
 #include "attn_tree.h"
 
 #include <limits.h>
@@ -1107,13 +1117,19 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 2) k_own(sg::BatchArgs a) {
   for (int s = 0; s < kStages - 1; s++) walk.fetch(s);
   const float scale = 1.4426950408889634f / sqrtf((float)HD);  // scores in units of log2
 
+  // r / group: mul is above 2^16 / group by 1 at most, which r < 64 does not carry into
+  // the quotient.
+  static_assert(kRows <= 64, "all rows of a request");
+  const unsigned mul = 65536u / a.group + 1;
+  auto token = [&](int r) { return (int)(r * mul >> 16); };
+
   int at = 0;  // tiles gone through
   do {
     const Rows rows_of = walk.rows(at);
     const int head = walk.head(at), R = rows_of.t * a.group, r0 = rows_of.r0;
     const int parts = walk.parts(at);
     auto query = [&](int r) {  // of row r of the request
-      const int tok = r / a.group;
+      const int tok = token(r);
       return static_cast<const uint16_t*>(a.q) + (rows_of.token0 + tok) * a.ldq +
              (size_t)(head * a.group + r - tok * a.group) * HD;
     };
@@ -1137,7 +1153,7 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 2) k_own(sg::BatchArgs a) {
 #pragma unroll
       for (int e = 0; e < 2; e++) {
         const int r = r0 + 8 * j + 2 * c4 + e;
-        last[j][e] = r < R ? r / a.group - rows_of.late : -1;
+        last[j][e] = r < R ? token(r) - rows_of.late : -1;
         m[j][e] = -INFINITY;
         l[j][e] = 0.f;
       }
@@ -1298,75 +1314,67 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 2) k_own(sg::BatchArgs a) {
     }
 
     // The warps' parts are joined in shared memory, in the last tile's place (tiles
-    // behind it may be on their way), those of the upper half into the lower.
-#pragma unroll
-    for (int j = 0; j < NT; j++)
-#pragma unroll
-      for (int e = 0; e < 2; e++)
-#pragma unroll
-        for (int d = 4; d < 32; d *= 2) l[j][e] += __shfl_xor_sync(0xFFFFFFFFu, l[j][e], d);
-    constexpr int kLane = NT * (4 * kQ + 4);  // values a lane hands over
-    static_assert(kOwnWarps / 2 * 32 * kLane * 4 <= L::kStage, "join fits a tile");
+    // behind it may be on their way), kAtOnce tiles of rows at a time: every warp
+    // hands over all that it has, and adds up a quarter of the outputs.
+    constexpr int kLane = 4 * kQ + 4;  // values a lane hands over per tile of rows
+    constexpr int kFits = L::kStage / (kOwnWarps * 32 * kLane * 4);
+    constexpr int kAtOnce = kFits < NT ? kFits : NT, kApart = 32 * kOwnWarps;
+    static_assert(kAtOnce > 0, "a tile of rows fits");
+    // [value][warp][lane]: lanes side by side.
     float* const x = reinterpret_cast<float*>(smem + (at - 1) % kStages * L::kStage);
 #pragma unroll
-    for (int half = kOwnWarps / 2; half > 0; half /= 2) {
-      constexpr int kApart = kOwnWarps / 2 * 32;
+    for (int j0 = 0; j0 < NT; j0 += kAtOnce) {
       __syncthreads();
-      // [value][warp][lane]: lanes side by side.
-      if (warp >= half && warp < 2 * half) {
-        float* p = x + (warp - half) * 32 + lane;
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
+      for (int j = j0; j < j0 + kAtOnce && j < NT; j++) {
+        float* p = x + (j - j0) * kLane * kApart + threadIdx.x;
 #pragma unroll
-          for (int i = 0; i < kQ; i++)
+        for (int i = 0; i < kQ; i++)
 #pragma unroll
-            for (int e = 0; e < 4; e++, p += kApart) *p = o[j][i][e];
+          for (int e = 0; e < 4; e++, p += kApart) *p = o[j][i][e];
 #pragma unroll
-          for (int e = 0; e < 2; e++, p += 2 * kApart) {
-            p[0] = m[j][e];
-            p[kApart] = l[j][e];
-          }
+        for (int e = 0; e < 2; e++, p += 2 * kApart) {
+#pragma unroll
+          for (int d = 4; d < 32; d *= 2) l[j][e] += __shfl_xor_sync(0xFFFFFFFFu, l[j][e], d);
+          p[0] = m[j][e];
+          p[kApart] = l[j][e];
         }
       }
       __syncthreads();
-      if (warp < half) {
-        const float* p = x + warp * 32 + lane;
 #pragma unroll
-        for (int j = 0; j < NT; j++, p += (4 * kQ + 4) * kApart) {
-          float f[2], g[2];
-#pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const float m2 = p[(4 * kQ + 2 * e) * kApart], l2 = p[(4 * kQ + 2 * e + 1) * kApart];
-            const float next = fmaxf(m[j][e], m2);
-            f[e] = next == -INFINITY ? 0.f : ex2(m[j][e] - next);
-            g[e] = next == -INFINITY ? 0.f : ex2(m2 - next);
-            m[j][e] = next;
-            l[j][e] = l[j][e] * f[e] + l2 * g[e];
-          }
-#pragma unroll
-          for (int i = 0; i < kQ; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-              o[j][i][e] = o[j][i][e] * f[e & 1] + p[(4 * i + e) * kApart] * g[e & 1];
-        }
-      }
-    }
-    if (warp == 0) {
-#pragma unroll
-      for (int j = 0; j < NT; j++)
+      for (int j = j0; j < j0 + kAtOnce && j < NT; j++) {
+        const float* const p = x + (j - j0) * kLane * kApart + lane;
+        float f[2][kOwnWarps];
+        float* to[2];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-          const int r = r0 + 8 * j + 2 * c4 + e;
-          if (r >= R) continue;
-          const size_t to = walk.part(a, rows_of, head, parts, r);
-          if (g8 == 0) a.ml[to] = make_float2(m[j][e], l[j][e]);
-          float* const part = a.part + to * HD + g8;
+          const float* const ml = p + (4 * kQ + 2 * e) * kApart;
+          float top = -INFINITY, sum = 0.f;
 #pragma unroll
-          for (int i = 0; i < kQ; i++) {
-            part[16 * i] = o[j][i][e];
-            part[16 * i + 8] = o[j][i][2 + e];
+          for (int w = 0; w < kOwnWarps; w++) top = fmaxf(top, ml[32 * w]);
+#pragma unroll
+          for (int w = 0; w < kOwnWarps; w++) {
+            f[e][w] = top == -INFINITY ? 0.f : ex2(ml[32 * w] - top);
+            sum += f[e][w] * ml[kApart + 32 * w];
+          }
+          const int r = r0 + 8 * j + 2 * c4 + e;
+          const size_t at_row = r < R ? walk.part(a, rows_of, head, parts, r) : 0;
+          to[e] = r < R ? a.part + at_row * HD + g8 : nullptr;
+          if (r < R && g8 == 0 && warp == 0) a.ml[at_row] = make_float2(top, sum);
+        }
+#pragma unroll
+        for (int u = 0; u < 2 * kQ; u += kOwnWarps) {
+          const int of = u + warp;  // outputs 8 of + g8
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const float* const v = p + (of / 2 * 4 + of % 2 * 2 + e) * kApart;
+            float y = 0.f;
+#pragma unroll
+            for (int w = 0; w < kOwnWarps; w++) y = fmaf(f[e][w], v[32 * w], y);
+            if (to[e]) to[e][8 * of] = y;
           }
         }
+      }
     }
   } while (at < walk.count());
   sg::pdl_wait();
@@ -1650,20 +1658,33 @@ bool on_tc(int t, int group, int hd) {
   return t <= 256 && hd >= 64 && t * group > (hd == 128 ? 16 : 32);
 }
 
-// Rows of a tile of requests' rows.
-// Tiles of eight rows of k_own that take a request's `rows`; 0: none does.
+// Tiles of eight rows of k_own that take a request's `rows`; 0: k_tree takes them.
+// Measured with 8 kv heads behind a prefix of 64 rows, us of a call with k_own /
+// k_tree, for 48 requests of 1000 rows, 8 of 4000 and 16 of 200:
+//   head_dim 128,  4 rows: 49 / 57, 36 / 42, 13.3 / 15.8
+//                 16 rows: 60 / 61, 44 / 45, 18.7 / 18.4
+//   head_dim 64,   8 rows: 34 / 41, 21 / 26, 13.5 / 15.9
+//                 16 rows: 37 / 40, 26 / 28, 16.0 / 16.7
+//                 32 rows: 52 / 54, 34 / 34, 22.9 / 20.5
+//                 48 rows: 76 / 73, 46 / 51, 25.3 / 18.9
+//   head_dim 32,  32 rows: 42 / 48, 29 / 33, 20.5 / 18.2
+//                 48 rows: 57 / 73, 38 / 48, 20.7 / 16.6
+// (k_tree takes 48 rows as 64.) Where neither is always ahead, it goes by the longer
+// ones.
 int own_tiles(int hd, int rows) {
   if (rows <= 8) return 1;
   if (rows <= 16) return 2;
-  return hd > 64 || rows > 48 ? 0 : rows <= 32 ? 4 : 6;
+  if (rows <= 32) return hd == 32 ? 4 : 0;
+  return rows <= 48 && hd < 128 ? 6 : 0;
 }
+// Rows of a tile of requests' rows.
 int own_rows(int hd, bool f32, int rows) {
   if (f32 && hd == kFewHeadDim && rows <= kFewRows) return kFewRows;
   const int tiles = f32 ? 0 : own_tiles(hd, rows);
   return tiles ? 8 * tiles : 16 * shape_of(rows).mw;
 }
 
-// Whether a shared prefix's keys, which every row sees, go to tcgen05.
+// Whether a shared prefix's keys go to tcgen05: on_tc's rule, whatever the tokens.
 bool prefix_on_tc(int rows, int hd) { return hd >= 64 && rows > (hd == 128 ? 16 : 32); }
 
 // Splits of the keys: as many CTAs as the GPU holds at once.
@@ -1759,12 +1780,10 @@ cudaError_t launch_own(const sg::BatchArgs& a, int dev, cudaStream_t s) {
       case 1: return launch_own_as<HD, 1>(a, dev, s);
       case 2: return launch_own_as<HD, 2>(a, dev, s);
     }
-    if constexpr (HD <= 64) {
-      switch (own_tiles(HD, rows)) {
-        case 4: return launch_own_as<HD, 4>(a, dev, s);
-        case 6: return launch_own_as<HD, 6>(a, dev, s);
-      }
-    }
+    if constexpr (HD == 32)
+      if (own_tiles(HD, rows) == 4) return launch_own_as<HD, 4>(a, dev, s);
+    if constexpr (HD < 128)
+      if (own_tiles(HD, rows) == 6) return launch_own_as<HD, 6>(a, dev, s);
   }
   int none = 0;
   return launch_mma<T, HD>(a, rows, &none, dev, s);
