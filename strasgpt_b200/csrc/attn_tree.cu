@@ -1088,25 +1088,35 @@ __device__ __forceinline__ uint32_t transpose(uint32_t v) {
   return t;
 }
 
-// A batch's own tiles, bf16, up to 8 NT rows a request and kv head: the keys are the
-// 16 rows of matrix instructions, the queries their columns, so that one token of
-// eight heads fills what k_tree's 16 rows would leave half empty, and the scores come
-// out as the weights go in. Rows rescale only when a score is 2^8 above what their
-// weights are relative to. A warp has a quarter of a tile's keys, 32 at a time.
+// A batch's own tiles, up to 8 NT rows a request and kv head: the keys are the 16 rows
+// of matrix instructions, the queries their columns, so that one token of eight heads
+// fills what k_tree's 16 rows would leave half empty, and the scores come out as the
+// weights go in. Rows rescale only when a score is 2^8 above what their weights are
+// relative to. A warp has the same keys of each tile, 16 or 32 at a time, and all of the
+// outputs or (fp32, 128 entries, where a tile has 32 keys) half of them.
 //   S^T = K Q^T;  O^T += V^T P^T
+// fp32: tf32 parts as in k_tree. A matrix instruction cuts its sums, so those of small
+// products and of large ones are kept apart, and outputs start from zero at each step
+// and are added with rounding. Entries of a row, and keys, are numbered so that a lane's
+// are neighbours: any order serves, if both operands have it.
 constexpr int kOwnWarps = 4;
 
-template <int HD, int NT>
+template <typename T, int HD, int NT>
 __global__ void __launch_bounds__(32 * kOwnWarps, 2) k_own(sg::BatchArgs a) {
+  constexpr bool kF32 = sizeof(T) == 4;
   constexpr int kThreads = 32 * kOwnWarps, kRows = 8 * NT;
-  using L = Tile<uint16_t, HD, kOwnWarps>;
-  constexpr int kKeys = L::kKeys, kWarpKeys = kKeys / kOwnWarps;
+  using L = Tile<T, HD, kOwnWarps>;
+  // Warps side by side in keys, and in outputs.
+  constexpr int kKeys = L::kKeys, kSide = kKeys / 16 < kOwnWarps ? kKeys / 16 : kOwnWarps;
+  constexpr int kShares = kOwnWarps / kSide, kWarpKeys = kKeys / kSide;
   constexpr int kStep = NT > 2 || kWarpKeys < 32 ? 16 : 32, kGroups = kStep / 16;
-  constexpr int kQ = HD / 16;  // k steps of the scores, row tiles of the outputs
+  constexpr int kQ = HD / 16, kO = kQ / kShares;  // 16 entries: of the scores, of a warp's outputs
+  static_assert(!kF32 || kGroups == 1, "16 keys a step");
   extern __shared__ __align__(16) unsigned char smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, c4 = lane & 3;
   sg::pdl_trigger();  // (see k_tree)
-  using W = Stream<uint16_t, HD, kThreads, kRows>;
+  const int side = warp % kSide, share = warp / kSide;
+  using W = Stream<T, HD, kThreads, kRows>;
   __shared__ typename W::Shared shared;
   W walk(a, shared, smem);
   if (walk.count() == 0) {
@@ -1130,24 +1140,40 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 2) k_own(sg::BatchArgs a) {
     const int parts = walk.parts(at);
     auto query = [&](int r) {  // of row r of the request
       const int tok = token(r);
-      return static_cast<const uint16_t*>(a.q) + (rows_of.token0 + tok) * a.ldq +
+      return static_cast<const T*>(a.q) + (rows_of.token0 + tok) * a.ldq +
              (size_t)(head * a.group + r - tok * a.group) * HD;
     };
-    uint32_t q[NT][kQ][2];
+    // bf16: operands as they are; fp32: the parts of entries 16 k + 4 c4 + {0, 1} and
+    // {2, 3}.
+    uint32_t q[NT][kQ][kF32 ? 8 : 2];
 #pragma unroll
     for (int j = 0; j < NT; j++) {
       const int r = r0 + 8 * j + g8;
-      const uint16_t* const from = query(r < R ? r : r0) + 2 * c4;
+      const T* const from = query(r < R ? r : r0) + (kF32 ? 4 : 2) * c4;
 #pragma unroll
-      for (int k = 0; k < kQ; k++)
+      for (int k = 0; k < kQ; k++) {
+        if constexpr (kF32) {
+          const float4 x = r < R ? *reinterpret_cast<const float4*>(from + 16 * k)
+                                 : make_float4(0.f, 0.f, 0.f, 0.f);
+          split_tf32(x.x, q[j][k][0], q[j][k][4]);
+          split_tf32(x.y, q[j][k][1], q[j][k][5]);
+          split_tf32(x.z, q[j][k][2], q[j][k][6]);
+          split_tf32(x.w, q[j][k][3], q[j][k][7]);
+        } else {
 #pragma unroll
-        for (int h = 0; h < 2; h++)
-          q[j][k][h] = r < R ? *reinterpret_cast<const uint32_t*>(from + 16 * k + 8 * h) : 0u;
+          for (int h = 0; h < 2; h++)
+            q[j][k][h] = r < R ? *reinterpret_cast<const uint32_t*>(from + 16 * k + 8 * h) : 0u;
+        }
+      }
     }
     // This lane's rows 8 j + 2 c4 + e: their last drafted key, maximum and (this
-    // lane's keys') sum; outputs 16 i + g8 + 8 h of them.
+    // lane's keys') sum; outputs entry(i, h) of them.
+    auto entry = [&](int i, int h) {
+      return kF32 ? share * (HD / kShares) + 32 * (i / 2) + 4 * g8 + i % 2 * 2 + h
+                  : 16 * i + g8 + 8 * h;
+    };
     int last[NT][2];
-    float m[NT][2], l[NT][2], o[NT][kQ][4];
+    float m[NT][2], l[NT][2], o[NT][kO][4];
 #pragma unroll
     for (int j = 0; j < NT; j++) {
 #pragma unroll
@@ -1158,7 +1184,7 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 2) k_own(sg::BatchArgs a) {
         l[j][e] = 0.f;
       }
 #pragma unroll
-      for (int i = 0; i < kQ; i++) o[j][i][0] = o[j][i][1] = o[j][i][2] = o[j][i][3] = 0.f;
+      for (int i = 0; i < kO; i++) o[j][i][0] = o[j][i][1] = o[j][i][2] = o[j][i][3] = 0.f;
     }
 
     for (bool more = true; more; at++) {
@@ -1174,31 +1200,73 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 2) k_own(sg::BatchArgs a) {
       bool slow = false;
       if (first >= 0) {
         bool bad = false;
-        constexpr int kVecs = HD * 2 / 16;
-        for (int i = threadIdx.x; i < kKeys * kVecs; i += kThreads)
-          bad = bad || !finite_bf16x8(*reinterpret_cast<const uint4*>(
-                           vs + i / kVecs * L::kVRow + i % kVecs * 16));
+        constexpr int kVecs = HD * (int)sizeof(T) / 16;
+        for (int i = threadIdx.x; i < kKeys * kVecs; i += kThreads) {
+          const unsigned char* p = vs + i / kVecs * L::kVRow + i % kVecs * 16;
+          if constexpr (kF32)
+            bad = bad || !finite4(*reinterpret_cast<const float4*>(p));
+          else
+            bad = bad || !finite_bf16x8(*reinterpret_cast<const uint4*>(p));
+        }
         slow = __syncthreads_or(bad);
       }
 #pragma unroll 1
       for (int ch = 0; ch < kWarpKeys; ch += kStep) {
-        const int k0 = warp * kWarpKeys + ch;  // first key of the step in the tile
+        const int k0 = side * kWarpKeys + ch;  // first key of the step in the tile
         if (k0 >= rows) break;
         float s[NT][kGroups][4];
-        const uint32_t kp = saddr(ks) + (k0 + (lane & 15)) * L::kKRow + (lane >> 4) * 16;
+        if constexpr (kF32) {
+          float big[NT][2][4], small[NT][2][4];
 #pragma unroll
-        for (int j = 0; j < NT; j++)
+          for (int j = 0; j < NT; j++)
 #pragma unroll
-          for (int b = 0; b < kGroups; b++) s[j][b][0] = s[j][b][1] = s[j][b][2] = s[j][b][3] = 0.f;
+            for (int x = 0; x < 8; x++) (&big[j][0][0])[x] = (&small[j][0][0])[x] = 0.f;
+          const unsigned char* const kp = ks + (k0 + g8) * L::kKRow + c4 * 16;
 #pragma unroll
-        for (int k = 0; k < kQ; k++)
+          for (int k = 0; k < kQ; k++) {
+            const float4 x = *reinterpret_cast<const float4*>(kp + k * 64);
+            const float4 y = *reinterpret_cast<const float4*>(kp + 8 * L::kKRow + k * 64);
+            uint32_t hi[2][4], lo[2][4];
+            split_tf32(x.x, hi[0][0], lo[0][0]);
+            split_tf32(y.x, hi[0][1], lo[0][1]);
+            split_tf32(x.y, hi[0][2], lo[0][2]);
+            split_tf32(y.y, hi[0][3], lo[0][3]);
+            split_tf32(x.z, hi[1][0], lo[1][0]);
+            split_tf32(y.z, hi[1][1], lo[1][1]);
+            split_tf32(x.w, hi[1][2], lo[1][2]);
+            split_tf32(y.w, hi[1][3], lo[1][3]);
 #pragma unroll
-          for (int b = 0; b < kGroups; b++) {
-            uint32_t x[4];
-            ldsm4(kp + b * 16 * L::kKRow + k * 32, x);
+            for (int j = 0; j < NT; j++)
 #pragma unroll
-            for (int j = 0; j < NT; j++) mma_bf16(s[j][b], x, q[j][k][0], q[j][k][1]);
+              for (int h = 0; h < 2; h++) {
+                const uint32_t* const w = q[j][k] + 2 * h;
+                mma_tf32(small[j][h], lo[h], w[0], w[1]);
+                mma_tf32(big[j][h], hi[h], w[0], w[1]);
+                mma_tf32(small[j][h], hi[h], w[4], w[5]);
+              }
           }
+#pragma unroll
+          for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int x = 0; x < 4; x++)
+              s[j][0][x] = (small[j][0][x] + small[j][1][x]) + (big[j][0][x] + big[j][1][x]);
+        } else {
+          const uint32_t kp = saddr(ks) + (k0 + (lane & 15)) * L::kKRow + (lane >> 4) * 16;
+#pragma unroll
+          for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int b = 0; b < kGroups; b++)
+              s[j][b][0] = s[j][b][1] = s[j][b][2] = s[j][b][3] = 0.f;
+#pragma unroll
+          for (int k = 0; k < kQ; k++)
+#pragma unroll
+            for (int b = 0; b < kGroups; b++) {
+              uint32_t x[4];
+              ldsm4(kp + b * 16 * L::kKRow + k * 32, x);
+#pragma unroll
+              for (int j = 0; j < NT; j++) mma_bf16(s[j][b], x, q[j][k][0], q[j][k][1]);
+            }
+        }
         // What the rows do not see.
         if (first >= 0 || k0 + kStep > rows) {
 #pragma unroll
@@ -1239,14 +1307,14 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 2) k_own(sg::BatchArgs a) {
               m[j][e] = next;
               l[j][e] *= f;
 #pragma unroll
-              for (int i = 0; i < kQ; i++) {
+              for (int i = 0; i < kO; i++) {
                 o[j][i][e] *= f;
                 o[j][i][2 + e] *= f;
               }
             }
         }
-        // Weights, as two bf16 parts; transposed, they are operands.
-        uint32_t ph[NT][kGroups][2], pl[NT][kGroups][2];
+        // Weights, as two bf16 parts, or tf32 parts; transposed, they are operands.
+        uint32_t ph[NT][kGroups][kF32 ? 4 : 2], pl[NT][kGroups][kF32 ? 4 : 2];
 #pragma unroll
         for (int j = 0; j < NT; j++) {
           const float z0 = m[j][0] == -INFINITY ? 0.f : m[j][0];
@@ -1261,17 +1329,27 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 2) k_own(sg::BatchArgs a) {
               y = ex2(fmaf(y, scale, -z1));
               l[j][0] += x;
               l[j][1] += y;
-              uint32_t hi, lo;
-              split_bf16(x, y, hi, lo);
-              ph[j][b][h] = transpose(hi);
-              pl[j][b][h] = transpose(lo);
+              if constexpr (kF32) {
+                // Upper and lower halves; then keys 8 h + 2 c4 and the next one.
+                const uint32_t u = __float_as_uint(x), v = __float_as_uint(y);
+                const uint32_t up = transpose(__byte_perm(u, v, 0x7632));
+                const uint32_t down = transpose(__byte_perm(u, v, 0x5410));
+                split_tf32(__uint_as_float(__byte_perm(down, up, 0x5410)), ph[j][b][2 * h],
+                           pl[j][b][2 * h]);
+                split_tf32(__uint_as_float(__byte_perm(down, up, 0x7632)), ph[j][b][2 * h + 1],
+                           pl[j][b][2 * h + 1]);
+              } else {
+                uint32_t hi, lo;
+                split_bf16(x, y, hi, lo);
+                ph[j][b][h] = transpose(hi);
+                pl[j][b][h] = transpose(lo);
+              }
             }
         }
         if (slow) {
           // Key by key, weights of exactly 0 left out.
           for (int kk = 0; kk < kStep && k0 + kk < rows; kk++) {
-            const uint16_t* const row =
-                reinterpret_cast<const uint16_t*>(vs + (k0 + kk) * L::kVRow) + g8;
+            const T* const row = reinterpret_cast<const T*>(vs + (k0 + kk) * L::kVRow);
 #pragma unroll
             for (int j = 0; j < NT; j++) {
               float w[2] = {0.f, 0.f};
@@ -1287,36 +1365,79 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 2) k_own(sg::BatchArgs a) {
               w[0] = __shfl_sync(0xFFFFFFFFu, w[0], from);
               w[1] = __shfl_sync(0xFFFFFFFFu, w[1], from);
 #pragma unroll
-              for (int i = 0; i < kQ; i++)
+              for (int i = 0; i < kO; i++)
 #pragma unroll
-                for (int x = 0; x < 4; x++)
-                  if (w[x & 1] != 0.f)
-                    o[j][i][x] = fmaf(w[x & 1], sg::bf16_to_f32(row[16 * i + 8 * (x >> 1)]), o[j][i][x]);
+                for (int x = 0; x < 4; x++) {
+                  if (w[x & 1] == 0.f) continue;
+                  const T v = row[entry(i, x >> 1)];
+                  if constexpr (kF32)
+                    o[j][i][x] = fmaf(w[x & 1], v, o[j][i][x]);
+                  else
+                    o[j][i][x] = fmaf(w[x & 1], sg::bf16_to_f32(v), o[j][i][x]);
+                }
             }
           }
           continue;
         }
-        const uint32_t vp = saddr(vs) + (k0 + (lane & 7) + (lane >> 4) * 8) * L::kVRow +
-                            ((lane >> 3) & 1) * 16;
+        if constexpr (kF32) {
+          const unsigned char* const vp =
+              vs + (k0 + 2 * c4) * L::kVRow + (share * (HD / kShares) + 4 * g8) * 4;
 #pragma unroll
-        for (int b = 0; b < kGroups; b++)
+          for (int i = 0; i < kO; i += 2) {
+            uint32_t hi[2][2][4], lo[2][2][4];  // [half of the keys][tile]
 #pragma unroll
-          for (int i = 0; i < kQ; i++) {
-            uint32_t x[4];
-            ldsm4t(vp + b * 16 * L::kVRow + i * 32, x);
-#pragma unroll
-            for (int j = 0; j < NT; j++) {
-              mma_bf16(o[j][i], x, pl[j][b][0], pl[j][b][1]);
-              mma_bf16(o[j][i], x, ph[j][b][0], ph[j][b][1]);
+            for (int h = 0; h < 2; h++) {
+              const unsigned char* const p = vp + 8 * h * L::kVRow + i * 64;
+              const float4 x = *reinterpret_cast<const float4*>(p);
+              const float4 y = *reinterpret_cast<const float4*>(p + L::kVRow);
+              split_tf32(x.x, hi[h][0][0], lo[h][0][0]);
+              split_tf32(x.y, hi[h][0][1], lo[h][0][1]);
+              split_tf32(y.x, hi[h][0][2], lo[h][0][2]);
+              split_tf32(y.y, hi[h][0][3], lo[h][0][3]);
+              split_tf32(x.z, hi[h][1][0], lo[h][1][0]);
+              split_tf32(x.w, hi[h][1][1], lo[h][1][1]);
+              split_tf32(y.z, hi[h][1][2], lo[h][1][2]);
+              split_tf32(y.w, hi[h][1][3], lo[h][1][3]);
             }
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+              for (int t = 0; t < 2; t++) {
+                const uint32_t *const wh = ph[j][0], *const wl = pl[j][0];
+                float y[4] = {0.f, 0.f, 0.f, 0.f};
+                mma_tf32(y, lo[0][t], wh[0], wh[1]);
+                mma_tf32(y, lo[1][t], wh[2], wh[3]);
+                mma_tf32(y, hi[0][t], wl[0], wl[1]);
+                mma_tf32(y, hi[1][t], wl[2], wl[3]);
+                mma_tf32(y, hi[0][t], wh[0], wh[1]);
+                mma_tf32(y, hi[1][t], wh[2], wh[3]);
+#pragma unroll
+                for (int x = 0; x < 4; x++) o[j][i + t][x] += y[x];
+              }
           }
+        } else {
+          const uint32_t vp = saddr(vs) + (k0 + (lane & 7) + (lane >> 4) * 8) * L::kVRow +
+                              ((lane >> 3) & 1) * 16;
+#pragma unroll
+          for (int b = 0; b < kGroups; b++)
+#pragma unroll
+            for (int i = 0; i < kO; i++) {
+              uint32_t x[4];
+              ldsm4t(vp + b * 16 * L::kVRow + i * 32, x);
+#pragma unroll
+              for (int j = 0; j < NT; j++) {
+                mma_bf16(o[j][i], x, pl[j][b][0], pl[j][b][1]);
+                mma_bf16(o[j][i], x, ph[j][b][0], ph[j][b][1]);
+              }
+            }
+        }
       }
     }
 
     // The warps' parts are joined in shared memory, in the last tile's place (tiles
     // behind it may be on their way), kAtOnce tiles of rows at a time: every warp
     // hands over all that it has, and adds up a quarter of the outputs.
-    constexpr int kLane = 4 * kQ + 4;  // values a lane hands over per tile of rows
+    constexpr int kLane = 4 * kO + 4;  // values a lane hands over per tile of rows
     constexpr int kFits = L::kStage / (kOwnWarps * 32 * kLane * 4);
     constexpr int kAtOnce = kFits < NT ? kFits : NT, kApart = 32 * kOwnWarps;
     static_assert(kAtOnce > 0, "a tile of rows fits");
@@ -1329,7 +1450,7 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 2) k_own(sg::BatchArgs a) {
       for (int j = j0; j < j0 + kAtOnce && j < NT; j++) {
         float* p = x + (j - j0) * kLane * kApart + threadIdx.x;
 #pragma unroll
-        for (int i = 0; i < kQ; i++)
+        for (int i = 0; i < kO; i++)
 #pragma unroll
           for (int e = 0; e < 4; e++, p += kApart) *p = o[j][i][e];
 #pragma unroll
@@ -1344,34 +1465,52 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 2) k_own(sg::BatchArgs a) {
 #pragma unroll
       for (int j = j0; j < j0 + kAtOnce && j < NT; j++) {
         const float* const p = x + (j - j0) * kLane * kApart + lane;
-        float f[2][kOwnWarps];
+        float f[2][kSide];
         float* to[2];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-          const float* const ml = p + (4 * kQ + 2 * e) * kApart;
+          const float* const ml = p + (4 * kO + 2 * e) * kApart;
           float top = -INFINITY, sum = 0.f;
 #pragma unroll
-          for (int w = 0; w < kOwnWarps; w++) top = fmaxf(top, ml[32 * w]);
+          for (int w = 0; w < kSide; w++) top = fmaxf(top, ml[32 * w]);
 #pragma unroll
-          for (int w = 0; w < kOwnWarps; w++) {
+          for (int w = 0; w < kSide; w++) {
             f[e][w] = top == -INFINITY ? 0.f : ex2(ml[32 * w] - top);
             sum += f[e][w] * ml[kApart + 32 * w];
           }
           const int r = r0 + 8 * j + 2 * c4 + e;
           const size_t at_row = r < R ? walk.part(a, rows_of, head, parts, r) : 0;
-          to[e] = r < R ? a.part + at_row * HD + g8 : nullptr;
+          to[e] = r < R ? a.part + at_row * HD : nullptr;
           if (r < R && g8 == 0 && warp == 0) a.ml[at_row] = make_float2(top, sum);
         }
+        auto sum_of = [&](int e, int value, int from) {  // of warps `from` on
+          const float* const v = p + value * kApart + 32 * from;
+          float y = 0.f;
 #pragma unroll
-        for (int u = 0; u < 2 * kQ; u += kOwnWarps) {
-          const int of = u + warp;  // outputs 8 of + g8
+          for (int w = 0; w < kSide; w++) y = fmaf(f[e][w], v[32 * w], y);
+          return y;
+        };
+        if constexpr (kF32) {
+          // 32 entries, four to a lane.
+          if (warp < HD / 32) {
+            const int from = warp / (kO / 2) * kSide, i = warp % (kO / 2) * 8;
 #pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const float* const v = p + (of / 2 * 4 + of % 2 * 2 + e) * kApart;
-            float y = 0.f;
+            for (int e = 0; e < 2; e++) {
+              const float4 y =
+                  make_float4(sum_of(e, i + e, from), sum_of(e, i + 2 + e, from),
+                              sum_of(e, i + 4 + e, from), sum_of(e, i + 6 + e, from));
+              if (to[e]) *reinterpret_cast<float4*>(to[e] + 32 * warp + 4 * g8) = y;
+            }
+          }
+        } else {
 #pragma unroll
-            for (int w = 0; w < kOwnWarps; w++) y = fmaf(f[e][w], v[32 * w], y);
-            if (to[e]) to[e][8 * of] = y;
+          for (int u = 0; u < 2 * kO; u += kOwnWarps) {
+            const int of = u + warp;  // outputs 8 of + g8
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              const float y = sum_of(e, of / 2 * 4 + of % 2 * 2 + e, 0);
+              if (to[e]) to[e][8 * of + g8] = y;
+            }
           }
         }
       }
@@ -1644,6 +1783,9 @@ Shape shape_of(int rows) {
   return {8, 1};
 }
 
+// Whether fp32 rows go to k_tree_few.
+bool few_rows(int hd, int rows) { return hd == kFewHeadDim && rows <= kFewRows; }
+
 // Whether the cached keys go to tcgen05 (attn_tree_tc.cu): where mma.sync, not
 // the cache's bytes, is what bounds this file's kernel. Measured with 8 kv
 // heads, us here / there:
@@ -1658,8 +1800,8 @@ bool on_tc(int t, int group, int hd) {
   return t <= 256 && hd >= 64 && t * group > (hd == 128 ? 16 : 32);
 }
 
-// Tiles of eight rows of k_own that take a request's `rows`; 0: k_tree takes them.
-// Measured with 8 kv heads behind a prefix of 64 rows, us of a call with k_own /
+// Tiles of eight rows of k_own that take a request's `rows`; 0: k_tree (or k_tree_few)
+// takes them. Measured with 8 kv heads behind a prefix of 64 rows, us of a call with k_own /
 // k_tree, for 48 requests of 1000 rows, 8 of 4000 and 16 of 200:
 //   head_dim 128,  4 rows: 49 / 57, 36 / 42, 13.3 / 15.8
 //                 16 rows: 60 / 61, 44 / 45, 18.7 / 18.4
@@ -1670,8 +1812,16 @@ bool on_tc(int t, int group, int hd) {
 //   head_dim 32,  32 rows: 42 / 48, 29 / 33, 20.5 / 18.2
 //                 48 rows: 57 / 73, 38 / 48, 20.7 / 16.6
 // (k_tree takes 48 rows as 64.) Where neither is always ahead, it goes by the longer
-// ones.
-int own_tiles(int hd, int rows) {
+// ones. fp32, k_own / k_tree or (128 entries, 4 rows) k_tree_few:
+//   head_dim 128,  4 rows: 111 / 105, 87 / 79, 16.9 / 17.9
+//                  8 rows: 115 / 141, 86 / 105, 20.0 / 22.4
+//                 16 rows: 146 / 145, 111 / 109, 23.1 / 25.4
+//   head_dim 64,   8 rows: 61 / 73, 45 / 54, 15.3 / 17.3
+//                 16 rows: 72 / 73, 56 / 56, 17.5 / 17.8
+//   head_dim 32,   8 rows: 44 / 53, 29 / 36, 13.0 / 13.7
+//                 16 rows: 52 / 52, 37 / 37, 15.7 / 15.6
+int own_tiles(int hd, bool f32, int rows) {
+  if (f32) return rows > 8 || few_rows(hd, rows) ? 0 : 1;
   if (rows <= 8) return 1;
   if (rows <= 16) return 2;
   if (rows <= 32) return hd == 32 ? 4 : 0;
@@ -1679,8 +1829,8 @@ int own_tiles(int hd, int rows) {
 }
 // Rows of a tile of requests' rows.
 int own_rows(int hd, bool f32, int rows) {
-  if (f32 && hd == kFewHeadDim && rows <= kFewRows) return kFewRows;
-  const int tiles = f32 ? 0 : own_tiles(hd, rows);
+  if (f32 && few_rows(hd, rows)) return kFewRows;
+  const int tiles = own_tiles(hd, f32, rows);
   return tiles ? 8 * tiles : 16 * shape_of(rows).mw;
 }
 
@@ -1729,10 +1879,10 @@ cudaError_t launch_shape(const Args& a, int dev, cudaStream_t s) {
 
 // This file's kernels for `rows` rows of a kv head (of a tree, of a request);
 // *keys: of a tile of theirs.
-template <typename T, int HD, typename Args>
-cudaError_t launch_mma(const Args& a, int rows, int* keys, int dev, cudaStream_t s) {
+template <typename T, int HD>
+cudaError_t launch_mma(const TreeArgs& a, int rows, int* keys, int dev, cudaStream_t s) {
   if constexpr (sizeof(T) == 4 && HD == kFewHeadDim)
-    if (rows <= kFewRows) {
+    if (few_rows(HD, rows)) {
       *keys = Tile<float, HD, kFewWarps>::kKeys;
       return launch_few(a, dev, s);
     }
@@ -1762,31 +1912,35 @@ cudaError_t launch_hd(const TreeArgs& a, int dev, cudaStream_t s) {
   return sg::try_launch(k_merge<T, HD, false>, rows, dim3(kMergeThreads), 0, 1, s, a, keys);
 }
 
-template <int HD, int NT>
+template <typename T, int HD, int NT>
 cudaError_t launch_own_as(const sg::BatchArgs& a, int dev, cudaStream_t s) {
   static std::atomic<size_t> allowed[sg::kDevices];
-  constexpr size_t bytes = Tile<uint16_t, HD, kOwnWarps>::kBytes;
-  const cudaError_t e = sg::allow_smem(k_own<HD, NT>, bytes, dev, allowed);
+  constexpr size_t bytes = Tile<T, HD, kOwnWarps>::kBytes;
+  const cudaError_t e = sg::allow_smem(k_own<T, HD, NT>, bytes, dev, allowed);
   if (e != cudaSuccess) return e;
-  return sg::try_launch(k_own<HD, NT>, dim3(a.ctas), dim3(32 * kOwnWarps), bytes, 1, s, a);
+  return sg::try_launch(k_own<T, HD, NT>, dim3(a.ctas), dim3(32 * kOwnWarps), bytes, 1, s, a);
 }
 
 // A batch's own tiles.
 template <typename T, int HD>
 cudaError_t launch_own(const sg::BatchArgs& a, int dev, cudaStream_t s) {
-  const int rows = a.most * a.group;
-  if constexpr (sizeof(T) == 2) {
-    switch (own_tiles(HD, rows)) {
-      case 1: return launch_own_as<HD, 1>(a, dev, s);
-      case 2: return launch_own_as<HD, 2>(a, dev, s);
-    }
-    if constexpr (HD == 32)
-      if (own_tiles(HD, rows) == 4) return launch_own_as<HD, 4>(a, dev, s);
-    if constexpr (HD < 128)
-      if (own_tiles(HD, rows) == 6) return launch_own_as<HD, 6>(a, dev, s);
+  const int rows = a.most * a.group, tiles = own_tiles(HD, sizeof(T) == 4, rows);
+  if (tiles == 1) return launch_own_as<T, HD, 1>(a, dev, s);
+  if constexpr (sizeof(T) == 2)
+    if (tiles == 2) return launch_own_as<T, HD, 2>(a, dev, s);
+  if constexpr (sizeof(T) == 2 && HD == 32)
+    if (tiles == 4) return launch_own_as<T, HD, 4>(a, dev, s);
+  if constexpr (sizeof(T) == 2 && HD < 128)
+    if (tiles == 6) return launch_own_as<T, HD, 6>(a, dev, s);
+  const int mw = shape_of(rows).mw;
+  if constexpr (sizeof(T) == 4) {
+    if constexpr (HD == kFewHeadDim)
+      if (few_rows(HD, rows)) return launch_few(a, dev, s);
+    if (mw == 1) return launch_shape<T, HD, 1, 4>(a, dev, s);
   }
-  int none = 0;
-  return launch_mma<T, HD>(a, rows, &none, dev, s);
+  if constexpr (sizeof(T) == 4 || HD > 32)
+    if (mw == 2) return launch_shape<T, HD, 2, 2>(a, dev, s);
+  return mw == 4 ? launch_shape<T, HD, 4, 1>(a, dev, s) : launch_shape<T, HD, 8, 1>(a, dev, s);
 }
 
 // Behind a shared prefix: parts of the prefix for all rows, parts of each
@@ -1863,7 +2017,7 @@ Batch batch_of(int sms, int type, int t, int tokens, int kh, int group, int hd) 
   }
   // As many CTAs as an SM takes (k_own has four warps).
   const Shape s = shape_of(t * group);
-  const bool own = type == STRASGPT_BF16 && own_tiles(hd, t * group) > 0;
+  const bool own = own_tiles(hd, type == STRASGPT_F32, t * group) > 0;
   b.ctas = sms * (own || s.mw * s.kw <= kOwnWarps ? 2 : 1);
   b.parts = (b.splits + 1) * rows + (size_t)b.ctas * own_rows(hd, type == STRASGPT_F32, t * group);
   b.where = b.parts * (hd + 2) * sizeof(float);
