@@ -153,6 +153,60 @@ def test_rows_nobody_sees_may_hold_anything(cuda, type_, g, most):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("type_", [F32, BF16])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("g,most", [(1, 8), (8, 1), (5, 3), (16, 2), (8, 6), (3, 21), (1, 130)])
+def test_hidden_new_rows_may_hold_anything(cuda, type_, hd, g, most):
+    """Every size of a request's rows: NaN and infinities in all new rows but the first
+    token's, which alone is looked at then, and behind the rows."""
+    torch = cuda
+    b = Batch(torch, 2, g, hd, 40, [most] * 3, [most, most + 64, most + 131], type_, hd + g)
+    b.run()
+    b.check()
+    clean = b.att.clone()
+    for r, n in enumerate(b.rows):
+        b.k[r, :, n:], b.v[r, :, n:] = float("nan"), float("inf")
+    b.run()
+    assert torch.equal(b.att, clean)
+    for r, n in enumerate(b.rows):
+        b.v[r, :, n - most + 1:] = torch.tensor([float("inf"), float("nan")] * (hd // 2)).to(b.v)
+        b.k[r, :, n - most + 1:] = float("nan")
+    b.run()
+    b.v[:] = torch.nan_to_num(b.v, 0.0, 0.0, 0.0)
+    got = b.att[0::most].clone()
+    b.att.copy_(clean)
+    b.att[0::most] = got
+    for r, n in enumerate(b.rows):     # what the first tokens see is as it was
+        own = n - most + 1
+        for x in (b.k, b.v):
+            assert torch.isfinite(x[r, :, :own]).all()
+    b.new, first = [1] * 3, b.first
+    b.first, b.rows = first[:-1], [n - most + 1 for n in b.rows]
+    b.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [F32, BF16])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("g,most", [(4, 1), (8, 1), (4, 4), (8, 6), (4, 20)])
+@pytest.mark.parametrize("way", [1, -1])
+def test_scores_that_rise_and_fall(cuda, type_, hd, g, most, way):
+    """Scores that climb (or fall) along the keys, slowly and by more than any weight's
+    range: maxima that move all the time, and such as never do."""
+    torch = cuda
+    b = Batch(torch, 2, g, hd, 333, [most] * 4, [most + 500, most + 37, most, most + 200], type_, 6)
+    q = torch.randn(hd, device="cuda")
+    b.q[:] = (q + 0.1 * torch.randn_like(b.q.float())).to(b.q)
+    def slope(n):
+        return way * torch.linspace(-4, 4, n, device="cuda")[:, None]
+    unit = q / q.norm() ** 2 * math.sqrt(hd) * 12
+    b.kp[:] = (slope(b.kp.shape[1]) * unit + 0.05 * torch.randn_like(b.kp.float())).to(b.kp)
+    b.k[:] = (slope(b.k.shape[2]) * unit + 0.05 * torch.randn_like(b.k.float())).to(b.k)
+    b.run()
+    b.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [F32, BF16])
 def test_equal_counts_need_no_first_in_place(cuda, type_):
     torch = cuda
     b = Batch(torch, 2, 4, 128, 500, [3] * 9, [3, 4, 100, 65, 64, 63, 7, 30, 300], type_, 7)

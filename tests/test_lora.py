@@ -157,6 +157,33 @@ def test_strides_no_base_no_scale_in_place(cuda, type_, odd):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("type_", [F32, BF16])
+@pytest.mark.parametrize("m,k,n,r", [(257, 72, 65, 8), (1000, 200, 190, 72), (9000, 64, 34, 8)])
+@pytest.mark.parametrize("epi", [STORE, ADD, SWIGLU])
+def test_many_tokens_within_wider_rows(cuda, type_, m, k, n, r, epi):
+    """Many tokens, whose rows of base and out are off 16 bytes and lie in wider ones;
+    runs of adapters, and more tokens than one look at the adapters takes."""
+    torch = cuda
+    n += n % 2 if epi == SWIGLU else 0
+    x, a, b, adapter, scale, base = inputs(torch, m, k, n, r, 5, type_, m)
+    adapter[m // 4:m // 2] = 3
+    adapter[m // 2:m // 2 + 130] = -1
+    wide_x = torch.full((m, k + 48), float("nan"), device="cuda").to(x.dtype)
+    wide_x[:, 16:16 + k] = x
+    wide_b = torch.full((m, n + 11), float("nan"), device="cuda").to(x.dtype)
+    wide_b[:, 5:5 + n] = base
+    outs = n // 2 if epi == SWIGLU else n
+    wide = torch.randn(m, outs + 9, device="cuda").to(x.dtype)
+    before = wide.clone()
+    want, err = reference(torch, x, a, b, adapter, scale, base, wide[:, 3:3 + outs], epi, type_)
+    assert call(torch, wide_x[:, 16:16 + k], a, b, adapter, scale, wide_b[:, 5:5 + n],
+                wide[:, 3:3 + outs], epi, type_) == 0
+    assert ((wide[:, 3:3 + outs].double() - want).abs() <= err).all()
+    assert torch.equal(wide[:, :3], before[:, :3])
+    assert torch.equal(wide[:, 3 + outs:], before[:, 3 + outs:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [F32, BF16])
 @pytest.mark.parametrize("m", [5, 200, 900])
 def test_other_tokens_rows_and_adapters_stay_out(cuda, type_, m):
     """Infinities and NaN in one token's row, in an adapter that others do not
