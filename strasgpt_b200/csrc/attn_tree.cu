@@ -1687,53 +1687,57 @@ template <typename T, int HD, int WARPS>
 __global__ void __launch_bounds__(32 * kJoinWarps) k_join(JoinArgs a, int keys_per_tile) {
   constexpr int V = HD / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part_of = warp % WARPS;
-  const size_t all = (size_t)a.t * a.group;
-  const long long row = (long long)blockIdx.x * (kJoinWarps / WARPS) + warp / WARPS;
+  // (Rows are fewer than 2^31; parts that a GPU's memory holds, than 2^32.)
+  const unsigned all = (unsigned)a.t * a.group, rows = all * a.kh;
+  const unsigned row = blockIdx.x * (kJoinWarps / WARPS) + warp / WARPS;
+  const unsigned head = row / all, r = row - head * all;
+  const int tok = (int)(r / (unsigned)a.group);
   sg::pdl_trigger();
   sg::pdl_wait();
-  const int head = (int)(row / all), r = (int)(row - head * all), tok = r / a.group;
-  const bool in = head < a.kh && (a.first ? tok >= a.first[0] && tok < a.first[a.requests]
-                                          : tok < (long long)a.requests * a.most);
+  const bool in = row < rows && (a.first ? tok >= a.first[0] && tok < a.first[a.requests]
+                                         : tok < (long long)a.requests * a.most);
   if (WARPS == 1 && !in) return;
   float m = -INFINITY, l = 0.f, o[V];
 #pragma unroll
   for (int i = 0; i < V; i++) o[i] = 0.f;
   if (in) {
-    const int tiles = (sg::tree_cached(a) + keys_per_tile - 1) / keys_per_tile;
-    const int per = (tiles + a.splits - 1) / a.splits, prefix = tiles ? (tiles + per - 1) / per : 0;
+    const unsigned tiles = (sg::tree_cached(a) + keys_per_tile - 1) / keys_per_tile;
+    const unsigned per = (tiles + a.splits - 1) / a.splits;
+    const int prefix = tiles ? (int)((tiles + per - 1) / per) : 0;
     // (Within the workspace, whatever stands there.)
     const int2 w = a.where[row];
     const int cta = min(max(w.x, 0), a.ctas - 1), place = min(w.y & 127, a.rows - 1);
     const int parts = prefix + min(max(w.y >> 7, 1), a.ctas - cta);
-    auto index = [&](int i) {
-      return i <= prefix ? (size_t)(i < prefix ? i : a.splits) * a.kh * all + row
-                         : (size_t)(a.splits + 1) * a.kh * all +
-                               (size_t)(cta + i - prefix) * a.rows + place;
-    };
     const int share = (parts + WARPS - 1) / WARPS, end = min(parts, (part_of + 1) * share);
     for (int from = part_of * share; from < end; from += 32) {
-      const int n = min(32, end - from);
-      const float2 p = lane < n ? a.ml[index(from + lane)] : make_float2(-INFINITY, 0.f);
+      const int n = min(32, end - from), i = from + lane;  // i: this lane's part
+      const unsigned at = i <= prefix ? (i < prefix ? i : a.splits) * rows + row
+                                      : (a.splits + 1) * rows + (cta + i - prefix) * a.rows + place;
+      const float2 p = lane < n ? a.ml[at] : make_float2(-INFINITY, 0.f);
       const float next = fmaxf(m, sg::warp_max(p.x));
       const float f = next == -INFINITY ? 1.f : exp2f(m - next);
       const float g = next == -INFINITY || p.y == 0.f ? 0.f : exp2f(p.x - next);
       m = next;
       l = l * f + sg::warp_sum(p.y == 0.f ? 0.f : p.y * g);
 #pragma unroll
-      for (int i = 0; i < V; i++) o[i] *= f;
+      for (int v = 0; v < V; v++) o[v] *= f;
 #pragma unroll 4
       for (int j = 0; j < n; j++) {
         const float weight = __shfl_sync(0xFFFFFFFFu, g, j);
-        if (weight == 0.f) continue;  // no keys, or too far below: may hold anything
-        const float* x = a.part + index(from + j) * HD + lane * V;
+        const float* x = a.part + (size_t)__shfl_sync(0xFFFFFFFFu, at, j) * HD + lane * V;
+        float y[V];
         if constexpr (V == 4) {
-          const float4 y = *reinterpret_cast<const float4*>(x);
-          o[0] = fmaf(weight, y.x, o[0]); o[1] = fmaf(weight, y.y, o[1]);
-          o[2] = fmaf(weight, y.z, o[2]); o[3] = fmaf(weight, y.w, o[3]);
+          const float4 z = *reinterpret_cast<const float4*>(x);
+          y[0] = z.x; y[1] = z.y; y[2] = z.z; y[3] = z.w;
+        } else if constexpr (V == 2) {
+          const float2 z = *reinterpret_cast<const float2*>(x);
+          y[0] = z.x; y[1] = z.y;
         } else {
-#pragma unroll
-          for (int i = 0; i < V; i++) o[i] = fmaf(weight, x[i], o[i]);
+          y[0] = *x;
         }
+        // Weight 0: no keys, or too far below; the part may hold anything.
+#pragma unroll
+        for (int v = 0; v < V; v++) o[v] = weight == 0.f ? o[v] : fmaf(weight, y[v], o[v]);
       }
     }
   }
@@ -1763,13 +1767,20 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_join(JoinArgs a, int keys_p
   const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   T* to = static_cast<T*>(a.att) + tok * a.ldo + (size_t)(head * a.group + r - tok * a.group) * HD +
           lane * V;
-  if constexpr (sizeof(T) == 4) {
+  union {
+    T entry[V];
+    std::conditional_t<V * sizeof(T) == 16, uint4,
+        std::conditional_t<V * sizeof(T) == 8, uint2,
+            std::conditional_t<V * sizeof(T) == 4, uint32_t, uint16_t>>> all;
+  } out;
 #pragma unroll
-    for (int i = 0; i < V; i++) to[i] = o[i] * f;
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; i++) asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(to[i]) : "f"(o[i] * f));
+  for (int i = 0; i < V; i++) {
+    if constexpr (sizeof(T) == 4)
+      out.entry[i] = o[i] * f;
+    else
+      asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(out.entry[i]) : "f"(o[i] * f));
   }
+  *reinterpret_cast<decltype(out.all)*>(to) = out.all;
 }
 
 // Rows of a kv head -> warps in rows and in keys.
