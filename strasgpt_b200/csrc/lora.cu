@@ -26,9 +26,9 @@
 //
 // Measured on a B200: 3.8 us for one token of 2048 x 2048, rank 8; 7.7 us for 61
 // tokens, most with one of 48 adapters of rank 16, on 4096 x 6144 (latency: a read of
-// A, the cluster's sums and a read of B, one after the other); 46 us for 2047 fp32
-// tokens of six prompts, rank 32, on 4096 x 4096 (2.2 TB/s); 149 us for 4001 bf16
-// tokens, rank 64, on 4096 x 28672 with SwiGLU (2.6 TB/s). What bounds the last two is
+// A, the cluster's sums and a read of B, one after the other); 47 us for 2047 fp32
+// tokens of six prompts, rank 32, on 4096 x 4096 (2.2 TB/s); 142 us for 4001 bf16
+// tokens, rank 64, on 4096 x 28672 with SwiGLU (2.8 TB/s). What bounds the last two is
 // noted at k_lora_many.
 #include "entry.h"
 
@@ -726,6 +726,30 @@ __device__ __forceinline__ T* entry(uint8_t* row, int r, int e) {
   return reinterpret_cast<T*>(row + (((e / kV) ^ (r & 7)) << 4)) + e % kV;
 }
 
+// A warp reads `outs` entries each of `mine` rows, ld apart, into a swizzled tile. Several
+// rows are on their way at once (287 bf16 tokens on 1672 x 2284, SwiGLU, 42 us one after
+// the other, now 20), and apart from the rows that TMA brings, which need its registers.
+template <typename T>
+__device__ __noinline__ void read_rows(uint8_t* rows, const T* from, long long ld, int mine,
+                                          int outs) {
+  constexpr int kOf = 128 / (int)sizeof(T) / 32, kAtOnce = 16 / kOf;  // entries a lane; rows
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int j0 = 0; j0 < mine; j0 += kAtOnce) {
+    T v[kAtOnce][kOf];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; j++)
+#pragma unroll
+      for (int e = 0; e < kOf; e++)
+        v[j][e] = j0 + j < mine && lane + 32 * e < outs ? from[(j0 + j) * ld + lane + 32 * e] : T(0);
+#pragma unroll
+    for (int j = 0; j < kAtOnce; j++)
+#pragma unroll
+      for (int e = 0; e < kOf; e++)
+        if (j0 + j < mine) *entry<T>(rows + (j0 + j) * 128, j0 + j, lane + 32 * e) = v[j][e];
+  }
+}
+
 // Adds 32 entries of a row that lies swizzled in a tile (its first or second 64
 // bytes: bf16; all of it: fp32).
 template <typename T>
@@ -1199,14 +1223,11 @@ __global__ void __launch_bounds__(kManyThreads, P == 1 ? 2 : 1)
           // Rows that TMA cannot read.
           const T* const b = static_cast<const T*>(p.base ? p.base : p.out);
           const long long ld = p.base ? p.ldb : p.ldo;
-          for (int j = 0; j < mine; j++)
-            for (int e = lane; e < outs; e += 32) {
-              const size_t t = (size_t)token0 + 32 * quarter + j;
-              *entry<T>(rows + j * 128, j, e) = b[t * ld + n + e];
-              if (both)
-                *entry<T>(rows + second + j * 128, j, e) =
-                    static_cast<const T*>(p.out)[t * p.ldo + n + e];
-            }
+          const size_t t = (size_t)token0 + 32 * quarter;
+          read_rows(rows, b + t * ld + n, ld, mine, outs);
+          if (both)
+            read_rows(rows + second, static_cast<const T*>(p.out) + t * p.ldo + n, p.ldo, mine,
+                      outs);
           __syncwarp();
         }
         if (d >= 0) {
@@ -1254,7 +1275,7 @@ __global__ void __launch_bounds__(kManyThreads, P == 1 ? 2 : 1)
             for (int c = 0; c < 8; c++)
               *reinterpret_cast<uint4*>(row + 16 * c) = make_uint4(~0u, ~0u, ~0u, ~0u);
           }
-          const int wide = gated ? kCols / 2 : kCols, x = gated ? n / 2 : n;
+          const int x = gated ? n / 2 : n;
           if (mine == 32 && p.out_tma) {
             fence_async();
             __syncwarp();
@@ -1264,9 +1285,11 @@ __global__ void __launch_bounds__(kManyThreads, P == 1 ? 2 : 1)
           } else {
             __syncwarp();
             const int last = gated ? outs / 2 : outs;
+#pragma unroll 4
             for (int j = 0; j < mine; j++) {
               T* const to = static_cast<T*>(p.out) + ((size_t)token0 + 32 * quarter + j) * p.ldo + x;
-              for (int e = lane; e < wide; e += 32)
+#pragma unroll
+              for (int e = lane; e < kCols; e += 32)
                 if (e < last)
                   to[e] = gated ? reinterpret_cast<const T*>(
                                       rows + j * 64 + (((e / kV) ^ ((j >> 1) & 3)) << 4))[e % kV]
