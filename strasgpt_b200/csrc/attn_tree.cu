@@ -2015,10 +2015,11 @@ Batch batch_of(int sms, int type, int t, int tokens, int kh, int group, int hd) 
   if (tc) {
     // One CTA to an SM: whole rounds of them, in units of a tile's time, for a
     // prefix of 128 tiles (its length is not known here); a CTA's start and end cost
-    // as much as six.
+    // as much as six. (16 splits at most: one kv head, 93 fp32 rows of 64 entries over 64543,
+    // 115 us, now 37.)
     const long long units = (long long)kh * ((tokens * group + sg::kTreeTcRows - 1) / sg::kTreeTcRows);
     double best = 1e30;
-    for (int n = 1; n <= 16; n++) {
+    for (int n = 1; n <= kMaxSplits; n++) {
       const double cost = (double)((units * n + sms - 1) / sms) * (128.0 / n + 6);
       if (cost < best) {
         best = cost;
