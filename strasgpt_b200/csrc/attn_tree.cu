@@ -31,10 +31,10 @@
 // rows by tiles of keys, are shared out evenly over as many CTAs as the GPU holds,
 // which start as the prefix's leave room; k_join adds up both. Measured, 8 kv heads:
 // 64 requests of four heads of 128 bf16 entries, up to 1021 rows each behind 32768,
-// 90 us (prefix 47, own rows 41, alone: 4.9 TB/s; join 11); 48 in fp32, 700 behind
-// 8191, 107 us (50, 58, 8); 31 requests with up to six drafted tokens of eight heads of
-// 64 bf16 entries, 2000 behind 16001, 117 us (66, 57, 10); 16 prompts of up to 96
-// tokens behind 8192 rows 210 us (173, 32, 27); two requests behind 613 rows 11 us.
+// 90 us (prefix 47, own rows 41, alone: 4.9 TB/s; join 10); 48 in fp32, 700 behind
+// 8191, 107 us (50, 58, 7); 31 requests with up to six drafted tokens of eight heads of
+// 64 bf16 entries, 2000 behind 16001, 117 us (66, 57, 9); 16 prompts of up to 96
+// tokens behind 8192 rows 205 us (172, 32, 21); two requests behind 613 rows 10 us.
 #include "attn_tree.h"
 
 #include <limits.h>
@@ -442,7 +442,8 @@ struct Stream {
   }
   __device__ int parts(int i) const { return s.notes[i % kNotes].parts; }
   // Where the part of row r of these lies; the first run notes who goes on.
-  __device__ size_t part(const sg::BatchArgs& a, const Rows& rows, int head, int parts, int r) const {
+  __device__ size_t part(const sg::BatchArgs& a, const Rows& rows, int head, int parts,
+                         int r) const {
     const size_t all = (size_t)a.t * a.group, row = head * all + (size_t)rows.token0 * a.group + r;
     if (!parts) return (a.split0 + 1) * a.kh * all + (size_t)blockIdx.x * ROWS + (r - rows.r0);
     a.where[row] = make_int2(blockIdx.x, parts * 128 + r - rows.r0);
@@ -494,393 +495,393 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Args
 
   int at = 0;  // tiles gone through
   do {
-  const Rows rows_of = walk.rows(at);
-  const int head = walk.head(at), R = rows_of.t * a.group, r0 = rows_of.r0;
-  const int parts = walk.parts(at);
-  // This lane's rows g8 and g8 + 8 of the warp's 16.
-  const int rA = r0 + 16 * mw + g8, rB = rA + 8;
-  const int tA = rA / a.group, tB = rB / a.group;
-  const bool inA = rA < R, inB = rB < R;
-  const T* qA = static_cast<const T*>(a.q) + (rows_of.token0 + (inA ? tA : 0)) * a.ldq +
-                (size_t)(head * a.group + (inA ? rA - tA * a.group : 0)) * HD;
-  const T* qB = static_cast<const T*>(a.q) + (rows_of.token0 + (inB ? tB : 0)) * a.ldq +
-                (size_t)(head * a.group + (inB ? rB - tB * a.group : 0)) * HD;
-  // Scores in units of log2, so that the softmax is exp2.
-  const float scale = 1.4426950408889634f / sqrtf((float)HD);
+    const Rows rows_of = walk.rows(at);
+    const int head = walk.head(at), R = rows_of.t * a.group, r0 = rows_of.r0;
+    const int parts = walk.parts(at);
+    // This lane's rows g8 and g8 + 8 of the warp's 16.
+    const int rA = r0 + 16 * mw + g8, rB = rA + 8;
+    const int tA = rA / a.group, tB = rB / a.group;
+    const bool inA = rA < R, inB = rB < R;
+    const T* qA = static_cast<const T*>(a.q) + (rows_of.token0 + (inA ? tA : 0)) * a.ldq +
+                  (size_t)(head * a.group + (inA ? rA - tA * a.group : 0)) * HD;
+    const T* qB = static_cast<const T*>(a.q) + (rows_of.token0 + (inB ? tB : 0)) * a.ldq +
+                  (size_t)(head * a.group + (inB ? rB - tB * a.group : 0)) * HD;
+    // Scores in units of log2, so that the softmax is exp2.
+    const float scale = 1.4426950408889634f / sqrtf((float)HD);
 
-  // Queries as A operands. fp32: raw values, 16 entries of the head per step;
-  // slots (c, c + 4) of its two k8 steps hold entries 4c, 4c+1 and 4c+2, 4c+3
-  // (keys are read in the same order, so one float4 feeds both steps).
-  // bf16: the fragment of m16n8k16.
-  constexpr int kQ = HD / 16;
-  float4 q4[kF32 ? kQ : 1][2];
-  uint32_t q16[kF32 ? 1 : kQ][4];
+    // Queries as A operands. fp32: raw values, 16 entries of the head per step;
+    // slots (c, c + 4) of its two k8 steps hold entries 4c, 4c+1 and 4c+2, 4c+3
+    // (keys are read in the same order, so one float4 feeds both steps).
+    // bf16: the fragment of m16n8k16.
+    constexpr int kQ = HD / 16;
+    float4 q4[kF32 ? kQ : 1][2];
+    uint32_t q16[kF32 ? 1 : kQ][4];
 #pragma unroll
-  for (int j = 0; j < kQ; j++) {
-    if constexpr (kF32) {
-      auto load = [&](const T* p, bool in) {
-        float4 v = *reinterpret_cast<const float4*>(p + 16 * j + 4 * c4);
-        return in ? make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale)
-                  : make_float4(0.f, 0.f, 0.f, 0.f);
-      };
-      q4[j][0] = load(qA, inA);
-      q4[j][1] = load(qB, inB);
-    } else {
-      auto load = [&](const T* p, bool in, int at) {
-        return in ? *reinterpret_cast<const uint32_t*>(p + 16 * j + at) : 0u;
-      };
-      q16[j][0] = load(qA, inA, 2 * c4);
-      q16[j][1] = load(qB, inB, 2 * c4);
-      q16[j][2] = load(qA, inA, 2 * c4 + 8);
-      q16[j][3] = load(qB, inB, 2 * c4 + 8);
-    }
-  }
-
-  // Output accumulators. fp32: n8 tile 4b + i holds head entries
-  // 32b + 4 column + i (one float4 of a value row feeds four tiles).
-  float o[kOut][4];
-#pragma unroll
-  for (int i = 0; i < kOut; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float mA = -INFINITY, mB = -INFINITY, lA = 0.f, lB = 0.f;
-
-  for (bool more = true; more; at++) {
-    cp_async_wait<kStages - 2>();
-    __syncthreads();
-    walk.fetch(at + kStages - 1);  // into the buffer that the last tile left
-    int rows, first;
-    walk.keys(at, rows, first);
-    more = !walk.last(at);
-    const bool old = first < 0;
-    const unsigned char* ks = smem + at % kStages * L::kStage;
-    const unsigned char* vs = ks + kKeys * L::kKRow;
-    // A drafted value row with an infinity or NaN may be hidden from some of
-    // the rows: 0 * NaN in a matrix instruction would reach them. Such a tile
-    // takes the slow product below. (Cached rows are seen by all.)
-    bool slow = false;
-    if (!old) {
-      bool bad = false;
-      constexpr int kVecs = HD * (int)sizeof(T) / 16;
-      for (int i = threadIdx.x; i < kKeys * kVecs; i += kThreads) {
-        const unsigned char* p = vs + i / kVecs * L::kVRow + i % kVecs * 16;
-        if constexpr (kF32)
-          bad = bad || !finite4(*reinterpret_cast<const float4*>(p));
-        else
-          bad = bad || !finite_bf16x8(*reinterpret_cast<const uint4*>(p));
+    for (int j = 0; j < kQ; j++) {
+      if constexpr (kF32) {
+        auto load = [&](const T* p, bool in) {
+          float4 v = *reinterpret_cast<const float4*>(p + 16 * j + 4 * c4);
+          return in ? make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale)
+                    : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
+        q4[j][0] = load(qA, inA);
+        q4[j][1] = load(qB, inB);
+      } else {
+        auto load = [&](const T* p, bool in, int at) {
+          return in ? *reinterpret_cast<const uint32_t*>(p + 16 * j + at) : 0u;
+        };
+        q16[j][0] = load(qA, inA, 2 * c4);
+        q16[j][1] = load(qB, inB, 2 * c4);
+        q16[j][2] = load(qA, inA, 2 * c4 + 8);
+        q16[j][3] = load(qB, inB, 2 * c4 + 8);
       }
-      slow = __syncthreads_or(bad);
     }
+
+    // Output accumulators. fp32: n8 tile 4b + i holds head entries
+    // 32b + 4 column + i (one float4 of a value row feeds four tiles).
+    float o[kOut][4];
+#pragma unroll
+    for (int i = 0; i < kOut; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float mA = -INFINITY, mB = -INFINITY, lA = 0.f, lB = 0.f;
+
+    for (bool more = true; more; at++) {
+      cp_async_wait<kStages - 2>();
+      __syncthreads();
+      walk.fetch(at + kStages - 1);  // into the buffer that the last tile left
+      int rows, first;
+      walk.keys(at, rows, first);
+      more = !walk.last(at);
+      const bool old = first < 0;
+      const unsigned char* ks = smem + at % kStages * L::kStage;
+      const unsigned char* vs = ks + kKeys * L::kKRow;
+      // A drafted value row with an infinity or NaN may be hidden from some of
+      // the rows: 0 * NaN in a matrix instruction would reach them. Such a tile
+      // takes the slow product below. (Cached rows are seen by all.)
+      bool slow = false;
+      if (!old) {
+        bool bad = false;
+        constexpr int kVecs = HD * (int)sizeof(T) / 16;
+        for (int i = threadIdx.x; i < kKeys * kVecs; i += kThreads) {
+          const unsigned char* p = vs + i / kVecs * L::kVRow + i % kVecs * 16;
+          if constexpr (kF32)
+            bad = bad || !finite4(*reinterpret_cast<const float4*>(p));
+          else
+            bad = bad || !finite_bf16x8(*reinterpret_cast<const uint4*>(p));
+        }
+        slow = __syncthreads_or(bad);
+      }
 
 #pragma unroll 1
-    for (int ch = 0; ch < kWarpKeys; ch += kChunk) {
-      const int k0 = kw * kWarpKeys + ch;  // first key of the chunk in the tile
-      if (k0 >= rows) break;
-      float s[kN8][4];
+      for (int ch = 0; ch < kWarpKeys; ch += kChunk) {
+        const int k0 = kw * kWarpKeys + ch;  // first key of the chunk in the tile
+        if (k0 >= rows) break;
+        float s[kN8][4];
 #pragma unroll
-      for (int i = 0; i < kN8; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
-      if constexpr (kF32) {
-        // The tensor cores cut their sums: 16 entries at a time from zero,
-        // small products first, then added with rounding.
-        const unsigned char* kp = ks + (k0 + g8) * L::kKRow + c4 * 16;
+        for (int i = 0; i < kN8; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+        if constexpr (kF32) {
+          // The tensor cores cut their sums: 16 entries at a time from zero,
+          // small products first, then added with rounding.
+          const unsigned char* kp = ks + (k0 + g8) * L::kKRow + c4 * 16;
 #pragma unroll
-        for (int j = 0; j < kQ; j++) {
-          uint32_t ah[2][4], al[2][4];
-          split_tf32(q4[j][0].x, ah[0][0], al[0][0]);
-          split_tf32(q4[j][1].x, ah[0][1], al[0][1]);
-          split_tf32(q4[j][0].y, ah[0][2], al[0][2]);
-          split_tf32(q4[j][1].y, ah[0][3], al[0][3]);
-          split_tf32(q4[j][0].z, ah[1][0], al[1][0]);
-          split_tf32(q4[j][1].z, ah[1][1], al[1][1]);
-          split_tf32(q4[j][0].w, ah[1][2], al[1][2]);
-          split_tf32(q4[j][1].w, ah[1][3], al[1][3]);
+          for (int j = 0; j < kQ; j++) {
+            uint32_t ah[2][4], al[2][4];
+            split_tf32(q4[j][0].x, ah[0][0], al[0][0]);
+            split_tf32(q4[j][1].x, ah[0][1], al[0][1]);
+            split_tf32(q4[j][0].y, ah[0][2], al[0][2]);
+            split_tf32(q4[j][1].y, ah[0][3], al[0][3]);
+            split_tf32(q4[j][0].z, ah[1][0], al[1][0]);
+            split_tf32(q4[j][1].z, ah[1][1], al[1][1]);
+            split_tf32(q4[j][0].w, ah[1][2], al[1][2]);
+            split_tf32(q4[j][1].w, ah[1][3], al[1][3]);
 #pragma unroll
-          for (int i = 0; i < kN8; i++) {
-            const float4 kv = *reinterpret_cast<const float4*>(kp + i * 8 * L::kKRow + j * 64);
-            uint32_t bh[4], bl[4];
-            split_tf32(kv.x, bh[0], bl[0]);
-            split_tf32(kv.y, bh[1], bl[1]);
-            split_tf32(kv.z, bh[2], bl[2]);
-            split_tf32(kv.w, bh[3], bl[3]);
-            float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_tf32(x, ah[0], bl[0], bl[1]);
-            mma_tf32(y, ah[1], bl[2], bl[3]);
-            mma_tf32(x, al[0], bh[0], bh[1]);
-            mma_tf32(y, al[1], bh[2], bh[3]);
-            mma_tf32(x, ah[0], bh[0], bh[1]);
-            mma_tf32(y, ah[1], bh[2], bh[3]);
+            for (int i = 0; i < kN8; i++) {
+              const float4 kv = *reinterpret_cast<const float4*>(kp + i * 8 * L::kKRow + j * 64);
+              uint32_t bh[4], bl[4];
+              split_tf32(kv.x, bh[0], bl[0]);
+              split_tf32(kv.y, bh[1], bl[1]);
+              split_tf32(kv.z, bh[2], bl[2]);
+              split_tf32(kv.w, bh[3], bl[3]);
+              float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+              mma_tf32(x, ah[0], bl[0], bl[1]);
+              mma_tf32(y, ah[1], bl[2], bl[3]);
+              mma_tf32(x, al[0], bh[0], bh[1]);
+              mma_tf32(y, al[1], bh[2], bh[3]);
+              mma_tf32(x, ah[0], bh[0], bh[1]);
+              mma_tf32(y, ah[1], bh[2], bh[3]);
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[i][e] += x[e] + y[e];
+              for (int e = 0; e < 4; e++) s[i][e] += x[e] + y[e];
+            }
           }
-        }
-      } else {
-        const uint32_t kp = saddr(ks) + (k0 + (lane & 7) + (lane >> 4) * 8) * L::kKRow +
-                            ((lane >> 3) & 1) * 16;
+        } else {
+          const uint32_t kp = saddr(ks) + (k0 + (lane & 7) + (lane >> 4) * 8) * L::kKRow +
+                              ((lane >> 3) & 1) * 16;
 #pragma unroll
-        for (int j = 0; j < kQ; j++)
+          for (int j = 0; j < kQ; j++)
 #pragma unroll
-          for (int i = 0; i < kN8; i += 2) {
-            uint32_t b[4];
-            ldsm4(kp + i * 8 * L::kKRow + j * 32, b);
-            mma_bf16(s[i], q16[j], b[0], b[1]);
-            mma_bf16(s[i + 1], q16[j], b[2], b[3]);
-          }
-#pragma unroll
-        for (int i = 0; i < kN8; i++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) s[i][e] *= scale;
-      }
-
-      // What the rows may see: all cached keys, or the mask's bits.
-      if (!old) {
-        const int j0 = first + k0;  // drafted index, a multiple of 8
-        const u64 wA = inA ? seen_of(a, rows_of, tA, j0) : 0;
-        const u64 wB = inB ? seen_of(a, rows_of, tB, j0) : 0;
-#pragma unroll
-        for (int i = 0; i < kN8; i++)
-#pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const int j = 8 * i + 2 * c4 + e;
-            const bool in = k0 + j < rows;
-            if (!(in && (wA >> j & 1))) s[i][e] = -INFINITY;
-            if (!(in && (wB >> j & 1))) s[i][2 + e] = -INFINITY;
-          }
-      } else if (k0 + kChunk > rows) {
-#pragma unroll
-        for (int i = 0; i < kN8; i++)
-#pragma unroll
-          for (int e = 0; e < 2; e++)
-            if (k0 + 8 * i + 2 * c4 + e >= rows) s[i][e] = s[i][2 + e] = -INFINITY;
-      }
-
-      // Online softmax; the four lanes of a row share its keys.
-      float xA = -INFINITY, xB = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < kN8; i++) {
-        xA = fmaxf(xA, fmaxf(s[i][0], s[i][1]));
-        xB = fmaxf(xB, fmaxf(s[i][2], s[i][3]));
-      }
-      xA = fmaxf(xA, __shfl_xor_sync(0xFFFFFFFFu, xA, 1));
-      xA = fmaxf(xA, __shfl_xor_sync(0xFFFFFFFFu, xA, 2));
-      xB = fmaxf(xB, __shfl_xor_sync(0xFFFFFFFFu, xB, 1));
-      xB = fmaxf(xB, __shfl_xor_sync(0xFFFFFFFFu, xB, 2));
-      const float nA = fmaxf(mA, xA), nB = fmaxf(mB, xB);
-      if (__any_sync(0xFFFFFFFFu, nA > mA || nB > mB)) {
-        // A row that has seen no key yet keeps m = -inf and zeros.
-        const float fA = nA == -INFINITY ? 1.f : exp2f(mA - nA);
-        const float fB = nB == -INFINITY ? 1.f : exp2f(mB - nB);
-        mA = nA;
-        mB = nB;
-        lA *= fA;
-        lB *= fB;
-#pragma unroll
-        for (int i = 0; i < kOut; i++) {
-          o[i][0] *= fA;
-          o[i][1] *= fA;
-          o[i][2] *= fB;
-          o[i][3] *= fB;
-        }
-      }
-      const float zA = mA == -INFINITY ? 0.f : mA, zB = mB == -INFINITY ? 0.f : mB;
-#pragma unroll
-      for (int i = 0; i < kN8; i++) {
-        s[i][0] = exp2f(s[i][0] - zA);
-        s[i][1] = exp2f(s[i][1] - zA);
-        s[i][2] = exp2f(s[i][2] - zB);
-        s[i][3] = exp2f(s[i][3] - zB);
-        lA += s[i][0] + s[i][1];
-        lB += s[i][2] + s[i][3];
-      }
-
-      if (slow) {
-        // Key by key, weights of exactly 0 left out.
-        for (int kk = 0; kk < kChunk && k0 + kk < rows; kk++) {
-          float pA = 0.f, pB = 0.f;
+            for (int i = 0; i < kN8; i += 2) {
+              uint32_t b[4];
+              ldsm4(kp + i * 8 * L::kKRow + j * 32, b);
+              mma_bf16(s[i], q16[j], b[0], b[1]);
+              mma_bf16(s[i + 1], q16[j], b[2], b[3]);
+            }
 #pragma unroll
           for (int i = 0; i < kN8; i++)
-            if (i == kk / 8) {
-              pA = kk & 1 ? s[i][1] : s[i][0];
-              pB = kk & 1 ? s[i][3] : s[i][2];
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[i][e] *= scale;
+        }
+
+        // What the rows may see: all cached keys, or the mask's bits.
+        if (!old) {
+          const int j0 = first + k0;  // drafted index, a multiple of 8
+          const u64 wA = inA ? seen_of(a, rows_of, tA, j0) : 0;
+          const u64 wB = inB ? seen_of(a, rows_of, tB, j0) : 0;
+#pragma unroll
+          for (int i = 0; i < kN8; i++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              const int j = 8 * i + 2 * c4 + e;
+              const bool in = k0 + j < rows;
+              if (!(in && (wA >> j & 1))) s[i][e] = -INFINITY;
+              if (!(in && (wB >> j & 1))) s[i][2 + e] = -INFINITY;
             }
-          const int from = (lane & ~3) | (kk % 8 / 2);
-          pA = __shfl_sync(0xFFFFFFFFu, pA, from);
-          pB = __shfl_sync(0xFFFFFFFFu, pB, from);
-          const T* vr = reinterpret_cast<const T*>(vs + (k0 + kk) * L::kVRow);
+        } else if (k0 + kChunk > rows) {
+#pragma unroll
+          for (int i = 0; i < kN8; i++)
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+              if (k0 + 8 * i + 2 * c4 + e >= rows) s[i][e] = s[i][2 + e] = -INFINITY;
+        }
+
+        // Online softmax; the four lanes of a row share its keys.
+        float xA = -INFINITY, xB = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kN8; i++) {
+          xA = fmaxf(xA, fmaxf(s[i][0], s[i][1]));
+          xB = fmaxf(xB, fmaxf(s[i][2], s[i][3]));
+        }
+        xA = fmaxf(xA, __shfl_xor_sync(0xFFFFFFFFu, xA, 1));
+        xA = fmaxf(xA, __shfl_xor_sync(0xFFFFFFFFu, xA, 2));
+        xB = fmaxf(xB, __shfl_xor_sync(0xFFFFFFFFu, xB, 1));
+        xB = fmaxf(xB, __shfl_xor_sync(0xFFFFFFFFu, xB, 2));
+        const float nA = fmaxf(mA, xA), nB = fmaxf(mB, xB);
+        if (__any_sync(0xFFFFFFFFu, nA > mA || nB > mB)) {
+          // A row that has seen no key yet keeps m = -inf and zeros.
+          const float fA = nA == -INFINITY ? 1.f : exp2f(mA - nA);
+          const float fB = nB == -INFINITY ? 1.f : exp2f(mB - nB);
+          mA = nA;
+          mB = nB;
+          lA *= fA;
+          lB *= fB;
+#pragma unroll
+          for (int i = 0; i < kOut; i++) {
+            o[i][0] *= fA;
+            o[i][1] *= fA;
+            o[i][2] *= fB;
+            o[i][3] *= fB;
+          }
+        }
+        const float zA = mA == -INFINITY ? 0.f : mA, zB = mB == -INFINITY ? 0.f : mB;
+#pragma unroll
+        for (int i = 0; i < kN8; i++) {
+          s[i][0] = exp2f(s[i][0] - zA);
+          s[i][1] = exp2f(s[i][1] - zA);
+          s[i][2] = exp2f(s[i][2] - zB);
+          s[i][3] = exp2f(s[i][3] - zB);
+          lA += s[i][0] + s[i][1];
+          lB += s[i][2] + s[i][3];
+        }
+
+        if (slow) {
+          // Key by key, weights of exactly 0 left out.
+          for (int kk = 0; kk < kChunk && k0 + kk < rows; kk++) {
+            float pA = 0.f, pB = 0.f;
+#pragma unroll
+            for (int i = 0; i < kN8; i++)
+              if (i == kk / 8) {
+                pA = kk & 1 ? s[i][1] : s[i][0];
+                pB = kk & 1 ? s[i][3] : s[i][2];
+              }
+            const int from = (lane & ~3) | (kk % 8 / 2);
+            pA = __shfl_sync(0xFFFFFFFFu, pA, from);
+            pB = __shfl_sync(0xFFFFFFFFu, pB, from);
+            const T* vr = reinterpret_cast<const T*>(vs + (k0 + kk) * L::kVRow);
+#pragma unroll
+            for (int i = 0; i < kOut; i++)
+#pragma unroll
+              for (int e = 0; e < 2; e++) {
+                float v;
+                if constexpr (kF32)
+                  v = vr[32 * (i / 4) + 4 * (2 * c4 + e) + i % 4];
+                else
+                  v = sg::bf16_to_f32(vr[8 * i + 2 * c4 + e]);
+                if (pA != 0.f) o[i][e] += pA * v;
+                if (pB != 0.f) o[i][2 + e] += pB * v;
+              }
+          }
+          continue;
+        }
+
+        if constexpr (kF32) {
+          // The score accumulators are the A operand as they lie: slots c and
+          // c + 4 of a k8 step are keys 2c and 2c + 1. A chunk's products are
+          // summed from zero and then added, as above.
+          uint32_t ph[kN8][4], pl[kN8][4];
+#pragma unroll
+          for (int i = 0; i < kN8; i++) {
+            split_tf32(s[i][0], ph[i][0], pl[i][0]);
+            split_tf32(s[i][2], ph[i][1], pl[i][1]);
+            split_tf32(s[i][1], ph[i][2], pl[i][2]);
+            split_tf32(s[i][3], ph[i][3], pl[i][3]);
+          }
+          const unsigned char* vp = vs + (k0 + 2 * c4) * L::kVRow + g8 * 16;
+#pragma unroll
+          for (int b = 0; b < HD / 32; b++) {
+            float x[4][4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e][0] = x[e][1] = x[e][2] = x[e][3] = 0.f;
+#pragma unroll
+            for (int i = 0; i < kN8; i++) {
+              const float4 v0 =
+                  *reinterpret_cast<const float4*>(vp + i * 8 * L::kVRow + b * 128);
+              const float4 v1 =
+                  *reinterpret_cast<const float4*>(vp + (i * 8 + 1) * L::kVRow + b * 128);
+              uint32_t h0[4], l0[4], h1[4], l1[4];
+              split_tf32(v0.x, h0[0], l0[0]);
+              split_tf32(v0.y, h0[1], l0[1]);
+              split_tf32(v0.z, h0[2], l0[2]);
+              split_tf32(v0.w, h0[3], l0[3]);
+              split_tf32(v1.x, h1[0], l1[0]);
+              split_tf32(v1.y, h1[1], l1[1]);
+              split_tf32(v1.z, h1[2], l1[2]);
+              split_tf32(v1.w, h1[3], l1[3]);
+#pragma unroll
+              for (int e = 0; e < 4; e++) mma_tf32(x[e], ph[i], l0[e], l1[e]);
+#pragma unroll
+              for (int e = 0; e < 4; e++) mma_tf32(x[e], pl[i], h0[e], h1[e]);
+#pragma unroll
+              for (int e = 0; e < 4; e++) mma_tf32(x[e], ph[i], h0[e], h1[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+              for (int y = 0; y < 4; y++) o[4 * b + e][y] += x[e][y];
+          }
+        } else {
+          const uint32_t vp = saddr(vs) + (k0 + (lane & 7) + ((lane >> 3) & 1) * 8) * L::kVRow +
+                              (lane >> 4) * 16;
+#pragma unroll
+          for (int i = 0; i < kN8; i += 2) {
+            uint32_t ph[4], pl[4];
+            split_bf16(s[i][0], s[i][1], ph[0], pl[0]);
+            split_bf16(s[i][2], s[i][3], ph[1], pl[1]);
+            split_bf16(s[i + 1][0], s[i + 1][1], ph[2], pl[2]);
+            split_bf16(s[i + 1][2], s[i + 1][3], ph[3], pl[3]);
+#pragma unroll
+            for (int b = 0; b < kOut; b += 2) {
+              uint32_t v[4];
+              ldsm4t(vp + i * 8 * L::kVRow + b * 16, v);
+              mma_bf16(o[b], ph, v[0], v[1]);
+              mma_bf16(o[b + 1], ph, v[2], v[3]);
+              mma_bf16(o[b], pl, v[0], v[1]);
+              mma_bf16(o[b + 1], pl, v[2], v[3]);
+            }
+          }
+        }
+      }
+    }
+    if constexpr (!kBatch) cp_async_wait<0>();
+    lA += __shfl_xor_sync(0xFFFFFFFFu, lA, 1);
+    lA += __shfl_xor_sync(0xFFFFFFFFu, lA, 2);
+    lB += __shfl_xor_sync(0xFFFFFFFFu, lB, 1);
+    lB += __shfl_xor_sync(0xFFFFFFFFu, lB, 2);
+
+    // The key warps' parts of the rows are joined in shared memory, warps of
+    // the upper half into the lower one, in the last tile's place (tiles behind it
+    // may be on their way).
+    if constexpr (KW > 1) {
+      constexpr int kLane = kOut * 4 + 4;  // values a lane hands over
+      float* x = reinterpret_cast<float*>(smem + (kBatch ? (at - 1) % kStages * L::kStage : 0));
+      static_assert((size_t)MW * (KW / 2) * 32 * kLane * 4 <= L::kStage, "join fits a tile");
+#pragma unroll
+      for (int half = KW / 2; half > 0; half /= 2) {
+        __syncthreads();
+        // [value][warp][lane]: lanes side by side.
+        if (kw >= half && kw < 2 * half) {
+          float* p = x + ((kw - half) * MW + mw) * 32 + lane;
+          constexpr int kStep = MW * (KW / 2) * 32;
 #pragma unroll
           for (int i = 0; i < kOut; i++)
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-              float v;
-              if constexpr (kF32)
-                v = vr[32 * (i / 4) + 4 * (2 * c4 + e) + i % 4];
-              else
-                v = sg::bf16_to_f32(vr[8 * i + 2 * c4 + e]);
-              if (pA != 0.f) o[i][e] += pA * v;
-              if (pB != 0.f) o[i][2 + e] += pB * v;
-            }
+            for (int e = 0; e < 4; e++) p[(4 * i + e) * kStep] = o[i][e];
+          p[(4 * kOut) * kStep] = mA;
+          p[(4 * kOut + 1) * kStep] = mB;
+          p[(4 * kOut + 2) * kStep] = lA;
+          p[(4 * kOut + 3) * kStep] = lB;
         }
-        continue;
-      }
-
-      if constexpr (kF32) {
-        // The score accumulators are the A operand as they lie: slots c and
-        // c + 4 of a k8 step are keys 2c and 2c + 1. A chunk's products are
-        // summed from zero and then added, as above.
-        uint32_t ph[kN8][4], pl[kN8][4];
+        __syncthreads();
+        if (kw < half) {
+          const float* p = x + (kw * MW + mw) * 32 + lane;
+          constexpr int kStep = MW * (KW / 2) * 32;
+          const float m2A = p[(4 * kOut) * kStep], m2B = p[(4 * kOut + 1) * kStep];
+          const float nA = fmaxf(mA, m2A), nB = fmaxf(mB, m2B);
+          const float fA = nA == -INFINITY ? 0.f : exp2f(mA - nA);
+          const float fB = nB == -INFINITY ? 0.f : exp2f(mB - nB);
+          const float gA = nA == -INFINITY ? 0.f : exp2f(m2A - nA);
+          const float gB = nB == -INFINITY ? 0.f : exp2f(m2B - nB);
+          lA = lA * fA + p[(4 * kOut + 2) * kStep] * gA;
+          lB = lB * fB + p[(4 * kOut + 3) * kStep] * gB;
+          mA = nA;
+          mB = nB;
 #pragma unroll
-        for (int i = 0; i < kN8; i++) {
-          split_tf32(s[i][0], ph[i][0], pl[i][0]);
-          split_tf32(s[i][2], ph[i][1], pl[i][1]);
-          split_tf32(s[i][1], ph[i][2], pl[i][2]);
-          split_tf32(s[i][3], ph[i][3], pl[i][3]);
-        }
-        const unsigned char* vp = vs + (k0 + 2 * c4) * L::kVRow + g8 * 16;
-#pragma unroll
-        for (int b = 0; b < HD / 32; b++) {
-          float x[4][4];
-#pragma unroll
-          for (int e = 0; e < 4; e++) x[e][0] = x[e][1] = x[e][2] = x[e][3] = 0.f;
-#pragma unroll
-          for (int i = 0; i < kN8; i++) {
-            const float4 v0 =
-                *reinterpret_cast<const float4*>(vp + i * 8 * L::kVRow + b * 128);
-            const float4 v1 =
-                *reinterpret_cast<const float4*>(vp + (i * 8 + 1) * L::kVRow + b * 128);
-            uint32_t h0[4], l0[4], h1[4], l1[4];
-            split_tf32(v0.x, h0[0], l0[0]);
-            split_tf32(v0.y, h0[1], l0[1]);
-            split_tf32(v0.z, h0[2], l0[2]);
-            split_tf32(v0.w, h0[3], l0[3]);
-            split_tf32(v1.x, h1[0], l1[0]);
-            split_tf32(v1.y, h1[1], l1[1]);
-            split_tf32(v1.z, h1[2], l1[2]);
-            split_tf32(v1.w, h1[3], l1[3]);
-#pragma unroll
-            for (int e = 0; e < 4; e++) mma_tf32(x[e], ph[i], l0[e], l1[e]);
-#pragma unroll
-            for (int e = 0; e < 4; e++) mma_tf32(x[e], pl[i], h0[e], h1[e]);
-#pragma unroll
-            for (int e = 0; e < 4; e++) mma_tf32(x[e], ph[i], h0[e], h1[e]);
-          }
-#pragma unroll
-          for (int e = 0; e < 4; e++)
-#pragma unroll
-            for (int y = 0; y < 4; y++) o[4 * b + e][y] += x[e][y];
-        }
-      } else {
-        const uint32_t vp = saddr(vs) + (k0 + (lane & 7) + ((lane >> 3) & 1) * 8) * L::kVRow +
-                            (lane >> 4) * 16;
-#pragma unroll
-        for (int i = 0; i < kN8; i += 2) {
-          uint32_t ph[4], pl[4];
-          split_bf16(s[i][0], s[i][1], ph[0], pl[0]);
-          split_bf16(s[i][2], s[i][3], ph[1], pl[1]);
-          split_bf16(s[i + 1][0], s[i + 1][1], ph[2], pl[2]);
-          split_bf16(s[i + 1][2], s[i + 1][3], ph[3], pl[3]);
-#pragma unroll
-          for (int b = 0; b < kOut; b += 2) {
-            uint32_t v[4];
-            ldsm4t(vp + i * 8 * L::kVRow + b * 16, v);
-            mma_bf16(o[b], ph, v[0], v[1]);
-            mma_bf16(o[b + 1], ph, v[2], v[3]);
-            mma_bf16(o[b], pl, v[0], v[1]);
-            mma_bf16(o[b + 1], pl, v[2], v[3]);
+          for (int i = 0; i < kOut; i++) {
+            o[i][0] = o[i][0] * fA + p[(4 * i) * kStep] * gA;
+            o[i][1] = o[i][1] * fA + p[(4 * i + 1) * kStep] * gA;
+            o[i][2] = o[i][2] * fB + p[(4 * i + 2) * kStep] * gB;
+            o[i][3] = o[i][3] * fB + p[(4 * i + 3) * kStep] * gB;
           }
         }
       }
     }
-  }
-  if constexpr (!kBatch) cp_async_wait<0>();
-  lA += __shfl_xor_sync(0xFFFFFFFFu, lA, 1);
-  lA += __shfl_xor_sync(0xFFFFFFFFu, lA, 2);
-  lB += __shfl_xor_sync(0xFFFFFFFFu, lB, 1);
-  lB += __shfl_xor_sync(0xFFFFFFFFu, lB, 2);
+    if (kw == 0) {
 
-  // The key warps' parts of the rows are joined in shared memory, warps of
-  // the upper half into the lower one, in the last tile's place (tiles behind it
-  // may be on their way).
-  if constexpr (KW > 1) {
-    constexpr int kLane = kOut * 4 + 4;  // values a lane hands over
-    float* x = reinterpret_cast<float*>(smem + (kBatch ? (at - 1) % kStages * L::kStage : 0));
-    static_assert((size_t)MW * (KW / 2) * 32 * kLane * 4 <= L::kStage, "join fits a tile");
+    // One split: the rows are complete (a row without keys is zeros). Else the
+    // parts go to the workspace as they are, in 32 bits.
+    const bool whole = !kBatch && a.whole && a.splits == 1;
 #pragma unroll
-    for (int half = KW / 2; half > 0; half /= 2) {
-      __syncthreads();
-      // [value][warp][lane]: lanes side by side.
-      if (kw >= half && kw < 2 * half) {
-        float* p = x + ((kw - half) * MW + mw) * 32 + lane;
-        constexpr int kStep = MW * (KW / 2) * 32;
+    for (int half = 0; half < 2; half++) {
+      const int r = half ? rB : rA, tok = half ? tB : tA;
+      if (r >= R) continue;
+      const float m = half ? mB : mA, l = half ? lB : lA;
+      const float f = whole ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
+      const size_t at = walk.part(a, rows_of, head, parts, r);
+      if (!whole && c4 == 0) a.ml[at] = make_float2(m, l);
+      T* out = static_cast<T*>(a.att) + tok * a.ldo +
+               (size_t)(head * a.group + r - tok * a.group) * HD;
+      float* part = a.part + at * HD;
+      if constexpr (kF32) {
+        float* to = whole ? reinterpret_cast<float*>(out) : part;
 #pragma unroll
-        for (int i = 0; i < kOut; i++)
+        for (int b = 0; b < HD / 32; b++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) p[(4 * i + e) * kStep] = o[i][e];
-        p[(4 * kOut) * kStep] = mA;
-        p[(4 * kOut + 1) * kStep] = mB;
-        p[(4 * kOut + 2) * kStep] = lA;
-        p[(4 * kOut + 3) * kStep] = lB;
-      }
-      __syncthreads();
-      if (kw < half) {
-        const float* p = x + (kw * MW + mw) * 32 + lane;
-        constexpr int kStep = MW * (KW / 2) * 32;
-        const float m2A = p[(4 * kOut) * kStep], m2B = p[(4 * kOut + 1) * kStep];
-        const float nA = fmaxf(mA, m2A), nB = fmaxf(mB, m2B);
-        const float fA = nA == -INFINITY ? 0.f : exp2f(mA - nA);
-        const float fB = nB == -INFINITY ? 0.f : exp2f(mB - nB);
-        const float gA = nA == -INFINITY ? 0.f : exp2f(m2A - nA);
-        const float gB = nB == -INFINITY ? 0.f : exp2f(m2B - nB);
-        lA = lA * fA + p[(4 * kOut + 2) * kStep] * gA;
-        lB = lB * fB + p[(4 * kOut + 3) * kStep] * gB;
-        mA = nA;
-        mB = nB;
+          for (int e = 0; e < 2; e++)
+            *reinterpret_cast<float4*>(to + 32 * b + 8 * c4 + 4 * e) =
+                make_float4(o[4 * b][2 * half + e] * f, o[4 * b + 1][2 * half + e] * f,
+                            o[4 * b + 2][2 * half + e] * f, o[4 * b + 3][2 * half + e] * f);
+      } else {
 #pragma unroll
         for (int i = 0; i < kOut; i++) {
-          o[i][0] = o[i][0] * fA + p[(4 * i) * kStep] * gA;
-          o[i][1] = o[i][1] * fA + p[(4 * i + 1) * kStep] * gA;
-          o[i][2] = o[i][2] * fB + p[(4 * i + 2) * kStep] * gB;
-          o[i][3] = o[i][3] * fB + p[(4 * i + 3) * kStep] * gB;
+          const float x0 = o[i][2 * half] * f, x1 = o[i][2 * half + 1] * f;
+          if (whole) {
+            uint32_t w;
+            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(x1), "f"(x0));
+            *reinterpret_cast<uint32_t*>(out + 8 * i + 2 * c4) = w;
+          } else {
+            *reinterpret_cast<float2*>(part + 8 * i + 2 * c4) = make_float2(x0, x1);
+          }
         }
       }
     }
-  }
-  if (kw == 0) {
-
-  // One split: the rows are complete (a row without keys is zeros). Else the
-  // parts go to the workspace as they are, in 32 bits.
-  const bool whole = !kBatch && a.whole && a.splits == 1;
-#pragma unroll
-  for (int half = 0; half < 2; half++) {
-    const int r = half ? rB : rA, tok = half ? tB : tA;
-    if (r >= R) continue;
-    const float m = half ? mB : mA, l = half ? lB : lA;
-    const float f = whole ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
-    const size_t at = walk.part(a, rows_of, head, parts, r);
-    if (!whole && c4 == 0) a.ml[at] = make_float2(m, l);
-    T* out = static_cast<T*>(a.att) + tok * a.ldo +
-             (size_t)(head * a.group + r - tok * a.group) * HD;
-    float* part = a.part + at * HD;
-    if constexpr (kF32) {
-      float* to = whole ? reinterpret_cast<float*>(out) : part;
-#pragma unroll
-      for (int b = 0; b < HD / 32; b++)
-#pragma unroll
-        for (int e = 0; e < 2; e++)
-          *reinterpret_cast<float4*>(to + 32 * b + 8 * c4 + 4 * e) =
-              make_float4(o[4 * b][2 * half + e] * f, o[4 * b + 1][2 * half + e] * f,
-                          o[4 * b + 2][2 * half + e] * f, o[4 * b + 3][2 * half + e] * f);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kOut; i++) {
-        const float x0 = o[i][2 * half] * f, x1 = o[i][2 * half + 1] * f;
-        if (whole) {
-          uint32_t w;
-          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(x1), "f"(x0));
-          *reinterpret_cast<uint32_t*>(out + 8 * i + 2 * c4) = w;
-        } else {
-          *reinterpret_cast<float2*>(part + 8 * i + 2 * c4) = make_float2(x0, x1);
-        }
-      }
     }
-  }
-  }
   } while (kBatch && at < walk.count());
   if constexpr (kBatch) sg::pdl_wait();
 }
@@ -924,153 +925,153 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(Args a) {
 
   int at = 0;  // tiles gone through
   do {
-  const Rows rows_of = walk.rows(at);
-  const int head = walk.head(at), R = rows_of.t * a.group, parts = walk.parts(at);
-  // Scores in units of log2, so that the softmax is exp2.
-  const float scale = 1.4426950408889634f / sqrtf((float)HD);
-  ulonglong2 q[kFewRows][kQ];
-  float m[kFewRows], l[kFewRows];
-  f32x2 o[kFewRows][kO / 2];
+    const Rows rows_of = walk.rows(at);
+    const int head = walk.head(at), R = rows_of.t * a.group, parts = walk.parts(at);
+    // Scores in units of log2, so that the softmax is exp2.
+    const float scale = 1.4426950408889634f / sqrtf((float)HD);
+    ulonglong2 q[kFewRows][kQ];
+    float m[kFewRows], l[kFewRows];
+    f32x2 o[kFewRows][kO / 2];
 #pragma unroll
-  for (int r = 0; r < kFewRows; r++) {
-    const int row = r < R ? r : 0, tok = row / a.group;
-    const float* from = static_cast<const float*>(a.q) + (rows_of.token0 + tok) * a.ldq +
-                        (size_t)(head * a.group + row - tok * a.group) * HD + 4 * c4;
-#pragma unroll
-    for (int j = 0; j < kQ; j++) {
-      const float4 x = *reinterpret_cast<const float4*>(from + 16 * j);
-      q[r][j].x = pack2(x.x * scale, x.y * scale);
-      q[r][j].y = pack2(x.z * scale, x.w * scale);
-    }
-    m[r] = -INFINITY;
-    l[r] = 0.f;
-#pragma unroll
-    for (int i = 0; i < kO / 2; i++) o[r][i] = 0;
-  }
-
-  for (bool more = true; more; at++) {
-    cp_async_wait<kStages - 2>();
-    __syncthreads();
-    walk.fetch(at + kStages - 1);  // into the buffer that the last tile left
-    int rows, first;
-    walk.keys(at, rows, first);
-    more = !walk.last(at);
-    const bool old = first < 0;
-    const unsigned char* ks = smem + at % kStages * L::kStage;
-    const unsigned char* vs = ks + L::kKeys * L::kKRow;
-    const int k0 = warp * kWarpKeys;  // the warp's first key in the tile
-    if (k0 < rows) {
-      f32x2 s[kFewRows];
-#pragma unroll
-      for (int r = 0; r < kFewRows; r++) s[r] = 0;
-      const unsigned char* kp = ks + (k0 + g8) * L::kKRow + c4 * 16;
+    for (int r = 0; r < kFewRows; r++) {
+      const int row = r < R ? r : 0, tok = row / a.group;
+      const float* from = static_cast<const float*>(a.q) + (rows_of.token0 + tok) * a.ldq +
+                          (size_t)(head * a.group + row - tok * a.group) * HD + 4 * c4;
 #pragma unroll
       for (int j = 0; j < kQ; j++) {
-        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(kp + j * 64);
+        const float4 x = *reinterpret_cast<const float4*>(from + 16 * j);
+        q[r][j].x = pack2(x.x * scale, x.y * scale);
+        q[r][j].y = pack2(x.z * scale, x.w * scale);
+      }
+      m[r] = -INFINITY;
+      l[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kO / 2; i++) o[r][i] = 0;
+    }
+
+    for (bool more = true; more; at++) {
+      cp_async_wait<kStages - 2>();
+      __syncthreads();
+      walk.fetch(at + kStages - 1);  // into the buffer that the last tile left
+      int rows, first;
+      walk.keys(at, rows, first);
+      more = !walk.last(at);
+      const bool old = first < 0;
+      const unsigned char* ks = smem + at % kStages * L::kStage;
+      const unsigned char* vs = ks + L::kKeys * L::kKRow;
+      const int k0 = warp * kWarpKeys;  // the warp's first key in the tile
+      if (k0 < rows) {
+        f32x2 s[kFewRows];
+#pragma unroll
+        for (int r = 0; r < kFewRows; r++) s[r] = 0;
+        const unsigned char* kp = ks + (k0 + g8) * L::kKRow + c4 * 16;
+#pragma unroll
+        for (int j = 0; j < kQ; j++) {
+          const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(kp + j * 64);
+#pragma unroll
+          for (int r = 0; r < kFewRows; r++) {
+            s[r] = fma2(q[r][j].x, x.x, s[r]);
+            s[r] = fma2(q[r][j].y, x.y, s[r]);
+          }
+        }
+        float p[kFewRows], top[kFewRows];
 #pragma unroll
         for (int r = 0; r < kFewRows; r++) {
-          s[r] = fma2(q[r][j].x, x.x, s[r]);
-          s[r] = fma2(q[r][j].y, x.y, s[r]);
+          const float2 both = unpack2(s[r]);
+          p[r] = both.x + both.y;
+          p[r] += __shfl_xor_sync(0xFFFFFFFFu, p[r], 1);
+          p[r] += __shfl_xor_sync(0xFFFFFFFFu, p[r], 2);
+          bool in = k0 + g8 < rows && r < R;
+          if (!old && in) {
+            in = seen_of(a, rows_of, r / a.group, first + k0) >> g8 & 1;
+          }
+          if (!in) p[r] = -INFINITY;
+          top[r] = fmaxf(p[r], __shfl_xor_sync(0xFFFFFFFFu, p[r], 4));
+          top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 8));
+          top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 16));
         }
-      }
-      float p[kFewRows], top[kFewRows];
-#pragma unroll
-      for (int r = 0; r < kFewRows; r++) {
-        const float2 both = unpack2(s[r]);
-        p[r] = both.x + both.y;
-        p[r] += __shfl_xor_sync(0xFFFFFFFFu, p[r], 1);
-        p[r] += __shfl_xor_sync(0xFFFFFFFFu, p[r], 2);
-        bool in = k0 + g8 < rows && r < R;
-        if (!old && in) {
-          in = seen_of(a, rows_of, r / a.group, first + k0) >> g8 & 1;
-        }
-        if (!in) p[r] = -INFINITY;
-        top[r] = fmaxf(p[r], __shfl_xor_sync(0xFFFFFFFFu, p[r], 4));
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 8));
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 16));
-      }
-#pragma unroll
-      for (int r = 0; r < kFewRows; r++) {
-        if (top[r] > m[r]) {  // the same in all lanes
-          const float f = exp2f(m[r] - top[r]);
-          m[r] = top[r];
-          l[r] *= f;
-#pragma unroll
-          for (int i = 0; i < kO / 2; i++) o[r][i] = mul2(pack2(f, f), o[r][i]);
-        }
-        // A row that has seen no key yet keeps m = -inf and zeros.
-        p[r] = exp2f(p[r] - (m[r] == -INFINITY ? 0.f : m[r]));
-        l[r] += p[r];
-      }
-      const unsigned char* vp = vs + k0 * L::kVRow + lane * kO * 4;
-#pragma unroll
-      for (int kk = 0; kk < 8; kk++) {
-        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(vp + kk * L::kVRow);
 #pragma unroll
         for (int r = 0; r < kFewRows; r++) {
-          const float w = __shfl_sync(0xFFFFFFFFu, p[r], 4 * kk);
-          // A drafted row that is hidden may hold anything; cached ones are
-          // seen by all.
-          if (old || w != 0.f) {
-            o[r][0] = fma2(pack2(w, w), x.x, o[r][0]);
-            o[r][1] = fma2(pack2(w, w), x.y, o[r][1]);
+          if (top[r] > m[r]) {  // the same in all lanes
+            const float f = exp2f(m[r] - top[r]);
+            m[r] = top[r];
+            l[r] *= f;
+#pragma unroll
+            for (int i = 0; i < kO / 2; i++) o[r][i] = mul2(pack2(f, f), o[r][i]);
+          }
+          // A row that has seen no key yet keeps m = -inf and zeros.
+          p[r] = exp2f(p[r] - (m[r] == -INFINITY ? 0.f : m[r]));
+          l[r] += p[r];
+        }
+        const unsigned char* vp = vs + k0 * L::kVRow + lane * kO * 4;
+#pragma unroll
+        for (int kk = 0; kk < 8; kk++) {
+          const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(vp + kk * L::kVRow);
+#pragma unroll
+          for (int r = 0; r < kFewRows; r++) {
+            const float w = __shfl_sync(0xFFFFFFFFu, p[r], 4 * kk);
+            // A drafted row that is hidden may hold anything; cached ones are
+            // seen by all.
+            if (old || w != 0.f) {
+              o[r][0] = fma2(pack2(w, w), x.x, o[r][0]);
+              o[r][1] = fma2(pack2(w, w), x.y, o[r][1]);
+            }
           }
         }
       }
     }
-  }
-  if constexpr (!kBatch) cp_async_wait<0>();
-  __syncthreads();
+    if constexpr (!kBatch) cp_async_wait<0>();
+    __syncthreads();
 
-  // The warps' parts are joined in shared memory, a row by each warp, in the last
-  // tile's place.
-  float* part =  // [warp][row][HD + 2]
-      reinterpret_cast<float*>(smem + (kBatch ? (at - 1) % kStages * L::kStage : 0));
-  static_assert(kFewWarps * kFewRows * (HD + 2) * 4 <= (int)L::kStage, "join fits a tile");
-  static_assert(kFewWarps == kFewRows, "a warp per row");
+    // The warps' parts are joined in shared memory, a row by each warp, in the last
+    // tile's place.
+    float* part =  // [warp][row][HD + 2]
+        reinterpret_cast<float*>(smem + (kBatch ? (at - 1) % kStages * L::kStage : 0));
+    static_assert(kFewWarps * kFewRows * (HD + 2) * 4 <= (int)L::kStage, "join fits a tile");
+    static_assert(kFewWarps == kFewRows, "a warp per row");
 #pragma unroll
-  for (int r = 0; r < kFewRows; r++) {
-    l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 4);
-    l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 8);
-    l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 16);
-    float* to = part + (warp * kFewRows + r) * (HD + 2);
+    for (int r = 0; r < kFewRows; r++) {
+      l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 4);
+      l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 8);
+      l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 16);
+      float* to = part + (warp * kFewRows + r) * (HD + 2);
 #pragma unroll
-    for (int i = 0; i < kO / 2; i++)
-      *reinterpret_cast<float2*>(to + lane * kO + 2 * i) = unpack2(o[r][i]);
-    if (lane == 0) {
-      to[HD] = m[r];
-      to[HD + 1] = l[r];
+      for (int i = 0; i < kO / 2; i++)
+        *reinterpret_cast<float2*>(to + lane * kO + 2 * i) = unpack2(o[r][i]);
+      if (lane == 0) {
+        to[HD] = m[r];
+        to[HD + 1] = l[r];
+      }
     }
-  }
-  __syncthreads();
-  if (warp < R) {
-  float all = -INFINITY, sum = 0.f, out[kO];
+    __syncthreads();
+    if (warp < R) {
+    float all = -INFINITY, sum = 0.f, out[kO];
 #pragma unroll
-  for (int i = 0; i < kO; i++) out[i] = 0.f;
+    for (int i = 0; i < kO; i++) out[i] = 0.f;
 #pragma unroll
-  for (int w = 0; w < kFewWarps; w++)
-    all = fmaxf(all, part[(w * kFewRows + warp) * (HD + 2) + HD]);
+    for (int w = 0; w < kFewWarps; w++)
+      all = fmaxf(all, part[(w * kFewRows + warp) * (HD + 2) + HD]);
 #pragma unroll
-  for (int w = 0; w < kFewWarps; w++) {
-    const float* from = part + (w * kFewRows + warp) * (HD + 2);
-    const float f = all == -INFINITY ? 0.f : exp2f(from[HD] - all);
-    sum += from[HD + 1] * f;
+    for (int w = 0; w < kFewWarps; w++) {
+      const float* from = part + (w * kFewRows + warp) * (HD + 2);
+      const float f = all == -INFINITY ? 0.f : exp2f(from[HD] - all);
+      sum += from[HD + 1] * f;
 #pragma unroll
-    for (int i = 0; i < kO; i++) out[i] = fmaf(from[lane * kO + i], f, out[i]);
-  }
-  // One split: the row is complete (one without keys is zeros). Else its part
-  // goes to the workspace.
-  const bool whole = !kBatch && a.whole && a.splits == 1;
-  const float f = whole ? (sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum)) : 1.f;
-  const int tok = warp / a.group;
-  const size_t at = walk.part(a, rows_of, head, parts, warp);
-  if (!whole && lane == 0) a.ml[at] = make_float2(all, sum);
-  float* to = whole ? static_cast<float*>(a.att) + tok * a.ldo +
-                          (size_t)(head * a.group + warp - tok * a.group) * HD
-                    : a.part + at * HD;
+      for (int i = 0; i < kO; i++) out[i] = fmaf(from[lane * kO + i], f, out[i]);
+    }
+    // One split: the row is complete (one without keys is zeros). Else its part
+    // goes to the workspace.
+    const bool whole = !kBatch && a.whole && a.splits == 1;
+    const float f = whole ? (sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum)) : 1.f;
+    const int tok = warp / a.group;
+    const size_t at = walk.part(a, rows_of, head, parts, warp);
+    if (!whole && lane == 0) a.ml[at] = make_float2(all, sum);
+    float* to = whole ? static_cast<float*>(a.att) + tok * a.ldo +
+                            (size_t)(head * a.group + warp - tok * a.group) * HD
+                      : a.part + at * HD;
 #pragma unroll
-  for (int i = 0; i < kO; i++) to[lane * kO + i] = out[i] * f;
-  }
+    for (int i = 0; i < kO; i++) to[lane * kO + i] = out[i] * f;
+    }
   } while (kBatch && at < walk.count());
   if constexpr (kBatch) sg::pdl_wait();
 }
@@ -2017,7 +2018,8 @@ Batch batch_of(int sms, int type, int t, int tokens, int kh, int group, int hd) 
     // prefix of 128 tiles (its length is not known here); a CTA's start and end cost
     // as much as six. (16 splits at most: one kv head, 93 fp32 rows of 64 entries over 64543,
     // 115 us, now 37.)
-    const long long units = (long long)kh * ((tokens * group + sg::kTreeTcRows - 1) / sg::kTreeTcRows);
+    const int tiles = (tokens * group + sg::kTreeTcRows - 1) / sg::kTreeTcRows;
+    const long long units = (long long)kh * tiles;
     double best = 1e30;
     for (int n = 1; n <= kMaxSplits; n++) {
       const double cost = (double)((units * n + sms - 1) / sms) * (128.0 / n + 6);
