@@ -110,6 +110,19 @@ def test_matches_float64(cuda, type_, hd, kh, g, prefix, new, rows):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("type_", [F32, BF16])
+@pytest.mark.parametrize("hd,g,requests", [(64, 1, 40), (128, 2, 12), (128, 1, 3), (32, 3, 2),
+                                           (64, 8, 600)])
+def test_one_kv_head_and_a_long_prefix(cuda, type_, hd, g, requests):
+    """As many parts of a row as there are CTAs; one request's rows over many of them."""
+    torch = cuda
+    b = Batch(torch, 1, g, hd, 20000, [1] * requests, [9000] + [3] * (requests - 1), type_, hd,
+              ctx=9000 if requests < 100 else 9001)
+    b.run()
+    b.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [F32, BF16])
 @pytest.mark.parametrize("new", [[1] * 6, [3, 1, 0, 2]])
 def test_rows_of_no_request_stay_as_they_are(cuda, type_, new):
     """Padding before the first and behind the last request's tokens (q there

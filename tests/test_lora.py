@@ -131,6 +131,21 @@ def test_runs_of_tokens_have_one_adapter(cuda, type_):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("type_", [F32, BF16])
+@pytest.mark.parametrize("m,d,n", [(256, 1, 96), (256, 256, 40), (257, 257, 40), (65, 2, 8200),
+                                   (64, 70, 40), (256, 1, 8200)])
+def test_one_adapter_for_all_and_one_for_each(cuda, type_, m, d, n):
+    torch = cuda
+    x, a, b, adapter, scale, base = inputs(torch, m, 104, n, 8, d, type_, m + d, none=0)
+    if d >= m:
+        adapter = torch.randperm(d, device="cuda")[:m].int()
+    out = torch.full_like(base, float("nan"))
+    want, err = reference(torch, x, a, b, adapter, scale, base, None, STORE, type_)
+    assert call(torch, x, a, b, adapter, scale, base, out, STORE, type_) == 0
+    assert ((out.double() - want).abs() <= err).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [F32, BF16])
 @pytest.mark.parametrize("odd", [0, 1])
 def test_strides_no_base_no_scale_in_place(cuda, type_, odd):
     """Rows within wider ones, whose other entries stay as they are; odd: base
