@@ -262,7 +262,8 @@ int strasgpt_k_rope_axes(const void* x, long long x_token_stride,
 //                        up rows interleaved as in strasgpt_k_gemm_tc
 // A token whose adapter[i] is not in 0..adapters - 1 has none: v = base_i, and
 // nothing of a, b or x is read for it. Any tokens of a call may have any
-// adapters; neighbours that share one share its products. Adapters of a lower
+// adapters; neighbours that share one share its products (above 512 tokens they alone
+// do: tokens should be in order of their adapters there). Adapters of a lower
 // rank are padded with zeros.
 //
 // x, base and out have the type `type`; A x and all sums are held in 32 bits,

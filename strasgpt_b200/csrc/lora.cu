@@ -238,16 +238,21 @@ __device__ __forceinline__ void swiglu2(float* y, float g0, float u0, float g1, 
 }
 
 // --- Few tokens: a cluster per adapter -----------------------------------------
-// Up to kFew tokens in any order. Cluster c stands for token c: it is at work if
-// the number of earlier tokens with the same adapter is a multiple of kGroup,
-// and takes those of the next kGroup (this token the first) at once. So weights
-// are read once for eight tokens that share them, wherever they stand.
+// Up to kFew tokens in any order, kThreads of them looked at together. Cluster c stands
+// for token c: it is at work if the number of earlier ones with the same adapter is a
+// multiple of kGroup, and takes those of the next kGroup (this token the first) at
+// once. So weights are read once for eight tokens that share them, wherever they stand.
 //
 // Weights are the 16 rows of m16n8k16, the tokens its 8 columns. A warp takes 32
 // outputs at a time, two products: row g + 8 h of product t is output
 // 4 g + 2 t + h, so that a lane has four outputs in a row of two tokens. B's
 // first rows are on their way before the cluster's sums are there.
-constexpr int kFew = kThreads, kGroup = 8;
+//
+// kFew: tokens whose neighbours have other adapters are runs of one to the other kernel,
+// a round of which takes as long as one of 96. us there / here, 512 tokens on 4096 x
+// 6144, rank 32: fp32 one run 29 / 28, six 45 / 29, all mixed 645 / 27; bf16 17 / 25,
+// 22 / 25, 344 / 22. 1024 tokens in six runs: 50 / 59, 25 / 48.
+constexpr int kFew = 2 * kThreads, kGroup = 8;
 // CTAs of a cluster: eight for up to kWide tokens, or where an adapter has more than
 // kLong outputs, else four: 61 tokens on 4096 x 6144, rank 16, 10.9 us with eight and
 // 11.4 with four, 128 tokens 14.7 and 13.3, 256 tokens 21 and 18; 61 on 4096 x 28672,
@@ -295,11 +300,12 @@ __global__ void __launch_bounds__(kThreads, U <= 2 ? 2 : 1) k_lora_few(const Lor
     const int id = p.adapter[i];
     return id >= 0 && id < p.adapters ? id : -1;
   };
-  const int id = me < p.m ? adapter(me) : -2, d = adapter(token);
-  const int earlier = __syncthreads_count(me < token && id == d);
+  const int mine = token / kThreads * kThreads + me;  // this thread's token
+  const int id = mine < p.m ? adapter(mine) : -2, d = adapter(token);
+  const int earlier = __syncthreads_count(mine < token && id == d);
   if (earlier % kGroup) return;  // the same in all CTAs of the cluster
   cluster_started();
-  const unsigned peers = __ballot_sync(0xFFFFFFFFu, me >= token && id == d);
+  const unsigned peers = __ballot_sync(0xFFFFFFFFu, mine >= token && id == d);
   if (lane == 0) before[warp] = __popc(peers);
   __syncthreads();
   int at = __popc(peers & ((1u << lane) - 1)), count = 0;
@@ -308,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, U <= 2 ? 2 : 1) k_lora_few(const Lor
     if (w < warp) at += before[w];
     count += before[w];
   }
-  if ((peers >> lane & 1) && at < kGroup) members[at] = me;
+  if ((peers >> lane & 1) && at < kGroup) members[at] = mine;
   count = min(count, kGroup);
   __syncthreads();
 
@@ -727,8 +733,8 @@ __device__ __forceinline__ T* entry(uint8_t* row, int r, int e) {
 }
 
 // A warp reads `outs` entries each of `mine` rows, ld apart, into a swizzled tile. Several
-// rows are on their way at once (287 bf16 tokens on 1672 x 2284, SwiGLU, 42 us one after
-// the other, now 20), and apart from the rows that TMA brings, which need its registers.
+// rows are on their way at once (636 fp32 tokens on 776 x 2803, rank 8, 40 us one after
+// the other, now 33), and apart from the rows that TMA brings, which need its registers.
 template <typename T>
 __device__ __noinline__ void read_rows(uint8_t* rows, const T* from, long long ld, int mine,
                                           int outs) {

@@ -5,7 +5,7 @@ Tolerance, with h = 2^-24 (half a step of fp32) and b = 2^-8 (of bf16). A matrix
 instruction cuts its sums: 2 h of the sum of the products' sizes each. For a
 token, |A||x| (of a rank) and |B||s| stand for those sums.
 
-A x. fp32 rows: products are exact (three parts of 8 bits). Up to 256 tokens, 32
+A x. fp32 rows: products are exact (three parts of 8 bits). Up to 512 tokens, 32
 entries take six instructions from zero, 12 h; a warp's steps, at most k / 1024 + 1,
 are added with roundings of h. More tokens: two instructions per 32 entries in one sum
 of the large parts over at most k / 16 + 64 entries, 4 h (k / 512 + 2), and the small
@@ -131,7 +131,7 @@ def test_runs_of_tokens_have_one_adapter(cuda, type_):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("type_", [F32, BF16])
-@pytest.mark.parametrize("m,d,n", [(256, 1, 96), (256, 256, 40), (257, 257, 40), (65, 2, 8200),
+@pytest.mark.parametrize("m,d,n", [(256, 1, 96), (256, 256, 40), (512, 300, 40), (513, 600, 40), (300, 1, 96), (65, 2, 8200),
                                    (64, 70, 40), (256, 1, 8200)])
 def test_one_adapter_for_all_and_one_for_each(cuda, type_, m, d, n):
     torch = cuda
@@ -172,7 +172,7 @@ def test_strides_no_base_no_scale_in_place(cuda, type_, odd):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("type_", [F32, BF16])
-@pytest.mark.parametrize("m,k,n,r", [(257, 72, 65, 8), (1000, 200, 190, 72), (9000, 64, 34, 8)])
+@pytest.mark.parametrize("m,k,n,r", [(257, 72, 65, 8), (600, 72, 65, 8), (1000, 200, 190, 72), (9000, 64, 34, 8)])
 @pytest.mark.parametrize("epi", [STORE, ADD, SWIGLU])
 def test_many_tokens_within_wider_rows(cuda, type_, m, k, n, r, epi):
     """Many tokens, whose rows of base and out are off 16 bytes and lie in wider ones;
