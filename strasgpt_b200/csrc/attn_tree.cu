@@ -186,10 +186,9 @@ struct Rows {
   // that the call names.
   __device__ Rows(const sg::BatchArgs& a, int request, int first_row) {
     r0 = first_row;
-    const int from = a.first ? a.first[request] : min((long long)request * a.most, (long long)a.t);
-    const int to = a.first ? a.first[request + 1] : min((request + 1ll) * a.most, (long long)a.t);
-    token0 = min(max(from, 0), a.t);
-    t = min(max(min(to, a.t) - token0, 0), a.most);
+    sg::cut_tokens(a.first ? a.first[request] : (long long)request * a.most,
+                   a.first ? a.first[request + 1] : (request + 1ll) * a.most, a.t, a.most, &token0,
+                   &t);
     const int n = min(max(a.rows[request], 0), a.ctx);
     cached = max(n - t, 0);
     drafted = n - cached;

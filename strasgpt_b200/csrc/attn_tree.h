@@ -28,6 +28,17 @@ __device__ __forceinline__ int tree_cached(const TreeArgs& a) {
   return min(max(*a.cached, 0), a.ctx - a.drafted);
 }
 
+// Rows from..to - 1 of a call with `tokens` rows, as far as they are there and `most`
+// of them at most: the first one and how many. Any from and to, which device memory
+// holds, give rows of the call, or none: both ends are cut before they are subtracted.
+__host__ __device__ inline void cut_tokens(long long from, long long to, int tokens, int most,
+                                           int* token0, int* count) {
+  const int begin = (int)(from < 0 ? 0 : from > tokens ? tokens : from);
+  const int end = (int)(to < 0 ? 0 : to > tokens ? tokens : to);
+  *token0 = begin;
+  *count = end <= begin ? 0 : end - begin < most ? end - begin : most;
+}
+
 // A batch of requests whose t tokens are in all, each request's next to one
 // another: k, v and ctx are the requests' own caches', and a request's tokens
 // see each other in order.
