@@ -26,8 +26,8 @@
 //
 // Measured on a B200: 3.8 us for one token of 2048 x 2048, rank 8; 7.7 us for 61
 // tokens, most with one of 48 adapters of rank 16, on 4096 x 6144 (latency: a read of
-// A, the cluster's sums and a read of B, one after the other); 47 us for 2047 fp32
-// tokens of six prompts, rank 32, on 4096 x 4096 (2.2 TB/s); 142 us for 4001 bf16
+// A, the cluster's sums and a read of B, one after the other); 44 us for 2047 fp32
+// tokens of six prompts, rank 32, on 4096 x 4096 (2.4 TB/s); 144 us for 4001 bf16
 // tokens, rank 64, on 4096 x 28672 with SwiGLU (2.8 TB/s). What bounds the last two is
 // noted at k_lora_many.
 #include "entry.h"
@@ -208,33 +208,21 @@ __device__ __forceinline__ void load(const uint16_t* from, float* v, int count, 
   }
 }
 
-// silu(gate) up. For results that are rounded to bf16, exp and divide to 2^-20.
+// silu(gate) up. For results that are rounded to bf16, approximate exp and reciprocal:
+// 2^-19 of the result for gates of up to 10, 2^-16 at -95.
 __device__ __forceinline__ float swiglu(float gate, float up, float) {
   return sg::swiglu(gate, up);
 }
+// For bf16 results: with E = e^-|g| = h h, silu(g) is g / (1 + E), and g E / (1 + E) below
+// 0. There g takes one h and the up the other, so that neither what is small nor what is
+// large leaves 32 bits before the result does (1 + e^-g would be infinite from -89 on, and
+// its reciprocal below the normal numbers from -87; here gates below -174 give 0).
 __device__ __forceinline__ float swiglu(float gate, float up, uint16_t) {
-  float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(gate * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-  return gate * r * up;
-}
-// Two of them. For bf16 results one reciprocal serves both, 1/a = b / (a b): what
-// bounds this is the unit of exp and reciprocal. (exp is cut at 2^60, so that a b
-// is finite: gates below -41 give 2^-60 of themselves.)
-__device__ __forceinline__ void swiglu2(float* y, float g0, float u0, float g1, float u1, float) {
-  y[0] = sg::swiglu(g0, u0);
-  y[1] = sg::swiglu(g1, u1);
-}
-__device__ __forceinline__ void swiglu2(float* y, float g0, float u0, float g1, float u1,
-                                        uint16_t) {
-  float e0, e1, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(fminf(g0 * -1.4426950408889634f, 60.f)));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(fminf(g1 * -1.4426950408889634f, 60.f)));
-  e0 += 1.f;
-  e1 += 1.f;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e0 * e1));
-  y[0] = g0 * u0 * (r * e1);
-  y[1] = g1 * u1 * (r * e0);
+  float h, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(h) : "f"(fabsf(gate) * -0.7213475204444817f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(h, h, 1.f)));
+  const float a = gate < 0.f ? h : 1.f;
+  return gate * a * r * (up * a);
 }
 
 // --- Few tokens: a cluster per adapter -----------------------------------------
@@ -786,6 +774,54 @@ __device__ __forceinline__ uint4 packed(const float* v) {
                       bf16x2(v[6], v[7]));
 }
 
+// Sixteen gates and ups in turn -> silu(gate) up, packed. All lanes of a warp call it.
+__device__ __forceinline__ void swiglu16(const float (&v)[32], uint4 (&y)[4], float t) {
+#pragma unroll
+  for (int c = 0; c < 4; c++) {
+    float x[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) x[j] = swiglu(v[8 * c + 2 * j], v[8 * c + 2 * j + 1], t);
+    y[c] = packed<float>(x);
+  }
+}
+// For bf16 results one reciprocal serves two, 1/a = b / (a b): what bounds this is the
+// unit of exp and reciprocal. That is good while a b is below 2^120, two gates of -41 or
+// one of -83; where one of the warp's pairs is beyond, or has a NaN, each result is
+// computed by itself. It is looked for once the results are there, so that nothing waits
+// for the vote (before the exponentials it cost 4001 tokens on 4096 x 28672 8 us).
+__device__ __forceinline__ void swiglu16(const float (&v)[32], uint4 (&y)[2], uint16_t t) {
+  float least = 1.f;  // of the reciprocals
+#pragma unroll
+  for (int c = 0; c < 2; c++) {
+    float x[8], r[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const float* const p = v + 16 * c + 4 * j;
+      float e0, e1;
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(p[0] * -1.4426950408889634f));
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(p[2] * -1.4426950408889634f));
+      e0 += 1.f;
+      e1 += 1.f;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r[j]) : "f"(e0 * e1));
+      x[2 * j] = p[0] * (r[j] * e1) * p[1];
+      x[2 * j + 1] = p[2] * (r[j] * e0) * p[3];
+    }
+    asm("min.NaN.f32 %0, %0, %1, %2;" : "+f"(least) : "f"(r[0]), "f"(r[1]));
+    asm("min.NaN.f32 %0, %0, %1, %2;" : "+f"(least) : "f"(r[2]), "f"(r[3]));
+    y[c] = packed<uint16_t>(x);
+  }
+  if (!__all_sync(0xFFFFFFFFu, least >= 0x1p-120f)) {
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[j] = swiglu(v[16 * c + 2 * j], v[16 * c + 2 * j + 1], t);
+      y[c] = packed<uint16_t>(x);
+    }
+    __syncwarp();
+  }
+}
+
 // Sixteen entries of a row of a stage of fp32 x -> the same place in three parts'
 // rows of 64 bytes, 64-byte swizzle.
 __device__ __forceinline__ void split_row(const uint8_t* row, int r, int half, uint8_t* to,
@@ -891,7 +927,7 @@ __device__ __forceinline__ void each_item(const LoraArgs& p, unsigned* starts, i
 // SMs are at it); over the whole, that items come in rounds of the 33 or so clusters
 // that the GPU holds (46 items of 4001 tokens in five runs make two rounds) and that an item takes 20 us before its first output (finding
 // it 4, A x 6, the exchange 6). Tiles of 128 tokens have room for one stage a side:
-// 4001 tokens in five runs 221 us, now 142.
+// 4001 tokens in five runs 221 us, now 144.
 template <typename T, int P>
 __global__ void __launch_bounds__(kManyThreads, P == 1 ? 2 : 1)
     k_lora_many(const LoraArgs p, const Layout l, const __grid_constant__ ManyMaps maps) {
@@ -1241,7 +1277,7 @@ __global__ void __launch_bounds__(kManyThreads, P == 1 ? 2 : 1)
         }
         if (mine) {
           constexpr int kV = 16 / (int)sizeof(T);
-          uint4 y[kCols / 2 / kV];  // of SwiGLU
+          uint4 y[kHalves][16 / kV];  // of SwiGLU
 #pragma unroll
           for (int h = 0; h < kHalves; h++) {
             float v[32];
@@ -1254,11 +1290,7 @@ __global__ void __launch_bounds__(kManyThreads, P == 1 ? 2 : 1)
             if (has) add_row<T>(row, r, h, v);
             if (both) add_row<T>(row + second, r, h, v);
             if (gated) {
-#pragma unroll
-              for (int j = 0; j < 16; j += 2)
-                swiglu2(v + j, v[2 * j], v[2 * j + 1], v[2 * j + 2], v[2 * j + 3], T());
-#pragma unroll
-              for (int c = 0; c < 16 / kV; c++) y[h * 16 / kV + c] = packed<T>(v + kV * c);
+              swiglu16(v, y[h], T());
             } else {
 #pragma unroll
               for (int c = 0; c < 32 / kV; c++)
@@ -1272,7 +1304,8 @@ __global__ void __launch_bounds__(kManyThreads, P == 1 ? 2 : 1)
             __syncwarp();
 #pragma unroll
             for (int c = 0; c < 4; c++)
-              *reinterpret_cast<uint4*>(rows + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = y[c];
+              *reinterpret_cast<uint4*>(rows + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
+                  y[c / (16 / kV)][c % (16 / kV)];
           }
           // A wait that ran out leaves NaN: no result passes for a complete one.
           if (!ok || failed) {
