@@ -1313,8 +1313,10 @@ __global__ void __launch_bounds__(kManyThreads, P == 1 ? 2 : 1)
             for (int c = 0; c < 8; c++)
               *reinterpret_cast<uint4*>(row + 16 * c) = make_uint4(~0u, ~0u, ~0u, ~0u);
           }
-          const int x = gated ? n / 2 : n;
-          if (mine == 32 && p.out_tma) {
+          const int x = gated ? n / 2 : n, last = gated ? outs / 2 : outs;
+          // (TMA stores whole 16 bytes: where the row ends within them, zeros would take
+          // the place of what lies behind it.)
+          if (mine == 32 && p.out_tma && last * sizeof(T) % 16 == 0) {
             fence_async();
             __syncwarp();
             if (lane == 0)
@@ -1322,7 +1324,6 @@ __global__ void __launch_bounds__(kManyThreads, P == 1 ? 2 : 1)
                         ring_at + stage.at * l.stage + 32 * quarter * 128);
           } else {
             __syncwarp();
-            const int last = gated ? outs / 2 : outs;
 #pragma unroll 4
             for (int j = 0; j < mine; j++) {
               T* const to = static_cast<T*>(p.out) + ((size_t)token0 + 32 * quarter + j) * p.ldo + x;
