@@ -842,44 +842,43 @@ __global__ void __launch_bounds__(32 * MW * KW, MW* KW <= 4 ? 2 : 1) k_tree(Args
       }
     }
     if (kw == 0) {
-
-    // One split: the rows are complete (a row without keys is zeros). Else the
-    // parts go to the workspace as they are, in 32 bits.
-    const bool whole = !kBatch && a.whole && a.splits == 1;
+      // One split: the rows are complete (a row without keys is zeros). Else the
+      // parts go to the workspace as they are, in 32 bits.
+      const bool whole = !kBatch && a.whole && a.splits == 1;
 #pragma unroll
-    for (int half = 0; half < 2; half++) {
-      const int r = half ? rB : rA, tok = half ? tB : tA;
-      if (r >= R) continue;
-      const float m = half ? mB : mA, l = half ? lB : lA;
-      const float f = whole ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
-      const size_t at = walk.part(a, rows_of, head, parts, r);
-      if (!whole && c4 == 0) a.ml[at] = make_float2(m, l);
-      T* out = static_cast<T*>(a.att) + tok * a.ldo +
-               (size_t)(head * a.group + r - tok * a.group) * HD;
-      float* part = a.part + at * HD;
-      if constexpr (kF32) {
-        float* to = whole ? reinterpret_cast<float*>(out) : part;
+      for (int half = 0; half < 2; half++) {
+        const int r = half ? rB : rA, tok = half ? tB : tA;
+        if (r >= R) continue;
+        const float m = half ? mB : mA, l = half ? lB : lA;
+        const float f = whole ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
+        const size_t at = walk.part(a, rows_of, head, parts, r);
+        if (!whole && c4 == 0) a.ml[at] = make_float2(m, l);
+        T* out = static_cast<T*>(a.att) + tok * a.ldo +
+                 (size_t)(head * a.group + r - tok * a.group) * HD;
+        float* part = a.part + at * HD;
+        if constexpr (kF32) {
+          float* to = whole ? reinterpret_cast<float*>(out) : part;
 #pragma unroll
-        for (int b = 0; b < HD / 32; b++)
+          for (int b = 0; b < HD / 32; b++)
 #pragma unroll
-          for (int e = 0; e < 2; e++)
-            *reinterpret_cast<float4*>(to + 32 * b + 8 * c4 + 4 * e) =
-                make_float4(o[4 * b][2 * half + e] * f, o[4 * b + 1][2 * half + e] * f,
-                            o[4 * b + 2][2 * half + e] * f, o[4 * b + 3][2 * half + e] * f);
-      } else {
+            for (int e = 0; e < 2; e++)
+              *reinterpret_cast<float4*>(to + 32 * b + 8 * c4 + 4 * e) =
+                  make_float4(o[4 * b][2 * half + e] * f, o[4 * b + 1][2 * half + e] * f,
+                              o[4 * b + 2][2 * half + e] * f, o[4 * b + 3][2 * half + e] * f);
+        } else {
 #pragma unroll
-        for (int i = 0; i < kOut; i++) {
-          const float x0 = o[i][2 * half] * f, x1 = o[i][2 * half + 1] * f;
-          if (whole) {
-            uint32_t w;
-            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(x1), "f"(x0));
-            *reinterpret_cast<uint32_t*>(out + 8 * i + 2 * c4) = w;
-          } else {
-            *reinterpret_cast<float2*>(part + 8 * i + 2 * c4) = make_float2(x0, x1);
+          for (int i = 0; i < kOut; i++) {
+            const float x0 = o[i][2 * half] * f, x1 = o[i][2 * half + 1] * f;
+            if (whole) {
+              uint32_t w;
+              asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(x1), "f"(x0));
+              *reinterpret_cast<uint32_t*>(out + 8 * i + 2 * c4) = w;
+            } else {
+              *reinterpret_cast<float2*>(part + 8 * i + 2 * c4) = make_float2(x0, x1);
+            }
           }
         }
       }
-    }
     }
   } while (kBatch && at < walk.count());
   if constexpr (kBatch) sg::pdl_wait();
@@ -1044,32 +1043,32 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) k_tree_few(Args a) {
     }
     __syncthreads();
     if (warp < R) {
-    float all = -INFINITY, sum = 0.f, out[kO];
+      float all = -INFINITY, sum = 0.f, out[kO];
 #pragma unroll
-    for (int i = 0; i < kO; i++) out[i] = 0.f;
+      for (int i = 0; i < kO; i++) out[i] = 0.f;
 #pragma unroll
-    for (int w = 0; w < kFewWarps; w++)
-      all = fmaxf(all, part[(w * kFewRows + warp) * (HD + 2) + HD]);
+      for (int w = 0; w < kFewWarps; w++)
+        all = fmaxf(all, part[(w * kFewRows + warp) * (HD + 2) + HD]);
 #pragma unroll
-    for (int w = 0; w < kFewWarps; w++) {
-      const float* from = part + (w * kFewRows + warp) * (HD + 2);
-      const float f = all == -INFINITY ? 0.f : exp2f(from[HD] - all);
-      sum += from[HD + 1] * f;
+      for (int w = 0; w < kFewWarps; w++) {
+        const float* from = part + (w * kFewRows + warp) * (HD + 2);
+        const float f = all == -INFINITY ? 0.f : exp2f(from[HD] - all);
+        sum += from[HD + 1] * f;
 #pragma unroll
-      for (int i = 0; i < kO; i++) out[i] = fmaf(from[lane * kO + i], f, out[i]);
-    }
-    // One split: the row is complete (one without keys is zeros). Else its part
-    // goes to the workspace.
-    const bool whole = !kBatch && a.whole && a.splits == 1;
-    const float f = whole ? (sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum)) : 1.f;
-    const int tok = warp / a.group;
-    const size_t at = walk.part(a, rows_of, head, parts, warp);
-    if (!whole && lane == 0) a.ml[at] = make_float2(all, sum);
-    float* to = whole ? static_cast<float*>(a.att) + tok * a.ldo +
-                            (size_t)(head * a.group + warp - tok * a.group) * HD
-                      : a.part + at * HD;
+        for (int i = 0; i < kO; i++) out[i] = fmaf(from[lane * kO + i], f, out[i]);
+      }
+      // One split: the row is complete (one without keys is zeros). Else its part
+      // goes to the workspace.
+      const bool whole = !kBatch && a.whole && a.splits == 1;
+      const float f = whole ? (sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum)) : 1.f;
+      const int tok = warp / a.group;
+      const size_t at = walk.part(a, rows_of, head, parts, warp);
+      if (!whole && lane == 0) a.ml[at] = make_float2(all, sum);
+      float* to = whole ? static_cast<float*>(a.att) + tok * a.ldo +
+                              (size_t)(head * a.group + warp - tok * a.group) * HD
+                        : a.part + at * HD;
 #pragma unroll
-    for (int i = 0; i < kO; i++) to[lane * kO + i] = out[i] * f;
+      for (int i = 0; i < kO; i++) to[lane * kO + i] = out[i] * f;
     }
   } while (kBatch && at < walk.count());
   if constexpr (kBatch) sg::pdl_wait();

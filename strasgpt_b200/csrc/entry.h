@@ -1,6 +1,6 @@
 // Host side shared by the kernel-level entry points that refuse a call with
-// -1 and a message instead of ending the process (rope.cu, attn_tree.cu,
-// sample.cu).
+// -1 and a message instead of ending the process (rope.cu, lora.cu,
+// attn_tree.cu, sample.cu).
 #pragma once
 
 #include <atomic>

@@ -24,11 +24,11 @@
 // parts and the small ones, and added with rounding. A x is held in 32 bits, and is
 // three parts (fp32 rows) or two (bf16 rows: 2^-17 of it, where the result has 2^-9).
 //
-// Measured on a B200: 3.8 us for one token of 2048 x 2048, rank 8; 7.7 us for 61
-// tokens, most with one of 48 adapters of rank 16, on 4096 x 6144 (latency: a read of
-// A, the cluster's sums and a read of B, one after the other); 44 us for 2047 fp32
-// tokens of six prompts, rank 32, on 4096 x 4096 (2.4 TB/s); 144 us for 4001 bf16
-// tokens, rank 64, on 4096 x 28672 with SwiGLU (2.8 TB/s). What bounds the last two is
+// Measured on a B200, captured calls in short runs: 3.8 us for one token of 2048 x 2048,
+// rank 8; 7.7 us for 61 tokens, most with one of 48 adapters of rank 16, on 4096 x 6144
+// (latency: a read of A, the cluster's sums and a read of B, one after the other); 44 us
+// for 2047 fp32 tokens of six prompts, rank 32, on 4096 x 4096 (2.4 TB/s); 144 us for 4001
+// bf16 tokens, rank 64, on 4096 x 28672 with SwiGLU (2.8 TB/s). What bounds the last two is
 // noted at k_lora_many.
 #include "entry.h"
 
@@ -250,7 +250,6 @@ constexpr int kWide = 64, kLong = 8192;
 // U units of 32 ranks.
 template <int U>
 struct Few {
-  static constexpr int kAhead = 1;
   static constexpr int kRow = 32 * U + 4;                     // floats of a token's sums
   static constexpr size_t bytes(int ctas) {
     return sizeof(float) * (kWarps + ctas) * kGroup * kRow;
@@ -272,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, U <= 2 ? 2 : 1) k_lora_few(const Lor
   using F = Few<U>;
   constexpr bool kF32 = sizeof(T) == 4;
   constexpr int kXParts = kF32 ? 3 : 1, kSParts = kF32 ? 3 : 2;
-  constexpr int kAhead = F::kAhead, kRow = F::kRow;
+  constexpr int kRow = F::kRow;
   extern __shared__ __align__(16) float smem[];
   float* const sums = smem;                                // [warp][token][kRow]
   float* const exchange = smem + kWarps * kGroup * kRow;   // [cta][token][kRow]
@@ -331,13 +330,10 @@ __global__ void __launch_bounds__(kThreads, U <= 2 ? 2 : 1) k_lora_few(const Lor
     load<4>(base + token0 * p.ldb + n, v[0], in0 && p.base ? last : 0, p.wide);
     load<4>(base + token1 * p.ldb + n, v[1], in1 && p.base ? last : 0, p.wide);
   };
-  uint4 w[kAhead][U][4];
-  float base[kAhead][2][4];
-#pragma unroll
-  for (int i = 0; i < kAhead; i++) {
-    load_rows(tile + i * kWarps, w[i]);
-    load_base(tile + i * kWarps, base[i]);
-  }
+  uint4 w[U][4];
+  float base[2][4];
+  load_rows(tile, w);
+  load_base(tile, base);
 
   // A x: this CTA's steps of 32 entries, one in kWarps to each warp. This lane's
   // column is token g8.
@@ -428,54 +424,50 @@ __global__ void __launch_bounds__(kThreads, U <= 2 ? 2 : 1) k_lora_few(const Lor
     for (int i = 0; i < 4; i++) parts<kSParts>(v[2 * i], v[2 * i + 1], &sb[u][0][i], 4);
   }
 
-  for (; tile < tile1; tile += kAhead * kWarps) {
+  for (; tile < tile1; tile += kWarps) {
+    float big[2][4], small[2][4];
 #pragma unroll
-    for (int i = 0; i < kAhead; i++) {
-      const int now = tile + i * kWarps;
-      float big[2][4], small[2][4];
+    for (int t = 0; t < 2; t++)
 #pragma unroll
-      for (int t = 0; t < 2; t++)
+      for (int e = 0; e < 4; e++) big[t][e] = small[t][e] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; e++) big[t][e] = small[t][e] = 0.f;
+    for (int u = 0; u < U; u++)
 #pragma unroll
-      for (int u = 0; u < U; u++)
+      for (int t = 0; t < 2; t++) {
+        uint32_t wa[2][4];
+        operands(w[u][2 * t], w[u][2 * t + 1], wa);
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-          uint32_t wa[2][4];
-          operands(w[i][u][2 * t], w[i][u][2 * t + 1], wa);
+        for (int h = 0; h < 2; h++) {
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-#pragma unroll
-            for (int q = kSParts - 1; q > 0; q--)
-              mma_bf16(small[t], wa[h], sb[u][q][2 * h], sb[u][q][2 * h + 1]);
-            mma_bf16(big[t], wa[h], sb[u][0][2 * h], sb[u][0][2 * h + 1]);
-          }
+          for (int q = kSParts - 1; q > 0; q--)
+            mma_bf16(small[t], wa[h], sb[u][q][2 * h], sb[u][q][2 * h + 1]);
+          mma_bf16(big[t], wa[h], sb[u][0][2 * h], sb[u][0][2 * h + 1]);
         }
-      float v[2][4];
+      }
+    float v[2][4];
 #pragma unroll
-      for (int e = 0; e < 2; e++)
+    for (int e = 0; e < 2; e++)
 #pragma unroll
-        for (int j = 0; j < 4; j++)  // product j / 2, row j % 2
-          v[e][j] = base[i][e][j] + (big[j / 2][2 * (j % 2) + e] + small[j / 2][2 * (j % 2) + e]);
-      load_rows(now + kAhead * kWarps, w[i]);
-      load_base(now + kAhead * kWarps, base[i]);
-      const int n = 32 * now + 4 * g8, last = now < tile1 ? max(0, min(4, p.n - n)) : 0;
+      for (int j = 0; j < 4; j++)  // product j / 2, row j % 2
+        v[e][j] = base[e][j] + (big[j / 2][2 * (j % 2) + e] + small[j / 2][2 * (j % 2) + e]);
+    load_rows(tile + kWarps, w);
+    load_base(tile + kWarps, base);
+    const int n = 32 * tile + 4 * g8, last = tile < tile1 ? max(0, min(4, p.n - n)) : 0;
 #pragma unroll
-      for (int e = 0; e < 2; e++) {
-        if (!(e ? in1 : in0) || !last) continue;
-        T* const row = static_cast<T*>(p.out) + (e ? token1 : token0) * p.ldo;
-        if (p.epi == STRASGPT_EPI_SWIGLU) {
-          const float y[2] = {swiglu(v[e][0], v[e][1], T()), swiglu(v[e][2], v[e][3], T())};
-          store<2>(row + n / 2, y, last / 2, p.wide);
-        } else {
-          if (p.epi == STRASGPT_EPI_ADD) {
-            float old[4];
-            load<4>(row + n, old, last, p.wide);
+    for (int e = 0; e < 2; e++) {
+      if (!(e ? in1 : in0) || !last) continue;
+      T* const row = static_cast<T*>(p.out) + (e ? token1 : token0) * p.ldo;
+      if (p.epi == STRASGPT_EPI_SWIGLU) {
+        const float y[2] = {swiglu(v[e][0], v[e][1], T()), swiglu(v[e][2], v[e][3], T())};
+        store<2>(row + n / 2, y, last / 2, p.wide);
+      } else {
+        if (p.epi == STRASGPT_EPI_ADD) {
+          float old[4];
+          load<4>(row + n, old, last, p.wide);
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[e][j] += old[j];
-          }
-          store<4>(row + n, v[e], last, p.wide);
+          for (int j = 0; j < 4; j++) v[e][j] += old[j];
         }
+        store<4>(row + n, v[e], last, p.wide);
       }
     }
   }
@@ -513,8 +505,8 @@ cudaError_t launch_few_rank(const LoraArgs& p, int dev, cudaStream_t s) {
 //
 // B (A x): a stage has 128 bytes of the tokens' base rows, and B's for as many
 // outputs. A x lies in shared memory, as bf16 parts. The sums go to one of kSlots
-// places in tensor memory. A thread has a token, adds its sums to the base row in the stage, where the results take their place,
-// and each warp sends its 32 rows off by TMA.
+// places in tensor memory. A thread has a token, adds its sums to the base row in the
+// stage, where the results take their place, and each warp sends its 32 rows off by TMA.
 constexpr int kManyThreads = kThreads + 128;
 constexpr int kSlots = 2, kMaxStages = 4;  // of a side
 constexpr int kChunks = 256;  // of 32 tokens that are looked over at a time
@@ -553,7 +545,8 @@ Layout layout_of(int tokens, bool both) {
   l.operand = M::kParts * P * l.panel;
   l.stage = l.panel * (both ? 2 : 1) + P * M::kSide;
   // Operands have 128 rows, whatever the tile has: what lies behind is read too
-  // (and comes to nothing), so that behind the last stage there is room.
+  // (and comes to nothing), so that behind the last stage there is room. (There is one
+  // stage at least, for tiles of up to 96 tokens.)
   const int room = M::kMemory - l.operand - std::max(0, kMaxTokens * 128 - l.stage);
   l.stages = std::min(kMaxStages, room / l.stage / 2);
   return l;
@@ -735,7 +728,8 @@ __device__ __noinline__ void read_rows(uint8_t* rows, const T* from, long long l
     for (int j = 0; j < kAtOnce; j++)
 #pragma unroll
       for (int e = 0; e < kOf; e++)
-        v[j][e] = j0 + j < mine && lane + 32 * e < outs ? from[(j0 + j) * ld + lane + 32 * e] : T(0);
+        v[j][e] = j0 + j < mine && lane + 32 * e < outs ? from[(j0 + j) * ld + lane + 32 * e]
+                                                        : T(0);
 #pragma unroll
     for (int j = 0; j < kAtOnce; j++)
 #pragma unroll
@@ -925,9 +919,9 @@ __device__ __forceinline__ void each_item(const LoraArgs& p, unsigned* starts, i
 // What bounds it: in the second product, memory and its latency (1.3 us from a
 // stage's request to its arrival, two stages a side of 96 tokens: 5.7 TB/s while all
 // SMs are at it); over the whole, that items come in rounds of the 33 or so clusters
-// that the GPU holds (46 items of 4001 tokens in five runs make two rounds) and that an item takes 20 us before its first output (finding
-// it 4, A x 6, the exchange 6). Tiles of 128 tokens have room for one stage a side:
-// 4001 tokens in five runs 221 us, now 144.
+// that the GPU holds (46 items of 4001 tokens in five runs make two rounds) and that an
+// item takes 20 us before its first output (finding it 4, A x 6, the exchange 6). Tiles
+// of 128 tokens have room for one stage a side: 4001 tokens in five runs 221 us, now 144.
 template <typename T, int P>
 __global__ void __launch_bounds__(kManyThreads, P == 1 ? 2 : 1)
     k_lora_many(const LoraArgs p, const Layout l, const __grid_constant__ ManyMaps maps) {
@@ -936,7 +930,8 @@ __global__ void __launch_bounds__(kManyThreads, P == 1 ? 2 : 1)
   constexpr int kParts = M::kParts, kCols = M::kCols, kHalves = kCols / 32, kRow = M::kRow;
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t filled_[2][kMaxStages], frees_[2][kMaxStages],
-      full_[2][kSlots], empty_[2][kSlots], x_full[M::kXBuffers], x_empty[M::kXBuffers], sums_full, done;
+      full_[2][kSlots], empty_[2][kSlots], x_full[M::kXBuffers], x_empty[M::kXBuffers],
+      sums_full, done;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int failed;
   __shared__ unsigned starts[kChunks];
@@ -1158,7 +1153,8 @@ __global__ void __launch_bounds__(kManyThreads, P == 1 ? 2 : 1)
 #pragma unroll 1
         for (int i = side_of; i < k_mine; i += 2, stage.next(stages)) {
           if (!kF32) continue;
-          const bool ok = wait_filled() && warp_wait(saddr(&x_empty[side_of]), x_phase ^ 1, &failed);
+          const bool ok =
+              wait_filled() && warp_wait(saddr(&x_empty[side_of]), x_phase ^ 1, &failed);
           x_phase ^= 1;
           if constexpr (kF32) {
             if (ok && r < (count + 31) / 32 * 32) {
@@ -1326,7 +1322,8 @@ __global__ void __launch_bounds__(kManyThreads, P == 1 ? 2 : 1)
             __syncwarp();
 #pragma unroll 4
             for (int j = 0; j < mine; j++) {
-              T* const to = static_cast<T*>(p.out) + ((size_t)token0 + 32 * quarter + j) * p.ldo + x;
+              T* const to =
+                  static_cast<T*>(p.out) + ((size_t)token0 + 32 * quarter + j) * p.ldo + x;
 #pragma unroll
               for (int e = lane; e < kCols; e += 32)
                 if (e < last)
@@ -1403,9 +1400,8 @@ bool encode_map(PFN_cuTensorMapEncodeTiled_v12000 encode, CUtensorMap* map, bool
 int clusters_of(int rank, int sms) { return std::max(1, (rank <= 64 ? 2 : 1) * sms / kCluster); }
 
 template <typename T, int P>
-cudaError_t launch_many(LoraArgs p, int dev, int sms, cudaStream_t s) {
+cudaError_t launch_many(const LoraArgs& p, int dev, int sms, cudaStream_t s) {
   const bool both = p.base && p.epi == STRASGPT_EPI_ADD;
-  while (layout_of<T, P>(p.tokens, both).stages < 1) p.tokens -= 32;
   static std::atomic<size_t> allowed[sg::kDevices];
   using M = Many<T, P>;
   const cudaError_t e = sg::allow_smem(k_lora_many<T, P>, M::kBytes, dev, allowed);
@@ -1423,8 +1419,8 @@ cudaError_t launch_many(LoraArgs p, int dev, int sms, cudaStream_t s) {
       (p.base && p.base_tma &&
        !encode_map(encode, &maps.base, M::kF32, p.base, p.n, p.m, p.ldb, 0, kCols, 32, sw128)) ||
       (p.out_tma &&
-       !(gated ? encode_map(encode, &maps.out, M::kF32, p.out, p.n / 2, p.m, p.ldo, 0, kCols / 2, 32,
-                            CU_TENSOR_MAP_SWIZZLE_64B)
+       !(gated ? encode_map(encode, &maps.out, M::kF32, p.out, p.n / 2, p.m, p.ldo, 0, kCols / 2,
+                            32, CU_TENSOR_MAP_SWIZZLE_64B)
                : encode_map(encode, &maps.out, M::kF32, p.out, p.n, p.m, p.ldo, 0, kCols, 32,
                             sw128))))
     return cudaErrorInvalidValue;

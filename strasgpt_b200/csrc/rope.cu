@@ -112,7 +112,8 @@ constexpr int blocks_of(Layout l) { return l == kHalves ? 4 : 6; }
 // An item is the pairs of one access, or V entries behind the turned ones,
 // which are copied.
 template <typename T, int V, Layout LAYOUT, typename Args>
-__global__ void __launch_bounds__(kThreads, blocks_of(LAYOUT)) k_rope(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, blocks_of(LAYOUT))
+    k_rope(const __grid_constant__ Args a) {
   constexpr int kPairs = LAYOUT == kAdjacent ? V / 2 : V;  // of an item
   constexpr bool kTwo = LAYOUT != kAdjacent;               // two accesses
   __shared__ float2 cs[kSinesMax];
