@@ -238,8 +238,8 @@ __device__ __forceinline__ float swiglu(float gate, float up, uint16_t) {
 //
 // kFew: tokens whose neighbours have other adapters are runs of one to the other kernel,
 // a round of which takes as long as one of 96. us there / here, 512 tokens on 4096 x
-// 6144, rank 32: fp32 one run 29 / 28, six 45 / 29, all mixed 645 / 27; bf16 17 / 25,
-// 22 / 25, 344 / 22. 1024 tokens in six runs: 50 / 59, 25 / 48.
+// 6144, rank 32: fp32 one run 28 / 20, six 40 / 23, 48 adapters at random 644 / 37; bf16
+// 16 / 17, 23 / 18, 334 / 33. 1024 tokens in six runs: 46 / 43, 26 / 33.
 constexpr int kFew = 2 * kThreads, kGroup = 8;
 // CTAs of a cluster: eight for up to kWide tokens, or where an adapter has more than
 // kLong outputs, else four: 61 tokens on 4096 x 6144, rank 16, 10.9 us with eight and
